@@ -218,6 +218,72 @@ int launch_nf24_pack(const float* w, int out_f, int in_f, const float* alphabet,
 int launch_nf24_decode(const int16_t* code01_t, const int8_t* q2_t, const float* scale, float* out,
                        int in_f, int out_f, int transposed, hipStream_t stream);
 
+// ---- operators that serve a batch of several requests (include/tsplat_hip_requests.h) ----
+
+// out[m] = y[m] + scale[a] (x[m] down[a]^T) up[a]^T, a = rows[m]; out[m] = y[m] where a names no adapter.
+enum AdapterType : int { kAdapterF32 = 0, kAdapterBf16 = 1, kAdapterF16 = 2 };
+struct LowRankParams {
+  const float* y;
+  const float* x;
+  const int32_t* rows;  // [M] adapter of each row
+  const void* down;     // [slots][ceil(R/16)][ceil(K/32)][4][16][8]
+  const void* up;       // [slots][ceil(N/16)][ceil(R/32)][4][16][8]
+  const float* scale;   // [slots]
+  const int32_t* rank;  // [slots]
+  float* out;
+  int64_t y_stride, x_stride, out_stride;
+  int M, K, N, slots, R;
+  int dtype;
+  float* scratch;
+};
+int64_t low_rank_scratch_bytes(int M, int K, int N, int slots, int R, int dtype);
+int launch_low_rank_add(const LowRankParams& p, hipStream_t stream);
+
+// x' = c x + gate[b] post(h), normed = pre(x') (1 + scale[b]) + shift[b].
+enum NormKind : int { kNormNone = 0, kNormLayer = 1, kNormRms = 2 };
+struct NormSpec {
+  int kind;
+  const float* weight;  // or null
+  const float* bias;    // or null
+  float eps;
+};
+struct ResidualNormParams {
+  const float* x;
+  const float* h;
+  float* out;
+  float* normed;
+  int64_t x_stride, h_stride, out_stride, normed_stride;
+  int64_t rows;
+  int cols;
+  float residual_scale;
+  const float* gate;  // or null
+  int64_t gate_stride;
+  NormSpec post, pre;
+  const float* scale;  // or null
+  const float* shift;
+  int64_t mod_stride;
+  int64_t rows_per_batch;
+};
+int launch_residual_norm(const ResidualNormParams& p, hipStream_t stream);
+
+// Parts 0 and 1 turned by their positions and, with a gamma, normed per head; part 2 copied.
+struct RopeAxesParams {
+  const float* x;
+  int64_t part_stride, batch_stride, token_stride, head_stride;
+  int parts;
+  const float* gamma[2];
+  float* out[3];
+  const void* positions;  // [position_batches][L][axes], int32 or fp32
+  int position_type, position_batches, axes;
+  const double* turns;    // [D/2] revolutions per unit of position
+  const int32_t* axis;    // [D/2]
+  int interleaved;
+  float eps;
+  int B, L, H, D;
+  int out_bhld;
+};
+int launch_rope_axes(const RopeAxesParams& p, hipStream_t stream);
+
 // Device scratch owned by the library, one grow-only buffer per (device,
 // stream, slot); null on allocation failure, or when the stream is under
 // graph capture and its buffer is too small.  The policy (reuse, free after

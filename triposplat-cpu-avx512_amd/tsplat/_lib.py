@@ -90,6 +90,18 @@ SIGNATURES = {
     "tsplat_build_arch": ([], ctypes.c_char_p),
 }
 
+# The operators that serve a batch of several requests; declared in
+# include/tsplat_hip_requests.h, with a version of their own.
+REQUEST_SIGNATURES = {
+    "tsplat_requests_abi_version": ([], _i),
+    "tsplat_low_rank_scratch_bytes": ([_i] * 6, _i64),
+    "tsplat_low_rank_add_async": ([_vp, _i64, _vp, _i64] + [_vp] * 6 + [_i64] + [_i] * 6 + [_vp, _i64, _vp], _i),
+    "tsplat_residual_norm_async": ([_vp, _i64] * 4 + [_i64, _i, ctypes.c_float, _vp, _i64]
+                                   + [_i, _vp, _vp, ctypes.c_float] * 2 + [_vp, _vp, _i64, _i64, _vp], _i),
+    "tsplat_rope_axes_async": ([_vp] + [_i64] * 4 + [_i] + [_vp] * 6 + [_i] * 3 + [_vp] * 2
+                               + [_i, ctypes.c_float] + [_i] * 5 + [_vp], _i),
+}
+
 STATUS_TEXT = {
     -1: "null pointer",
     -2: "bad sizes / stages / head dim",
@@ -107,6 +119,8 @@ STATUS_TEXT = {
 # version would read its arguments shifted) or entries are added (ABI 4: the
 # bf16 weight planes; ABI 5: the packer's error figures).
 ABI_VERSION = 5
+# tsplat_requests_abi_version(), likewise, of REQUEST_SIGNATURES.
+REQUESTS_ABI_VERSION = 1
 
 _CACHE: dict[str, ctypes.CDLL] = {}
 
@@ -143,6 +157,18 @@ def load_library(path: str | os.PathLike | None = None) -> ctypes.CDLL:
             f"{resolved} reports ABI version {found}, these bindings expect {ABI_VERSION}; "
             "rebuild it with `make -C triposplat-cpu-avx512_amd`"
         )
+    for name, (argtypes, restype) in REQUEST_SIGNATURES.items():
+        fn = getattr(lib, name, None)
+        if fn is None:
+            raise RuntimeError(f"{resolved} has no {name}; rebuild it with `make -C triposplat-cpu-avx512_amd`")
+        fn.argtypes = argtypes
+        fn.restype = restype
+    found = lib.tsplat_requests_abi_version()
+    if found != REQUESTS_ABI_VERSION:
+        raise RuntimeError(
+            f"{resolved} reports version {found} of its request operators, these bindings expect "
+            f"{REQUESTS_ABI_VERSION}; rebuild it with `make -C triposplat-cpu-avx512_amd`"
+        )
     _CACHE[key] = lib
     return lib
 
@@ -157,3 +183,53 @@ def current_stream_handle(device) -> int:
     import torch
 
     return int(torch.cuda.current_stream(device).cuda_stream)
+
+
+# ---- shared by the wrappers of REQUEST_SIGNATURES
+def enqueue(lib, fn_name, device, *args) -> None:
+    """Calls an asynchronous entry on torch's current stream of `device`; raises on a nonzero status."""
+    import torch
+
+    fn = getattr(lib, fn_name)
+    stream = int(torch.cuda.current_stream(device).cuda_stream)
+    if torch.cuda.current_device() == device.index:
+        status = fn(*args, stream)
+    else:
+        with torch.cuda.device(device):
+            status = fn(*args, stream)
+    check_status(status, fn_name)
+
+
+def no_gradients(*tensors) -> None:
+    """These operators have no backward: a tensor that expects one is refused, not cut off in silence."""
+    import torch
+
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise ValueError("this operator has no backward: call it under torch.no_grad(), or detach its inputs")
+
+
+def rows_of(name, t, cols) -> tuple[int, int]:
+    """(rows, row stride) of a GPU fp32 tensor [..., cols] whose rows lie at one stride; ValueError otherwise."""
+    import torch
+
+    if not (torch.is_tensor(t) and t.device.type == "cuda" and t.dtype == torch.float32):
+        raise ValueError(f"{name} must be an fp32 GPU tensor")
+    shape = t.shape
+    if len(shape) == 0 or shape[-1] != cols:
+        raise ValueError(f"{name} must have {cols} columns, its shape is {list(shape)}")
+    if t.is_contiguous():
+        return t.numel() // cols, cols
+    steps = t.stride()
+    if cols > 1 and steps[-1] != 1:
+        raise ValueError(f"{name} must have unit column stride")
+    rows, stride = 1, None
+    for size, step in zip(reversed(shape[:-1]), reversed(steps[:-1])):
+        if size != 1:
+            if stride is None:
+                stride = step
+            elif step != stride * rows:
+                raise ValueError(f"the rows of {name} must lie at one stride")
+            rows *= size
+    if stride is not None and rows > 1 and stride < cols:
+        raise ValueError(f"the rows of {name} overlap")
+    return rows, cols if stride is None else stride

@@ -11,7 +11,7 @@ mode: no torch fallback).
 """
 from __future__ import annotations
 
-from ._lib import check_status, current_stream_handle, load_library
+from ._lib import check_status, current_stream_handle, enqueue, load_library, no_gradients, rows_of
 
 # epilogue ids of tsplat_nf24_gemm_epilogue_async (include/tsplat_hip.h)
 EPILOGUE_STORE, EPILOGUE_GELU, EPILOGUE_GATED, EPILOGUE_ADD = 0, 2, 3, 4
@@ -137,6 +137,87 @@ def add_inplace(x, h, library=None):
         raise ValueError("add_inplace operands differ in size")
     _call(load_library(library), "tsplat_add_async", x.device, x.data_ptr(), h.data_ptr(), x.numel())
     return x
+
+
+# norm kinds of tsplat_residual_norm_async (include/tsplat_hip_requests.h)
+NORM_KINDS = {None: 0, "layer": 1, "rms": 2}
+
+
+def _batch_rows(name, t, B, C, device):
+    """(pointer, row stride) of a per-batch [B, C] or shared [1, C] row of a modulation."""
+    import torch
+
+    if not (torch.is_tensor(t) and t.device == device and t.dtype == torch.float32 and t.dim() == 2
+            and t.shape[1] == C and t.shape[0] in (1, B) and (C == 1 or t.stride(1) == 1)):
+        raise ValueError(f"{name} must be [{B}, {C}] or [1, {C}], fp32 on {device} with unit column stride")
+    if t.shape[0] > 1 and t.stride(0) < C:
+        raise ValueError(f"the rows of {name} overlap")
+    return t.data_ptr(), int(t.stride(0)) if t.shape[0] > 1 else C
+
+
+def residual_norm(x, h, *, gate=None, residual_scale=1.0, post_norm=None, post_weight=None, post_bias=None,
+                  post_eps=1.0e-6, norm="layer", weight=None, bias=None, eps=1.0e-6, scale=None, shift=None,
+                  out=None, normed=None, library=None):
+    """A branch's end and the next branch's start in one pass over the residual stream:
+
+        x' = residual_scale * x + gate[b] * post_norm(h)
+        y  = norm(x') * (1 + scale[b]) + shift[b]
+
+    and returns (x', y).  x, h [..., C]: fp32 on the GPU, rows at one stride each, b the first dimension.
+    post_norm: None, "layer" or "rms" (h / sqrt(mean(h^2) + eps)); norm: "layer" or "rms"; each with an optional
+    weight and bias [C].  gate, scale, shift: [B, C] views whose rows may be strided (chunks of a [B, 6C] tensor;
+    scale and shift with one stride), or [1, C] for every row; scale and shift go together.  out may be x itself,
+    normed may be h itself; they may not overlap the inputs otherwise.  No gradients."""
+    import torch
+
+    if not torch.is_tensor(x) or x.dim() < 1:
+        raise ValueError("x must be an fp32 GPU tensor")
+    if norm not in ("layer", "rms") or post_norm not in NORM_KINDS:
+        raise ValueError(f"norm is 'layer' or 'rms', post_norm one of them or None, not {norm!r}, {post_norm!r}")
+    C = int(x.shape[-1])
+    if C < 1 or not torch.is_tensor(h) or h.shape != x.shape:
+        raise ValueError("x and h must be [..., C] of one shape")
+    M, x_stride = rows_of("x", x, C)
+    _, h_stride = rows_of("h", h, C)
+    B = int(x.shape[0]) if x.dim() > 1 else 1
+    no_gradients(x, h, gate, post_weight, post_bias, weight, bias, scale, shift)
+    vectors = []
+    for name, t in (("post_weight", post_weight), ("post_bias", post_bias), ("weight", weight), ("bias", bias)):
+        if t is not None and not (torch.is_tensor(t) and t.device == x.device and t.dtype == torch.float32
+                                  and tuple(t.shape) == (C,) and t.is_contiguous()):
+            raise ValueError(f"{name} must be a contiguous [{C}] fp32 tensor on {x.device}")
+        vectors.append(None if t is None else t.data_ptr())
+    if post_norm is None and (post_weight is not None or post_bias is not None):
+        raise ValueError("post_weight and post_bias belong to a post_norm")
+    if (scale is None) != (shift is None):
+        raise ValueError("scale and shift go together")
+    if not float(eps) >= 0.0 or not float(post_eps) >= 0.0:
+        raise ValueError("eps must not be negative")
+    gate_ptr, gate_stride = (None, 0) if gate is None else _batch_rows("gate", gate, B, C, x.device)
+    scale_ptr, mod_stride = (None, 0) if scale is None else _batch_rows("scale", scale, B, C, x.device)
+    shift_ptr, shift_stride = (None, 0) if shift is None else _batch_rows("shift", shift, B, C, x.device)
+    if scale is not None and (scale.shape[0] != shift.shape[0] or mod_stride != shift_stride):
+        raise ValueError("scale and shift must share the row stride")
+    groups = {int(t.shape[0]) for t in (gate, scale) if t is not None} or {1}
+    if len(groups) > 1:  # one is [1, C]: its row serves every batch entry
+        if gate.shape[0] == 1:
+            gate_stride = 0
+        else:
+            mod_stride = 0
+    out = torch.empty(x.shape, dtype=torch.float32, device=x.device) if out is None else out
+    normed = torch.empty(x.shape, dtype=torch.float32, device=x.device) if normed is None else normed
+    if out.shape != x.shape or normed.shape != x.shape or not x.device == h.device == out.device == normed.device:
+        raise ValueError("x, h, out and normed must be of one shape on one GPU")
+    _, out_stride = rows_of("out", out, C)
+    _, normed_stride = rows_of("normed", normed, C)
+    if M == 0:
+        return out, normed
+    enqueue(load_library(library), "tsplat_residual_norm_async", x.device, x.data_ptr(), x_stride, h.data_ptr(),
+            h_stride, out.data_ptr(), out_stride, normed.data_ptr(), normed_stride, M, C, float(residual_scale),
+            gate_ptr, gate_stride, NORM_KINDS[post_norm], vectors[0], vectors[1], float(post_eps),
+            NORM_KINDS[norm], vectors[2], vectors[3], float(eps), scale_ptr, shift_ptr, mod_stride,
+            M // max(groups))
+    return out, normed
 
 
 def _unary(fn_name, x, out, library):

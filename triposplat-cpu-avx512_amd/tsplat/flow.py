@@ -268,12 +268,21 @@ class FlowModel:
         lin["fc2"].epilogue(h, bo.EPILOGUE_GATED, out=x2, gate=gate_mlp)
         return x
 
-    def velocity(self, z, cond, t, observe=None):
+    def velocity(self, z, cond, t, observe=None, *, adapters=None, slots=None, positions=None, rope=None):
         """z [B, L, C], cond [B, Lc, C], t [B] (already x1000) -> v [B, L, C].
+        adapters (flow_requests.FlowAdapters) with slots, one of them per
+        batch entry, or positions with rope (qkv.RopeAxes): the batch's
+        requests with their own adapters and latent positions
+        (flow_requests.velocity).
         observe(i, x), when given, sees the hidden state x entering block i,
         and observe(len(blocks), x) the state the final layer receives (for
         checks that recompute single blocks elsewhere; x is updated in place
         afterwards, so keep a copy)."""
+        if adapters is not None or slots is not None or positions is not None or rope is not None:
+            from . import flow_requests
+
+            return flow_requests.velocity(self, z, cond, t, adapters=adapters, slots=slots, positions=positions,
+                                          rope=rope, observe=observe)
         torch = self.torch
         B, L, C = (int(s) for s in z.shape)
         t_emb, t_mod = self.timestep(t)

@@ -11,7 +11,9 @@ tail tokens zero -- the layout the packed SDPA consumes.
 """
 from __future__ import annotations
 
-from ._lib import check_status, current_stream_handle, load_library
+import math
+
+from ._lib import check_status, current_stream_handle, enqueue, load_library, no_gradients, rows_of
 
 
 # bf16 rounding of the stored k and/or v (the K/V sensitivity probe,
@@ -142,3 +144,118 @@ def q_kv_selected_rope_rmsnorm_pack(q, kv, frequencies, selected_indices, q_gamm
         )
     check_status(status, "tsplat_q_kv_selected_postprocess_async")
     return qo, pk, pv
+
+
+class RopeAxes:
+    """Which position each pair of a head's vector turns by, and how fast: the plan of rope_axes.
+
+    dim: the head's size, even, at most 512; sections: how many of its dim / 2 pairs each axis (time, height, width)
+    takes, in order.  An axis has a ramp of its own, frequency theta^(-j / n) of its j-th pair of n; with shared,
+    one ramp theta^(-p / (dim / 2)) over all pairs is dealt out to the axes.  interleaved: a pair is the neighbours
+    (2p, 2p + 1), as in rope_complex; else (p, p + dim / 2)."""
+
+    def __init__(self, dim, sections, theta=10000.0, *, shared=False, interleaved=True, device="cuda"):
+        import torch
+
+        sections = [int(n) for n in sections]
+        dim = int(dim)
+        if dim < 2 or dim % 2 or dim > 512 or not 1 <= len(sections) <= 8:
+            raise ValueError("dim must be even, 2..512, with 1..8 sections")
+        if min(sections) < 0 or sum(sections) != dim // 2:
+            raise ValueError(f"the sections of {dim // 2} pairs must add up to them, not {sections}")
+        if not float(theta) > 0.0:
+            raise ValueError("theta must be positive")
+        self.dim, self.sections, self.theta = dim, tuple(sections), float(theta)
+        self.shared, self.interleaved = bool(shared), bool(interleaved)
+        axis = [i for i, n in enumerate(sections) for _ in range(n)]
+        if shared:
+            ramp = [self.theta ** (-p / (dim // 2)) for p in range(dim // 2)]
+        else:
+            ramp = [self.theta ** (-j / n) for n in sections for j in range(n)]
+        # revolutions per unit of position, in 64 bits: the kernel keeps the fraction of position * turns
+        self.turns = torch.tensor([f / (2.0 * math.pi) for f in ramp], dtype=torch.float64, device=device)
+        self.axis = torch.tensor(axis, dtype=torch.int32, device=device)
+        self.device = self.turns.device
+
+    @property
+    def axes(self):
+        return len(self.sections)
+
+
+def _rope_call(torch, x, strides, parts, gammas, positions, rope, eps, B, L, H, outs, out_bhld, library):
+    if not isinstance(rope, RopeAxes):
+        raise ValueError("rope must be a RopeAxes")
+    D = rope.dim
+    device = x.device
+    if (not torch.is_tensor(positions) or positions.dtype not in (torch.int32, torch.float32)
+            or not positions.is_contiguous() or positions.dim() not in (2, 3)
+            or tuple(positions.shape[-2:]) != (L, rope.axes) or (positions.dim() == 3 and positions.shape[0] not in (1, B))):
+        raise ValueError(f"positions must be a contiguous [{L}, {rope.axes}] or [{B}, {L}, {rope.axes}] tensor of int32 "
+                         "or fp32")
+    for g in gammas:
+        if g is not None and not (torch.is_tensor(g) and g.dtype == torch.float32 and tuple(g.shape) == (H, D)
+                                  and g.is_contiguous()):
+            raise ValueError(f"gamma must be a contiguous [{H}, {D}] fp32 tensor")
+    no_gradients(x, positions, *gammas)
+    if not float(eps) >= 0.0:
+        raise ValueError("eps must not be negative")
+    shape = (B, H, L, D) if out_bhld else (B, L, H, D)
+    if outs is None:
+        outs = [torch.empty(shape, dtype=torch.float32, device=device) for _ in range(parts)]
+    for o in outs:
+        if not (torch.is_tensor(o) and o.dtype == torch.float32 and tuple(o.shape) == shape and o.is_contiguous()):
+            raise ValueError(f"out must be a contiguous {list(shape)} fp32 tensor")
+    if any(t is not None and t.device != device for t in (positions, *gammas, *outs)) or rope.device != device:
+        raise ValueError("x, positions, rope, gamma and out must be on one GPU")
+    if B * L * H == 0:
+        return outs
+    ptr = [None if g is None else g.data_ptr() for g in (*gammas, None)]
+    dst = [o.data_ptr() for o in outs] + [None, None]
+    enqueue(load_library(library), "tsplat_rope_axes_async", device, x.data_ptr(), *strides, parts, ptr[0], ptr[1],
+            dst[0], dst[1], dst[2], positions.data_ptr(), int(positions.dtype == torch.float32),
+            1 if positions.dim() == 2 else int(positions.shape[0]), rope.axes, rope.turns.data_ptr(),
+            rope.axis.data_ptr(), int(rope.interleaved), float(eps), B, L, H, D, int(out_bhld))
+    return outs
+
+
+def rope_axes(x, positions, rope, *, gamma=None, eps=1.0e-12, out=None, out_bhld=True, library=None):
+    """x [B, L, H, D] turned by positions of several axes, then with a gamma [H, D] the per-head RMSNorm
+    y * sqrt(D) / max(||y||, eps) * gamma, as [B, H, L, D] (out_bhld) or [B, L, H, D].
+
+    x: fp32 on the GPU, any strides that do not overlap, unit in D (a view into a projection's rows).  positions:
+    [L, axes] or [B, L, axes], int32 or fp32 (fractional places); an angle is taken in 64 bits, so far positions
+    keep their precision.  rope: RopeAxes.  out may not overlap x.  No gradients."""
+    import torch
+
+    if not (torch.is_tensor(x) and x.device.type == "cuda" and x.dtype == torch.float32 and x.dim() == 4):
+        raise ValueError("x must be a [B, L, H, D] fp32 GPU tensor")
+    B, L, H, D = (int(s) for s in x.shape)
+    if not isinstance(rope, RopeAxes) or D != rope.dim:
+        raise ValueError(f"rope must be a RopeAxes of the heads' size {D}")
+    sb, sl, sh, sd = x.stride()
+    if sd != 1:
+        raise ValueError("x must have unit stride within its vectors")
+    for size, step in ((B, sb), (L, sl), (H, sh)):
+        if size > 1 and step < D:
+            raise ValueError("the vectors of x overlap")
+    return _rope_call(torch, x, (0, sb, sl, sh), 1, (gamma,), positions, rope, eps, B, L, H,
+                      None if out is None else [out], out_bhld, library)[0]
+
+
+def qkv_rope_axes(qkv, positions, rope, q_gamma, k_gamma, B, L, H, *, eps=1.0e-12, outs=None, library=None):
+    """qkv [B*L, 3*H*D] = [q | k | v] of an unfused projection: q and k turned by positions of several axes and
+    normed per head as rope_axes does (a gamma of None: turned only), v moved; all three come back as [B, H, L, D],
+    what native_sdpa_f32_ex reads.  outs: three such tensors to write, or None.  The rows of qkv may be strided."""
+    import torch
+
+    if not isinstance(rope, RopeAxes):
+        raise ValueError("rope must be a RopeAxes")
+    B, L, H = int(B), int(L), int(H)
+    width = H * rope.dim
+    rows, stride = rows_of("qkv", qkv, 3 * width)
+    if rows != B * L:
+        raise ValueError(f"qkv has {rows} rows, not B * L = {B * L}")
+    if outs is not None and len(outs) != 3:
+        raise ValueError("outs must be three tensors")
+    return tuple(_rope_call(torch, qkv, (width, L * stride, stride, rope.dim), 3, (q_gamma, k_gamma), positions,
+                            rope, eps, B, L, H, outs, True, library))
