@@ -71,8 +71,8 @@ int tsplat_low_rank_add_async(const float* y, int64_t y_stride, const float* x, 
   if (!y || !x || !rows || !down || !up || !scale || !rank || !out) return kErrNull;
   if (M <= 0 || K <= 0 || N <= 0 || slots <= 0 || slots > kMaxSlots || max_rank <= 0 || max_rank > kMaxRank) return kErrDims;
   if (dtype != kAdapterF32 && dtype != kAdapterBf16 && dtype != kAdapterF16) return kErrDims;
-  // (the kernels number a matrix' tiles and a row's bytes in 32 bits)
-  if (K > (1 << 28) || N > (1 << 28)) return kErrDims;
+  // (the launches' grids hold these)
+  if (M > (1 << 28) || K > (1 << 20) || N > (1 << 20)) return kErrDims;
   const Rows ry{y, y_stride, M, N}, rx{x, x_stride, M, K}, ro{out, out_stride, M, N};
   if (!sane(ry) || !sane(rx) || !sane(ro)) return kErrRange;
   if ((!same(ro, ry) && !disjoint(ro, ry)) || !disjoint(ro, rx)) return kErrRange;
