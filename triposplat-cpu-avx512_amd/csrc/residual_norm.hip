@@ -1,42 +1,180 @@
 // A branch's norm, its gate and residual, and the next norm with its modulation, one pass over the rows:
 //   h' = post(h);  x' = c x + gate[b] h';  out = x';  normed = pre(x') (1 + scale[b]) + shift[b].
-// Statistics are fp32 sums of the row's values less its first mean, whose own sum corrects that mean: a row far from
-// zero keeps the precision of its differences.
+// 16 bytes a value from and to HBM, which bounds it.  Statistics are fp32 sums of the row's values less its first
+// mean, whose own sum corrects that mean: a row far from zero keeps the precision of its differences.
+
+#include <algorithm>
+#include <type_traits>
 
 #include "tsplat_common.h"
 #include "tsplat_launch.h"
+#include "wave_sum.h"
 
 namespace tsplat {
 namespace {
 
-constexpr int kThreads = 256;
+typedef float floatx4u __attribute__((ext_vector_type(4), aligned(4)));  // rows start at any float
 
-__device__ float block_sum(float v, float* lds) {
-  for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
-  __syncthreads();
-  float s = 0.0f;
-  for (int i = 0; i < kThreads / 64; ++i) s += lds[i];
-  return s;
+__device__ __forceinline__ int64_t block_index() { return (int64_t)blockIdx.y * gridDim.x + blockIdx.x; }
+
+// The sum over the RW waves of a row, in every lane.  lds: RW floats for each call that may be in flight.
+template <int RW>
+__device__ __forceinline__ float row_sum(float v, float* lds) {
+  v = group_sum<64>(v);
+  if constexpr (RW > 1) {
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = 0.0f;
+#pragma unroll
+    for (int i = 0; i < RW; ++i) v += lds[i];
+  }
+  return v;
 }
 
 struct Stats {
   float mean, left, inv;  // normed value = (v - mean - left) * inv
 };
 
+// A row in registers: RW waves, lane l of them holding columns 4 (64 RW i + l) .. + 3 for i < V.  All but the last i
+// are whole; `last` is how many of that one's four columns exist.
+template <int RW, int V>
+struct Row {
+  floatx4 v[V];
+};
+
+template <int RW, int V>
+__device__ __forceinline__ void load_row(Row<RW, V>& r, const float* src, int c0, int last) {
+#pragma unroll
+  for (int i = 0; i < V - 1; ++i) r.v[i] = *reinterpret_cast<const floatx4u*>(src + c0 + i * 256 * RW);
+  const float* tail = src + c0 + (V - 1) * 256 * RW;
+  if (last >= 4) {
+    r.v[V - 1] = *reinterpret_cast<const floatx4u*>(tail);
+  } else {
+    r.v[V - 1] = floatx4{};
+#pragma unroll
+    for (int e = 0; e < 3; ++e)
+      if (e < last) r.v[V - 1][e] = tail[e];
+  }
+}
+
+template <int RW, int V>
+__device__ __forceinline__ void store_row(const Row<RW, V>& r, float* dst, int c0, int last) {
+#pragma unroll
+  for (int i = 0; i < V - 1; ++i) *reinterpret_cast<floatx4u*>(dst + c0 + i * 256 * RW) = r.v[i];
+  float* tail = dst + c0 + (V - 1) * 256 * RW;
+  if (last >= 4) {
+    *reinterpret_cast<floatx4u*>(tail) = r.v[V - 1];
+  } else {
+#pragma unroll
+    for (int e = 0; e < 3; ++e)
+      if (e < last) tail[e] = r.v[V - 1][e];
+  }
+}
+
+// lds: 3 RW floats.
+template <int RW, int V>
+__device__ __forceinline__ Stats row_stats(const Row<RW, V>& r, int kind, float eps, float n, int last, float* lds) {
+  if (kind == kNormNone) return {0.0f, 0.0f, 1.0f};
+  float mean = 0.0f, left = 0.0f;
+  if (kind == kNormLayer) {
+    float s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < V; ++i) s += (r.v[i][0] + r.v[i][1]) + (r.v[i][2] + r.v[i][3]);  // (zeros past the end)
+    mean = row_sum<RW>(s, lds) / n;
+  }
+  float s = 0.0f, q = 0.0f;
+#pragma unroll
+  for (int i = 0; i < V; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float d = i == V - 1 && e >= last ? 0.0f : r.v[i][e] - mean;
+      s += d;
+      q = fmaf(d, d, q);
+    }
+  q = row_sum<RW>(q, lds + RW) / n;
+  if (kind == kNormLayer) {
+    left = row_sum<RW>(s, lds + 2 * RW) / n;
+    q = fmaxf(q - left * left, 0.0f);
+  }
+  return {mean, left, 1.0f / sqrtf(q + eps)};
+}
+
+// RW waves a row (one: four rows a workgroup); a row's x, h, gate and modulation are all asked for at once.
+template <int RW, int V>
+__global__ __launch_bounds__(RW == 1 ? 256 : RW * 64) void residual_norm_kernel(ResidualNormParams p) {
+  __shared__ float lds[RW == 1 ? 1 : 6 * RW];
+  const int64_t row = RW == 1 ? block_index() * 4 + (threadIdx.x >> 6) : block_index();
+  if (row >= p.rows) return;  // whole waves; with RW > 1 whole workgroups
+  const int c0 = (RW == 1 ? threadIdx.x & 63 : threadIdx.x) * 4, last = p.cols - c0 - (V - 1) * 256 * RW;
+  const int64_t b = p.gate || p.scale ? row / p.rows_per_batch : 0;
+  const float n = (float)p.cols;
+  Row<RW, V> x, h, gate;
+  load_row(h, p.h + row * p.h_stride, c0, last);
+  load_row(x, p.x + row * p.x_stride, c0, last);
+  if (p.gate) load_row(gate, p.gate + b * p.gate_stride, c0, last);
+  auto affine = [&](Row<RW, V>& r, const NormSpec& s, const Stats& st) {
+    if (s.kind == kNormNone) return;
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) r.v[i][e] = (r.v[i][e] - st.mean - st.left) * st.inv;
+    if (s.weight) {
+      Row<RW, V> w;
+      load_row(w, s.weight, c0, last);
+#pragma unroll
+      for (int i = 0; i < V; ++i) r.v[i] *= w.v[i];
+    }
+    if (s.bias) {
+      Row<RW, V> w;
+      load_row(w, s.bias, c0, last);
+#pragma unroll
+      for (int i = 0; i < V; ++i) r.v[i] += w.v[i];
+    }
+  };
+  affine(h, p.post, row_stats(h, p.post.kind, p.post.eps, n, last, lds));
+  if (p.gate) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) h.v[i] *= gate.v[i];
+  }
+#pragma unroll
+  for (int i = 0; i < V; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e)  // (past the end the statistics want zeros)
+      x.v[i][e] = i == V - 1 && e >= last ? 0.0f : fmaf(p.residual_scale, x.v[i][e], h.v[i][e]);
+  store_row(x, p.out + row * p.out_stride, c0, last);
+  affine(x, p.pre, row_stats(x, p.pre.kind, p.pre.eps, n, last, lds + (RW == 1 ? 0 : 3 * RW)));
+  if (p.scale) {
+    Row<RW, V> scale, shift;
+    load_row(scale, p.scale + b * p.mod_stride, c0, last);
+    load_row(shift, p.shift + b * p.mod_stride, c0, last);
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x.v[i][e] = fmaf(x.v[i][e], 1.0f + scale.v[i][e], shift.v[i][e]);
+  }
+  store_row(x, p.normed + row * p.normed_stride, c0, last);
+}
+
+// Rows too wide for registers: one workgroup a row, which is read again for each sum.
+constexpr int kWideThreads = 1024;
+
+__device__ float block_sum(float v, float* lds) {
+  __syncthreads();  // (the sums before have been read)
+  return row_sum<kWideThreads / 64>(v, lds);
+}
+
 template <typename F>
-__device__ Stats row_stats(int kind, float eps, int cols, float* lds, F value) {
+__device__ Stats wide_stats(int kind, float eps, int cols, float* lds, F value) {
   if (kind == kNormNone) return {0.0f, 0.0f, 1.0f};
   const float n = (float)cols;
   float mean = 0.0f, left = 0.0f;
   if (kind == kNormLayer) {
     float s = 0.0f;
-    for (int c = threadIdx.x; c < cols; c += kThreads) s += value(c);
+    for (int c = threadIdx.x; c < cols; c += kWideThreads) s += value(c);
     mean = block_sum(s, lds) / n;
   }
   float s = 0.0f, q = 0.0f;
-  for (int c = threadIdx.x; c < cols; c += kThreads) {
+  for (int c = threadIdx.x; c < cols; c += kWideThreads) {
     const float d = value(c) - mean;
     s += d;
     q = fmaf(d, d, q);
@@ -49,7 +187,7 @@ __device__ Stats row_stats(int kind, float eps, int cols, float* lds, F value) {
   return {mean, left, 1.0f / sqrtf(q + eps)};
 }
 
-__device__ __forceinline__ float normed_value(const NormSpec& s, const Stats& st, float v, int c) {
+__device__ __forceinline__ float wide_value(const NormSpec& s, const Stats& st, float v, int c) {
   if (s.kind == kNormNone) return v;
   v = (v - st.mean - st.left) * st.inv;
   if (s.weight) v *= s.weight[c];
@@ -57,33 +195,66 @@ __device__ __forceinline__ float normed_value(const NormSpec& s, const Stats& st
   return v;
 }
 
-// One workgroup a row of any width; the row is read again for each sum.
-__global__ __launch_bounds__(kThreads) void residual_norm_row_kernel(ResidualNormParams p) {
-  __shared__ float lds[kThreads / 64];
-  const int64_t row = blockIdx.x, b = row / p.rows_per_batch;
+__global__ __launch_bounds__(kWideThreads) void residual_norm_wide_kernel(ResidualNormParams p) {
+  __shared__ float lds[kWideThreads / 64];
+  const int64_t row = block_index();
+  if (row >= p.rows) return;
+  const int64_t b = p.gate || p.scale ? row / p.rows_per_batch : 0;
   const float* x = p.x + row * p.x_stride;
   const float* h = p.h + row * p.h_stride;
   float* out = p.out + row * p.out_stride;
   float* normed = p.normed + row * p.normed_stride;
   const float* gate = p.gate ? p.gate + b * p.gate_stride : nullptr;
-  const Stats post = row_stats(p.post.kind, p.post.eps, p.cols, lds, [&](int c) { return h[c]; });
-  for (int c = threadIdx.x; c < p.cols; c += kThreads) {
-    const float v = normed_value(p.post, post, h[c], c);
+  const Stats post = wide_stats(p.post.kind, p.post.eps, p.cols, lds, [&](int c) { return h[c]; });
+  for (int c = threadIdx.x; c < p.cols; c += kWideThreads) {
+    const float v = wide_value(p.post, post, h[c], c);
     out[c] = fmaf(p.residual_scale, x[c], gate ? gate[c] * v : v);
   }
   // (a thread reads back what it wrote itself)
-  const Stats pre = row_stats(p.pre.kind, p.pre.eps, p.cols, lds, [&](int c) { return out[c]; });
-  for (int c = threadIdx.x; c < p.cols; c += kThreads) {
-    float v = normed_value(p.pre, pre, out[c], c);
+  const Stats pre = wide_stats(p.pre.kind, p.pre.eps, p.cols, lds, [&](int c) { return out[c]; });
+  for (int c = threadIdx.x; c < p.cols; c += kWideThreads) {
+    float v = wide_value(p.pre, pre, out[c], c);
     if (p.scale) v = fmaf(v, 1.0f + p.scale[b * p.mod_stride + c], p.shift[b * p.mod_stride + c]);
     normed[c] = v;
+  }
+}
+
+dim3 grid_of(int64_t blocks) {
+  const int64_t x = std::min<int64_t>(blocks, 1 << 20);
+  return dim3((unsigned)x, (unsigned)((blocks + x - 1) / x));
+}
+
+template <int RW>
+void launch_rows(const ResidualNormParams& p, hipStream_t stream) {
+  const dim3 grid = grid_of(RW == 1 ? (p.rows + 3) / 4 : p.rows);
+  const int threads = RW == 1 ? 256 : RW * 64;
+  auto run = [&](auto v) {
+    residual_norm_kernel<RW, decltype(v)::value><<<grid, threads, 0, stream>>>(p);
+  };
+  const int chunks = (p.cols + 256 * RW - 1) / (256 * RW);
+  if constexpr (RW == 1) {  // (wider rows have three chunks at least)
+    if (chunks == 1) return run(std::integral_constant<int, 1>{});
+    if (chunks == 2) return run(std::integral_constant<int, 2>{});
+  }
+  switch (chunks) {
+    case 3: run(std::integral_constant<int, 3>{}); break;
+    case 4: run(std::integral_constant<int, 4>{}); break;
+    case 5: run(std::integral_constant<int, 5>{}); break;
+    case 6: run(std::integral_constant<int, 6>{}); break;
+    case 7: run(std::integral_constant<int, 7>{}); break;
+    default: run(std::integral_constant<int, 8>{}); break;
   }
 }
 
 }  // namespace
 
 int launch_residual_norm(const ResidualNormParams& p, hipStream_t stream) {
-  residual_norm_row_kernel<<<(unsigned)p.rows, kThreads, 0, stream>>>(p);
+  if (p.cols <= 256 * 8)
+    launch_rows<1>(p, stream);
+  else if (p.cols <= 4 * 256 * 8)
+    launch_rows<4>(p, stream);
+  else
+    residual_norm_wide_kernel<<<grid_of(p.rows), kWideThreads, 0, stream>>>(p);
   return hipGetLastError() == hipSuccess ? kOk : kErrLaunch;
 }
 
