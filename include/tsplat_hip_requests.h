@@ -43,7 +43,7 @@ int tsplat_low_rank_add_async(const float* y, int64_t y_stride, const float* x, 
 /* ---------------- norm, gate, residual, norm ---------------------------- */
 
 /* h' = post(h);  x' = residual_scale * x + gate[b] * h';  out = x';  normed = pre(x') * (1 + scale[b]) + shift[b],
- * over `rows` rows of `cols` fp32 values; b = row / rows_per_batch.
+ * over `rows` (below 2^31) rows of `cols` fp32 values; b = row / rows_per_batch.
  * norm kinds: 0 none (post only), 1 LayerNorm, 2 RMS norm (x / sqrt(mean(x^2) + eps)); each with its weight and
  * bias [cols], either null.  gate null: 1; scale and shift: both or neither; their rows mod_stride floats apart
  * (gate: gate_stride), 0 for one row that serves every b.  x, h, out, normed rows are x_stride ... floats apart.  out may be x, normed may be h (same
@@ -64,7 +64,7 @@ int tsplat_residual_norm_async(const float* x, int64_t x_stride, const float* h,
  * [H, D], become y * sqrt(D) / max(||y||, eps) * gamma.  Part 2 (v) is copied.  A pair is (2p, 2p + 1) with
  * interleaved, else (p, p + D/2).
  * positions: [position_batches][L][axes], position_batches 1 or B, int32 (position_type 0) or fp32 (1); an axis[p]
- * outside [0, axes) counts as 0.  axes 1..8; D even, 2..512.  The outputs must not overlap each other or an input
+ * outside [0, axes) counts as 0.  axes 1..8; D even, 2..512; H up to 2^16, B * L below 2^31.  The outputs must not overlap each other or an input
  * (-3). */
 int tsplat_rope_axes_async(const float* x, int64_t part_stride, int64_t batch_stride, int64_t token_stride,
                            int64_t head_stride, int parts, const float* gamma0, const float* gamma1,

@@ -104,7 +104,7 @@ def _rope(lib, x=P[0], ps=0, sb=0, sl=128, sh=64, parts=1, g0=None, g1=None, o0=
     (dict(x=None), -1), (dict(o0=None), -1), (dict(pos=None), -1), (dict(turns=None), -1), (dict(axis=None), -1),
     (dict(parts=2, ps=64), -1), (dict(parts=3, ps=64, o1=P[2]), -1),
     (dict(parts=0), -2), (dict(parts=4), -2), (dict(B=0), -2), (dict(L=0), -2), (dict(H=0), -2), (dict(D=63), -2),
-    (dict(D=514), -2), (dict(axes=0), -2), (dict(axes=9), -2), (dict(ptype=2), -2), (dict(eps=-1.0), -2),
+    (dict(D=514), -2), (dict(H=(1 << 16) + 1), -2), (dict(axes=0), -2), (dict(axes=9), -2), (dict(ptype=2), -2), (dict(eps=-1.0), -2),
     (dict(B=1 << 16, L=1 << 16, sb=64), -2),
     (dict(pb=2), -3), (dict(sh=63), -3), (dict(sl=-128), -3), (dict(sl=1 << 62), -3), (dict(B=2, sb=0), -3),
     (dict(o0=P[0]), -3), (dict(parts=2, ps=64, o1=P[1] + 4), -3),

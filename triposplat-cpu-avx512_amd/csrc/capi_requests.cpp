@@ -18,6 +18,7 @@ constexpr int kRequestsAbiVersion = 1;
 constexpr int kMaxRank = 512;
 constexpr int kMaxSlots = 1 << 20;
 constexpr int kMaxHeadDim = 512;
+constexpr int kMaxHeads = 1 << 16;
 constexpr int kMaxAxes = 8;
 
 int launched(int st) {
@@ -108,7 +109,6 @@ int tsplat_residual_norm_async(const float* x, int64_t x_stride, const float* h,
                                const float* pre_weight, const float* pre_bias, float pre_eps, const float* scale,
                                const float* shift, int64_t mod_stride, int64_t rows_per_batch, void* stream) {
   if (!x || !h || !out || !normed) return kErrNull;
-  // (one workgroup or wave a row: the launch's grid holds 2^31 - 1)
   if (rows <= 0 || rows > INT32_MAX || cols <= 0 || !(post_eps >= 0.0f) || !(pre_eps >= 0.0f)) return kErrDims;
   if (post_kind != kNormNone && post_kind != kNormLayer && post_kind != kNormRms) return kErrDims;
   if (pre_kind != kNormLayer && pre_kind != kNormRms) return kErrDims;
@@ -157,7 +157,8 @@ int tsplat_rope_axes_async(const float* x, int64_t part_stride, int64_t batch_st
                            int position_batches, int axes, const double* turns, const int32_t* axis,
                            int interleaved, float eps, int B, int L, int H, int D, int out_bhld, void* stream) {
   if (!x || !out0 || !positions || !turns || !axis) return kErrNull;
-  if (parts < 1 || parts > 3 || B <= 0 || L <= 0 || H <= 0 || D <= 0 || (D & 1) || D > kMaxHeadDim) return kErrDims;
+  if (parts < 1 || parts > 3 || B <= 0 || L <= 0 || H <= 0 || D <= 0 || (D & 1) || D > kMaxHeadDim || H > kMaxHeads)
+    return kErrDims;
   if ((parts > 1 && !out1) || (parts > 2 && !out2)) return kErrNull;
   if (axes < 1 || axes > kMaxAxes || (position_type != 0 && position_type != 1) || !(eps >= 0.0f)) return kErrDims;
   if (position_batches != 1 && position_batches != B) return kErrRange;

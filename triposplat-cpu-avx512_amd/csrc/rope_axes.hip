@@ -1,60 +1,138 @@
 // Rotary positions of several axes, the per-head RMS norm and the attention's layout in one pass:
 //   (a, b) of pair p -> (a cos t - b sin t, a sin t + b cos t),  t = 2 pi positions[axis[p]] turns[p],
-//   z = y sqrt(D) / max(||y||, eps) gamma[h].
+//   z = y sqrt(D) / max(||y||, eps) gamma[h]     (||y|| = ||x||: a rotation keeps it).
 // The angle is taken in revolutions and in 64 bits, where only its fraction counts: a far position keeps the
-// precision that its fp32 product with a frequency would lose.
+// precision that its fp32 product with a frequency would lose.  8 bytes a value from and to HBM, which bounds it.
+
+#include <algorithm>
+#include <type_traits>
 
 #include "tsplat_common.h"
 #include "tsplat_launch.h"
+#include "wave_sum.h"
 
 namespace tsplat {
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kMaxPairs = 256;
+typedef float floatx4u __attribute__((ext_vector_type(4), aligned(4)));  // vectors start at any float
 
-// One workgroup a token, one wave a head's vector.
-__global__ __launch_bounds__(kThreads) void rope_axes_token_kernel(RopeAxesParams p) {
-  __shared__ float cos_lds[kMaxPairs], sin_lds[kMaxPairs];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int64_t token = blockIdx.x;
-  const int64_t b = token / p.L, l = token % p.L;
-  const int pairs = p.D / 2;
-  for (int i = tid; i < pairs; i += kThreads) {
-    int axis = p.axis[i];
-    if (axis < 0 || axis >= p.axes) axis = 0;
-    const int64_t at = ((p.position_batches > 1 ? b : 0) * p.L + l) * p.axes + axis;
-    const double pos = p.position_type ? (double)static_cast<const float*>(p.positions)[at]
-                                       : (double)static_cast<const int32_t*>(p.positions)[at];
-    const double t = pos * p.turns[i];
-    float s, c;
-    sincospif(2.0f * (float)(t - rint(t)), &s, &c);
-    cos_lds[i] = c;
-    sin_lds[i] = s;
+constexpr int kWaves = 4;
+constexpr int kAhead = 4;  // vectors that a lane asks for at once
+
+// G lanes a vector, lane i of them its pairs 4 i .. 4 i + 3; a wave turns 64 / G tokens, whose sines and cosines stay
+// in registers while it goes through its share of the parts' heads.
+template <int G, bool INTERLEAVED>
+__global__ __launch_bounds__(kWaves * 64) void rope_axes_kernel(RopeAxesParams p, int shares) {
+  constexpr int kTokens = 64 / G;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i0 = (lane % G) * 4;
+  const int64_t tokens = (int64_t)p.B * p.L;
+  const int64_t token = ((int64_t)blockIdx.z * gridDim.x + blockIdx.x) * kTokens + lane / G;
+  const int share = blockIdx.y * kWaves + wave;
+  const int pairs = p.D / 2, vectors = p.parts * p.H;
+  const int n = token < tokens ? min(4, pairs - i0) : 0;  // pairs of this lane
+  const int64_t b = n > 0 ? token / p.L : 0, l = n > 0 ? token % p.L : 0;
+  float cs[4], sn[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    cs[e] = 1.0f;
+    sn[e] = 0.0f;
+    if (e < n) {
+      int axis = p.axis[i0 + e];
+      if (axis < 0 || axis >= p.axes) axis = 0;
+      const int64_t at = ((p.position_batches > 1 ? b : 0) * p.L + l) * p.axes + axis;
+      const double pos = p.position_type ? (double)static_cast<const float*>(p.positions)[at]
+                                         : (double)static_cast<const int32_t*>(p.positions)[at];
+      const double t = pos * p.turns[i0 + e];
+      sincospif(2.0f * (float)(t - rint(t)), &sn[e], &cs[e]);
+    }
   }
-  __syncthreads();
-  for (int v = wave; v < p.parts * p.H; v += kThreads / 64) {
-    const int part = v / p.H, h = v % p.H;
-    const float* src = p.x + part * p.part_stride + b * p.batch_stride + l * p.token_stride + h * p.head_stride;
-    float* dst = p.out[part] + (p.out_bhld ? (b * p.H + h) * p.L + l : (b * p.L + l) * p.H + h) * p.D;
-    if (part == 2) {
-      for (int d = lane; d < p.D; d += 64) dst[d] = src[d];
-      continue;
+  const float root = sqrtf((float)p.D);
+  // element offsets of the pairs' first and second values: 8 neighbours, or 4 of each half
+  const int j0 = INTERLEAVED ? 2 * i0 : i0, j1 = INTERLEAVED ? 2 * i0 + 4 : i0 + pairs;
+  const float* src = p.x + b * p.batch_stride + l * p.token_stride;
+  const bool whole = n == 4;
+  auto load = [&](const float* v, floatx4& lo, floatx4& hi) {
+    lo = hi = floatx4{};
+    if (whole) {
+      lo = *reinterpret_cast<const floatx4u*>(v + j0);
+      hi = *reinterpret_cast<const floatx4u*>(v + j1);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (INTERLEAVED) {
+          if (e < 2 * n) lo[e] = v[j0 + e];
+          if (e + 4 < 2 * n) hi[e] = v[j1 + e];
+        } else if (e < n) {
+          lo[e] = v[j0 + e];
+          hi[e] = v[j1 + e];
+        }
+      }
     }
-    const float* gamma = p.gamma[part] ? p.gamma[part] + h * p.D : nullptr;
-    float scale = 1.0f;
-    if (gamma) {
-      float q = 0.0f;
-      for (int d = lane; d < p.D; d += 64) q = fmaf(src[d], src[d], q);
-      for (int d = 32; d; d >>= 1) q += __shfl_xor(q, d);
-      scale = sqrtf((float)p.D) / fmaxf(sqrtf(q), p.eps);
+  };
+  auto store = [&](float* v, const floatx4& lo, const floatx4& hi) {
+    if (whole) {
+      *reinterpret_cast<floatx4u*>(v + j0) = lo;
+      *reinterpret_cast<floatx4u*>(v + j1) = hi;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (INTERLEAVED) {
+          if (e < 2 * n) v[j0 + e] = lo[e];
+          if (e + 4 < 2 * n) v[j1 + e] = hi[e];
+        } else if (e < n) {
+          v[j0 + e] = lo[e];
+          v[j1 + e] = hi[e];
+        }
+      }
     }
-    for (int i = lane; i < pairs; i += 64) {
-      const int j0 = p.interleaved ? 2 * i : i, j1 = p.interleaved ? 2 * i + 1 : i + pairs;
-      const float a0 = src[j0], a1 = src[j1], c = cos_lds[i], s = sin_lds[i];
-      const float y0 = a0 * c - a1 * s, y1 = a0 * s + a1 * c;
-      dst[j0] = gamma ? y0 * scale * gamma[j0] : y0;
-      dst[j1] = gamma ? y1 * scale * gamma[j1] : y1;
+  };
+  for (int first = share; first < vectors; first += shares * kAhead) {
+    floatx4 lo[kAhead], hi[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const int v = first + u * shares;
+      if (v < vectors) load(src + (v / p.H) * p.part_stride + (v % p.H) * p.head_stride, lo[u], hi[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const int v = first + u * shares;
+      if (v >= vectors) break;  // the same for the whole wave
+      const int part = v / p.H, h = v % p.H;
+      floatx4 a = lo[u], c = hi[u];
+      if (part < 2) {
+        const float* gamma = p.gamma[part];
+        float scale = 1.0f;
+        floatx4 g0, g1;
+        if (gamma) {
+          load(gamma + (int64_t)h * p.D, g0, g1);
+          float q = 0.0f;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) q = fmaf(a[e], a[e], fmaf(c[e], c[e], q));
+          scale = root / fmaxf(sqrtf(group_sum<G>(q)), p.eps);
+        }
+        floatx4 y0, y1;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (INTERLEAVED) {
+            const float re = e < 2 ? a[2 * e] : c[2 * e - 4], im = e < 2 ? a[2 * e + 1] : c[2 * e - 3];
+            const float t0 = re * cs[e] - im * sn[e], t1 = re * sn[e] + im * cs[e];
+            if (e < 2)
+              y0[2 * e] = t0, y0[2 * e + 1] = t1;
+            else
+              y1[2 * e - 4] = t0, y1[2 * e - 3] = t1;
+          } else {
+            y0[e] = a[e] * cs[e] - c[e] * sn[e];
+            y1[e] = a[e] * sn[e] + c[e] * cs[e];
+          }
+        }
+        if (gamma) {
+          y0 = y0 * scale * g0;
+          y1 = y1 * scale * g1;
+        }
+        a = y0;
+        c = y1;
+      }
+      if (n > 0) store(p.out[part] + (p.out_bhld ? (b * p.H + h) * p.L + l : (b * p.L + l) * p.H + h) * p.D, a, c);
     }
   }
 }
@@ -62,7 +140,34 @@ __global__ __launch_bounds__(kThreads) void rope_axes_token_kernel(RopeAxesParam
 }  // namespace
 
 int launch_rope_axes(const RopeAxesParams& p, hipStream_t stream) {
-  rope_axes_token_kernel<<<p.B * p.L, kThreads, 0, stream>>>(p);
+  const int lanes = (p.D / 2 + 3) / 4;
+  auto run = [&](auto g) {
+    constexpr int G = decltype(g)::value;
+    const int64_t tokens = (int64_t)p.B * p.L, groups = (tokens + 64 / G - 1) / (64 / G);
+    // A wave of many vectors computes its sines for all of them; few tokens need more waves to fill the chip.
+    const int vectors = p.parts * p.H;
+    const int blocks = (int)std::min<int64_t>((vectors + kWaves - 1) / kWaves, std::max<int64_t>(1, 2048 / groups));
+    const int64_t row = std::min<int64_t>(groups, 1 << 20);
+    const dim3 grid((unsigned)row, (unsigned)blocks, (unsigned)((groups + row - 1) / row));
+    if (p.interleaved)
+      rope_axes_kernel<G, true><<<grid, kWaves * 64, 0, stream>>>(p, blocks * kWaves);
+    else
+      rope_axes_kernel<G, false><<<grid, kWaves * 64, 0, stream>>>(p, blocks * kWaves);
+  };
+  if (lanes <= 1)
+    run(std::integral_constant<int, 1>{});
+  else if (lanes <= 2)
+    run(std::integral_constant<int, 2>{});
+  else if (lanes <= 4)
+    run(std::integral_constant<int, 4>{});
+  else if (lanes <= 8)
+    run(std::integral_constant<int, 8>{});
+  else if (lanes <= 16)
+    run(std::integral_constant<int, 16>{});
+  else if (lanes <= 32)
+    run(std::integral_constant<int, 32>{});
+  else
+    run(std::integral_constant<int, 64>{});
   return hipGetLastError() == hipSuccess ? kOk : kErrLaunch;
 }
 
