@@ -134,12 +134,19 @@ def library_path(path: str | os.PathLike | None = None) -> Path:
 
 def load_library(path: str | os.PathLike | None = None) -> ctypes.CDLL:
     """Open libtsplat_hip.so once per path and set every argtypes/restype."""
+    # the name as it is given, so that a loaded library is found again without touching the file system
+    given = os.environ.get("TSPLAT_HIP_LIBRARY", "") if path is None else path
+    lib = _CACHE.get(given) if isinstance(given, str) else None
+    if lib is not None:
+        return lib
     import torch  # noqa: F401  (binds the library to torch's HIP runtime)
 
     resolved = library_path(path)
     key = resolved.as_posix()
     lib = _CACHE.get(key)
     if lib is not None:
+        if isinstance(given, str) and (given == "" or os.path.isabs(given)):
+            _CACHE[given] = lib  # (a relative name means another file in another folder)
         return lib
     if not resolved.is_file():
         raise FileNotFoundError(
@@ -185,34 +192,35 @@ def current_stream_handle(device) -> int:
     return int(torch.cuda.current_stream(device).cuda_stream)
 
 
-# ---- shared by the wrappers of REQUEST_SIGNATURES
+# ---- shared by the wrappers of REQUEST_SIGNATURES.  Small calls are bound by the host, a microsecond for every few
+# attribute reads: these take each fact about a tensor once.
 def enqueue(lib, fn_name, device, *args) -> None:
     """Calls an asynchronous entry on torch's current stream of `device`; raises on a nonzero status."""
     import torch
 
     fn = getattr(lib, fn_name)
-    stream = int(torch.cuda.current_stream(device).cuda_stream)
+    stream = torch.cuda.current_stream(device).cuda_stream
     if torch.cuda.current_device() == device.index:
         status = fn(*args, stream)
     else:
         with torch.cuda.device(device):
             status = fn(*args, stream)
-    check_status(status, fn_name)
+    if status != 0:
+        check_status(status, fn_name)
 
 
 def no_gradients(*tensors) -> None:
     """These operators have no backward: a tensor that expects one is refused, not cut off in silence."""
     import torch
 
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise ValueError("this operator has no backward: call it under torch.no_grad(), or detach its inputs")
+    for t in tensors:
+        if t is not None and t.requires_grad and torch.is_grad_enabled():
+            raise ValueError("this operator has no backward: call it under torch.no_grad(), or detach its inputs")
 
 
-def rows_of(name, t, cols) -> tuple[int, int]:
+def rows_of(torch, name, t, cols) -> tuple[int, int]:
     """(rows, row stride) of a GPU fp32 tensor [..., cols] whose rows lie at one stride; ValueError otherwise."""
-    import torch
-
-    if not (torch.is_tensor(t) and t.device.type == "cuda" and t.dtype == torch.float32):
+    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype == torch.float32):
         raise ValueError(f"{name} must be an fp32 GPU tensor")
     shape = t.shape
     if len(shape) == 0 or shape[-1] != cols:

@@ -143,16 +143,25 @@ def add_inplace(x, h, library=None):
 NORM_KINDS = {None: 0, "layer": 1, "rms": 2}
 
 
-def _batch_rows(name, t, B, C, device):
-    """(pointer, row stride) of a per-batch [B, C] or shared [1, C] row of a modulation."""
-    import torch
-
-    if not (torch.is_tensor(t) and t.device == device and t.dtype == torch.float32 and t.dim() == 2
-            and t.shape[1] == C and t.shape[0] in (1, B) and (C == 1 or t.stride(1) == 1)):
-        raise ValueError(f"{name} must be [{B}, {C}] or [1, {C}], fp32 on {device} with unit column stride")
-    if t.shape[0] > 1 and t.stride(0) < C:
+def _batch_rows(torch, name, t, B, C, device):
+    """(pointer, row stride, rows) of a per-batch [B, C] or shared [1, C] row of a modulation."""
+    if not (isinstance(t, torch.Tensor) and t.get_device() == device and t.dtype == torch.float32 and t.dim() == 2):
+        raise ValueError(f"{name} must be [{B}, {C}] or [1, {C}], fp32 on the GPU of x")
+    (rows, cols), (step, unit) = t.shape, t.stride()
+    if cols != C or (rows != B and rows != 1) or (unit != 1 and C > 1):
+        raise ValueError(f"{name} must be [{B}, {C}] or [1, {C}] with unit column stride")
+    if rows == 1:
+        return t.data_ptr(), C, 1
+    if step < C:
         raise ValueError(f"the rows of {name} overlap")
-    return t.data_ptr(), int(t.stride(0)) if t.shape[0] > 1 else C
+    return t.data_ptr(), step, rows
+
+
+def _norm_vector(torch, name, t, C, device):
+    if not (isinstance(t, torch.Tensor) and t.get_device() == device and t.dtype == torch.float32
+            and t.dim() == 1 and t.shape[0] == C and t.is_contiguous()):
+        raise ValueError(f"{name} must be a contiguous [{C}] fp32 tensor on the GPU of x")
+    return t.data_ptr()
 
 
 def residual_norm(x, h, *, gate=None, residual_scale=1.0, post_norm=None, post_weight=None, post_bias=None,
@@ -170,53 +179,65 @@ def residual_norm(x, h, *, gate=None, residual_scale=1.0, post_norm=None, post_w
     normed may be h itself; they may not overlap the inputs otherwise.  No gradients."""
     import torch
 
-    if not torch.is_tensor(x) or x.dim() < 1:
-        raise ValueError("x must be an fp32 GPU tensor")
+    if not isinstance(x, torch.Tensor) or not isinstance(h, torch.Tensor):
+        raise ValueError("x and h must be fp32 GPU tensors")
     if norm not in ("layer", "rms") or post_norm not in NORM_KINDS:
         raise ValueError(f"norm is 'layer' or 'rms', post_norm one of them or None, not {norm!r}, {post_norm!r}")
-    C = int(x.shape[-1])
-    if C < 1 or not torch.is_tensor(h) or h.shape != x.shape:
+    shape = x.shape
+    if len(shape) == 0 or shape[-1] < 1 or h.shape != shape:
         raise ValueError("x and h must be [..., C] of one shape")
-    M, x_stride = rows_of("x", x, C)
-    _, h_stride = rows_of("h", h, C)
-    B = int(x.shape[0]) if x.dim() > 1 else 1
+    C, B = shape[-1], shape[0] if len(shape) > 1 else 1
+    M, x_stride = rows_of(torch, "x", x, C)
+    _, h_stride = rows_of(torch, "h", h, C)
     no_gradients(x, h, gate, post_weight, post_bias, weight, bias, scale, shift)
-    vectors = []
-    for name, t in (("post_weight", post_weight), ("post_bias", post_bias), ("weight", weight), ("bias", bias)):
-        if t is not None and not (torch.is_tensor(t) and t.device == x.device and t.dtype == torch.float32
-                                  and tuple(t.shape) == (C,) and t.is_contiguous()):
-            raise ValueError(f"{name} must be a contiguous [{C}] fp32 tensor on {x.device}")
-        vectors.append(None if t is None else t.data_ptr())
+    at = x.get_device()
     if post_norm is None and (post_weight is not None or post_bias is not None):
         raise ValueError("post_weight and post_bias belong to a post_norm")
+    pw, pb, w, b = (None if t is None else _norm_vector(torch, name, t, C, at) for name, t in
+                    (("post_weight", post_weight), ("post_bias", post_bias), ("weight", weight), ("bias", bias)))
     if (scale is None) != (shift is None):
         raise ValueError("scale and shift go together")
-    if not float(eps) >= 0.0 or not float(post_eps) >= 0.0:
+    if not eps >= 0.0 or not post_eps >= 0.0:
         raise ValueError("eps must not be negative")
-    gate_ptr, gate_stride = (None, 0) if gate is None else _batch_rows("gate", gate, B, C, x.device)
-    scale_ptr, mod_stride = (None, 0) if scale is None else _batch_rows("scale", scale, B, C, x.device)
-    shift_ptr, shift_stride = (None, 0) if shift is None else _batch_rows("shift", shift, B, C, x.device)
-    if scale is not None and (scale.shape[0] != shift.shape[0] or mod_stride != shift_stride):
-        raise ValueError("scale and shift must share the row stride")
-    groups = {int(t.shape[0]) for t in (gate, scale) if t is not None} or {1}
-    if len(groups) > 1:  # one is [1, C]: its row serves every batch entry
-        if gate.shape[0] == 1:
-            gate_stride = 0
-        else:
-            mod_stride = 0
-    out = torch.empty(x.shape, dtype=torch.float32, device=x.device) if out is None else out
-    normed = torch.empty(x.shape, dtype=torch.float32, device=x.device) if normed is None else normed
-    if out.shape != x.shape or normed.shape != x.shape or not x.device == h.device == out.device == normed.device:
-        raise ValueError("x, h, out and normed must be of one shape on one GPU")
-    _, out_stride = rows_of("out", out, C)
-    _, normed_stride = rows_of("normed", normed, C)
+    gate_ptr, gate_stride, scale_ptr, shift_ptr, mod_stride, groups = None, 0, None, None, 0, 1
+    if gate is not None:
+        gate_ptr, gate_stride, groups = _batch_rows(torch, "gate", gate, B, C, at)
+    if scale is not None:
+        scale_ptr, mod_stride, mods = _batch_rows(torch, "scale", scale, B, C, at)
+        shift_ptr, shift_stride, shifts = _batch_rows(torch, "shift", shift, B, C, at)
+        if mods != shifts or mod_stride != shift_stride:
+            raise ValueError("scale and shift must share the row stride")
+        if gate is not None and mods != groups:  # one is [1, C]: its row serves every batch entry
+            if groups == 1:
+                gate_stride = 0
+            else:
+                mod_stride = 0
+        groups = max(groups, mods)
+    out_stride = normed_stride = C
+    if out is None:
+        out = torch.empty(shape, dtype=torch.float32, device=x.device)
+    elif out is x:
+        out_stride = x_stride
+    else:
+        if out.shape != shape:
+            raise ValueError("out must have the shape of x")
+        _, out_stride = rows_of(torch, "out", out, C)
+    if normed is None:
+        normed = torch.empty(shape, dtype=torch.float32, device=x.device)
+    elif normed is h:
+        normed_stride = h_stride
+    else:
+        if normed.shape != shape:
+            raise ValueError("normed must have the shape of x")
+        _, normed_stride = rows_of(torch, "normed", normed, C)
+    if not at == h.get_device() == out.get_device() == normed.get_device():
+        raise ValueError("x, h, out and normed must be on one GPU")
     if M == 0:
         return out, normed
     enqueue(load_library(library), "tsplat_residual_norm_async", x.device, x.data_ptr(), x_stride, h.data_ptr(),
-            h_stride, out.data_ptr(), out_stride, normed.data_ptr(), normed_stride, M, C, float(residual_scale),
-            gate_ptr, gate_stride, NORM_KINDS[post_norm], vectors[0], vectors[1], float(post_eps),
-            NORM_KINDS[norm], vectors[2], vectors[3], float(eps), scale_ptr, shift_ptr, mod_stride,
-            M // max(groups))
+            h_stride, out.data_ptr(), out_stride, normed.data_ptr(), normed_stride, M, C, residual_scale, gate_ptr,
+            gate_stride, NORM_KINDS[post_norm], pw, pb, post_eps, NORM_KINDS[norm], w, b, eps, scale_ptr, shift_ptr,
+            mod_stride, M // groups)
     return out, normed
 
 

@@ -175,46 +175,45 @@ class RopeAxes:
         # revolutions per unit of position, in 64 bits: the kernel keeps the fraction of position * turns
         self.turns = torch.tensor([f / (2.0 * math.pi) for f in ramp], dtype=torch.float64, device=device)
         self.axis = torch.tensor(axis, dtype=torch.int32, device=device)
-        self.device = self.turns.device
-
-    @property
-    def axes(self):
-        return len(self.sections)
+        self.device, self.index, self.axes = self.turns.device, self.turns.get_device(), len(sections)
 
 
 def _rope_call(torch, x, strides, parts, gammas, positions, rope, eps, B, L, H, outs, out_bhld, library):
-    if not isinstance(rope, RopeAxes):
-        raise ValueError("rope must be a RopeAxes")
-    D = rope.dim
-    device = x.device
-    if (not torch.is_tensor(positions) or positions.dtype not in (torch.int32, torch.float32)
-            or not positions.is_contiguous() or positions.dim() not in (2, 3)
-            or tuple(positions.shape[-2:]) != (L, rope.axes) or (positions.dim() == 3 and positions.shape[0] not in (1, B))):
+    D, at = rope.dim, x.get_device()
+    shape = (B, H, L, D) if out_bhld else (B, L, H, D)
+    fresh = outs is None
+    if fresh:
+        outs = [torch.empty(shape, dtype=torch.float32, device=x.device) for _ in range(parts)]
+    if not isinstance(positions, torch.Tensor) or positions.get_device() != at or rope.index != at:
+        raise ValueError("x, positions and rope must be on one GPU")
+    fractional = positions.dtype == torch.float32
+    places = positions.shape
+    batches = places[0] if len(places) == 3 else 1
+    if (not (fractional or positions.dtype == torch.int32) or not positions.is_contiguous()
+            or not 2 <= len(places) <= 3 or places[-2] != L or places[-1] != rope.axes or batches not in (1, B)):
         raise ValueError(f"positions must be a contiguous [{L}, {rope.axes}] or [{B}, {L}, {rope.axes}] tensor of int32 "
                          "or fp32")
-    for g in gammas:
-        if g is not None and not (torch.is_tensor(g) and g.dtype == torch.float32 and tuple(g.shape) == (H, D)
-                                  and g.is_contiguous()):
-            raise ValueError(f"gamma must be a contiguous [{H}, {D}] fp32 tensor")
     no_gradients(x, positions, *gammas)
-    if not float(eps) >= 0.0:
+    ptr = [None, None]
+    for i, g in enumerate(gammas):
+        if g is not None:
+            if not (isinstance(g, torch.Tensor) and g.dtype == torch.float32 and g.shape == (H, D)
+                    and g.is_contiguous() and g.get_device() == at):
+                raise ValueError(f"gamma must be a contiguous [{H}, {D}] fp32 tensor on the GPU of x")
+            ptr[i] = g.data_ptr()
+    if not eps >= 0.0:
         raise ValueError("eps must not be negative")
-    shape = (B, H, L, D) if out_bhld else (B, L, H, D)
-    if outs is None:
-        outs = [torch.empty(shape, dtype=torch.float32, device=device) for _ in range(parts)]
-    for o in outs:
-        if not (torch.is_tensor(o) and o.dtype == torch.float32 and tuple(o.shape) == shape and o.is_contiguous()):
-            raise ValueError(f"out must be a contiguous {list(shape)} fp32 tensor")
-    if any(t is not None and t.device != device for t in (positions, *gammas, *outs)) or rope.device != device:
-        raise ValueError("x, positions, rope, gamma and out must be on one GPU")
+    if not fresh:
+        for o in outs:
+            if not (isinstance(o, torch.Tensor) and o.dtype == torch.float32 and o.shape == shape and o.is_contiguous()
+                    and o.get_device() == at):
+                raise ValueError(f"out must be a contiguous {list(shape)} fp32 tensor on the GPU of x")
     if B * L * H == 0:
         return outs
-    ptr = [None if g is None else g.data_ptr() for g in (*gammas, None)]
     dst = [o.data_ptr() for o in outs] + [None, None]
-    enqueue(load_library(library), "tsplat_rope_axes_async", device, x.data_ptr(), *strides, parts, ptr[0], ptr[1],
-            dst[0], dst[1], dst[2], positions.data_ptr(), int(positions.dtype == torch.float32),
-            1 if positions.dim() == 2 else int(positions.shape[0]), rope.axes, rope.turns.data_ptr(),
-            rope.axis.data_ptr(), int(rope.interleaved), float(eps), B, L, H, D, int(out_bhld))
+    enqueue(load_library(library), "tsplat_rope_axes_async", x.device, x.data_ptr(), *strides, parts, ptr[0], ptr[1],
+            dst[0], dst[1], dst[2], positions.data_ptr(), fractional, batches, rope.axes, rope.turns.data_ptr(),
+            rope.axis.data_ptr(), rope.interleaved, eps, B, L, H, D, out_bhld)
     return outs
 
 
@@ -227,17 +226,16 @@ def rope_axes(x, positions, rope, *, gamma=None, eps=1.0e-12, out=None, out_bhld
     keep their precision.  rope: RopeAxes.  out may not overlap x.  No gradients."""
     import torch
 
-    if not (torch.is_tensor(x) and x.device.type == "cuda" and x.dtype == torch.float32 and x.dim() == 4):
+    if not (isinstance(x, torch.Tensor) and x.is_cuda and x.dtype == torch.float32 and x.dim() == 4):
         raise ValueError("x must be a [B, L, H, D] fp32 GPU tensor")
-    B, L, H, D = (int(s) for s in x.shape)
+    B, L, H, D = x.shape
     if not isinstance(rope, RopeAxes) or D != rope.dim:
         raise ValueError(f"rope must be a RopeAxes of the heads' size {D}")
     sb, sl, sh, sd = x.stride()
     if sd != 1:
         raise ValueError("x must have unit stride within its vectors")
-    for size, step in ((B, sb), (L, sl), (H, sh)):
-        if size > 1 and step < D:
-            raise ValueError("the vectors of x overlap")
+    if (B > 1 and sb < D) or (L > 1 and sl < D) or (H > 1 and sh < D):
+        raise ValueError("the vectors of x overlap")
     return _rope_call(torch, x, (0, sb, sl, sh), 1, (gamma,), positions, rope, eps, B, L, H,
                       None if out is None else [out], out_bhld, library)[0]
 
@@ -252,7 +250,7 @@ def qkv_rope_axes(qkv, positions, rope, q_gamma, k_gamma, B, L, H, *, eps=1.0e-1
         raise ValueError("rope must be a RopeAxes")
     B, L, H = int(B), int(L), int(H)
     width = H * rope.dim
-    rows, stride = rows_of("qkv", qkv, 3 * width)
+    rows, stride = rows_of(torch, "qkv", qkv, 3 * width)
     if rows != B * L:
         raise ValueError(f"qkv has {rows} rows, not B * L = {B * L}")
     if outs is not None and len(outs) != 3:
