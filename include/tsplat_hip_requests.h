@@ -29,7 +29,8 @@ int tsplat_requests_abi_version(void);
  * piece, zero past K, N and each adapter's rank:
  *   down: [slots][ceil(R/16)][ceil(K/32)][4][16][8], value (r, k) at [r/16][k/32][k%32/8][r%16][k%8];
  *   up:   [slots][ceil(N/16)][ceil(R/32)][4][16][8], value (n, r) at [n/16][r/32][r%32/8][n%16][r%8];
- * R = max_rank, 1..512; rank[a] <= R (a larger one counts as R).  16-byte aligned (-4).  M up to 2^28, K and N up
+ * fp32: [slots][..][..][3][4][16][8] bf16, three planes whose sum is the value: its upper 16 bits, those of what is
+ * left, and those of what is left then.  R = max_rank, 1..512; rank[a] <= R (a larger one counts as R).  16-byte aligned (-4).  M up to 2^28, K and N up
  * to 2^20, slots up to 2^20 (-2).  A row of x that holds an infinity or NaN gives NaN.
  * scratch: at least tsplat_low_rank_scratch_bytes(...) of device memory that no other work uses until the call's
  * kernels are done (-5 when too small), 16-byte aligned. */

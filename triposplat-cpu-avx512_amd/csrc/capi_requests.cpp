@@ -82,7 +82,7 @@ int tsplat_low_rank_add_async(const float* y, int64_t y_stride, const float* x, 
     return kErrAlign;
   const int64_t need = low_rank_scratch_bytes(M, K, N, slots, max_rank, dtype);
   if (need > 0 && (scratch == nullptr || scratch_bytes < need)) return kErrWorkspace;
-  const int64_t size = dtype == kAdapterF32 ? 4 : 2;
+  const int64_t size = dtype == kAdapterF32 ? 6 : 2;  // (fp32: three bf16 planes)
   const int64_t k_pad = ((int64_t)K + 31) / 32 * 32, n_pad = ((int64_t)N + 15) / 16 * 16;
   const int64_t down_values = ((int64_t)max_rank + 15) / 16 * 16 * k_pad;
   const int64_t up_values = ((int64_t)max_rank + 31) / 32 * 32 * n_pad;

@@ -84,19 +84,17 @@ struct Weights<kAdapterF16> {
 };
 
 template <>
-struct Weights<kAdapterF32> {
-  static constexpr int kTerms = 3, kBytes = 4;
-  floatx4 raw[2];
+struct Weights<kAdapterF32> {  // three planes of the tile, split when the bank was laid out
+  static constexpr int kTerms = 3, kBytes = 6;
+  bf16x8 raw[3];
   __device__ __forceinline__ void load(const char* p) {
-    raw[0] = reinterpret_cast<const floatx4*>(p)[0];
-    raw[1] = reinterpret_cast<const floatx4*>(p)[1];
-  }
-  __device__ __forceinline__ void clear() { raw[0] = raw[1] = floatx4{}; }
-  __device__ __forceinline__ void terms(bf16x8* t) const {
-    float v[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = raw[i >> 2][i & 3];
-    split<3>(v, t);
+    for (int i = 0; i < 3; ++i) raw[i] = *reinterpret_cast<const bf16x8*>(p + i * 1024);
+  }
+  __device__ __forceinline__ void clear() { raw[0] = raw[1] = raw[2] = bf16x8{}; }
+  __device__ __forceinline__ void terms(bf16x8* t) const {
+#pragma unroll
+    for (int i = 0; i < 3; ++i) t[i] = raw[i];
   }
 };
 
@@ -121,85 +119,99 @@ __device__ __forceinline__ floatx4 mfma16(const bf16x8& w, const bf16x8& v, floa
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, v, c, 0, 0, 0);
 }
 
-// The adapter of row m and its rank; id -1 for none.
-__device__ __forceinline__ int row_adapter(const LowRankParams& p, int64_t m, bool live) {
-  int id = live && m < p.M ? p.rows[m] : -1;
-  if (id < 0 || id >= p.slots) return -1;
-  return p.rank[id] > 0 ? id : -1;
-}
+// Scratch: what the first kernel finds out about each row, its adapter and that one's rank in one number (-1: none),
+// then its inner values [splits][M][ceil(R/16) 16].  With that the second kernel's loads hang on one load, not three,
+// each of which takes microseconds while memory is saturated.
+__host__ __device__ constexpr int64_t meta_floats(int M) { return ((int64_t)M + 63) / 64 * 64; }
+constexpr int kIdBits = 20;
+static_assert((1 << (31 - kIdBits)) > 512, "a rank of 512 has room above the adapter's number");
 
-// Goes through the distinct adapters of a tile of at most 64 rows (lane l holds row l's): f(adapter, mask of its
-// rows).  With several passes (gridDim.z), every workgroup takes its share of them.
+// Goes through the distinct adapters of a tile of at most 64 rows: lane l holds row l's number, negative for none;
+// f(number, its first row, mask of its rows).  Of several passes, this workgroup's share of them.
 template <typename F>
-__device__ __forceinline__ void each_adapter(int id, F f) {
-  uint64_t left = __ballot(id >= 0);
+__device__ __forceinline__ void each_adapter(int number, uint64_t rows, int passes, F f) {
+  uint64_t left = __ballot(number >= 0) & rows;
   int pass = 0;
   while (left != 0) {
-    const int a = __builtin_amdgcn_readlane(id, __ffsll((unsigned long long)left) - 1);
-    const uint64_t mask = __ballot(id == a);
+    const int first = __ffsll((unsigned long long)left) - 1;
+    const int a = __builtin_amdgcn_readlane(number, first);
+    const uint64_t mask = __ballot(number == a) & rows;
     left &= ~mask;
-    if (pass % (int)gridDim.z == (int)blockIdx.z) f(a, mask);
+    if (passes == 1 || pass % passes == (int)blockIdx.z) f(a, first, mask);
     ++pass;
   }
 }
 
 // ------------------------------------------------------------------ t = scale x down^T
-// A workgroup: RT * 16 rows x up to RB * 16 ranks; its W waves share the K axis in steps of 32 (neighbouring waves at
-// neighbouring steps) and add their sums in LDS.  x goes from HBM to the registers that feed the matrix cores, each
-// value read once by a wave; an adapter's tile of 16 ranks by 32 values is one contiguous load.
+// A workgroup: RT * 16 rows x up to RB * 16 ranks; its W waves share the K axis in runs of 32-value steps and add their
+// sums in LDS.  x goes from HBM to the registers that feed the matrix cores, a step ahead, each value read once by one
+// wave; an adapter's tile of 16 ranks by 32 values is one contiguous load, a step ahead too.  (Two or four steps of x
+// ahead are 5-40 % slower: the loads of all waves fill memory's queues as it is.)
 template <int DTYPE, int RT, int RB, int W>
-__global__ __launch_bounds__(W * 64) void low_rank_down_kernel(LowRankParams p, int rank_blocks, int splits) {
+__global__ __launch_bounds__(W * 64) void low_rank_down_kernel(LowRankParams p, int rank_blocks, int splits,
+                                                               int passes) {
   using Wt = Weights<DTYPE>;
-  __shared__ floatx4 sums[W][W][64];
+  constexpr int kRound = RT * RB < W ? RT * RB : W;  // tiles added up at once
+  __shared__ floatx4 sums[kRound][W][64];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, q = lane >> 4;
   const int64_t row0 = (int64_t)blockIdx.x * (RT * 16);
   const int rb0 = (int)(blockIdx.y % rank_blocks) * RB, part = (int)(blockIdx.y / rank_blocks);
   const int k_tiles = ceil_div(p.K, 32), r_tiles = ceil_div(p.R, 16), t_stride = r_tiles * 16;
-  const int per_part = ceil_div(k_tiles, splits);
-  const int s_end = min(k_tiles, (part + 1) * per_part);
-  const int id = row_adapter(p, row0 + lane, lane < RT * 16);
+  const int share = ceil_div(k_tiles, splits * W);
+  const int s_begin = (part * W + wave) * share, s_end = min(k_tiles, s_begin + share);
   const float* xrow[RT];
 #pragma unroll
   for (int t = 0; t < RT; ++t) {
     const int64_t m = row0 + t * 16 + (lane & 15);
     xrow[t] = p.x + (m < p.M ? m : p.M - 1) * p.x_stride + q * 8;
   }
-  each_adapter(id, [&](int a, uint64_t mask) {
-    const int tiles = min(RB, ceil_div(min(p.rank[a], p.R), 16) - rb0);
-    if (tiles <= 0) return;  // the same for the whole workgroup
-    const char* down = static_cast<const char*>(p.down) +
-                       (((int64_t)a * r_tiles + rb0) * k_tiles * 512 + lane * 8) * Wt::kBytes;
-    const int64_t tile_bytes = (int64_t)k_tiles * 512 * Wt::kBytes;
-    floatx4 acc[RT][RB] = {};
-    float raw[RT][8];
-    auto load_x = [&](int s) {
-      const int k = s * 32;
-      if (k + 32 <= p.K) {
+  float raw[RT][8];
+  auto load_x = [&](int s) {
+    const int k = s * 32;
+    if (k + 32 <= p.K) {
 #pragma unroll
-        for (int t = 0; t < RT; ++t) {
-          const floatx4u lo = *reinterpret_cast<const floatx4u*>(xrow[t] + k);
-          const floatx4u hi = *reinterpret_cast<const floatx4u*>(xrow[t] + k + 4);
+      for (int t = 0; t < RT; ++t) {
+        const floatx4u lo = *reinterpret_cast<const floatx4u*>(xrow[t] + k);
+        const floatx4u hi = *reinterpret_cast<const floatx4u*>(xrow[t] + k + 4);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) raw[t][i] = lo[i], raw[t][4 + i] = hi[i];
-        }
-      } else {  // the last step of a K that is no multiple of 32
-#pragma unroll
-        for (int t = 0; t < RT; ++t)
-#pragma unroll
-          for (int i = 0; i < 8; ++i) raw[t][i] = k + q * 8 + i < p.K ? xrow[t][k + i] : 0.0f;
+        for (int i = 0; i < 4; ++i) raw[t][i] = lo[i], raw[t][4 + i] = hi[i];
       }
-    };
-    int s = part * per_part + wave;
-    if (s < s_end) load_x(s);
-    for (; s < s_end; s += W) {
-      Wt w[RB];
+    } else {  // the last step of a K that is no multiple of 32
 #pragma unroll
-      for (int j = 0; j < RB; ++j)
-        if (j < tiles) w[j].load(down + j * tile_bytes + (int64_t)s * 512 * Wt::kBytes);
+      for (int t = 0; t < RT; ++t)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) raw[t][i] = k + q * 8 + i < p.K ? xrow[t][k + i] : 0.0f;
+    }
+  };
+  // x is on its way before its rows' adapters are known; passes after the first may have none
+  bool held = blockIdx.z == 0;
+  if (held && s_begin < s_end) load_x(s_begin);
+  int id = lane < RT * 16 && row0 + lane < p.M ? p.rows[row0 + lane] : -1;
+  if (id >= p.slots) id = -1;
+  const int row_rank = id >= 0 ? min(p.rank[id], p.R) : 0;
+  each_adapter(id, ~0ull, passes, [&](int a, int first_row, uint64_t mask) {
+    const char* down = static_cast<const char*>(p.down) +
+                       ((int64_t)a * r_tiles + rb0) * k_tiles * 512 * Wt::kBytes + lane * 16;
+    const int64_t tile_bytes = (int64_t)k_tiles * 512 * Wt::kBytes;
+    const float scale = p.scale[a];
+    int tiles = min(RB, r_tiles - rb0);  // (of the bank: the first loads do not wait for the adapter's own rank)
+    Wt w[RB];
+    auto load_w = [&](int j, int s) {
+      if (j < tiles && s < s_end) w[j].load(down + j * tile_bytes + (int64_t)s * 512 * Wt::kBytes);
+    };
+#pragma unroll
+    for (int j = 0; j < RB; ++j) load_w(j, s_begin);
+    const int rank = __builtin_amdgcn_readlane(row_rank, first_row);
+    tiles = rank > 0 ? min(RB, ceil_div(rank, 16) - rb0) : 0;
+    if (tiles <= 0) return;  // the same for the whole workgroup
+    if (!held && s_begin < s_end) load_x(s_begin);
+    held = false;
+    floatx4 acc[RT][RB] = {};
+    for (int s = s_begin; s < s_end; ++s) {
       bf16x8 xs[RT][3];
 #pragma unroll
       for (int t = 0; t < RT; ++t) split<3>(raw[t], xs[t]);
-      if (s + W < s_end) load_x(s + W);
+      if (s + 1 < s_end) load_x(s + 1);
 #pragma unroll
       for (int j = 0; j < RB; ++j) {
         if (j >= tiles) break;
@@ -210,20 +222,20 @@ __global__ __launch_bounds__(W * 64) void low_rank_down_kernel(LowRankParams p, 
 #pragma unroll
           for (int t = 0; t < RT; ++t)
             acc[t][j] = mfma16(ws[weight_term<Wt::kTerms>(i)], xs[t][value_term<Wt::kTerms>(i)], acc[t][j]);
+        load_w(j, s + 1);
       }
     }
     // the waves' sums, W tiles at a time: wave w adds up tile w
-    const float scale = p.scale[a];
-    float* out = p.scratch + (int64_t)part * p.M * t_stride;
+    float* out = p.scratch + meta_floats(p.M) + (int64_t)part * p.M * t_stride;
 #pragma unroll
-    for (int first = 0; first < RT * RB; first += W) {
+    for (int at = 0; at < RT * RB; at += kRound) {
       __syncthreads();
 #pragma unroll
-      for (int i = 0; i < W; ++i)
-        if (first + i < RT * RB) sums[i][wave][lane] = acc[(first + i) % RT][(first + i) / RT];
+      for (int i = 0; i < kRound; ++i)
+        if (at + i < RT * RB) sums[i][wave][lane] = acc[(at + i) % RT][(at + i) / RT];
       __syncthreads();
-      const int mine = first + wave, t = mine % RT, j = mine / RT;
-      if (mine < RT * RB && j < tiles && (mask >> (t * 16 + (lane & 15)) & 1)) {
+      const int mine = at + wave, t = mine % RT, j = mine / RT;
+      if (wave < kRound && mine < RT * RB && j < tiles && (mask >> (t * 16 + (lane & 15)) & 1)) {
         floatx4 sum = sums[wave][0][lane];
 #pragma unroll
         for (int i = 1; i < W; ++i) sum += sums[wave][i][lane];
@@ -232,118 +244,142 @@ __global__ __launch_bounds__(W * 64) void low_rank_down_kernel(LowRankParams p, 
       }
     }
   });
+  if (blockIdx.y == 0 && blockIdx.z == 0 && wave == 0 && lane < RT * 16 && row0 + lane < p.M)
+    reinterpret_cast<int*>(p.scratch)[row0 + lane] = row_rank > 0 ? row_rank << kIdBits | id : -1;
 }
 
 // ------------------------------------------------------------------ out = y + t up^T
-// A wave: RT * 16 rows x NT * 16 columns; its y is asked for before the products and joined after them.  A lane holds
-// four neighbouring columns of a row.
-template <int DTYPE, int RT, int NT, int W>
-__global__ __launch_bounds__(W * 64) void low_rank_up_kernel(LowRankParams p, int splits) {
+// A wave: 16 rows x NT * 16 columns.  Its y, its rows' numbers and inner values are asked for at once, then the
+// weights, 32 ranks at a time.  A lane holds four neighbouring columns of a row.  Workgroups follow one another along the
+// rows, as the values lie in memory: that order alone is worth 15 % of the bandwidth.
+template <int DTYPE, int NT, int W>
+__global__ __launch_bounds__(W * 64) void low_rank_up_kernel(LowRankParams p, int splits, int passes) {
   using Wt = Weights<DTYPE>;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, q = lane >> 4;
-  const int64_t row0 = (int64_t)blockIdx.x * (RT * 16);
-  const int tile0 = (int)(blockIdx.y * W + wave) * NT;
+  const int64_t row0 = (blockIdx.y + (passes == 1 ? (int64_t)blockIdx.z * gridDim.y : 0)) * 16;
+  const int tile0 = (int)(blockIdx.x * W + wave) * NT;
   const int n_tiles = ceil_div(p.N, 16), r_steps = ceil_div(p.R, 32), t_stride = ceil_div(p.R, 16) * 16;
-  if (tile0 >= n_tiles) return;
-  const int tiles = min(NT, n_tiles - tile0), n0 = tile0 * 16 + q * 4;
-  const int id = row_adapter(p, row0 + lane, lane < RT * 16);
-  auto load_y = [&](int t, int j) {
-    const float* src = p.y + (row0 + t * 16 + (lane & 15)) * p.y_stride;
-    const int n = n0 + j * 16;
-    if (n + 4 <= p.N) return (floatx4)*reinterpret_cast<const floatx4u*>(src + n);
-    floatx4 v = {};
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (n + i < p.N) v[i] = src[n + i];
-    return v;
-  };
-  auto store = [&](int t, int j, floatx4 v) {
-    float* dst = p.out + (row0 + t * 16 + (lane & 15)) * p.out_stride;
-    const int n = n0 + j * 16;
-    if (n + 4 <= p.N) {
-      *reinterpret_cast<floatx4u*>(dst + n) = v;
-      return;
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (n + i < p.N) dst[n + i] = v[i];
-  };
-  each_adapter(id, [&](int a, uint64_t mask) {
-    const int rank = min(p.rank[a], p.R), t_rank = ceil_div(rank, 16) * 16;
-    floatx4 yv[RT][NT];
-#pragma unroll
-    for (int t = 0; t < RT; ++t)
-      if (mask >> (t * 16 + (lane & 15)) & 1) {
-#pragma unroll
-        for (int j = 0; j < NT; ++j)
-          if (j < tiles) yv[t][j] = load_y(t, j);
-      }
-    floatx4 acc[RT][NT] = {};
-    const char* up = static_cast<const char*>(p.up) +
-                     (((int64_t)a * n_tiles + tile0) * r_steps * 512 + lane * 8) * Wt::kBytes;
-    for (int s = 0; s * 32 < rank; ++s) {
-      const int k = s * 32 + q * 8;
-      Wt w[NT];
+  if (tile0 >= n_tiles || row0 >= p.M) return;
+  const int64_t m = row0 + (lane & 15);
+  const bool there = m < p.M;
+  const float* yrow = p.y + m * p.y_stride + tile0 * 16 + q * 4;
+  float* orow = p.out + m * p.out_stride + tile0 * 16 + q * 4;
+  const float* trow = p.scratch + meta_floats(p.M) + m * t_stride + q * 8;
+  const int left = p.N - tile0 * 16 - q * 4;  // columns from this lane's first
+  auto run = [&](auto whole) {
+    constexpr bool kWhole = decltype(whole)::value;  // all NT tiles have all their columns
+    floatx4 yv[NT];
+    auto load_y = [&] {
 #pragma unroll
       for (int j = 0; j < NT; ++j) {
-        w[j].clear();
-        if (j < tiles && k < rank) w[j].load(up + ((int64_t)j * r_steps + s) * 512 * Wt::kBytes);
-      }
-      bf16x8 ts[RT][3];
+        if (kWhole || left >= j * 16 + 4) {
+          yv[j] = *reinterpret_cast<const floatx4u*>(yrow + j * 16);
+        } else {
 #pragma unroll
-      for (int t = 0; t < RT; ++t) {
-        float v[8] = {};
-        if (k < t_rank && (mask >> (t * 16 + (lane & 15)) & 1)) {
-          const float* src = p.scratch + (row0 + t * 16 + (lane & 15)) * t_stride + k;
-          for (int i = 0; i < splits; ++i, src += (int64_t)p.M * t_stride)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] += src[e];
+          for (int i = 0; i < 4; ++i)
+            if (left > j * 16 + i) yv[j][i] = yrow[j * 16 + i];
         }
-        split<3>(v, ts[t]);
       }
+    };
+    auto store = [&](const floatx4 (&v)[NT]) {
 #pragma unroll
       for (int j = 0; j < NT; ++j) {
-        bf16x8 ws[Wt::kTerms];
-        w[j].terms(ws);
+        if (kWhole || left >= j * 16 + 4) {
+          *reinterpret_cast<floatx4u*>(orow + j * 16) = v[j];
+        } else {
 #pragma unroll
-        for (int i = 0; i < kProducts<Wt::kTerms>; ++i)
-#pragma unroll
-          for (int t = 0; t < RT; ++t)
-            acc[t][j] = mfma16(ws[weight_term<Wt::kTerms>(i)], ts[t][value_term<Wt::kTerms>(i)], acc[t][j]);
+          for (int i = 0; i < 4; ++i)
+            if (left > j * 16 + i) orow[j * 16 + i] = v[j][i];
+        }
       }
-    }
+    };
+    float inner[8];  // past the adapter's rank: whatever scratch holds
+    auto load_inner = [&](int k) {
+      if (k + q * 8 >= t_stride) return;
+      const float* src = trow + k;
 #pragma unroll
-    for (int t = 0; t < RT; ++t)
-      if (mask >> (t * 16 + (lane & 15)) & 1) {
+      for (int e = 0; e < 8; ++e) inner[e] = src[e];
+      for (int i = 1; i < splits; ++i) {
+        src += (int64_t)p.M * t_stride;
 #pragma unroll
-        for (int j = 0; j < NT; ++j)
-          if (j < tiles) store(t, j, yv[t][j] + acc[t][j]);
+        for (int e = 0; e < 8; ++e) inner[e] += src[e];
       }
-  });
-  if (p.out == p.y || blockIdx.z != 0) return;
-  const uint64_t bare = __ballot(id < 0);  // rows without an adapter
-#pragma unroll
-  for (int t = 0; t < RT; ++t)
-    if ((bare >> (t * 16 + (lane & 15)) & 1) && row0 + t * 16 + (lane & 15) < p.M) {
-#pragma unroll
-      for (int j = 0; j < NT; ++j)
-        if (j < tiles) store(t, j, load_y(t, j));
+    };
+    int meta = -1;
+    if (there) {
+      meta = reinterpret_cast<const int*>(p.scratch)[m];
+      load_inner(0);
+      if (passes == 1) load_y();
     }
+    bool held = true;
+    each_adapter(meta, 0xffff, passes, [&](int number, int, uint64_t) {
+      const int a = number & ((1 << kIdBits) - 1), rank = number >> kIdBits;
+      const char* up = static_cast<const char*>(p.up) +
+                       ((int64_t)a * n_tiles + tile0) * r_steps * 512 * Wt::kBytes + lane * 16;
+      const bool mine = meta == number;
+      const int t_rank = mine ? ceil_div(rank, 16) * 16 : 0;
+      floatx4 acc[NT] = {};
+      for (int k = 0; k < rank; k += 32, up += 512 * Wt::kBytes) {
+        Wt w[NT];
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          w[j].clear();
+          if (k + q * 8 < rank && (kWhole || tile0 + j < n_tiles)) w[j].load(up + (int64_t)j * r_steps * 512 * Wt::kBytes);
+        }
+        if (!held && there) load_inner(k);
+        held = r_steps == 1;
+        if (k == 0 && passes != 1 && mine) load_y();
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = k + q * 8 < t_rank ? inner[e] : 0.0f;
+        bf16x8 ts[3];
+        split<3>(v, ts);
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          bf16x8 ws[Wt::kTerms];
+          w[j].terms(ws);
+#pragma unroll
+          for (int i = 0; i < kProducts<Wt::kTerms>; ++i)
+            acc[j] = mfma16(ws[weight_term<Wt::kTerms>(i)], ts[value_term<Wt::kTerms>(i)], acc[j]);
+        }
+      }
+      if (mine) {
+#pragma unroll
+        for (int j = 0; j < NT; ++j) acc[j] += yv[j];
+        store(acc);
+      }
+    });
+    if (p.out == p.y || (passes != 1 && blockIdx.z != 0)) return;
+    if (there && meta < 0) {  // rows without an adapter
+      if (passes != 1) load_y();
+      store(yv);
+    }
+  };
+  if ((tile0 + NT) * 16 <= p.N)
+    run(std::true_type{});
+  else
+    run(std::false_type{});
 }
 
-// Rows a workgroup of the first kernel, the parts that it splits K into and the workgroups that share a row tile's
-// adapters.  Few rows leave the chip idle without the last two.
+// Rows a workgroup of the first kernel, the parts that it splits K into, and the workgroups that share a tile's
+// adapters.  Few rows leave the chip idle without the last two: 64 rows of an adapter each, K 1024 -> N 6144, rank 32,
+// take 68 + 17 us with one workgroup a tile, 6.8 + 8.1 with 16 and 8.  Many rows: a second workgroup for the tiles at
+// the border of two requests, which would otherwise end last (12294 x 1024, rank 16: 20 -> 15 us); 32 rows a
+// workgroup, but 64 where an adapter's values are read often enough to count (16384 x 4096, rank 64: 91 against 75 us;
+// rank 16, K 1024: 18 against 20).
 struct Plan {
-  int row_tiles, splits, passes;
+  int row_tiles, splits, down_passes, up_tiles, up_passes;
 };
-constexpr int kDownWaves = 8;
+constexpr int kDownWaves = 8, kUpWaves = 4;
 
-Plan plan_of(int M, int K, int slots) {
-  Plan pl{M > 8192 ? 4 : M > 4096 ? 2 : 1, 1, 1};
-  const int wgs = ceil_div(M, 16 * pl.row_tiles);
-  if (pl.row_tiles == 1) {
-    pl.splits = std::max(1, std::min({256 / wgs, ceil_div(K, 32) / (2 * kDownWaves), 8}));
-    pl.passes = std::max(1, std::min({1024 / wgs, 16, M, slots}));
+Plan plan_of(int M, int K, int N, int slots, int R) {
+  Plan pl{M > 8192 && R > 32 ? 4 : M > 4096 ? 2 : 1, 1, std::min({2, M, slots}), 8, 1};
+  if (M <= 4096) {
+    const int tiles = ceil_div(M, 16), most = std::min({16, M, slots});
+    pl.splits = std::max(1, std::min({256 / tiles, ceil_div(K, 32) / (2 * kDownWaves), 8}));
+    pl.down_passes = std::max(1, std::min(1024 / tiles, most));
+    pl.up_tiles = 4;
+    pl.up_passes = std::max(1, std::min(1024 / (tiles * ceil_div(N, 16 * kUpWaves * pl.up_tiles)), most));
   }
   return pl;
 }
@@ -355,14 +391,22 @@ void launch_down(const LowRankParams& p, const Plan& pl, hipStream_t stream) {
     constexpr int RB = decltype(rb)::value;
     const int blocks = ceil_div(tiles, RB);
     low_rank_down_kernel<DTYPE, RT, RB, kDownWaves>
-        <<<dim3(m_blocks, blocks * pl.splits, pl.passes), kDownWaves * 64, 0, stream>>>(p, blocks, pl.splits);
+        <<<dim3(m_blocks, blocks * pl.splits, pl.down_passes), kDownWaves * 64, 0, stream>>>(p, blocks, pl.splits,
+                                                                                            pl.down_passes);
   };
-  if (tiles == 1)
-    run(std::integral_constant<int, 1>{});
-  else if (tiles == 2)
-    run(std::integral_constant<int, 2>{});
-  else
-    run(std::integral_constant<int, 4>{});
+  if constexpr (RT < 4) {
+    if (tiles == 1) return run(std::integral_constant<int, 1>{});
+    if (tiles == 2) return run(std::integral_constant<int, 2>{});
+  }
+  run(std::integral_constant<int, 4>{});
+}
+
+template <int DTYPE, int NT>
+void launch_up(const LowRankParams& p, const Plan& pl, hipStream_t stream) {
+  const int row_blocks = ceil_div(p.M, 16), rows = std::min(row_blocks, 65535);
+  const dim3 grid(ceil_div(p.N, 16 * NT * kUpWaves), rows,
+                  pl.up_passes > 1 ? pl.up_passes : ceil_div(row_blocks, rows));
+  low_rank_up_kernel<DTYPE, NT, kUpWaves><<<grid, kUpWaves * 64, 0, stream>>>(p, pl.splits, pl.up_passes);
 }
 
 template <int DTYPE>
@@ -372,25 +416,20 @@ void launch_typed(const LowRankParams& p, const Plan& pl, hipStream_t stream) {
     case 2: launch_down<DTYPE, 2>(p, pl, stream); break;
     default: launch_down<DTYPE, 4>(p, pl, stream); break;
   }
-  constexpr int W = 4;
-  const int n_tiles = ceil_div(p.N, 16);
-  if (pl.row_tiles == 1) {
-    low_rank_up_kernel<DTYPE, 1, 1, W>
-        <<<dim3(ceil_div(p.M, 16), ceil_div(n_tiles, W), pl.passes), W * 64, 0, stream>>>(p, pl.splits);
-  } else {
-    low_rank_up_kernel<DTYPE, 2, 4, W>
-        <<<dim3(ceil_div(p.M, 32), ceil_div(n_tiles, 4 * W), 1), W * 64, 0, stream>>>(p, pl.splits);
-  }
+  if (pl.up_tiles == 4)
+    launch_up<DTYPE, 4>(p, pl, stream);
+  else
+    launch_up<DTYPE, 8>(p, pl, stream);
 }
 
 }  // namespace
 
-int64_t low_rank_scratch_bytes(int M, int K, int, int slots, int R, int) {
-  return (int64_t)plan_of(M, K, slots).splits * M * ceil_div(R, 16) * 64;
+int64_t low_rank_scratch_bytes(int M, int K, int N, int slots, int R, int) {
+  return 4 * (meta_floats(M) + (int64_t)plan_of(M, K, N, slots, R).splits * M * ceil_div(R, 16) * 16);
 }
 
 int launch_low_rank_add(const LowRankParams& p, hipStream_t stream) {
-  const Plan pl = plan_of(p.M, p.K, p.slots);
+  const Plan pl = plan_of(p.M, p.K, p.N, p.slots, p.R);
   switch (p.dtype) {
     case kAdapterF32: launch_typed<kAdapterF32>(p, pl, stream); break;
     case kAdapterBf16: launch_typed<kAdapterBf16>(p, pl, stream); break;

@@ -23,7 +23,8 @@ def _types(torch):
 
 def _tiled(torch, values, tile):
     """values [S, rows, cols] -> [S, ceil(rows/16), ceil(cols/32), 4, 16, 8], the tiles that the kernels read, zero
-    past rows and cols; written to `tile`, or a new tensor."""
+    past rows and cols; fp32 as three bf16 planes of each tile, [.., 3, 4, 16, 8], whose sum is the value bit for bit
+    (8 bits each, by truncation).  Written to `tile`, or a new tensor."""
     S, rows, cols = (int(s) for s in values.shape)
     r16, c32 = -(-rows // 16), -(-cols // 32)
     if (rows, cols) != (16 * r16, 32 * c32):
@@ -31,13 +32,23 @@ def _tiled(torch, values, tile):
         padded[:, :rows, :cols] = values
         values = padded
     tiles = values.reshape(S, r16, 16, c32, 4, 8).permute(0, 1, 3, 4, 2, 5)
-    return tiles.contiguous() if tile is None else tile.copy_(tiles)
+    if values.dtype != torch.float32:
+        return tiles.contiguous() if tile is None else tile.copy_(tiles)
+    if tile is None:
+        tile = torch.empty((S, r16, c32, 3, 4, 16, 8), dtype=torch.bfloat16, device=values.device)
+    left = tiles
+    for i in range(3):
+        upper = (left.view(torch.int32) & -65536).view(torch.float32)
+        tile[:, :, :, i] = upper
+        left = left - upper
+    return tile
 
 
 class AdapterBank:
     """Adapters of one Linear [in_features -> out_features] in `slots` slots of at most max_rank.
 
-    The bank holds its own copies, in `dtype` (fp32, bf16 or fp16; values of another type are rounded to it).
+    The bank holds its own copies, in `dtype` (fp32, bf16 or fp16; values of another type are rounded to it; fp32 takes
+    6 bytes a value: the three bf16 terms that the matrix cores multiply).
     load and unload run on torch's current stream: calls that use the bank on another stream have to be ordered
     after them, and before them when they still read the slot."""
 
@@ -52,8 +63,9 @@ class AdapterBank:
         if min(self.slots, self.in_features, self.out_features) < 1 or not 1 <= self.max_rank <= MAX_RANK:
             raise ValueError(f"an AdapterBank needs slots, features and a max_rank of 1..{MAX_RANK}")
         k32, n16 = -(-self.in_features // 32), -(-self.out_features // 16)
-        self.down = torch.zeros((self.slots, -(-self.max_rank // 16), k32, 4, 16, 8), dtype=dtype, device=device)
-        self.up = torch.zeros((self.slots, n16, -(-self.max_rank // 32), 4, 16, 8), dtype=dtype, device=device)
+        tile, held = ((3, 4, 16, 8), torch.bfloat16) if dtype == torch.float32 else ((4, 16, 8), dtype)
+        self.down = torch.zeros((self.slots, -(-self.max_rank // 16), k32, *tile), dtype=held, device=device)
+        self.up = torch.zeros((self.slots, n16, -(-self.max_rank // 32), *tile), dtype=held, device=device)
         self.scale = torch.zeros(self.slots, dtype=torch.float32, device=device)
         self.rank = torch.zeros(self.slots, dtype=torch.int32, device=device)  # 0: nothing loaded
         self.device, self.type_id = self.down.device, _types(torch)[dtype]
