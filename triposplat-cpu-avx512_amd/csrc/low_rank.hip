@@ -361,6 +361,125 @@ __global__ __launch_bounds__(W * 64) void low_rank_up_kernel(LowRankParams p, in
     run(std::false_type{});
 }
 
+// ------------------------------------------------------------------ few rows: both products in one launch
+// A workgroup: 16 rows x W NT * 16 columns, ranks up to 32.  Its waves share the K axis for the inner values of every
+// row, add their sums in LDS, and each multiplies them with its own columns' weights.  Every column block computes the
+// inner values anew, which costs less than a second launch and the wait between the two while that is little work:
+// 2 rows, 1024 -> 1024, rank 16: 5.0 us against 7.0, and 4 us less of the host; see few_rows() for where it turns.
+template <int DTYPE, int NT, int W>
+__global__ __launch_bounds__(W * 64) void low_rank_few_kernel(LowRankParams p, int passes) {
+  using Wt = Weights<DTYPE>;
+  constexpr int kInner = 32 + 4;  // floats a row in LDS: 16-byte reads of neighbouring rows in other banks
+  __shared__ floatx4 sums[2][W][64];
+  __shared__ __attribute__((aligned(16))) float inner[16 * kInner];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, q = lane >> 4;
+  const int64_t row0 = (int64_t)blockIdx.y * 16, m = row0 + (lane & 15);
+  const int k_tiles = ceil_div(p.K, 32), r_tiles = ceil_div(p.R, 16);
+  const int n_tiles = ceil_div(p.N, 16), tile0 = (int)(blockIdx.x * W + wave) * NT;
+  const int share = ceil_div(k_tiles, W), s_begin = wave * share, s_end = min(k_tiles, s_begin + share);
+  const float* xrow = p.x + (m < p.M ? m : p.M - 1) * p.x_stride + q * 8;
+  const int n0 = tile0 * 16 + q * 4;
+  int id = m < p.M ? p.rows[m] : -1;
+  if (id >= p.slots) id = -1;
+  const int row_rank = id >= 0 ? min(p.rank[id], p.R) : 0;
+  floatx4 yv[NT];
+  auto load_y = [&] {
+    const float* src = p.y + m * p.y_stride;
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (n0 + j * 16 + i < p.N) yv[j][i] = src[n0 + j * 16 + i];
+  };
+  auto store = [&](const floatx4 (&v)[NT]) {
+    float* dst = p.out + m * p.out_stride;
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (n0 + j * 16 + i < p.N) dst[n0 + j * 16 + i] = v[j][i];
+  };
+  each_adapter(id, 0xffff, passes, [&](int a, int first_row, uint64_t mask) {
+    const int rank = __builtin_amdgcn_readlane(row_rank, first_row);
+    if (rank <= 0) return;  // the same for the whole workgroup
+    const bool mine = mask >> (lane & 15) & 1;
+    const float scale = p.scale[a];
+    if (mine) load_y();
+    floatx4 acc[NT] = {};
+    const int tiles = ceil_div(rank, 16);
+    const char* down = static_cast<const char*>(p.down) + (int64_t)a * r_tiles * k_tiles * 512 * Wt::kBytes + lane * 16;
+    const char* up = static_cast<const char*>(p.up) + ((int64_t)a * n_tiles + tile0) * 512 * Wt::kBytes + lane * 16;
+    Wt wu[NT];  // the second product's weights come while the first runs
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      wu[j].clear();
+      if (tile0 + j < n_tiles && q * 8 < rank) wu[j].load(up + j * 512 * Wt::kBytes);
+    }
+    floatx4 t[2] = {};
+    for (int s = s_begin; s < s_end; ++s) {
+      const int k = s * 32;
+      Wt w[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+        if (j < tiles) w[j].load(down + ((int64_t)j * k_tiles + s) * 512 * Wt::kBytes);
+      float v[8];
+      if (k + 32 <= p.K) {
+        const floatx4u lo = *reinterpret_cast<const floatx4u*>(xrow + k);
+        const floatx4u hi = *reinterpret_cast<const floatx4u*>(xrow + k + 4);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = lo[i], v[4 + i] = hi[i];
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = k + q * 8 + i < p.K ? xrow[k + i] : 0.0f;
+      }
+      bf16x8 xs[3];
+      split<3>(v, xs);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        if (j >= tiles) break;
+        bf16x8 ws[Wt::kTerms];
+        w[j].terms(ws);
+#pragma unroll
+        for (int i = 0; i < kProducts<Wt::kTerms>; ++i)
+          t[j] = mfma16(ws[weight_term<Wt::kTerms>(i)], xs[value_term<Wt::kTerms>(i)], t[j]);
+      }
+    }
+    sums[0][wave][lane] = t[0];
+    sums[1][wave][lane] = t[1];
+    __syncthreads();  // (this one also keeps an adapter's inner values from the next's until all have read them)
+    if (wave < 2) {
+      floatx4 sum = sums[wave][0][lane];
+#pragma unroll
+      for (int i = 1; i < W; ++i) sum += sums[wave][i][lane];
+      *reinterpret_cast<floatx4*>(&inner[(lane & 15) * kInner + wave * 16 + q * 4]) =
+          wave < tiles ? sum * scale : floatx4{};
+    }
+    __syncthreads();
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = inner[(lane & 15) * kInner + q * 8 + i];
+    bf16x8 ts[3];
+    split<3>(v, ts);
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      bf16x8 ws[Wt::kTerms];
+      wu[j].terms(ws);
+#pragma unroll
+      for (int i = 0; i < kProducts<Wt::kTerms>; ++i)
+        acc[j] = mfma16(ws[weight_term<Wt::kTerms>(i)], ts[value_term<Wt::kTerms>(i)], acc[j]);
+    }
+    if (mine) {
+#pragma unroll
+      for (int j = 0; j < NT; ++j) acc[j] += yv[j];
+      store(acc);
+    }
+  });
+  if (p.out != p.y && blockIdx.z == 0 && m < p.M && row_rank <= 0) {  // rows without an adapter
+    load_y();
+    store(yv);
+  }
+}
+
 // Rows a workgroup of the first kernel, the parts that it splits K into, and the workgroups that share a tile's
 // adapters.  Few rows leave the chip idle without the last two: 64 rows of an adapter each, K 1024 -> N 6144, rank 32,
 // take 68 + 17 us with one workgroup a tile, 6.8 + 8.1 with 16 and 8.  Many rows: a second workgroup for the tiles at
@@ -370,6 +489,14 @@ __global__ __launch_bounds__(W * 64) void low_rank_up_kernel(LowRankParams p, in
 struct Plan {
   int row_tiles, splits, down_passes, up_tiles, up_passes;
 };
+
+// Whether both products go in one launch: where a column block's own sums are little work, and not many of them.  16
+// rows of 16 adapters, 1024 -> 1024, rank 16: 7.1 us against 9.4; 64 rows of 64: 8.5 against 9.3; but 64 rows of 64,
+// 1024 -> 6144, rank 32: 32 against 15, and 2 rows, 4096 -> 1024, rank 64: 37 against 13.
+bool few_rows(int M, int K, int N, int R) {
+  return R <= 32 && K <= 2048 && (M <= 16 || (M <= 64 && N <= 2048));
+}
+constexpr int kFewTiles = 2, kFewWaves = 8;
 constexpr int kDownWaves = 8, kUpWaves = 4;
 
 Plan plan_of(int M, int K, int N, int slots, int R) {
@@ -410,7 +537,15 @@ void launch_up(const LowRankParams& p, const Plan& pl, hipStream_t stream) {
 }
 
 template <int DTYPE>
-void launch_typed(const LowRankParams& p, const Plan& pl, hipStream_t stream) {
+void launch_typed(const LowRankParams& p, hipStream_t stream) {
+  if (few_rows(p.M, p.K, p.N, p.R)) {
+    const int passes = std::min({16, p.M, p.slots});
+    low_rank_few_kernel<DTYPE, kFewTiles, kFewWaves>
+        <<<dim3(ceil_div(p.N, 16 * kFewTiles * kFewWaves), ceil_div(p.M, 16), passes), kFewWaves * 64, 0, stream>>>(
+            p, passes);
+    return;
+  }
+  const Plan pl = plan_of(p.M, p.K, p.N, p.slots, p.R);
   switch (pl.row_tiles) {
     case 1: launch_down<DTYPE, 1>(p, pl, stream); break;
     case 2: launch_down<DTYPE, 2>(p, pl, stream); break;
@@ -425,15 +560,15 @@ void launch_typed(const LowRankParams& p, const Plan& pl, hipStream_t stream) {
 }  // namespace
 
 int64_t low_rank_scratch_bytes(int M, int K, int N, int slots, int R, int) {
+  if (few_rows(M, K, N, R)) return 0;
   return 4 * (meta_floats(M) + (int64_t)plan_of(M, K, N, slots, R).splits * M * ceil_div(R, 16) * 16);
 }
 
 int launch_low_rank_add(const LowRankParams& p, hipStream_t stream) {
-  const Plan pl = plan_of(p.M, p.K, p.N, p.slots, p.R);
   switch (p.dtype) {
-    case kAdapterF32: launch_typed<kAdapterF32>(p, pl, stream); break;
-    case kAdapterBf16: launch_typed<kAdapterBf16>(p, pl, stream); break;
-    default: launch_typed<kAdapterF16>(p, pl, stream); break;
+    case kAdapterF32: launch_typed<kAdapterF32>(p, stream); break;
+    case kAdapterBf16: launch_typed<kAdapterBf16>(p, stream); break;
+    default: launch_typed<kAdapterF16>(p, stream); break;
   }
   return hipGetLastError() == hipSuccess ? kOk : kErrLaunch;
 }

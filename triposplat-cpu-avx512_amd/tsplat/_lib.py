@@ -194,28 +194,39 @@ def current_stream_handle(device) -> int:
 
 # ---- shared by the wrappers of REQUEST_SIGNATURES.  Small calls are bound by the host, a microsecond for every few
 # attribute reads: these take each fact about a tensor once.
-def enqueue(lib, fn_name, device, *args) -> None:
-    """Calls an asynchronous entry on torch's current stream of `device`; raises on a nonzero status."""
+_RAW_STREAM = None
+
+
+def _raw_stream(index: int) -> int:
+    """hipStream_t of torch's current stream on device `index`, without building a torch.cuda.Stream (1.8 us)."""
+    global _RAW_STREAM
+    if _RAW_STREAM is None:
+        import torch
+
+        _RAW_STREAM = getattr(torch._C, "_cuda_getCurrentRawStream", None) or current_stream_handle
+    return _RAW_STREAM(index)
+
+
+def enqueue(lib, fn_name, index, *args) -> None:
+    """Calls an asynchronous entry on torch's current stream of device `index`; raises on a nonzero status."""
     import torch
 
-    fn = getattr(lib, fn_name)
-    stream = torch.cuda.current_stream(device).cuda_stream
-    if torch.cuda.current_device() == device.index:
-        status = fn(*args, stream)
+    stream = _raw_stream(index)
+    if torch.cuda.current_device() == index:
+        status = getattr(lib, fn_name)(*args, stream)
     else:
-        with torch.cuda.device(device):
-            status = fn(*args, stream)
+        with torch.cuda.device(index):
+            status = getattr(lib, fn_name)(*args, stream)
     if status != 0:
         check_status(status, fn_name)
 
 
-def no_gradients(*tensors) -> None:
+def no_gradients(torch, *tensors) -> None:
     """These operators have no backward: a tensor that expects one is refused, not cut off in silence."""
-    import torch
-
-    for t in tensors:
-        if t is not None and t.requires_grad and torch.is_grad_enabled():
-            raise ValueError("this operator has no backward: call it under torch.no_grad(), or detach its inputs")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise ValueError("this operator has no backward: call it under torch.no_grad(), or detach its inputs")
 
 
 def rows_of(torch, name, t, cols) -> tuple[int, int]:

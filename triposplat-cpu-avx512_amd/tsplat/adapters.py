@@ -68,7 +68,7 @@ class AdapterBank:
         self.up = torch.zeros((self.slots, n16, -(-self.max_rank // 32), *tile), dtype=held, device=device)
         self.scale = torch.zeros(self.slots, dtype=torch.float32, device=device)
         self.rank = torch.zeros(self.slots, dtype=torch.int32, device=device)  # 0: nothing loaded
-        self.device, self.type_id = self.down.device, _types(torch)[dtype]
+        self.device, self.index, self.type_id = self.down.device, self.down.get_device(), _types(torch)[dtype]
 
     def _slot(self, slot):
         if not 0 <= int(slot) < self.slots:
@@ -124,7 +124,8 @@ class AdapterBank:
         if down.dtype not in _types(torch) or S < 1 or K < 1 or int(up.shape[1]) < 1 or not 1 <= R <= MAX_RANK:
             raise ValueError(f"an AdapterBank holds fp32, bf16 or fp16 adapters of rank 1..{MAX_RANK}")
         bank.slots, bank.in_features, bank.out_features, bank.max_rank = S, K, int(up.shape[1]), R
-        bank.dtype, bank.device, bank.type_id = down.dtype, down.device, _types(torch)[down.dtype]
+        bank.dtype, bank.device, bank.index = down.dtype, down.device, down.get_device()
+        bank.type_id = _types(torch)[down.dtype]
         with torch.no_grad():
             bank.rank = torch.tensor(ranks, dtype=torch.int32, device=down.device)
             bank.scale = scale.clone()
@@ -162,30 +163,30 @@ def low_rank_add(y, x, bank, rows, *, out=None, library=None):
         raise ValueError("low_rank_add needs an AdapterBank")
     M, y_stride = rows_of(torch, "y", y, bank.out_features)
     Mx, x_stride = rows_of(torch, "x", x, bank.in_features)
-    no_gradients(y, x)
+    no_gradients(torch, y, x)
     if Mx != M:
         raise ValueError(f"y has {M} rows, x has {Mx}")
     if not (isinstance(rows, torch.Tensor) and rows.dtype == torch.int32 and rows.numel() == M
             and rows.is_contiguous()):
         raise ValueError(f"rows must be a contiguous int32 tensor of {M} slots")
-    device = y.device
+    at = y.get_device()
     if out is None:
-        out, out_stride = torch.empty(y.shape, dtype=torch.float32, device=device), bank.out_features
+        out, out_stride = torch.empty_like(y, memory_format=torch.contiguous_format), bank.out_features
     elif out is y:
         out_stride = y_stride
     else:
         Mo, out_stride = rows_of(torch, "out", out, bank.out_features)
         if Mo != M:
             raise ValueError(f"out has {Mo} rows, y has {M}")
-    if not (bank.device == device and y.get_device() == x.get_device() == rows.get_device() == out.get_device()):
+    if not at == x.get_device() == rows.get_device() == out.get_device() == bank.index:
         raise ValueError("y, x, rows, out and the bank must be on one GPU")
     if M == 0:
         return out
     lib = load_library(library)
     sizes = (M, bank.in_features, bank.out_features, bank.slots, bank.max_rank, bank.type_id)
     need = lib.tsplat_low_rank_scratch_bytes(*sizes)
-    scratch = torch.empty(need, dtype=torch.uint8, device=device) if need else None
-    enqueue(lib, "tsplat_low_rank_add_async", device, y.data_ptr(), y_stride, x.data_ptr(), x_stride,
-            rows.data_ptr(), bank.down.data_ptr(), bank.up.data_ptr(), bank.scale.data_ptr(), bank.rank.data_ptr(),
-            out.data_ptr(), out_stride, *sizes, scratch.data_ptr() if need else None, need)
+    scratch = torch.empty(need, dtype=torch.uint8, device=y.device) if need else None
+    enqueue(lib, "tsplat_low_rank_add_async", at, y.data_ptr(), y_stride, x.data_ptr(), x_stride, rows.data_ptr(),
+            bank.down.data_ptr(), bank.up.data_ptr(), bank.scale.data_ptr(), bank.rank.data_ptr(), out.data_ptr(),
+            out_stride, *sizes, scratch.data_ptr() if need else None, need)
     return out

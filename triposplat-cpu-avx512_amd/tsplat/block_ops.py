@@ -145,9 +145,12 @@ NORM_KINDS = {None: 0, "layer": 1, "rms": 2}
 
 def _batch_rows(torch, name, t, B, C, device):
     """(pointer, row stride, rows) of a per-batch [B, C] or shared [1, C] row of a modulation."""
-    if not (isinstance(t, torch.Tensor) and t.get_device() == device and t.dtype == torch.float32 and t.dim() == 2):
-        raise ValueError(f"{name} must be [{B}, {C}] or [1, {C}], fp32 on the GPU of x")
-    (rows, cols), (step, unit) = t.shape, t.stride()
+    if not (isinstance(t, torch.Tensor) and t.get_device() == device and t.dtype == torch.float32):
+        raise ValueError(f"{name} must be an fp32 tensor on the GPU of x")
+    shape = t.shape
+    if len(shape) != 2:
+        raise ValueError(f"{name} must be [{B}, {C}] or [1, {C}]")
+    (rows, cols), (step, unit) = shape, t.stride()
     if cols != C or (rows != B and rows != 1) or (unit != 1 and C > 1):
         raise ValueError(f"{name} must be [{B}, {C}] or [1, {C}] with unit column stride")
     if rows == 1:
@@ -189,12 +192,14 @@ def residual_norm(x, h, *, gate=None, residual_scale=1.0, post_norm=None, post_w
     C, B = shape[-1], shape[0] if len(shape) > 1 else 1
     M, x_stride = rows_of(torch, "x", x, C)
     _, h_stride = rows_of(torch, "h", h, C)
-    no_gradients(x, h, gate, post_weight, post_bias, weight, bias, scale, shift)
+    no_gradients(torch, x, h, gate, post_weight, post_bias, weight, bias, scale, shift)
     at = x.get_device()
     if post_norm is None and (post_weight is not None or post_bias is not None):
         raise ValueError("post_weight and post_bias belong to a post_norm")
-    pw, pb, w, b = (None if t is None else _norm_vector(torch, name, t, C, at) for name, t in
-                    (("post_weight", post_weight), ("post_bias", post_bias), ("weight", weight), ("bias", bias)))
+    pw = None if post_weight is None else _norm_vector(torch, "post_weight", post_weight, C, at)
+    pb = None if post_bias is None else _norm_vector(torch, "post_bias", post_bias, C, at)
+    w = None if weight is None else _norm_vector(torch, "weight", weight, C, at)
+    b = None if bias is None else _norm_vector(torch, "bias", bias, C, at)
     if (scale is None) != (shift is None):
         raise ValueError("scale and shift go together")
     if not eps >= 0.0 or not post_eps >= 0.0:
@@ -215,7 +220,7 @@ def residual_norm(x, h, *, gate=None, residual_scale=1.0, post_norm=None, post_w
         groups = max(groups, mods)
     out_stride = normed_stride = C
     if out is None:
-        out = torch.empty(shape, dtype=torch.float32, device=x.device)
+        out = torch.empty_like(x, memory_format=torch.contiguous_format)
     elif out is x:
         out_stride = x_stride
     else:
@@ -223,7 +228,7 @@ def residual_norm(x, h, *, gate=None, residual_scale=1.0, post_norm=None, post_w
             raise ValueError("out must have the shape of x")
         _, out_stride = rows_of(torch, "out", out, C)
     if normed is None:
-        normed = torch.empty(shape, dtype=torch.float32, device=x.device)
+        normed = torch.empty_like(x, memory_format=torch.contiguous_format)
     elif normed is h:
         normed_stride = h_stride
     else:
@@ -234,7 +239,7 @@ def residual_norm(x, h, *, gate=None, residual_scale=1.0, post_norm=None, post_w
         raise ValueError("x, h, out and normed must be on one GPU")
     if M == 0:
         return out, normed
-    enqueue(load_library(library), "tsplat_residual_norm_async", x.device, x.data_ptr(), x_stride, h.data_ptr(),
+    enqueue(load_library(library), "tsplat_residual_norm_async", at, x.data_ptr(), x_stride, h.data_ptr(),
             h_stride, out.data_ptr(), out_stride, normed.data_ptr(), normed_stride, M, C, residual_scale, gate_ptr,
             gate_stride, NORM_KINDS[post_norm], pw, pb, post_eps, NORM_KINDS[norm], w, b, eps, scale_ptr, shift_ptr,
             mod_stride, M // groups)

@@ -193,7 +193,7 @@ def _rope_call(torch, x, strides, parts, gammas, positions, rope, eps, B, L, H, 
             or not 2 <= len(places) <= 3 or places[-2] != L or places[-1] != rope.axes or batches not in (1, B)):
         raise ValueError(f"positions must be a contiguous [{L}, {rope.axes}] or [{B}, {L}, {rope.axes}] tensor of int32 "
                          "or fp32")
-    no_gradients(x, positions, *gammas)
+    no_gradients(torch, x, positions, *gammas)
     ptr = [None, None]
     for i, g in enumerate(gammas):
         if g is not None:
@@ -211,7 +211,7 @@ def _rope_call(torch, x, strides, parts, gammas, positions, rope, eps, B, L, H, 
     if B * L * H == 0:
         return outs
     dst = [o.data_ptr() for o in outs] + [None, None]
-    enqueue(load_library(library), "tsplat_rope_axes_async", x.device, x.data_ptr(), *strides, parts, ptr[0], ptr[1],
+    enqueue(load_library(library), "tsplat_rope_axes_async", at, x.data_ptr(), *strides, parts, ptr[0], ptr[1],
             dst[0], dst[1], dst[2], positions.data_ptr(), fractional, batches, rope.axes, rope.turns.data_ptr(),
             rope.axis.data_ptr(), rope.interleaved, eps, B, L, H, D, out_bhld)
     return outs
