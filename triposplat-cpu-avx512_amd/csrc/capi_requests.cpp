@@ -163,7 +163,7 @@ int tsplat_rope_axes_async(const float* x, int64_t part_stride, int64_t batch_st
   if (axes < 1 || axes > kMaxAxes || (position_type != 0 && position_type != 1) || !(eps >= 0.0f)) return kErrDims;
   if (position_batches != 1 && position_batches != B) return kErrRange;
   const int64_t tokens = (int64_t)B * L;
-  if (tokens > INT32_MAX) return kErrDims;
+  if (tokens > INT32_MAX) return kErrDims;  // (the launch's grid holds 2^32 groups of a token at least)
   const int64_t steps[4][2] = {{parts, part_stride}, {B, batch_stride}, {L, token_stride}, {H, head_stride}};
   __int128 last = D;
   for (const auto& s : steps) {

@@ -16,35 +16,47 @@ namespace {
 
 typedef float floatx4u __attribute__((ext_vector_type(4), aligned(4)));  // vectors start at any float
 
-constexpr int kWaves = 4;
-constexpr int kAhead = 4;  // vectors that a lane asks for at once
+// A workgroup: kTokenWaves waves along the tokens, each with kVectorWaves shares of their parts' heads.  16384 tokens x
+// 16 x 64, q, k and v: 87 us; one token wave with 4 shares 94-110 (writes of 2 KiB a head instead of 8), workgroups in
+// the order of the tokens 90 and more.
+constexpr int kTokenWaves = 4, kVectorWaves = 4, kThreads = kTokenWaves * kVectorWaves * 64;
+constexpr int kAhead = 2;  // vectors that a lane asks for at once (4: 107 us, 1: 87)
 
-// G lanes a vector, lane i of them its pairs 4 i .. 4 i + 3; a wave turns 64 / G tokens, whose sines and cosines stay
-// in registers while it goes through its share of the parts' heads.
+// G lanes a vector, lane i of them its pairs 4 i .. 4 i + 3; a wave turns 64 / G tokens.  The workgroup computes its
+// tokens' sines and cosines once, into LDS, and a lane keeps its own while it goes through its share of the vectors.
 template <int G, bool INTERLEAVED>
-__global__ __launch_bounds__(kWaves * 64) void rope_axes_kernel(RopeAxesParams p, int shares) {
-  constexpr int kTokens = 64 / G;
+__global__ __launch_bounds__(kThreads) void rope_axes_kernel(RopeAxesParams p) {
+  constexpr int kTokens = 64 / G, kAllTokens = kTokens * kTokenWaves;
+  __shared__ float2 circle[kAllTokens * G * 4];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i0 = (lane % G) * 4;
   const int64_t tokens = (int64_t)p.B * p.L;
-  const int64_t token = ((int64_t)blockIdx.z * gridDim.x + blockIdx.x) * kTokens + lane / G;
-  const int share = blockIdx.y * kWaves + wave;
+  const int64_t token0 = ((int64_t)blockIdx.z * gridDim.y + blockIdx.y) * kAllTokens;
+  const int64_t token = token0 + wave / kVectorWaves * kTokens + lane / G;
+  const int share = blockIdx.x * kVectorWaves + wave % kVectorWaves, shares = gridDim.x * kVectorWaves;
   const int pairs = p.D / 2, vectors = p.parts * p.H;
+  for (int i = threadIdx.x; i < kAllTokens * pairs; i += kThreads) {
+    const int t = i / pairs, pair = i % pairs;
+    if (token0 + t >= tokens) break;
+    const int64_t l = (token0 + t) % p.L, b = (token0 + t) / p.L;
+    int axis = p.axis[pair];
+    if (axis < 0 || axis >= p.axes) axis = 0;
+    const int64_t at = ((p.position_batches > 1 ? b : 0) * p.L + l) * p.axes + axis;
+    const double pos = p.position_type ? (double)static_cast<const float*>(p.positions)[at]
+                                       : (double)static_cast<const int32_t*>(p.positions)[at];
+    const double turn = pos * p.turns[pair];
+    float2 v;
+    sincospif(2.0f * (float)(turn - rint(turn)), &v.y, &v.x);
+    circle[t * G * 4 + pair] = v;
+  }
+  __syncthreads();
   const int n = token < tokens ? min(4, pairs - i0) : 0;  // pairs of this lane
   const int64_t b = n > 0 ? token / p.L : 0, l = n > 0 ? token % p.L : 0;
   float cs[4], sn[4];
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
-    cs[e] = 1.0f;
-    sn[e] = 0.0f;
-    if (e < n) {
-      int axis = p.axis[i0 + e];
-      if (axis < 0 || axis >= p.axes) axis = 0;
-      const int64_t at = ((p.position_batches > 1 ? b : 0) * p.L + l) * p.axes + axis;
-      const double pos = p.position_type ? (double)static_cast<const float*>(p.positions)[at]
-                                         : (double)static_cast<const int32_t*>(p.positions)[at];
-      const double t = pos * p.turns[i0 + e];
-      sincospif(2.0f * (float)(t - rint(t)), &sn[e], &cs[e]);
-    }
+    const float2 v = e < n ? circle[(int)(token - token0) * G * 4 + i0 + e] : make_float2(1.0f, 0.0f);
+    cs[e] = v.x;
+    sn[e] = v.y;
   }
   const float root = sqrtf((float)p.D);
   // element offsets of the pairs' first and second values: 8 neighbours, or 4 of each half
@@ -143,16 +155,18 @@ int launch_rope_axes(const RopeAxesParams& p, hipStream_t stream) {
   const int lanes = (p.D / 2 + 3) / 4;
   auto run = [&](auto g) {
     constexpr int G = decltype(g)::value;
-    const int64_t tokens = (int64_t)p.B * p.L, groups = (tokens + 64 / G - 1) / (64 / G);
-    // A wave of many vectors computes its sines for all of them; few tokens need more waves to fill the chip.
+    const int64_t tokens = (int64_t)p.B * p.L, groups = (tokens + 64 / G * kTokenWaves - 1) / (64 / G * kTokenWaves);
+    // four vectors a wave; fewer where few tokens leave the chip idle
     const int vectors = p.parts * p.H;
-    const int blocks = (int)std::min<int64_t>((vectors + kWaves - 1) / kWaves, std::max<int64_t>(1, 2048 / groups));
-    const int64_t row = std::min<int64_t>(groups, 1 << 20);
-    const dim3 grid((unsigned)row, (unsigned)blocks, (unsigned)((groups + row - 1) / row));
+    const int64_t blocks = std::min<int64_t>((vectors + kVectorWaves - 1) / kVectorWaves,
+                                             std::max<int64_t>((vectors + 4 * kVectorWaves - 1) / (4 * kVectorWaves),
+                                                               512 / groups));
+    const int64_t row = std::min<int64_t>(groups, 65535);
+    const dim3 grid((unsigned)blocks, (unsigned)row, (unsigned)((groups + row - 1) / row));
     if (p.interleaved)
-      rope_axes_kernel<G, true><<<grid, kWaves * 64, 0, stream>>>(p, blocks * kWaves);
+      rope_axes_kernel<G, true><<<grid, kThreads, 0, stream>>>(p);
     else
-      rope_axes_kernel<G, false><<<grid, kWaves * 64, 0, stream>>>(p, blocks * kWaves);
+      rope_axes_kernel<G, false><<<grid, kThreads, 0, stream>>>(p);
   };
   if (lanes <= 1)
     run(std::integral_constant<int, 1>{});
