@@ -147,71 +147,47 @@ __device__ __forceinline__ void each_adapter(int number, uint64_t rows, int pass
 // sums in LDS.  x goes from HBM to the registers that feed the matrix cores, a step ahead, each value read once by one
 // wave; an adapter's tile of 16 ranks by 32 values is one contiguous load, a step ahead too.  (Two or four steps of x
 // ahead are 5-40 % slower: the loads of all waves fill memory's queues as it is.)
+struct DownRange {
+  int rb0, part, s_begin, s_end;  // first rank tile, part of K, the wave's steps
+};
+
+// RT row tiles from row0 through adapter a's `tiles` rank tiles; bit i of mask: row0 + i is the adapter's.
 template <int DTYPE, int RT, int RB, int W>
-__global__ __launch_bounds__(W * 64) void low_rank_down_kernel(LowRankParams p, int rank_blocks, int splits,
-                                                               int passes) {
+struct DownTile {
   using Wt = Weights<DTYPE>;
-  constexpr int kRound = RT * RB < W ? RT * RB : W;  // tiles added up at once
-  __shared__ floatx4 sums[kRound][W][64];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, q = lane >> 4;
-  const int64_t row0 = (int64_t)blockIdx.x * (RT * 16);
-  const int rb0 = (int)(blockIdx.y % rank_blocks) * RB, part = (int)(blockIdx.y / rank_blocks);
-  const int k_tiles = ceil_div(p.K, 32), r_tiles = ceil_div(p.R, 16), t_stride = r_tiles * 16;
-  const int share = ceil_div(k_tiles, splits * W);
-  const int s_begin = (part * W + wave) * share, s_end = min(k_tiles, s_begin + share);
-  const float* xrow[RT];
-#pragma unroll
-  for (int t = 0; t < RT; ++t) {
-    const int64_t m = row0 + t * 16 + (lane & 15);
-    xrow[t] = p.x + (m < p.M ? m : p.M - 1) * p.x_stride + q * 8;
-  }
+  static constexpr int kRound = RT * RB < W ? RT * RB : W;  // tiles added up at once
   float raw[RT][8];
-  auto load_x = [&](int s) {
-    const int k = s * 32;
-    if (k + 32 <= p.K) {
+
+  __device__ __forceinline__ void load_x(const LowRankParams& p, int64_t row0, int s) {
+    const int lane = threadIdx.x & 63, k = s * 32 + (lane >> 4) * 8;
 #pragma unroll
-      for (int t = 0; t < RT; ++t) {
-        const floatx4u lo = *reinterpret_cast<const floatx4u*>(xrow[t] + k);
-        const floatx4u hi = *reinterpret_cast<const floatx4u*>(xrow[t] + k + 4);
+    for (int t = 0; t < RT; ++t) {
+      const int64_t m = row0 + t * 16 + (lane & 15);
+      const float* src = p.x + (m < p.M ? m : p.M - 1) * p.x_stride + k;
+      if (s * 32 + 32 <= p.K) {
+        const floatx4u lo = *reinterpret_cast<const floatx4u*>(src);
+        const floatx4u hi = *reinterpret_cast<const floatx4u*>(src + 4);
 #pragma unroll
         for (int i = 0; i < 4; ++i) raw[t][i] = lo[i], raw[t][4 + i] = hi[i];
+      } else {  // the last step of a K that is no multiple of 32
+#pragma unroll
+        for (int i = 0; i < 8; ++i) raw[t][i] = k + i < p.K ? src[i] : 0.0f;
       }
-    } else {  // the last step of a K that is no multiple of 32
-#pragma unroll
-      for (int t = 0; t < RT; ++t)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) raw[t][i] = k + q * 8 + i < p.K ? xrow[t][k + i] : 0.0f;
     }
-  };
-  // x is on its way before its rows' adapters are known; passes after the first may have none
-  bool held = blockIdx.z == 0;
-  if (held && s_begin < s_end) load_x(s_begin);
-  int id = lane < RT * 16 && row0 + lane < p.M ? p.rows[row0 + lane] : -1;
-  if (id >= p.slots) id = -1;
-  const int row_rank = id >= 0 ? min(p.rank[id], p.R) : 0;
-  each_adapter(id, ~0ull, passes, [&](int a, int first_row, uint64_t mask) {
-    const char* down = static_cast<const char*>(p.down) +
-                       ((int64_t)a * r_tiles + rb0) * k_tiles * 512 * Wt::kBytes + lane * 16;
-    const int64_t tile_bytes = (int64_t)k_tiles * 512 * Wt::kBytes;
-    const float scale = p.scale[a];
-    int tiles = min(RB, r_tiles - rb0);  // (of the bank: the first loads do not wait for the adapter's own rank)
-    Wt w[RB];
-    auto load_w = [&](int j, int s) {
-      if (j < tiles && s < s_end) w[j].load(down + j * tile_bytes + (int64_t)s * 512 * Wt::kBytes);
-    };
-#pragma unroll
-    for (int j = 0; j < RB; ++j) load_w(j, s_begin);
-    const int rank = __builtin_amdgcn_readlane(row_rank, first_row);
-    tiles = rank > 0 ? min(RB, ceil_div(rank, 16) - rb0) : 0;
-    if (tiles <= 0) return;  // the same for the whole workgroup
-    if (!held && s_begin < s_end) load_x(s_begin);
-    held = false;
+  }
+
+  // x of the first step is in raw; w holds the first step's weights.
+  __device__ __forceinline__ void run(const LowRankParams& p, const DownRange& r, int64_t row0, Wt (&w)[RB],
+                                      const char* down, int64_t tile_bytes, int tiles, float scale, uint64_t mask,
+                                      floatx4 (*sums)[W][64]) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, q = lane >> 4;
+    const int t_stride = ceil_div(p.R, 16) * 16;
     floatx4 acc[RT][RB] = {};
-    for (int s = s_begin; s < s_end; ++s) {
+    for (int s = r.s_begin; s < r.s_end; ++s) {
       bf16x8 xs[RT][3];
 #pragma unroll
       for (int t = 0; t < RT; ++t) split<3>(raw[t], xs[t]);
-      if (s + 1 < s_end) load_x(s + 1);
+      if (s + 1 < r.s_end) load_x(p, row0, s + 1);
 #pragma unroll
       for (int j = 0; j < RB; ++j) {
         if (j >= tiles) break;
@@ -222,11 +198,11 @@ __global__ __launch_bounds__(W * 64) void low_rank_down_kernel(LowRankParams p, 
 #pragma unroll
           for (int t = 0; t < RT; ++t)
             acc[t][j] = mfma16(ws[weight_term<Wt::kTerms>(i)], xs[t][value_term<Wt::kTerms>(i)], acc[t][j]);
-        load_w(j, s + 1);
+        if (s + 1 < r.s_end) w[j].load(down + j * tile_bytes + (int64_t)(s + 1) * 512 * Wt::kBytes);
       }
     }
-    // the waves' sums, W tiles at a time: wave w adds up tile w
-    float* out = p.scratch + meta_floats(p.M) + (int64_t)part * p.M * t_stride;
+    // the waves' sums, kRound tiles at a time: wave i adds up tile i
+    float* out = p.scratch + meta_floats(p.M) + (int64_t)r.part * p.M * t_stride;
 #pragma unroll
     for (int at = 0; at < RT * RB; at += kRound) {
       __syncthreads();
@@ -239,11 +215,74 @@ __global__ __launch_bounds__(W * 64) void low_rank_down_kernel(LowRankParams p, 
         floatx4 sum = sums[wave][0][lane];
 #pragma unroll
         for (int i = 1; i < W; ++i) sum += sums[wave][i][lane];
-        *reinterpret_cast<floatx4*>(out + (row0 + t * 16 + (lane & 15)) * t_stride + (rb0 + j) * 16 + q * 4) =
+        *reinterpret_cast<floatx4*>(out + (row0 + t * 16 + (lane & 15)) * t_stride + (r.rb0 + j) * 16 + q * 4) =
             sum * scale;
       }
     }
-  });
+  }
+};
+
+template <int DTYPE, int RT, int RB, int W>
+__global__ __launch_bounds__(W * 64) void low_rank_down_kernel(LowRankParams p, int rank_blocks, int splits,
+                                                               int passes) {
+  using Wt = Weights<DTYPE>;
+  __shared__ floatx4 sums[DownTile<DTYPE, RT, RB, W>::kRound][W][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t row0 = (int64_t)blockIdx.x * (RT * 16);
+  const int k_tiles = ceil_div(p.K, 32), r_tiles = ceil_div(p.R, 16), share = ceil_div(k_tiles, splits * W);
+  DownRange r;
+  r.rb0 = (int)(blockIdx.y % rank_blocks) * RB;
+  r.part = (int)(blockIdx.y / rank_blocks);
+  r.s_begin = (r.part * W + wave) * share;
+  r.s_end = min(k_tiles, r.s_begin + share);
+  // x is on its way before its rows' adapters are known; passes after the first may have none
+  DownTile<DTYPE, RT, RB, W> all;
+  bool held = blockIdx.z == 0;
+  if (held && r.s_begin < r.s_end) all.load_x(p, row0, r.s_begin);
+  int id = lane < RT * 16 && row0 + lane < p.M ? p.rows[row0 + lane] : -1;
+  if (id >= p.slots) id = -1;
+  const int row_rank = id >= 0 ? min(p.rank[id], p.R) : 0;
+  auto adapter = [&](int a, int first_row, uint64_t mask) {
+    const char* down = static_cast<const char*>(p.down) +
+                       ((int64_t)a * r_tiles + r.rb0) * k_tiles * 512 * Wt::kBytes + lane * 16;
+    const int64_t tile_bytes = (int64_t)k_tiles * 512 * Wt::kBytes;
+    const float scale = p.scale[a];
+    Wt w[RB];
+    auto load_w = [&](int tiles) {
+#pragma unroll
+      for (int j = 0; j < RB; ++j)
+        if (j < tiles && r.s_begin < r.s_end) w[j].load(down + j * tile_bytes + (int64_t)r.s_begin * 512 * Wt::kBytes);
+    };
+    load_w(min(RB, r_tiles - r.rb0));  // (of the bank: these do not wait for the adapter's own rank)
+    const int rank = __builtin_amdgcn_readlane(row_rank, first_row);
+    const int tiles = rank > 0 ? min(RB, ceil_div(rank, 16) - r.rb0) : 0;
+    if (tiles <= 0) return;  // the same for the whole workgroup
+    if (RT == 1 || held) {
+      if (!held && r.s_begin < r.s_end) all.load_x(p, row0, r.s_begin);
+      held = false;
+      all.run(p, r, row0, w, down, tile_bytes, tiles, scale, mask, sums);
+      return;
+    }
+    // A further adapter of a wider tile, at the border of two requests: its row tiles by themselves.
+    bool again = false;
+    for (int t = 0; t < RT; ++t) {
+      const uint64_t rows = mask >> (t * 16) & 0xffff;
+      if (rows == 0) continue;
+      if (again) load_w(tiles);
+      again = true;
+      DownTile<DTYPE, 1, RB, W> one;
+      if (r.s_begin < r.s_end) one.load_x(p, row0 + t * 16, r.s_begin);
+      one.run(p, r, row0 + t * 16, w, down, tile_bytes, tiles, scale, rows, sums);
+    }
+  };
+  if constexpr (RT == 1) {
+    each_adapter(id, ~0ull, passes, adapter);
+  } else {
+    // the middle row's adapter has the most rows of a border tile: it goes first, through all row tiles at once
+    const int middle = __builtin_amdgcn_readlane(id, RT * 8);
+    if (middle >= 0) adapter(middle, RT * 8, __ballot(id == middle));
+    each_adapter(id == middle ? -1 : id, ~0ull, 1, adapter);
+  }
   if (blockIdx.y == 0 && blockIdx.z == 0 && wave == 0 && lane < RT * 16 && row0 + lane < p.M)
     reinterpret_cast<int*>(p.scratch)[row0 + lane] = row_rank > 0 ? row_rank << kIdBits | id : -1;
 }
@@ -480,14 +519,13 @@ __global__ __launch_bounds__(W * 64) void low_rank_few_kernel(LowRankParams p, i
   }
 }
 
-// Rows a workgroup of the first kernel, the parts that it splits K into, and the workgroups that share a tile's
+// Row tiles a workgroup of the first kernel, the parts that it splits K into, and the workgroups that share a tile's
 // adapters.  Few rows leave the chip idle without the last two: 64 rows of an adapter each, K 1024 -> N 6144, rank 32,
-// take 68 + 17 us with one workgroup a tile, 6.8 + 8.1 with 16 and 8.  Many rows: a second workgroup for the tiles at
-// the border of two requests, which would otherwise end last (12294 x 1024, rank 16: 20 -> 15 us); 32 rows a
-// workgroup, but 64 where an adapter's values are read often enough to count (16384 x 4096, rank 64: 91 against 75 us;
-// rank 16, K 1024: 18 against 20).
+// take 68 + 17 us with one workgroup a tile, 6.8 + 8.1 with 16 and 8.  Many rows: two row tiles, so that an adapter's
+// values are read half as often (12294 x 1024, rank 16: 15.3 us against 16.9; four: 15.6, and 20 where requests meet,
+// since a workgroup that fills a compute unit by itself then ends last).
 struct Plan {
-  int row_tiles, splits, down_passes, up_tiles, up_passes;
+  int row_tiles, splits, down_passes, up_passes;
 };
 
 // Whether both products go in one launch: where a column block's own sums are little work, and not many of them.  16
@@ -500,13 +538,12 @@ constexpr int kFewTiles = 2, kFewWaves = 8;
 constexpr int kDownWaves = 8, kUpWaves = 4;
 
 Plan plan_of(int M, int K, int N, int slots, int R) {
-  Plan pl{M > 8192 && R > 32 ? 4 : M > 4096 ? 2 : 1, 1, std::min({2, M, slots}), 8, 1};
+  Plan pl{M > 4096 ? 2 : 1, 1, 1, 1};
   if (M <= 4096) {
     const int tiles = ceil_div(M, 16), most = std::min({16, M, slots});
     pl.splits = std::max(1, std::min({256 / tiles, ceil_div(K, 32) / (2 * kDownWaves), 8}));
     pl.down_passes = std::max(1, std::min(1024 / tiles, most));
-    pl.up_tiles = 4;
-    pl.up_passes = std::max(1, std::min(1024 / (tiles * ceil_div(N, 16 * kUpWaves * pl.up_tiles)), most));
+    pl.up_passes = std::max(1, std::min(1024 / (tiles * ceil_div(N, 64 * kUpWaves)), most));
   }
   return pl;
 }
@@ -521,11 +558,12 @@ void launch_down(const LowRankParams& p, const Plan& pl, hipStream_t stream) {
         <<<dim3(m_blocks, blocks * pl.splits, pl.down_passes), kDownWaves * 64, 0, stream>>>(p, blocks, pl.splits,
                                                                                             pl.down_passes);
   };
-  if constexpr (RT < 4) {
-    if (tiles == 1) return run(std::integral_constant<int, 1>{});
-    if (tiles == 2) return run(std::integral_constant<int, 2>{});
-  }
-  run(std::integral_constant<int, 4>{});
+  if (tiles == 1)
+    run(std::integral_constant<int, 1>{});
+  else if (tiles == 2)
+    run(std::integral_constant<int, 2>{});
+  else
+    run(std::integral_constant<int, 4>{});
 }
 
 template <int DTYPE, int NT>
@@ -546,15 +584,13 @@ void launch_typed(const LowRankParams& p, hipStream_t stream) {
     return;
   }
   const Plan pl = plan_of(p.M, p.K, p.N, p.slots, p.R);
-  switch (pl.row_tiles) {
-    case 1: launch_down<DTYPE, 1>(p, pl, stream); break;
-    case 2: launch_down<DTYPE, 2>(p, pl, stream); break;
-    default: launch_down<DTYPE, 4>(p, pl, stream); break;
-  }
-  if (pl.up_tiles == 4)
+  if (pl.row_tiles == 1) {
+    launch_down<DTYPE, 1>(p, pl, stream);
     launch_up<DTYPE, 4>(p, pl, stream);
-  else
+  } else {
+    launch_down<DTYPE, 2>(p, pl, stream);
     launch_up<DTYPE, 8>(p, pl, stream);
+  }
 }
 
 }  // namespace
