@@ -112,26 +112,27 @@ __global__ __launch_bounds__(RW == 1 ? 256 : RW * 64) void residual_norm_kernel(
   load_row(h, p.h + row * p.h_stride, c0, last);
   load_row(x, p.x + row * p.x_stride, c0, last);
   if (p.gate) load_row(gate, p.gate + b * p.gate_stride, c0, last);
-  auto affine = [&](Row<RW, V>& r, const NormSpec& s, const Stats& st) {
+  // a norm's vectors are asked for before its sums, which take their time
+  auto norm = [&](Row<RW, V>& r, const NormSpec& s, float* sums) {
     if (s.kind == kNormNone) return;
+    Row<RW, V> w, bias;
+    if (s.weight) load_row(w, s.weight, c0, last);
+    if (s.bias) load_row(bias, s.bias, c0, last);
+    const Stats st = row_stats(r, s.kind, s.eps, n, last, sums);
 #pragma unroll
     for (int i = 0; i < V; ++i)
 #pragma unroll
       for (int e = 0; e < 4; ++e) r.v[i][e] = (r.v[i][e] - st.mean - st.left) * st.inv;
     if (s.weight) {
-      Row<RW, V> w;
-      load_row(w, s.weight, c0, last);
 #pragma unroll
       for (int i = 0; i < V; ++i) r.v[i] *= w.v[i];
     }
     if (s.bias) {
-      Row<RW, V> w;
-      load_row(w, s.bias, c0, last);
 #pragma unroll
-      for (int i = 0; i < V; ++i) r.v[i] += w.v[i];
+      for (int i = 0; i < V; ++i) r.v[i] += bias.v[i];
     }
   };
-  affine(h, p.post, row_stats(h, p.post.kind, p.post.eps, n, last, lds));
+  norm(h, p.post, lds);
   if (p.gate) {
 #pragma unroll
     for (int i = 0; i < V; ++i) h.v[i] *= gate.v[i];
@@ -142,11 +143,13 @@ __global__ __launch_bounds__(RW == 1 ? 256 : RW * 64) void residual_norm_kernel(
     for (int e = 0; e < 4; ++e)  // (past the end the statistics want zeros)
       x.v[i][e] = i == V - 1 && e >= last ? 0.0f : fmaf(p.residual_scale, x.v[i][e], h.v[i][e]);
   store_row(x, p.out + row * p.out_stride, c0, last);
-  affine(x, p.pre, row_stats(x, p.pre.kind, p.pre.eps, n, last, lds + (RW == 1 ? 0 : 3 * RW)));
+  Row<RW, V> scale, shift;
   if (p.scale) {
-    Row<RW, V> scale, shift;
     load_row(scale, p.scale + b * p.mod_stride, c0, last);
     load_row(shift, p.shift + b * p.mod_stride, c0, last);
+  }
+  norm(x, p.pre, lds + (RW == 1 ? 0 : 3 * RW));
+  if (p.scale) {
 #pragma unroll
     for (int i = 0; i < V; ++i)
 #pragma unroll
