@@ -191,6 +191,10 @@ def test_bank_refusals():
             bank.load(slot, torch.zeros(down), torch.zeros(up))
     with pytest.raises(ValueError):
         AdapterBank(2, 8, 6, 513, device="cpu")
+    for sizes in ((0, 8, 6, 4), (2, 0, 6, 4), (2, 8, 0, 4), (2, 8, 6, 0), ((1 << 20) + 1, 8, 6, 4),
+                  (2, (1 << 20) + 1, 6, 4), (2, 8, (1 << 20) + 1, 4)):
+        with pytest.raises(ValueError):
+            AdapterBank(*sizes, device="meta")
     with pytest.raises(ValueError):
         AdapterBank(2, 8, 6, 4, torch.float64, device="cpu")
     with pytest.raises(ValueError):

@@ -223,15 +223,14 @@ def enqueue(lib, fn_name, index, *args) -> None:
 
 def no_gradients(torch, *tensors) -> None:
     """These operators have no backward: a tensor that expects one is refused, not cut off in silence."""
-    if torch.is_grad_enabled():
-        for t in tensors:
-            if t is not None and t.requires_grad:
-                raise ValueError("this operator has no backward: call it under torch.no_grad(), or detach its inputs")
+    for t in tensors:
+        if t is not None and t.requires_grad and torch.is_grad_enabled():
+            raise ValueError("this operator has no backward: call it under torch.no_grad(), or detach its inputs")
 
 
 def rows_of(torch, name, t, cols) -> tuple[int, int]:
     """(rows, row stride) of a GPU fp32 tensor [..., cols] whose rows lie at one stride; ValueError otherwise."""
-    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype == torch.float32):
+    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype is torch.float32):
         raise ValueError(f"{name} must be an fp32 GPU tensor")
     shape = t.shape
     if len(shape) == 0 or shape[-1] != cols:

@@ -14,7 +14,10 @@ from __future__ import annotations
 
 from ._lib import enqueue, load_library, no_gradients, rows_of
 
-MAX_RANK = 512  # the library's limit
+# the library's limits
+MAX_RANK = 512
+MAX_SLOTS = MAX_FEATURES = 1 << 20
+MAX_ROWS = 1 << 28
 
 
 def _types(torch):
@@ -44,6 +47,13 @@ def _tiled(torch, values, tile):
     return tile
 
 
+def _sizes_fit(slots, in_features, out_features, max_rank):
+    if not (1 <= slots <= MAX_SLOTS and 1 <= in_features <= MAX_FEATURES and 1 <= out_features <= MAX_FEATURES
+            and 1 <= max_rank <= MAX_RANK):
+        raise ValueError(f"an AdapterBank has 1..{MAX_SLOTS} slots, 1..{MAX_FEATURES} features in and out and a rank of "
+                         f"1..{MAX_RANK}")
+
+
 class AdapterBank:
     """Adapters of one Linear [in_features -> out_features] in `slots` slots of at most max_rank.
 
@@ -60,8 +70,7 @@ class AdapterBank:
             raise ValueError("an AdapterBank holds fp32, bf16 or fp16")
         self.slots, self.in_features, self.out_features = int(slots), int(in_features), int(out_features)
         self.max_rank, self.dtype = int(max_rank), dtype
-        if min(self.slots, self.in_features, self.out_features) < 1 or not 1 <= self.max_rank <= MAX_RANK:
-            raise ValueError(f"an AdapterBank needs slots, features and a max_rank of 1..{MAX_RANK}")
+        _sizes_fit(self.slots, self.in_features, self.out_features, self.max_rank)
         k32, n16 = -(-self.in_features // 32), -(-self.out_features // 16)
         tile, held = ((3, 4, 16, 8), torch.bfloat16) if dtype == torch.float32 else ((4, 16, 8), dtype)
         self.down = torch.zeros((self.slots, -(-self.max_rank // 16), k32, *tile), dtype=held, device=device)
@@ -121,8 +130,9 @@ class AdapterBank:
         if tuple(scale.shape) != (S,):
             raise ValueError(f"scale must be [{S}]")
         bank = cls.__new__(cls)
-        if down.dtype not in _types(torch) or S < 1 or K < 1 or int(up.shape[1]) < 1 or not 1 <= R <= MAX_RANK:
-            raise ValueError(f"an AdapterBank holds fp32, bf16 or fp16 adapters of rank 1..{MAX_RANK}")
+        if down.dtype not in _types(torch):
+            raise ValueError("an AdapterBank holds fp32, bf16 or fp16")
+        _sizes_fit(S, K, int(up.shape[1]), R)
         bank.slots, bank.in_features, bank.out_features, bank.max_rank = S, K, int(up.shape[1]), R
         bank.dtype, bank.device, bank.index = down.dtype, down.device, down.get_device()
         bank.type_id = _types(torch)[down.dtype]
@@ -164,14 +174,15 @@ def low_rank_add(y, x, bank, rows, *, out=None, library=None):
     M, y_stride = rows_of(torch, "y", y, bank.out_features)
     Mx, x_stride = rows_of(torch, "x", x, bank.in_features)
     no_gradients(torch, y, x)
-    if Mx != M:
-        raise ValueError(f"y has {M} rows, x has {Mx}")
+    if Mx != M or M > MAX_ROWS:
+        raise ValueError(f"y has {M} rows, x has {Mx}: as many of both are wanted, at most {MAX_ROWS}")
     if not (isinstance(rows, torch.Tensor) and rows.dtype == torch.int32 and rows.numel() == M
             and rows.is_contiguous()):
         raise ValueError(f"rows must be a contiguous int32 tensor of {M} slots")
     at = y.get_device()
     if out is None:
-        out, out_stride = torch.empty_like(y, memory_format=torch.contiguous_format), bank.out_features
+        out_stride = bank.out_features  # (rows at that stride are contiguous)
+        out = torch.empty_like(y) if y_stride == out_stride else y.new_empty(y.shape)
     elif out is y:
         out_stride = y_stride
     else:

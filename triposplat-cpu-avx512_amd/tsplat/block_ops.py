@@ -145,19 +145,16 @@ NORM_KINDS = {None: 0, "layer": 1, "rms": 2}
 
 def _batch_rows(torch, name, t, B, C, device):
     """(pointer, row stride, rows) of a per-batch [B, C] or shared [1, C] row of a modulation."""
-    if not (isinstance(t, torch.Tensor) and t.get_device() == device and t.dtype == torch.float32):
-        raise ValueError(f"{name} must be an fp32 tensor on the GPU of x")
-    shape = t.shape
-    if len(shape) != 2:
-        raise ValueError(f"{name} must be [{B}, {C}] or [1, {C}]")
-    (rows, cols), (step, unit) = shape, t.stride()
-    if cols != C or (rows != B and rows != 1) or (unit != 1 and C > 1):
-        raise ValueError(f"{name} must be [{B}, {C}] or [1, {C}] with unit column stride")
-    if rows == 1:
-        return t.data_ptr(), C, 1
-    if step < C:
-        raise ValueError(f"the rows of {name} overlap")
-    return t.data_ptr(), step, rows
+    if isinstance(t, torch.Tensor) and t.get_device() == device and t.dtype is torch.float32 and t.dim() == 2:
+        rows, cols = t.shape
+        step, unit = t.stride()
+        if cols == C and (unit == 1 or C == 1):
+            if rows == 1:
+                return t.data_ptr(), C, 1
+            if rows == B and step >= C:
+                return t.data_ptr(), step, rows
+    raise ValueError(f"{name} must be [{B}, {C}] or [1, {C}], fp32 on the GPU of x, with unit column stride and rows "
+                     "that do not overlap")
 
 
 def _norm_vector(torch, name, t, C, device):
@@ -187,8 +184,8 @@ def residual_norm(x, h, *, gate=None, residual_scale=1.0, post_norm=None, post_w
     if norm not in ("layer", "rms") or post_norm not in NORM_KINDS:
         raise ValueError(f"norm is 'layer' or 'rms', post_norm one of them or None, not {norm!r}, {post_norm!r}")
     shape = x.shape
-    if len(shape) == 0 or shape[-1] < 1 or h.shape != shape:
-        raise ValueError("x and h must be [..., C] of one shape")
+    if len(shape) == 0 or not 1 <= shape[-1] < 1 << 31 or h.shape != shape or x.numel() // shape[-1] >= 1 << 31:
+        raise ValueError("x and h must be [..., C] of one shape, with fewer than 2^31 rows and columns")
     C, B = shape[-1], shape[0] if len(shape) > 1 else 1
     M, x_stride = rows_of(torch, "x", x, C)
     _, h_stride = rows_of(torch, "h", h, C)
@@ -220,7 +217,7 @@ def residual_norm(x, h, *, gate=None, residual_scale=1.0, post_norm=None, post_w
         groups = max(groups, mods)
     out_stride = normed_stride = C
     if out is None:
-        out = torch.empty_like(x, memory_format=torch.contiguous_format)
+        out = torch.empty_like(x) if x_stride == C else x.new_empty(shape)  # (rows at stride C are contiguous)
     elif out is x:
         out_stride = x_stride
     else:
@@ -228,7 +225,7 @@ def residual_norm(x, h, *, gate=None, residual_scale=1.0, post_norm=None, post_w
             raise ValueError("out must have the shape of x")
         _, out_stride = rows_of(torch, "out", out, C)
     if normed is None:
-        normed = torch.empty_like(x, memory_format=torch.contiguous_format)
+        normed = torch.empty_like(x) if x_stride == C else x.new_empty(shape)
     elif normed is h:
         normed_stride = h_stride
     else:

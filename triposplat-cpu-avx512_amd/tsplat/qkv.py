@@ -178,42 +178,45 @@ class RopeAxes:
         self.device, self.index, self.axes = self.turns.device, self.turns.get_device(), len(sections)
 
 
-def _rope_call(torch, x, strides, parts, gammas, positions, rope, eps, B, L, H, outs, out_bhld, library):
+def _gamma(torch, g, H, D, device):
+    if g is None:
+        return None
+    if not (isinstance(g, torch.Tensor) and g.dtype is torch.float32 and g.shape == (H, D) and g.is_contiguous()
+            and g.get_device() == device):
+        raise ValueError(f"gamma must be a contiguous [{H}, {D}] fp32 tensor on the GPU of x")
+    return g.data_ptr()
+
+
+def _rope_call(torch, x, strides, parts, gamma0, gamma1, positions, rope, eps, B, L, H, outs, out_bhld, library):
     D, at = rope.dim, x.get_device()
     shape = (B, H, L, D) if out_bhld else (B, L, H, D)
-    fresh = outs is None
-    if fresh:
-        outs = [torch.empty(shape, dtype=torch.float32, device=x.device) for _ in range(parts)]
+    if outs is None:
+        outs = [x.new_empty(shape) for _ in range(parts)]
+    else:
+        for o in outs:
+            if not (isinstance(o, torch.Tensor) and o.dtype is torch.float32 and o.shape == shape
+                    and o.is_contiguous() and o.get_device() == at):
+                raise ValueError(f"out must be a contiguous {list(shape)} fp32 tensor on the GPU of x")
     if not isinstance(positions, torch.Tensor) or positions.get_device() != at or rope.index != at:
         raise ValueError("x, positions and rope must be on one GPU")
-    fractional = positions.dtype == torch.float32
-    places = positions.shape
-    batches = places[0] if len(places) == 3 else 1
-    if (not (fractional or positions.dtype == torch.int32) or not positions.is_contiguous()
-            or not 2 <= len(places) <= 3 or places[-2] != L or places[-1] != rope.axes or batches not in (1, B)):
+    kind, places = positions.dtype, positions.shape
+    fractional, batches = kind is torch.float32, places[0] if len(places) == 3 else 1
+    if (not (fractional or kind is torch.int32) or not positions.is_contiguous() or not 2 <= len(places) <= 3
+            or places[-2] != L or places[-1] != rope.axes or batches not in (1, B)):
         raise ValueError(f"positions must be a contiguous [{L}, {rope.axes}] or [{B}, {L}, {rope.axes}] tensor of int32 "
                          "or fp32")
-    no_gradients(torch, x, positions, *gammas)
-    ptr = [None, None]
-    for i, g in enumerate(gammas):
-        if g is not None:
-            if not (isinstance(g, torch.Tensor) and g.dtype == torch.float32 and g.shape == (H, D)
-                    and g.is_contiguous() and g.get_device() == at):
-                raise ValueError(f"gamma must be a contiguous [{H}, {D}] fp32 tensor on the GPU of x")
-            ptr[i] = g.data_ptr()
+    no_gradients(torch, x, positions, gamma0, gamma1)
     if not eps >= 0.0:
         raise ValueError("eps must not be negative")
-    if not fresh:
-        for o in outs:
-            if not (isinstance(o, torch.Tensor) and o.dtype == torch.float32 and o.shape == shape and o.is_contiguous()
-                    and o.get_device() == at):
-                raise ValueError(f"out must be a contiguous {list(shape)} fp32 tensor on the GPU of x")
+    if H > 1 << 16 or B * L >= 1 << 31:
+        raise ValueError("at most 2^16 heads, and fewer than 2^31 tokens")
+    gammas = _gamma(torch, gamma0, H, D, at), _gamma(torch, gamma1, H, D, at)
     if B * L * H == 0:
         return outs
-    dst = [o.data_ptr() for o in outs] + [None, None]
-    enqueue(load_library(library), "tsplat_rope_axes_async", at, x.data_ptr(), *strides, parts, ptr[0], ptr[1],
-            dst[0], dst[1], dst[2], positions.data_ptr(), fractional, batches, rope.axes, rope.turns.data_ptr(),
-            rope.axis.data_ptr(), rope.interleaved, eps, B, L, H, D, out_bhld)
+    dst = [outs[0].data_ptr(), outs[1].data_ptr(), outs[2].data_ptr()] if parts == 3 else [outs[0].data_ptr(), None, None]
+    enqueue(load_library(library), "tsplat_rope_axes_async", at, x.data_ptr(), *strides, parts, *gammas, *dst,
+            positions.data_ptr(), fractional, batches, rope.axes, rope.turns.data_ptr(), rope.axis.data_ptr(),
+            rope.interleaved, eps, B, L, H, D, out_bhld)
     return outs
 
 
@@ -236,7 +239,7 @@ def rope_axes(x, positions, rope, *, gamma=None, eps=1.0e-12, out=None, out_bhld
         raise ValueError("x must have unit stride within its vectors")
     if (B > 1 and sb < D) or (L > 1 and sl < D) or (H > 1 and sh < D):
         raise ValueError("the vectors of x overlap")
-    return _rope_call(torch, x, (0, sb, sl, sh), 1, (gamma,), positions, rope, eps, B, L, H,
+    return _rope_call(torch, x, (0, sb, sl, sh), 1, gamma, None, positions, rope, eps, B, L, H,
                       None if out is None else [out], out_bhld, library)[0]
 
 
@@ -255,5 +258,5 @@ def qkv_rope_axes(qkv, positions, rope, q_gamma, k_gamma, B, L, H, *, eps=1.0e-1
         raise ValueError(f"qkv has {rows} rows, not B * L = {B * L}")
     if outs is not None and len(outs) != 3:
         raise ValueError("outs must be three tensors")
-    return tuple(_rope_call(torch, qkv, (width, L * stride, stride, rope.dim), 3, (q_gamma, k_gamma), positions,
+    return tuple(_rope_call(torch, qkv, (width, L * stride, stride, rope.dim), 3, q_gamma, k_gamma, positions,
                             rope, eps, B, L, H, outs, True, library))
