@@ -85,7 +85,7 @@ def _norm(lib, x=P[0], xs=32, h=P[1], hs=32, out=P[2], os=32, normed=P[3], ns=32
     (dict(pre=0), -2), (dict(pre=3), -2), (dict(post=3), -2),
     (dict(xs=31), -3), (dict(hs=31), -3), (dict(os=31), -3), (dict(ns=31), -3),
     (dict(scale=P[5], ms=32), -3), (dict(shift=P[5], ms=32), -3), (dict(pw=P[5]), -3),
-    (dict(gate=P[5], gs=31), -3), (dict(gate=P[5], gs=32, per=0), -3),
+    (dict(gate=P[5], gs=31), -3), (dict(gate=P[2], gs=32, per=(1 << 63) - 1), -3), (dict(gate=P[5], gs=32, per=0), -3),
     (dict(out=P[0] + 4), -3), (dict(out=P[1]), -3), (dict(normed=P[0]), -3), (dict(normed=P[2]), -3),
     (dict(normed=P[1] + 4), -3), (dict(gate=P[2], gs=32), -3), (dict(scale=P[3], shift=P[5], ms=32), -3),
     (dict(x=P[0] + 1), -4),

@@ -3,6 +3,7 @@
 
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cstdint>
 
 #include "capi_internal.h"
@@ -119,7 +120,8 @@ int tsplat_residual_norm_async(const float* x, int64_t x_stride, const float* h,
   if (modulate && (!scale || !shift)) return kErrRange;
   if (post_kind == kNormNone && (post_weight || post_bias)) return kErrRange;
   if ((gate || modulate) && rows_per_batch <= 0) return kErrRange;
-  const int64_t batches = gate || modulate ? (rows + rows_per_batch - 1) / rows_per_batch : 1;
+  const int64_t per = gate || modulate ? std::min(rows_per_batch, rows) : rows;
+  const int64_t batches = (rows + per - 1) / per;
   // (a stride of 0: one row for every batch entry)
   const int64_t gates = gate_stride == 0 ? 1 : batches, mods = mod_stride == 0 ? 1 : batches;
   const Rows rg{gate, gate_stride, gates, cols}, rs{scale, mod_stride, mods, cols}, rt{shift, mod_stride, mods, cols};
@@ -147,7 +149,7 @@ int tsplat_residual_norm_async(const float* x, int64_t x_stride, const float* h,
                        residual_scale, gate, gate_stride,
                        NormSpec{post_kind, post_weight, post_bias, post_eps},
                        NormSpec{pre_kind, pre_weight, pre_bias, pre_eps},
-                       scale, shift, mod_stride, batches > 1 ? rows_per_batch : rows};
+                       scale, shift, mod_stride, per};
   return launched(launch_residual_norm(p, static_cast<hipStream_t>(stream)));
 }
 

@@ -1,6 +1,8 @@
 // A branch's norm, its gate and residual, and the next norm with its modulation, one pass over the rows:
 //   h' = post(h);  x' = c x + gate[b] h';  out = x';  normed = pre(x') (1 + scale[b]) + shift[b].
-// 16 bytes a value from and to HBM, which bounds it.  Statistics are fp32 sums of the row's values less its first
+// 16 bytes a value from and to HBM, which bounds it: 12294 x 1024 38 us (5.3 TB/s), 8202 x 4096 with both norms 94 us
+// (5.7).  A row stays in registers from the first load to the last store: in those of one wave up to 2048 columns, of
+// four up to 8192 (at 2048 columns the two are alike, 50 us for 7812 rows).  Statistics are fp32 sums of the row's values less its first
 // mean, whose own sum corrects that mean: a row far from zero keeps the precision of its differences.
 
 #include <algorithm>
@@ -103,10 +105,11 @@ __device__ __forceinline__ Stats row_stats(const Row<RW, V>& r, int kind, float 
 template <int RW, int V>
 __global__ __launch_bounds__(RW == 1 ? 256 : RW * 64) void residual_norm_kernel(ResidualNormParams p) {
   __shared__ float lds[RW == 1 ? 1 : 6 * RW];
-  const int64_t row = RW == 1 ? block_index() * 4 + (threadIdx.x >> 6) : block_index();
+  // (the wave's number as a scalar, so that what follows from the row is one too)
+  const int64_t row = RW == 1 ? block_index() * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : block_index();
   if (row >= p.rows) return;  // whole waves; with RW > 1 whole workgroups
   const int c0 = (RW == 1 ? threadIdx.x & 63 : threadIdx.x) * 4, last = p.cols - c0 - (V - 1) * 256 * RW;
-  const int64_t b = p.gate || p.scale ? row / p.rows_per_batch : 0;
+  const int64_t b = p.gate || p.scale ? (uint32_t)row / (uint32_t)p.rows_per_batch : 0;
   const float n = (float)p.cols;
   Row<RW, V> x, h, gate;
   load_row(h, p.h + row * p.h_stride, c0, last);
@@ -158,7 +161,7 @@ __global__ __launch_bounds__(RW == 1 ? 256 : RW * 64) void residual_norm_kernel(
   store_row(x, p.normed + row * p.normed_stride, c0, last);
 }
 
-// Rows too wide for registers: one workgroup a row, which is read again for each sum.
+// Rows too wide for registers: one workgroup a row, which is read again for each sum (1302 x 12288: 91 us, 2.8 TB/s).
 constexpr int kWideThreads = 1024;
 
 __device__ float block_sum(float v, float* lds) {
@@ -202,7 +205,7 @@ __global__ __launch_bounds__(kWideThreads) void residual_norm_wide_kernel(Residu
   __shared__ float lds[kWideThreads / 64];
   const int64_t row = block_index();
   if (row >= p.rows) return;
-  const int64_t b = p.gate || p.scale ? row / p.rows_per_batch : 0;
+  const int64_t b = p.gate || p.scale ? (uint32_t)row / (uint32_t)p.rows_per_batch : 0;
   const float* x = p.x + row * p.x_stride;
   const float* h = p.h + row * p.h_stride;
   float* out = p.out + row * p.out_stride;

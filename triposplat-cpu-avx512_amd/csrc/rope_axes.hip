@@ -17,10 +17,10 @@ namespace {
 typedef float floatx4u __attribute__((ext_vector_type(4), aligned(4)));  // vectors start at any float
 
 // A workgroup: kTokenWaves waves along the tokens, each with kVectorWaves shares of their parts' heads.  16384 tokens x
-// 16 x 64, q, k and v: 87 us; one token wave with 4 shares 94-110 (writes of 2 KiB a head instead of 8), workgroups in
-// the order of the tokens 90 and more.
+// 16 x 64, q, k and v: 89 us, 4.5 TB/s (a copy of as much: 73-79); one token wave with 4 shares 94-110 (writes of 2 KiB
+// a head instead of 8).
 constexpr int kTokenWaves = 4, kVectorWaves = 4, kThreads = kTokenWaves * kVectorWaves * 64;
-constexpr int kAhead = 2;  // vectors that a lane asks for at once (4: 107 us, 1: 87)
+constexpr int kAhead = 2;  // vectors that a lane asks for at once (with one token wave 4: 107 us, 2: 112, 1: 94)
 
 // G lanes a vector, lane i of them its pairs 4 i .. 4 i + 3; a wave turns 64 / G tokens.  The workgroup computes its
 // tokens' sines and cosines once, into LDS, and a lane keeps its own while it goes through its share of the vectors.
@@ -34,13 +34,13 @@ __global__ __launch_bounds__(kThreads) void rope_axes_kernel(RopeAxesParams p) {
   const int64_t token = token0 + wave / kVectorWaves * kTokens + lane / G;
   const int share = blockIdx.x * kVectorWaves + wave % kVectorWaves, shares = gridDim.x * kVectorWaves;
   const int pairs = p.D / 2, vectors = p.parts * p.H;
-  for (int i = threadIdx.x; i < kAllTokens * pairs; i += kThreads) {
-    const int t = i / pairs, pair = i % pairs;
+  for (uint32_t i = threadIdx.x; i < (uint32_t)(kAllTokens * pairs); i += kThreads) {
+    const uint32_t t = i / (uint32_t)pairs, pair = i - t * (uint32_t)pairs;
     if (token0 + t >= tokens) break;
-    const int64_t l = (token0 + t) % p.L, b = (token0 + t) / p.L;
+    const uint32_t b = (uint32_t)(token0 + t) / (uint32_t)p.L, l = (uint32_t)(token0 + t) - b * (uint32_t)p.L;
     int axis = p.axis[pair];
     if (axis < 0 || axis >= p.axes) axis = 0;
-    const int64_t at = ((p.position_batches > 1 ? b : 0) * p.L + l) * p.axes + axis;
+    const int64_t at = ((int64_t)(p.position_batches > 1 ? b : 0) * p.L + l) * p.axes + axis;
     const double pos = p.position_type ? (double)static_cast<const float*>(p.positions)[at]
                                        : (double)static_cast<const int32_t*>(p.positions)[at];
     const double turn = pos * p.turns[pair];
@@ -50,7 +50,9 @@ __global__ __launch_bounds__(kThreads) void rope_axes_kernel(RopeAxesParams p) {
   }
   __syncthreads();
   const int n = token < tokens ? min(4, pairs - i0) : 0;  // pairs of this lane
-  const int64_t b = n > 0 ? token / p.L : 0, l = n > 0 ? token % p.L : 0;
+  // (tokens are fewer than 2^31: a division of 32 bits takes a fifth of one of 64)
+  const uint32_t live = n > 0 ? (uint32_t)token : 0;
+  const int64_t b = live / (uint32_t)p.L, l = live - (uint32_t)b * (uint32_t)p.L;
   float cs[4], sn[4];
 #pragma unroll
   for (int e = 0; e < 4; ++e) {

@@ -173,8 +173,10 @@ class RopeAxes:
         else:
             ramp = [self.theta ** (-j / n) for n in sections for j in range(n)]
         # revolutions per unit of position, in 64 bits: the kernel keeps the fraction of position * turns
-        self.turns = torch.tensor([f / (2.0 * math.pi) for f in ramp], dtype=torch.float64, device=device)
-        self.axis = torch.tensor(axis, dtype=torch.int32, device=device)
+        turns = torch.tensor([f / (2.0 * math.pi) for f in ramp], dtype=torch.float64)
+        both = torch.cat((turns.view(torch.uint8), torch.tensor(axis, dtype=torch.int32).view(torch.uint8)))
+        both = both.to(device)  # (one copy to the device)
+        self.turns, self.axis = both[:4 * dim].view(torch.float64), both[4 * dim:].view(torch.int32)
         self.device, self.index, self.axes = self.turns.device, self.turns.get_device(), len(sections)
 
 
