@@ -30,8 +30,9 @@ int tsplat_requests_abi_version(void);
  *   down: [slots][ceil(R/16)][ceil(K/32)][4][16][8], value (r, k) at [r/16][k/32][k%32/8][r%16][k%8];
  *   up:   [slots][ceil(N/16)][ceil(R/32)][4][16][8], value (n, r) at [n/16][r/32][r%32/8][n%16][r%8];
  * fp32: [slots][..][..][3][4][16][8] bf16, three planes whose sum is the value: its upper 16 bits, those of what is
- * left, and those of what is left then.  R = max_rank, 1..512; rank[a] <= R (a larger one counts as R).  16-byte aligned (-4).  M up to 2^28, K and N up
- * to 2^20, slots up to 2^20 (-2).  A row of x that holds an infinity or NaN gives NaN.
+ * left, and those of what is left then.  R = max_rank, 1..512; rank[a] <= R (a larger one counts as R).  16-byte aligned (-4).  M up to 2^27, K and N up
+ * to 2^20, slots up to 2^20 (-2).  A row of x that holds an infinity or NaN gives NaN.  The factors of the products (x,
+ * the adapter, the inner sums) count in steps of 2^-133 where fp32's own are finer, below 2^-110.
  * scratch: at least tsplat_low_rank_scratch_bytes(...) of device memory that no other work uses until the call's
  * kernels are done (-5 when too small), 16-byte aligned. */
 int64_t tsplat_low_rank_scratch_bytes(int M, int K, int N, int slots, int max_rank, int dtype);

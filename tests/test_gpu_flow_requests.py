@@ -153,6 +153,27 @@ def test_without_anything_it_is_the_models_velocity(cuda, hiplib):
     assert torch.equal(model.velocity(z, c, t, adapters=FlowAdapters(model, 2, 8), slots=[1, -1]), got)
 
 
+def test_a_sampler_step_of_a_request(cuda, hiplib):
+    """euler_cfg_step passes a request's adapter and positions on: the guided pair's velocities, joined as ever."""
+    import torch
+    from tsplat.flow_requests import FlowAdapters
+    from tsplat.qkv import RopeAxes
+
+    model = _model(cuda)
+    z, c, _, pos, g = _inputs(torch, cuda, model.cfg, 1, 6)
+    adapters = FlowAdapters(model, 1, 8, torch.bfloat16)
+    adapters.load(0, _adapter(torch, cuda, model, g, 8, ["qkv", "out", "fc1"]))
+    request = dict(adapters=adapters, slots=[0, 0], positions=pos[0], rope=RopeAxes(64, SECTIONS, device=cuda))
+    z_next, v = model.euler_cfg_step(z[0], c[0], **request)
+    ts = model.schedule()
+    t = torch.full((2,), ts[0] * 1000.0, device=cuda)
+    pair = model.velocity(z.expand(2, -1, -1).contiguous(), torch.cat((c, torch.zeros_like(c))), t, **request)
+    want = 3.0 * pair[0].double() - 2.0 * pair[1].double()
+    assert _rel(v, want) <= 1e-6
+    assert _rel(z_next, z[0].double() - (ts[0] - ts[1]) * v.double()) <= 1e-6
+    assert _rel(v, model.euler_cfg_step(z[0], c[0])[1].double()) > 1e-3
+
+
 def test_a_captured_block_of_requests(cuda, hiplib):
     """The three operators and the projections between them, captured and replayed with eager work between."""
     import torch

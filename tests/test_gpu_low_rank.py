@@ -138,6 +138,26 @@ def bank_half(t, f):
     return (t.float() * f).to(t.dtype)
 
 
+@pytest.mark.parametrize("M", [3, 300, 5000])
+def test_values_near_the_smallest(cuda, hiplib, M):
+    """A factor counts in steps of 2^-133: x and t are each off by at most that, times the other factor."""
+    import torch
+    from tsplat.adapters import AdapterBank, low_rank_add
+
+    g = torch.Generator(device=cuda).manual_seed(M)
+    for size in (1e-33, 1e-36, 1e-38):
+        x = torch.randn(M, 64, generator=g, device=cuda) * size
+        down, up = torch.randn(1, 12, 64, generator=g, device=cuda), torch.randn(1, 40, 12, generator=g, device=cuda)
+        bank = AdapterBank.stack(down, up, [1.0])
+        rows = torch.zeros(M, dtype=torch.int32, device=cuda)
+        y = torch.zeros(M, 40, device=cuda)
+        want, bound = low_rank(torch, y, x, rows, {0: (down[0], up[0], 1.0)})
+        step = 2.0 ** -133
+        wide = (down[0].double().abs().sum(1) + 1) @ up[0].double().abs().t().contiguous()
+        # (three terms of x and of t, and the smallest fp32 steps of the sums)
+        assert_within(torch, low_rank_add(y, x, bank, rows), want, bound + 2 * step * wide, f"{size}")
+
+
 @pytest.mark.parametrize("M", [1, 2, 40, 300, 5000, 8300])
 def test_non_finite_values_stay_in_their_rows(cuda, hiplib, M):
     """NaN and infinities in an adapter, an unloaded slot's memory, scale or a row of x reach only the rows that

@@ -51,7 +51,7 @@ def _low_rank(lib, y=P[0], ys=64, x=P[1], xs=64, rows=P[2], down=P[3], up=P[4], 
     (dict(y=None), -1), (dict(x=None), -1), (dict(rows=None), -1), (dict(down=None), -1), (dict(up=None), -1),
     (dict(scale=None), -1), (dict(rank=None), -1), (dict(out=None), -1),
     (dict(M=0), -2), (dict(K=0), -2), (dict(N=0), -2), (dict(slots=0), -2), (dict(R=0), -2), (dict(R=513), -2),
-    (dict(dtype=3), -2), (dict(M=-1), -2), (dict(slots=(1 << 20) + 1), -2), (dict(K=(1 << 20) + 1), -2), (dict(N=(1 << 20) + 1), -2), (dict(M=(1 << 28) + 1), -2),
+    (dict(dtype=3), -2), (dict(M=-1), -2), (dict(slots=(1 << 20) + 1), -2), (dict(K=(1 << 20) + 1), -2), (dict(N=(1 << 20) + 1), -2), (dict(M=(1 << 27) + 1), -2),
     (dict(ys=63), -3), (dict(xs=63), -3), (dict(os=63), -3), (dict(ys=1 << 60), -3),
     (dict(out=P[0] + 64), -3),                 # over y, but not y itself
     (dict(out=P[0], os=65), -3),               # y at another stride

@@ -74,7 +74,7 @@ int tsplat_low_rank_add_async(const float* y, int64_t y_stride, const float* x, 
   if (M <= 0 || K <= 0 || N <= 0 || slots <= 0 || slots > kMaxSlots || max_rank <= 0 || max_rank > kMaxRank) return kErrDims;
   if (dtype != kAdapterF32 && dtype != kAdapterBf16 && dtype != kAdapterF16) return kErrDims;
   // (the launches' grids hold these)
-  if (M > (1 << 28) || K > (1 << 20) || N > (1 << 20)) return kErrDims;
+  if (M > (1 << 27) || K > (1 << 20) || N > (1 << 20)) return kErrDims;
   const Rows ry{y, y_stride, M, N}, rx{x, x_stride, M, K}, ro{out, out_stride, M, N};
   if (!sane(ry) || !sane(rx) || !sane(ro)) return kErrRange;
   if ((!same(ro, ry) && !disjoint(ro, ry)) || !disjoint(ro, rx)) return kErrRange;

@@ -17,7 +17,7 @@ from ._lib import enqueue, load_library, no_gradients, rows_of
 # the library's limits
 MAX_RANK = 512
 MAX_SLOTS = MAX_FEATURES = 1 << 20
-MAX_ROWS = 1 << 28
+MAX_ROWS = 1 << 27
 
 
 def _types(torch):
@@ -165,7 +165,8 @@ def low_rank_add(y, x, bank, rows, *, out=None, library=None):
     stride (column ranges of wider rows pass); rows [M] int32, contiguous.  A row whose number is no loaded slot of
     the bank (negative, out of range, unloaded) keeps y.  out: None for a new tensor, y itself (rows without an
     adapter are not touched), or another that overlaps neither y nor x.  A row of x that
-    holds an infinity or NaN gives NaN; other rows are not affected.  Runs on torch's current stream; capturable into
+    holds an infinity or NaN gives NaN; other rows are not affected.  fp32 factors below 2^-110 count in steps of
+    2^-133.  Runs on torch's current stream; capturable into
     a HIP graph.  No gradients."""
     import torch
 
@@ -173,7 +174,7 @@ def low_rank_add(y, x, bank, rows, *, out=None, library=None):
         raise ValueError("low_rank_add needs an AdapterBank")
     M, y_stride = rows_of(torch, "y", y, bank.out_features)
     Mx, x_stride = rows_of(torch, "x", x, bank.in_features)
-    no_gradients(torch, y, x)
+    no_gradients(torch, y, x, out)
     if Mx != M or M > MAX_ROWS:
         raise ValueError(f"y has {M} rows, x has {Mx}: as many of both are wanted, at most {MAX_ROWS}")
     if not (isinstance(rows, torch.Tensor) and rows.dtype == torch.int32 and rows.numel() == M

@@ -189,7 +189,7 @@ def residual_norm(x, h, *, gate=None, residual_scale=1.0, post_norm=None, post_w
     C, B = shape[-1], shape[0] if len(shape) > 1 else 1
     M, x_stride = rows_of(torch, "x", x, C)
     _, h_stride = rows_of(torch, "h", h, C)
-    no_gradients(torch, x, h, gate, post_weight, post_bias, weight, bias, scale, shift)
+    no_gradients(torch, x, h, gate, post_weight, post_bias, weight, bias, scale, shift, out, normed)
     at = x.get_device()
     if post_norm is None and (post_weight is not None or post_bias is not None):
         raise ValueError("post_weight and post_bias belong to a post_norm")

@@ -306,16 +306,17 @@ class FlowModel:
         u = [1.0 - i / self.cfg.steps for i in range(self.cfg.steps + 1)]
         return [s * x / (1.0 + (s - 1.0) * x) for x in u]
 
-    def euler_cfg_step(self, z, cond, step=0, observe=None):
+    def euler_cfg_step(self, z, cond, step=0, observe=None, **request):
         """One sampler step with CFG: z [L, C], cond [Lc, C] -> (z_next, v).
-        observe: as in velocity(), over the CFG batch of 2."""
+        observe: as in velocity(), over the CFG batch of 2; request: its
+        adapters, slots (one for each of the pair), positions and rope."""
         torch = self.torch
         ts = self.schedule()
         t = torch.full((2,), ts[step] * 1000.0, dtype=torch.float32, device=self.device)
         dt = float(ts[step] - ts[step + 1])
         zz = torch.stack((z, z))
         cc = torch.stack((cond, torch.zeros_like(cond)))
-        v = self.velocity(zz, cc, t, observe=observe)
+        v = self.velocity(zz, cc, t, observe=observe, **request)
         v_cfg, z_next = v[0:1].clone(), z[None].clone()
         g = torch.full((1,), self.cfg.guidance, dtype=torch.float32, device=self.device)
         d = torch.full((1,), dt, dtype=torch.float32, device=self.device)

@@ -207,7 +207,7 @@ def _rope_call(torch, x, strides, parts, gamma0, gamma1, positions, rope, eps, B
             or places[-2] != L or places[-1] != rope.axes or batches not in (1, B)):
         raise ValueError(f"positions must be a contiguous [{L}, {rope.axes}] or [{B}, {L}, {rope.axes}] tensor of int32 "
                          "or fp32")
-    no_gradients(torch, x, positions, gamma0, gamma1)
+    no_gradients(torch, x, positions, gamma0, gamma1, *outs)
     if not eps >= 0.0:
         raise ValueError("eps must not be negative")
     if H > 1 << 16 or B * L >= 1 << 31:
