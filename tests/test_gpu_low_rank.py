@@ -46,7 +46,7 @@ def _check(torch, x, y, bank, adapters, rows, what):
 @pytest.mark.parametrize("M,K,N,R", [(1, 64, 64, 16), (1, 1, 1, 1), (2, 1024, 1024, 16), (3, 33, 17, 5), (16, 96, 80, 32),
                                      (17, 100, 50, 33), (33, 257, 130, 48), (63, 513, 65, 64), (64, 1024, 512, 128),
                                      (65, 40, 48, 100), (130, 64, 96, 7), (257, 130, 129, 24), (1030, 192, 160, 17),
-                                     (16, 4096, 64, 40), (7, 2050, 6144, 20), (40, 31, 33, 512), (4200, 70, 90, 12),
+                                     (16, 4096, 64, 40), (7, 2050, 6144, 20), (40, 31, 33, 512), (4200, 70, 90, 12), (4300, 200, 72, 100), (4130, 96, 50, 140),
                                      (9000, 64, 64, 16), (5, 64, 64, 260)])
 def test_one_adapter(cuda, hiplib, M, K, N, R, dtype):
     import torch
@@ -58,7 +58,8 @@ def test_one_adapter(cuda, hiplib, M, K, N, R, dtype):
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("M,K,N,R,slots", [(64, 256, 192, 16, 64), (64, 256, 192, 32, 5), (300, 128, 160, 24, 7),
-                                           (1100, 96, 64, 40, 3), (5000, 96, 80, 16, 9), (9100, 64, 48, 20, 30)])
+                                           (1100, 96, 64, 40, 3), (5000, 96, 80, 16, 9), (9100, 64, 48, 20, 30),
+                                           (4600, 130, 70, 128, 6)])
 @pytest.mark.parametrize("order", ["requests", "every row another"])
 def test_many_adapters(cuda, hiplib, M, K, N, R, slots, order, dtype):
     """Ranks from 0 (an empty slot) to R, rows without an adapter and rows of numbers that are no slots."""

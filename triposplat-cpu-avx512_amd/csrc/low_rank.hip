@@ -563,6 +563,11 @@ void launch_down(const LowRankParams& p, const Plan& pl, hipStream_t stream) {
         <<<dim3(m_blocks, blocks * pl.splits, pl.down_passes), kDownWaves * 64, 0, stream>>>(p, blocks, pl.splits,
                                                                                             pl.down_passes);
   };
+  // Ranks past 64 in one workgroup, which then reads x once: 16384 x 1024, rank 128, bf16 38 -> 26 us, fp16 52 -> 42.
+  // Not with fewer rows (fp16 45 -> 53) nor fp32's three planes, whose 96 registers for eight tiles are too many.
+  if constexpr (RT == 2 && DTYPE != kAdapterF32) {
+    if (tiles > 4) return run(std::integral_constant<int, 8>{});
+  }
   if (tiles == 1)
     run(std::integral_constant<int, 1>{});
   else if (tiles == 2)
