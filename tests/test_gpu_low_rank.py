@@ -46,7 +46,7 @@ def _check(torch, x, y, bank, adapters, rows, what):
 @pytest.mark.parametrize("M,K,N,R", [(1, 64, 64, 16), (1, 1, 1, 1), (2, 1024, 1024, 16), (3, 33, 17, 5), (16, 96, 80, 32),
                                      (17, 100, 50, 33), (33, 257, 130, 48), (63, 513, 65, 64), (64, 1024, 512, 128),
                                      (65, 40, 48, 100), (130, 64, 96, 7), (257, 130, 129, 24), (1030, 192, 160, 17),
-                                     (16, 4096, 64, 40), (7, 2050, 6144, 20), (40, 31, 33, 512), (4200, 70, 90, 12), (4300, 200, 72, 100), (4130, 96, 50, 140),
+                                     (16, 4096, 64, 40), (7, 2050, 6144, 20), (40, 31, 33, 512), (4200, 70, 90, 12), (4300, 200, 72, 100), (4130, 96, 50, 140), (2050, 1100, 70, 90), (2500, 64, 40, 200), (700, 1600, 300, 129),
                                      (9000, 64, 64, 16), (5, 64, 64, 260)])
 def test_one_adapter(cuda, hiplib, M, K, N, R, dtype):
     import torch

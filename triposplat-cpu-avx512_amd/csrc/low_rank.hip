@@ -524,15 +524,6 @@ __global__ __launch_bounds__(W * 64) void low_rank_few_kernel(LowRankParams p, i
   }
 }
 
-// Row tiles a workgroup of the first kernel, the parts that it splits K into, and the workgroups that share a tile's
-// adapters.  Few rows leave the chip idle without the last two: 64 rows of an adapter each, K 1024 -> N 6144, rank 32,
-// take 68 + 17 us with one workgroup a tile, 6.8 + 8.1 with 16 and 8.  Many rows: two row tiles, so that an adapter's
-// values are read half as often (12294 x 1024, rank 16: 15.3 us against 16.9; four: 15.6, and 20 where requests meet,
-// since a workgroup that fills a compute unit by itself then ends last).
-struct Plan {
-  int row_tiles, splits, down_passes, up_passes;
-};
-
 // Whether both products go in one launch: where a column block's own sums are little work, and not many of them.  16
 // rows of 16 adapters, 1024 -> 1024, rank 16: 7.1 us against 9.4; 64 rows of 64: 8.5 against 9.3; but 64 rows of 64,
 // 1024 -> 6144, rank 32: 32 against 15, and 2 rows, 4096 -> 1024, rank 64: 37 against 13.
@@ -542,35 +533,52 @@ bool few_rows(int M, int K, int N, int R) {
 constexpr int kFewTiles = 2, kFewWaves = 8;
 constexpr int kDownWaves = 8, kUpWaves = 4;
 
-Plan plan_of(int M, int K, int N, int slots, int R) {
-  Plan pl{M > 4096 ? 2 : 1, 1, 1, 1};
-  if (M <= 4096) {
-    const int tiles = ceil_div(M, 16), most = std::min({16, M, slots});
-    pl.splits = std::max(1, std::min({256 / tiles, ceil_div(K, 32) / (2 * kDownWaves), 8}));
-    pl.down_passes = std::max(1, std::min(1024 / tiles, most));
-    pl.up_passes = std::max(1, std::min(1024 / (tiles * ceil_div(N, 64 * kUpWaves)), most));
+// Row and rank tiles a workgroup of the first kernel, the parts that it splits K into, and the workgroups that share a
+// row tile's adapters.
+//   - Two row tiles where there are enough for that, so that an adapter's values are read half as often (12294 x 1024,
+//     rank 16: 15.3 us against 16.9; four: 15.6, and 20 where requests meet, since a workgroup that fills a compute
+//     unit by itself then ends last); with large ranks sooner (4000 x 4096, rank 128 in fp32, both products: 78 us
+//     against 99; rank 64, K 1024 in bf16: 51 against 48; 2000 rows: 61 against 47).
+//   - Eight rank tiles, which read x once, only there and not for fp32's three planes, whose 96 registers are too many
+//     (16384 x 1024, rank 128: bf16 38 -> 26 us, fp16 52 -> 42; one row tile: fp16 45 -> 53).
+//   - Few rows leave the chip idle without the last two: 64 rows of an adapter each, K 1024 -> N 6144, rank 32, take 68
+//     + 17 us with one workgroup a tile, 6.8 + 8.1 with 16 and 8.  Parts of K past that cost the second kernel more
+//     (1000 x 4096 x 4096, rank 128: two parts 44 us, four 57).
+struct Plan {
+  int row_tiles, rank_tiles, splits, down_passes, up_passes;
+};
+
+Plan plan_of(int M, int K, int N, int slots, int R, int dtype) {
+  const int tiles = ceil_div(R, 16), most = std::min({16, M, slots});
+  Plan pl{M > 4096 || (M > 2048 && R > 64) ? 2 : 1, 4, 1, 1, 1};
+  if (tiles <= 2)
+    pl.rank_tiles = tiles;
+  else if (tiles > 4 && pl.row_tiles == 2 && dtype != kAdapterF32)
+    pl.rank_tiles = 8;
+  const int workgroups = ceil_div(M, 16 * pl.row_tiles) * ceil_div(tiles, pl.rank_tiles);
+  if (M <= 4096) pl.splits = std::max(1, std::min({256 / workgroups, ceil_div(K, 32) / (2 * kDownWaves), 8}));
+  if (pl.row_tiles == 1) {
+    pl.down_passes = std::max(1, std::min(1024 / (workgroups * pl.splits), most));
+    pl.up_passes = std::max(1, std::min(1024 / (ceil_div(M, 16) * ceil_div(N, 64 * kUpWaves)), most));
   }
   return pl;
 }
 
 template <int DTYPE, int RT>
 void launch_down(const LowRankParams& p, const Plan& pl, hipStream_t stream) {
-  const int tiles = ceil_div(p.R, 16), m_blocks = ceil_div(p.M, 16 * RT);
   auto run = [&](auto rb) {
     constexpr int RB = decltype(rb)::value;
-    const int blocks = ceil_div(tiles, RB);
+    const int blocks = ceil_div(ceil_div(p.R, 16), RB);
     low_rank_down_kernel<DTYPE, RT, RB, kDownWaves>
-        <<<dim3(m_blocks, blocks * pl.splits, pl.down_passes), kDownWaves * 64, 0, stream>>>(p, blocks, pl.splits,
-                                                                                            pl.down_passes);
+        <<<dim3(ceil_div(p.M, 16 * RT), blocks * pl.splits, pl.down_passes), kDownWaves * 64, 0, stream>>>(
+            p, blocks, pl.splits, pl.down_passes);
   };
-  // Ranks past 64 in one workgroup, which then reads x once: 16384 x 1024, rank 128, bf16 38 -> 26 us, fp16 52 -> 42.
-  // Not with fewer rows (fp16 45 -> 53) nor fp32's three planes, whose 96 registers for eight tiles are too many.
   if constexpr (RT == 2 && DTYPE != kAdapterF32) {
-    if (tiles > 4) return run(std::integral_constant<int, 8>{});
+    if (pl.rank_tiles == 8) return run(std::integral_constant<int, 8>{});
   }
-  if (tiles == 1)
+  if (pl.rank_tiles == 1)
     run(std::integral_constant<int, 1>{});
-  else if (tiles == 2)
+  else if (pl.rank_tiles == 2)
     run(std::integral_constant<int, 2>{});
   else
     run(std::integral_constant<int, 4>{});
@@ -593,7 +601,7 @@ void launch_typed(const LowRankParams& p, hipStream_t stream) {
             p, passes);
     return;
   }
-  const Plan pl = plan_of(p.M, p.K, p.N, p.slots, p.R);
+  const Plan pl = plan_of(p.M, p.K, p.N, p.slots, p.R, DTYPE);
   if (pl.row_tiles == 1) {
     launch_down<DTYPE, 1>(p, pl, stream);
     launch_up<DTYPE, 4>(p, pl, stream);
@@ -605,9 +613,9 @@ void launch_typed(const LowRankParams& p, hipStream_t stream) {
 
 }  // namespace
 
-int64_t low_rank_scratch_bytes(int M, int K, int N, int slots, int R, int) {
+int64_t low_rank_scratch_bytes(int M, int K, int N, int slots, int R, int dtype) {
   if (few_rows(M, K, N, R)) return 0;
-  return 4 * (meta_floats(M) + (int64_t)plan_of(M, K, N, slots, R).splits * M * ceil_div(R, 16) * 16);
+  return 4 * (meta_floats(M) + (int64_t)plan_of(M, K, N, slots, R, dtype).splits * M * ceil_div(R, 16) * 16);
 }
 
 int launch_low_rank_add(const LowRankParams& p, hipStream_t stream) {
