@@ -221,6 +221,50 @@ def test_a_captured_block_of_requests(cuda, hiplib):
         low_rank_add(qkv, z.view(B * L, C), bank, rows)
 
 
+def test_two_threads_on_two_streams(cuda, hiplib):
+    """The operators keep nothing between calls: two host threads, each on a stream of its own, get what one gets."""
+    import threading
+
+    import torch
+    from tsplat import block_ops as bo
+    from tsplat.adapters import AdapterBank, low_rank_add
+    from tsplat.qkv import RopeAxes, rope_axes
+
+    def inputs(seed):
+        g = torch.Generator(device=cuda).manual_seed(seed)
+        r = lambda *s: torch.randn(*s, generator=g, device=cuda)  # noqa: E731
+        bank = AdapterBank.stack(r(3, 40, 256).half(), r(3, 256, 40).half(), [1.0, 0.5, 2.0])
+        rows = torch.randint(-1, 3, (900,), generator=g, device=cuda, dtype=torch.int32)
+        pos = torch.randint(0, 99, (900, 2), generator=g, device=cuda, dtype=torch.int32)
+        return r(900, 256), r(900, 256), bank, rows, pos, RopeAxes(64, [16, 16], device=cuda)
+
+    def step(x, y, bank, rows, pos, rope):
+        a = low_rank_add(y, x, bank, rows)
+        b, c = bo.residual_norm(x, a, norm="rms")
+        return a, b, c, rope_axes(c.view(1, 900, 4, 64), pos, rope)
+
+    sets = [inputs(s) for s in (1, 2)]
+    wants = [step(*s) for s in sets]
+    torch.cuda.synchronize(cuda)
+    wrong = []
+
+    def work(i):
+        stream = torch.cuda.Stream(device=cuda)
+        with torch.cuda.stream(stream):
+            for n in range(40):
+                got = step(*sets[i])
+                stream.synchronize()
+                if not all(torch.equal(p, q) for p, q in zip(got, wants[i])):
+                    wrong.append((i, n))
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong, wrong
+
+
 def test_refusals(cuda, hiplib):
     import torch
     from tsplat.flow_requests import FlowAdapters
