@@ -185,6 +185,34 @@ def test_non_finite_vectors_stay_alone(cuda, hiplib):
     assert got[0, ~keep].isnan().any(-1).all()
 
 
+def test_a_nan_is_its_vectors(cuda, hiplib):
+    """A NaN makes its vector's norm one, and so the whole normed vector, as max(||y||, eps) of the formula does."""
+    import torch
+    from tsplat.qkv import RopeAxes, rope_axes
+
+    for D in (6, 64, 72, 512):
+        x = torch.randn(1, 9, 2, D, device=cuda)
+        x[0, 3, 1, 5] = float("nan")
+        pos = torch.arange(9, dtype=torch.int32, device=cuda)[:, None]
+        got = rope_axes(x, pos, RopeAxes(D, [D // 2], device=cuda), gamma=torch.ones(2, D, device=cuda))
+        assert got[0, 1, 3].isnan().all()
+        assert int(got.isnan().sum()) == D
+
+
+def test_more_tokens_than_a_grid_dimension(cuda, hiplib):
+    """Workgroups past 65535 along the tokens: the last tokens come out as in a call of their own."""
+    import torch
+    from tsplat.qkv import RopeAxes, rope_axes
+
+    L, D = 65536 * 4 + 9, 512  # four tokens a workgroup
+    x = torch.randn(1, L, 1, D, device=cuda)
+    pos = torch.arange(L, dtype=torch.int32, device=cuda)[:, None]
+    rope = RopeAxes(D, [D // 2], device=cuda)
+    got = rope_axes(x, pos, rope)
+    for a, b in ((0, 64), (65535 * 4 - 20, 65535 * 4 + 20), (L - 30, L)):
+        assert torch.equal(got[:, :, a:b], rope_axes(x[:, a:b], pos[a:b].contiguous(), rope))
+
+
 def test_graph_and_stream(cuda, hiplib):
     import torch
     from tsplat.qkv import RopeAxes, qkv_rope_axes

@@ -122,7 +122,8 @@ __global__ __launch_bounds__(kThreads) void rope_axes_kernel(RopeAxesParams p) {
           float q = 0.0f;
 #pragma unroll
           for (int e = 0; e < 4; ++e) q = fmaf(a[e], a[e], fmaf(c[e], c[e], q));
-          scale = root / fmaxf(sqrtf(group_sum<G>(q)), p.eps);
+          const float norm = sqrtf(group_sum<G>(q));
+          scale = root / (norm < p.eps ? p.eps : norm);  // (a NaN stays one, which fmaxf would hide from its neighbours)
         }
         floatx4 y0, y1;
 #pragma unroll
