@@ -273,6 +273,19 @@ def test_offsets_past_32_bits(cuda, hiplib):
     assert torch.equal(vy, want)
 
 
+def test_more_rows_than_a_grid_dimension(cuda, hiplib):
+    """Row tiles past 65535: the last rows come out as in a call of their own."""
+    import torch
+    from tsplat.adapters import low_rank_add
+
+    M = 65536 * 16 + 37
+    x, y, bank, _, g = _case(torch, cuda, M, 32, 16, 8, 3, "float16", seed=8)
+    rows = torch.randint(-1, 4, (M,), generator=g, device=cuda, dtype=torch.int32)
+    got = low_rank_add(y, x, bank, rows)
+    for a, b in ((0, 5000), (65535 * 16 - 2500, 65535 * 16 + 2500), (M - 5000, M)):  # (rows enough for the same split)
+        assert torch.equal(got[a:b], low_rank_add(y[a:b], x[a:b], bank, rows[a:b]))
+
+
 @pytest.mark.parametrize("M", [2, 600, 8300])
 def test_graphs_and_streams(cuda, hiplib, M):
     """Captured without an eager call before, two graphs replayed on two streams at once, and again with eager work

@@ -265,3 +265,16 @@ def test_refusals(cuda, hiplib):
     empty = torch.empty(2, 0, 8, device=cuda)
     out, normed = call(empty, empty.clone(), gate=gate)
     assert out.shape == normed.shape == (2, 0, 8)
+
+
+def test_more_rows_than_a_grid_dimension(cuda, hiplib):
+    """Workgroups past 2^20 in a grid's first dimension: the last rows come out as in a call of their own."""
+    import torch
+    from tsplat.block_ops import residual_norm as call
+
+    M, C = (1 << 22) + 11, 8  # four rows a workgroup
+    x, h = torch.randn(M, C, device=cuda), torch.randn(M, C, device=cuda)
+    out, normed = call(x, h, post_norm="rms", eps=1e-5)
+    for a, b in ((0, 9), ((1 << 22) - 30, (1 << 22) + 3), (M - 13, M)):
+        want = call(x[a:b], h[a:b], post_norm="rms", eps=1e-5)
+        assert torch.equal(out[a:b], want[0]) and torch.equal(normed[a:b], want[1])
