@@ -267,14 +267,28 @@ def test_refusals(cuda, hiplib):
     assert out.shape == normed.shape == (2, 0, 8)
 
 
-def test_more_rows_than_a_grid_dimension(cuda, hiplib):
-    """Workgroups past 2^20 in a grid's first dimension: the last rows come out as in a call of their own."""
+@pytest.mark.parametrize("C,share", [(8, 32), (130, 4)])
+def test_more_rows_than_a_grid_dimension(cuda, hiplib, C, share):
+    """Workgroups (of `share` rows) past 2^20 in a grid's first dimension: the last rows come out as in a call of
+    their own."""
     import torch
     from tsplat.block_ops import residual_norm as call
 
-    M, C = (1 << 22) + 11, 8  # four rows a workgroup
+    edge = share << 20
+    M = edge + 11
     x, h = torch.randn(M, C, device=cuda), torch.randn(M, C, device=cuda)
     out, normed = call(x, h, post_norm="rms", eps=1e-5)
-    for a, b in ((0, 9), ((1 << 22) - 30, (1 << 22) + 3), (M - 13, M)):
+    for a, b in ((0, 9), (edge - 30, edge + 3), (M - 13, M)):
         want = call(x[a:b], h[a:b], post_norm="rms", eps=1e-5)
         assert torch.equal(out[a:b], want[0]) and torch.equal(normed[a:b], want[1])
+
+
+@pytest.mark.parametrize("C", [1, 2, 5, 31, 32, 33, 48, 64, 66, 72, 100, 127, 128, 129])
+@pytest.mark.parametrize("L", [1, 7, 33, 1001])
+def test_narrow_rows(cuda, hiplib, C, L):
+    """Several rows a wave, some of a workgroup's missing."""
+    import torch
+
+    x, h, mod, vectors = _inputs(torch, cuda, 3, L, C, C + L)
+    for post, pre in (("rms", "layer"), ("layer", "rms"), (None, "layer")):
+        _check(torch, x, h, mod, vectors, post, pre, True, True, True, what=f"{post} {pre}")
