@@ -70,7 +70,9 @@ def rope(torch, x, positions, sections, theta, shared, interleaved, gamma, eps):
 
 def assert_within(torch, got, want, bound, what=""):
     assert got.shape == want.shape and torch.isfinite(got).all(), what
+    assert torch.isfinite(want).all() and torch.isfinite(bound).all(), what
     off = (got.double() - want).abs()
-    worst = float((off / bound).max()) if off.numel() else 0.0
+    # (a zero that is kept as it is has a bound of zero and is off by none: 0 / 0 is no fault)
+    worst = float(torch.where(off == 0, off, off / bound).max()) if off.numel() else 0.0
     print(f"{what}: {worst:.3f} of the bound", flush=True)
     assert worst <= 1.0, (what, worst)

@@ -57,6 +57,22 @@ def test_one_adapter(cuda, hiplib, M, K, N, R, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M,K,N,R,slots", [(7000, 64, 40, 20, 5), (6150, 70, 100, 100, 4), (5900, 90, 66, 140, 3),
+                                           (9000, 40, 4200, 12, 3), (5000, 40, 6800, 40, 3), (4500, 40, 7500, 70, 1),
+                                           (2700, 1100, 90, 130, 6), (300, 1100, 90, 60, 20)])
+def test_many_requests_in_every_layout(cuda, hiplib, M, K, N, R, slots, dtype):
+    """Requests of ragged lengths that meet inside row tiles, at each count of row, rank and column tiles."""
+    import torch
+
+    print(f"layouts M={M} K={K} N={N} R={R} slots={slots} {dtype}", flush=True)
+    ranks = [max(1, R - 13 * i) for i in range(slots)]
+    x, y, bank, adapters, g = _case(torch, cuda, M, K, N, R, slots, dtype, seed=M, ranks=ranks)
+    of_request = torch.randint(-1, slots + 1, (M,), generator=g, device=cuda, dtype=torch.int32)
+    starts = torch.rand(M, generator=g, device=cuda) < 0.05
+    _check(torch, x, y, bank, adapters, of_request[starts.cumsum(0)], "layouts")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("M,K,N,R,slots", [(64, 256, 192, 16, 64), (64, 256, 192, 32, 5), (300, 128, 160, 24, 7),
                                            (1100, 96, 64, 40, 3), (5000, 96, 80, 16, 9), (9100, 64, 48, 20, 30),
                                            (4600, 130, 70, 128, 6)])

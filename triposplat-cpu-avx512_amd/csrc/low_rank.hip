@@ -533,34 +533,45 @@ bool few_rows(int M, int K, int N, int R) {
 constexpr int kFewTiles = 2, kFewWaves = 8;
 constexpr int kDownWaves = 8, kUpWaves = 4;
 
-// Row and rank tiles a workgroup of the first kernel, the parts that it splits K into, and the workgroups that share a
-// row tile's adapters.
-//   - Two row tiles where there are enough for that, so that an adapter's values are read half as often (12294 x 1024,
-//     rank 16: 15.3 us against 16.9; four: 15.6, and 20 where requests meet, since a workgroup that fills a compute
-//     unit by itself then ends last); with large ranks sooner (4000 x 4096, rank 128 in fp32, both products: 78 us
-//     against 99; rank 64, K 1024 in bf16: 51 against 48; 2000 rows: 61 against 47).
+// Row and rank tiles a workgroup of the first kernel, the parts that it splits K into, the workgroups that share a row
+// tile's adapters, and the second kernel's column tiles a wave.
+//   - Two row tiles read an adapter's values half as often: 12294 x 1024, rank 16: 15.3 us against 16.9 (four: 15.6, and
+//     20 where requests meet, since a workgroup that fills a compute unit by itself then ends last).  But half as many
+//     workgroups go through twice as many adapters one after the other where requests meet: 4380 x 1181, rank 25, 222
+//     requests: 36 us, 22 with one; 2100 x 4096, rank 128 in fp32, 4 adapters: 56, 36 with one.  So a bank of one slot
+//     takes them sooner, and with large ranks sooner still (that call with one adapter: 45 us, one row tile 60; rank 64,
+//     4000 x 4096: 40, one 39).
 //   - Eight rank tiles, which read x once, only there and not for fp32's three planes, whose 96 registers are too many
 //     (16384 x 1024, rank 128: bf16 38 -> 26 us, fp16 52 -> 42; one row tile: fp16 45 -> 53).
-//   - Few rows leave the chip idle without the last two: 64 rows of an adapter each, K 1024 -> N 6144, rank 32, take 68
+//   - Few rows leave the chip idle without the next two: 64 rows of an adapter each, K 1024 -> N 6144, rank 32, take 68
 //     + 17 us with one workgroup a tile, 6.8 + 8.1 with 16 and 8.  Parts of K past that cost the second kernel more
 //     (1000 x 4096 x 4096, rank 128: two parts 44 us, four 57).
+//   - Eight column tiles read t and each adapter's border least, from where the waves come in many rounds (8202 x 6144:
+//     109 us, four 117; 12294 x 2900: 91, 98; but 14644 x 1743: 54, 49); two where there are fewer waves than three a
+//     compute unit (130 x 3000: 8.3 us, four 8.8; but 300 x 6000: 15.3, 14.2), unless many parts of K make each wave
+//     add up t again (336 rows, 3099 -> 1046, six parts: 18.2, four 13.3).
 struct Plan {
-  int row_tiles, rank_tiles, splits, down_passes, up_passes;
+  int row_tiles, rank_tiles, splits, down_passes, column_tiles, up_passes;
 };
 
 Plan plan_of(int M, int K, int N, int slots, int R, int dtype) {
-  const int tiles = ceil_div(R, 16), most = std::min({16, M, slots});
-  Plan pl{M > 4096 || (M > 2048 && R > 64) ? 2 : 1, 4, 1, 1, 1};
+  const int tiles = ceil_div(R, 16), most = std::min({16, M, slots}), row_tiles = ceil_div(M, 16);
+  Plan pl{1, 4, 1, 1, 4, 1};
+  if (slots > 1 ? M > 6144 : M > 4096 || (M > 2048 && R > 64)) pl.row_tiles = 2;
   if (tiles <= 2)
     pl.rank_tiles = tiles;
   else if (tiles > 4 && pl.row_tiles == 2 && dtype != kAdapterF32)
     pl.rank_tiles = 8;
   const int workgroups = ceil_div(M, 16 * pl.row_tiles) * ceil_div(tiles, pl.rank_tiles);
-  if (M <= 4096) pl.splits = std::max(1, std::min({256 / workgroups, ceil_div(K, 32) / (2 * kDownWaves), 8}));
-  if (pl.row_tiles == 1) {
-    pl.down_passes = std::max(1, std::min(1024 / (workgroups * pl.splits), most));
-    pl.up_passes = std::max(1, std::min(1024 / (ceil_div(M, 16) * ceil_div(N, 64 * kUpWaves)), most));
-  }
+  pl.splits = std::max(1, std::min({256 / workgroups, ceil_div(K, 32) / (2 * kDownWaves), 8}));
+  if (pl.row_tiles == 1) pl.down_passes = std::max(1, std::min(1024 / (workgroups * pl.splits), most));
+  const int64_t waves = (int64_t)row_tiles * ceil_div(N, 64);
+  if (waves < 768 && pl.splits <= 2)
+    pl.column_tiles = 2;
+  else if (waves >= 32768)
+    pl.column_tiles = 8;
+  const int64_t shares = (int64_t)row_tiles * ceil_div(N, 16 * pl.column_tiles * kUpWaves);
+  pl.up_passes = (int)std::max<int64_t>(1, std::min<int64_t>(1024 / shares, most));
   return pl;
 }
 
@@ -602,13 +613,16 @@ void launch_typed(const LowRankParams& p, hipStream_t stream) {
     return;
   }
   const Plan pl = plan_of(p.M, p.K, p.N, p.slots, p.R, DTYPE);
-  if (pl.row_tiles == 1) {
+  if (pl.row_tiles == 1)
     launch_down<DTYPE, 1>(p, pl, stream);
-    launch_up<DTYPE, 4>(p, pl, stream);
-  } else {
+  else
     launch_down<DTYPE, 2>(p, pl, stream);
+  if (pl.column_tiles == 2)
+    launch_up<DTYPE, 2>(p, pl, stream);
+  else if (pl.column_tiles == 4)
+    launch_up<DTYPE, 4>(p, pl, stream);
+  else
     launch_up<DTYPE, 8>(p, pl, stream);
-  }
 }
 
 }  // namespace
