@@ -22,13 +22,16 @@ typedef float floatx4u __attribute__((ext_vector_type(4), aligned(4)));  // vect
 constexpr int kTokenWaves = 4, kVectorWaves = 4, kThreads = kTokenWaves * kVectorWaves * 64;
 constexpr int kAhead = 2;  // vectors that a lane asks for at once (with one token wave 4: 107 us, 2: 112, 1: 94)
 
-// G lanes a vector, lane i of them its pairs 4 i .. 4 i + 3; a wave turns 64 / G tokens.  The workgroup computes its
-// tokens' sines and cosines once, into LDS, and a lane keeps its own while it goes through its share of the vectors.
+// G lanes a vector, lane i of them its pairs 4 i .. 4 i + 3; the last one with any takes the vector's last four, some of
+// which its neighbour has too and writes alike (28899 x 3 x 182: 40 us, 63 with single values there, which all lanes
+// wait for).  A wave turns 64 / G tokens.  The workgroup computes its tokens' sines and cosines once, into LDS, and a
+// lane keeps its own while it goes through its share of the vectors.  64 registers let two workgroups share a compute
+// unit (without that bound neighbours take 84: 1640 x 17 x 150, q, k and v, 35 us, so 26).
 template <int G, bool INTERLEAVED>
-__global__ __launch_bounds__(kThreads) void rope_axes_kernel(RopeAxesParams p) {
+__global__ __launch_bounds__(kThreads, 8) void rope_axes_kernel(RopeAxesParams p) {
   constexpr int kTokens = 64 / G, kAllTokens = kTokens * kTokenWaves;
   __shared__ float2 circle[kAllTokens * G * 4];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i0 = (lane % G) * 4;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t tokens = (int64_t)p.B * p.L;
   const int64_t token0 = ((int64_t)blockIdx.z * gridDim.y + blockIdx.y) * kAllTokens;
   const int64_t token = token0 + wave / kVectorWaves * kTokens + lane / G;
@@ -49,9 +52,11 @@ __global__ __launch_bounds__(kThreads) void rope_axes_kernel(RopeAxesParams p) {
     circle[t * G * 4 + pair] = v;
   }
   __syncthreads();
-  const int n = token < tokens ? min(4, pairs - i0) : 0;  // pairs of this lane
+  const int own = lane % G * 4, i0 = max(0, min(own, pairs - 4));
+  const int n = token < tokens && own < pairs ? min(4, pairs) : 0;  // pairs of this lane
+  const int twice = own - i0;                                       // the first ones of them, which a neighbour has too
   // (tokens are fewer than 2^31: a division of 32 bits takes a fifth of one of 64)
-  const uint32_t live = n > 0 ? (uint32_t)token : 0;
+  const uint32_t live = token < tokens ? (uint32_t)token : 0;
   const int64_t b = live / (uint32_t)p.L, l = live - (uint32_t)b * (uint32_t)p.L;
   float cs[4], sn[4];
 #pragma unroll
@@ -64,13 +69,14 @@ __global__ __launch_bounds__(kThreads) void rope_axes_kernel(RopeAxesParams p) {
   // element offsets of the pairs' first and second values: 8 neighbours, or 4 of each half
   const int j0 = INTERLEAVED ? 2 * i0 : i0, j1 = INTERLEAVED ? 2 * i0 + 4 : i0 + pairs;
   const float* src = p.x + b * p.batch_stride + l * p.token_stride;
-  const bool whole = n == 4;
+  const bool few = G == 1 && pairs < 4;
+  // (lanes without a token or pairs load others')
   auto load = [&](const float* v, floatx4& lo, floatx4& hi) {
-    lo = hi = floatx4{};
-    if (whole) {
+    if (!few) {
       lo = *reinterpret_cast<const floatx4u*>(v + j0);
       hi = *reinterpret_cast<const floatx4u*>(v + j1);
     } else {
+      lo = hi = floatx4{};
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         if (INTERLEAVED) {
@@ -84,7 +90,7 @@ __global__ __launch_bounds__(kThreads) void rope_axes_kernel(RopeAxesParams p) {
     }
   };
   auto store = [&](float* v, const floatx4& lo, const floatx4& hi) {
-    if (whole) {
+    if (!few) {
       *reinterpret_cast<floatx4u*>(v + j0) = lo;
       *reinterpret_cast<floatx4u*>(v + j1) = hi;
     } else {
@@ -121,7 +127,11 @@ __global__ __launch_bounds__(kThreads) void rope_axes_kernel(RopeAxesParams p) {
           load(gamma + (int64_t)h * p.D, g0, g1);
           float q = 0.0f;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) q = fmaf(a[e], a[e], fmaf(c[e], c[e], q));
+          for (int e = 0; e < 4; ++e) {
+            const float re = INTERLEAVED ? (e < 2 ? a[2 * e] : c[2 * e - 4]) : a[e];
+            const float im = INTERLEAVED ? (e < 2 ? a[2 * e + 1] : c[2 * e - 3]) : c[e];
+            q += e < twice ? 0.0f : fmaf(re, re, im * im);
+          }
           const float norm = sqrtf(group_sum<G>(q));
           scale = root / (norm < p.eps ? p.eps : norm);  // (a NaN stays one, which fmaxf would hide from its neighbours)
         }
