@@ -23,7 +23,7 @@ constexpr int kTokenWaves = 4, kVectorWaves = 4, kThreads = kTokenWaves * kVecto
 constexpr int kAhead = 2;  // vectors that a lane asks for at once (with one token wave 4: 107 us, 2: 112, 1: 94)
 
 // G lanes a vector, lane i of them its pairs 4 i .. 4 i + 3; the last one with any takes the vector's last four, some of
-// which its neighbour has too and writes alike (28899 x 3 x 182: 40 us, 63 with single values there, which all lanes
+// which its neighbour has too and writes alike (28899 x 3 x 182: 38 us, 63 with single values there, which all lanes
 // wait for).  A wave turns 64 / G tokens.  The workgroup computes its tokens' sines and cosines once, into LDS, and a
 // lane keeps its own while it goes through its share of the vectors.  64 registers let two workgroups share a compute
 // unit (without that bound neighbours take 84: 1640 x 17 x 150, q, k and v, 35 us, so 26).
@@ -31,7 +31,8 @@ template <int G, bool INTERLEAVED>
 __global__ __launch_bounds__(kThreads, 8) void rope_axes_kernel(RopeAxesParams p) {
   constexpr int kTokens = 64 / G, kAllTokens = kTokens * kTokenWaves;
   __shared__ float2 circle[kAllTokens * G * 4];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  // (the wave's number as a scalar, so that what follows from it is one too)
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t tokens = (int64_t)p.B * p.L;
   const int64_t token0 = ((int64_t)blockIdx.z * gridDim.y + blockIdx.y) * kAllTokens;
   const int64_t token = token0 + wave / kVectorWaves * kTokens + lane / G;
@@ -57,7 +58,7 @@ __global__ __launch_bounds__(kThreads, 8) void rope_axes_kernel(RopeAxesParams p
   const int twice = own - i0;                                       // the first ones of them, which a neighbour has too
   // (tokens are fewer than 2^31: a division of 32 bits takes a fifth of one of 64)
   const uint32_t live = token < tokens ? (uint32_t)token : 0;
-  const int64_t b = live / (uint32_t)p.L, l = live - (uint32_t)b * (uint32_t)p.L;
+  const uint32_t b = live / (uint32_t)p.L, l = live - b * (uint32_t)p.L;
   float cs[4], sn[4];
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
@@ -69,6 +70,8 @@ __global__ __launch_bounds__(kThreads, 8) void rope_axes_kernel(RopeAxesParams p
   // element offsets of the pairs' first and second values: 8 neighbours, or 4 of each half
   const int j0 = INTERLEAVED ? 2 * i0 : i0, j1 = INTERLEAVED ? 2 * i0 + 4 : i0 + pairs;
   const float* src = p.x + b * p.batch_stride + l * p.token_stride;
+  const int64_t dst = (p.out_bhld ? (int64_t)b * p.H * p.L + l : (int64_t)live * p.H) * p.D;
+  const int64_t dst_head = (p.out_bhld ? (int64_t)p.L : 1) * p.D;
   const bool few = G == 1 && pairs < 4;
   // (lanes without a token or pairs load others')
   auto load = [&](const float* v, floatx4& lo, floatx4& hi) {
@@ -157,7 +160,7 @@ __global__ __launch_bounds__(kThreads, 8) void rope_axes_kernel(RopeAxesParams p
         a = y0;
         c = y1;
       }
-      if (n > 0) store(p.out[part] + (p.out_bhld ? (b * p.H + h) * p.L + l : (b * p.L + l) * p.H + h) * p.D, a, c);
+      if (n > 0) store(p.out[part] + h * dst_head + dst, a, c);
     }
   }
 }
