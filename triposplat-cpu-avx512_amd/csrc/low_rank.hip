@@ -185,7 +185,7 @@ struct DownTile {
   __device__ __forceinline__ void run(const LowRankParams& p, const DownRange& r, int64_t row0, Wt (&w)[RB],
                                       const char* down, int64_t tile_bytes, int tiles, float scale, uint64_t mask,
                                       floatx4 (*sums)[W][64]) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, q = lane >> 4;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), q = lane >> 4;
     const int t_stride = ceil_div(p.R, 16) * 16;
     floatx4 acc[RT][RB] = {};
     for (int s = r.s_begin; s < r.s_end; ++s) {
@@ -232,7 +232,7 @@ __global__ __launch_bounds__(W * 64) void low_rank_down_kernel(LowRankParams p, 
                                                                int passes) {
   using Wt = Weights<DTYPE>;
   __shared__ floatx4 sums[DownTile<DTYPE, RT, RB, W>::kRound][W][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t row0 = (int64_t)blockIdx.x * (RT * 16);
   const int k_tiles = ceil_div(p.K, 32), r_tiles = ceil_div(p.R, 16), share = ceil_div(k_tiles, splits * W);
   DownRange r;
@@ -240,9 +240,9 @@ __global__ __launch_bounds__(W * 64) void low_rank_down_kernel(LowRankParams p, 
   r.part = (int)(blockIdx.y / rank_blocks);
   r.s_begin = (r.part * W + wave) * share;
   r.s_end = min(k_tiles, r.s_begin + share);
-  // x is on its way before its rows' adapters are known; passes after the first may have none
+  // x is on its way before its rows' adapters are known; a pass that may have none waits
   DownTile<DTYPE, RT, RB, W> all;
-  bool held = blockIdx.z == 0;
+  bool held = RT == 1 ? blockIdx.z == 0 : (int)blockIdx.z == passes - 1;
   if (held && r.s_begin < r.s_end) all.load_x(p, row0, r.s_begin);
   int id = lane < RT * 16 && row0 + lane < p.M ? p.rows[row0 + lane] : -1;
   if (id >= p.slots) id = -1;
@@ -283,10 +283,12 @@ __global__ __launch_bounds__(W * 64) void low_rank_down_kernel(LowRankParams p, 
   if constexpr (RT == 1) {
     each_adapter(id, ~0ull, passes, adapter);
   } else {
-    // the middle row's adapter has the most rows of a border tile: it goes first, through all row tiles at once
+    // The middle row's adapter has the most rows of a border tile: it goes through all row tiles at once.  The others,
+    // where a pass of their own is asked for, go before: most of its workgroups end at once, and those of a border start
+    // early, where one workgroup would take twice its time and end last.
     const int middle = __builtin_amdgcn_readlane(id, RT * 8);
-    if (middle >= 0) adapter(middle, RT * 8, __ballot(id == middle));
-    each_adapter(id == middle ? -1 : id, ~0ull, 1, adapter);
+    if (held && middle >= 0) adapter(middle, RT * 8, __ballot(id == middle));
+    if (blockIdx.z == 0) each_adapter(id == middle ? -1 : id, ~0ull, 1, adapter);
   }
   if (blockIdx.y == 0 && blockIdx.z == 0 && wave == 0 && lane < RT * 16 && row0 + lane < p.M)
     reinterpret_cast<int*>(p.scratch)[row0 + lane] = row_rank > 0 ? row_rank << kIdBits | id : -1;
@@ -299,7 +301,7 @@ __global__ __launch_bounds__(W * 64) void low_rank_down_kernel(LowRankParams p, 
 template <int DTYPE, int NT, int W>
 __global__ __launch_bounds__(W * 64) void low_rank_up_kernel(LowRankParams p, int splits, int passes) {
   using Wt = Weights<DTYPE>;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, q = lane >> 4;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), q = lane >> 4;
   const int64_t row0 = (blockIdx.y + (passes == 1 ? (int64_t)blockIdx.z * gridDim.y : 0)) * 16;
   const int tile0 = (int)(blockIdx.x * W + wave) * NT;
   const int n_tiles = ceil_div(p.N, 16), r_steps = ceil_div(p.R, 32), t_stride = ceil_div(p.R, 16) * 16;
@@ -416,7 +418,7 @@ __global__ __launch_bounds__(W * 64) void low_rank_few_kernel(LowRankParams p, i
   constexpr int kInner = 32 + 4;  // floats a row in LDS: 16-byte reads of neighbouring rows in other banks
   __shared__ floatx4 sums[2][W][64];
   __shared__ __attribute__((aligned(16))) float inner[16 * kInner];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, q = lane >> 4;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), q = lane >> 4;
   const int64_t row0 = (int64_t)blockIdx.y * 16, m = row0 + (lane & 15);
   const int k_tiles = ceil_div(p.K, 32), r_tiles = ceil_div(p.R, 16);
   const int n_tiles = ceil_div(p.N, 16), tile0 = (int)(blockIdx.x * W + wave) * NT;
@@ -532,6 +534,7 @@ bool few_rows(int M, int K, int N, int R) {
 }
 constexpr int kFewTiles = 2, kFewWaves = 8;
 constexpr int kDownWaves = 8, kUpWaves = 4;
+constexpr int kUnits = 256;  // compute units
 
 // Row and rank tiles a workgroup of the first kernel, the parts that it splits K into, the workgroups that share a row
 // tile's adapters, and the second kernel's column tiles a wave.
@@ -541,6 +544,9 @@ constexpr int kDownWaves = 8, kUpWaves = 4;
 //     requests: 36 us, 22 with one; 2100 x 4096, rank 128 in fp32, 4 adapters: 56, 36 with one.  So a bank of one slot
 //     takes them sooner, and with large ranks sooner still (that call with one adapter: 45 us, one row tile 60; rank 64,
 //     4000 x 4096: 40, one 39).
+//   - With two row tiles the border between requests in a pass of its own: 7000 x 4096, rank 64, 2 to 6 adapters: 70-90 us
+//     -> 55-73; 12294 x 1024: 48-57 -> 44-53.  Not where the last round of workgroups is full and one more starts
+//     another (16384 x 4096, 2 adapters: 148 -> 157).
 //   - Eight rank tiles, which read x once, only there and not for fp32's three planes, whose 96 registers are too many
 //     (16384 x 1024, rank 128: bf16 38 -> 26 us, fp16 52 -> 42; one row tile: fp16 45 -> 53).
 //   - Few rows leave the chip idle without the next two: 64 rows of an adapter each, K 1024 -> N 6144, rank 32, take 68
@@ -563,8 +569,11 @@ Plan plan_of(int M, int K, int N, int slots, int R, int dtype) {
   else if (tiles > 4 && pl.row_tiles == 2 && dtype != kAdapterF32)
     pl.rank_tiles = 8;
   const int workgroups = ceil_div(M, 16 * pl.row_tiles) * ceil_div(tiles, pl.rank_tiles);
-  pl.splits = std::max(1, std::min({256 / workgroups, ceil_div(K, 32) / (2 * kDownWaves), 8}));
-  if (pl.row_tiles == 1) pl.down_passes = std::max(1, std::min(1024 / (workgroups * pl.splits), most));
+  pl.splits = std::max(1, std::min({kUnits / workgroups, ceil_div(K, 32) / (2 * kDownWaves), 8}));
+  if (pl.row_tiles == 1)
+    pl.down_passes = std::max(1, std::min(1024 / (workgroups * pl.splits), most));
+  else if (slots > 1 && (workgroups - 1) % kUnits < kUnits * 7 / 8)
+    pl.down_passes = 2;
   const int64_t waves = (int64_t)row_tiles * ceil_div(N, 64);
   if (waves < 768 && pl.splits <= 2)
     pl.column_tiles = 2;
