@@ -6,8 +6,8 @@
 // (8 + 8 + 8 bits, split by truncation, so exactly and without overflow), a bf16 weight one, an fp16 weight two, an
 // fp32 weight three; the products below 2^-23 of the whole are left out.
 //
-// What bounds it: 12294 x 1024 -> 4096, rank 16, HBM: 453 MB in 91-93 us (4.9 TB/s; x 15, y 76).  16384 x 4096 -> 1024,
-// rank 64 in fp32 (402 MB, 79 us at a copy's rate): 119 us for one adapter, 143 where two requests meet; every 32 rows
+// What bounds it: 12294 x 1024 -> 4096, rank 16, HBM: 453 MB in 90-92 us (5.0 TB/s; x 15, y 74).  16384 x 4096 -> 1024,
+// rank 64 in fp32 (402 MB, 79 us at a copy's rate): 119 us for one adapter, 147 where two requests meet; every 32 rows
 // read the adapter's 1.5 MB from L2, 1.05 GB at 11 TB/s, and the border tile's second adapter ends last.  Adapter values
 // staged in LDS for 64 or 128 rows were slower or no faster: a barrier a step of K, and t in parts.
 //

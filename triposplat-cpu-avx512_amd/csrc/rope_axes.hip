@@ -17,7 +17,7 @@ namespace {
 typedef float floatx4u __attribute__((ext_vector_type(4), aligned(4)));  // vectors start at any float
 
 // A workgroup: kTokenWaves waves along the tokens, each with kVectorWaves shares of their parts' heads.  16384 tokens x
-// 16 x 64, q, k and v: 89 us, 4.5 TB/s (a copy of as much: 73-79); one token wave with 4 shares 94-110 (writes of 2 KiB
+// 16 x 64, q, k and v: 87 us, 4.6 TB/s (a copy of as much: 73-79); one token wave with 4 shares 94-110 (writes of 2 KiB
 // a head instead of 8).
 constexpr int kTokenWaves = 4, kVectorWaves = 4, kThreads = kTokenWaves * kVectorWaves * 64;
 constexpr int kAhead = 2;  // vectors that a lane asks for at once (with one token wave 4: 107 us, 2: 112, 1: 94)
