@@ -66,8 +66,8 @@ int tsplat_residual_norm_async(const float* x, int64_t x_stride, const float* h,
  * [H, D], become y * sqrt(D) / max(||y||, eps) * gamma.  Part 2 (v) is copied.  A pair is (2p, 2p + 1) with
  * interleaved, else (p, p + D/2).
  * positions: [position_batches][L][axes], position_batches 1 or B, int32 (position_type 0) or fp32 (1); an axis[p]
- * outside [0, axes) counts as 0.  axes 1..8; D even, 2..512; H up to 2^16, B * L below 2^31.  The outputs must not overlap each other or the
- * memory that x spans (-3). */
+ * outside [0, axes) counts as 0.  axes 1..8; D even, 2..512; H up to 2^16, B * L below 2^31.  The outputs must not
+ * overlap each other, the memory that x spans or anything else that is read (-3). */
 int tsplat_rope_axes_async(const float* x, int64_t part_stride, int64_t batch_stride, int64_t token_stride,
                            int64_t head_stride, int parts, const float* gamma0, const float* gamma1,
                            float* out0, float* out1, float* out2, const void* positions, int position_type,

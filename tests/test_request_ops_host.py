@@ -114,6 +114,24 @@ def test_rope_refusals(lib, change, status):
     assert _rope(lib, **change) == status
 
 
+@pytest.mark.parametrize("change", [
+    dict(g0=P[1] + 2044), dict(g0=P[1] - 508), dict(pos=P[1]), dict(pos=P[1] - 28), dict(turns=P[1] + 2040),
+    dict(turns=P[1] - 248), dict(axis=P[1] + 1024), dict(axis=P[1] - 124),
+    dict(parts=2, ps=512, o1=P[2], g1=P[2]), dict(parts=2, ps=512, o1=P[2], pos=P[2] + 2044),
+    dict(parts=3, ps=512, o1=P[2], o2=P[3], g0=P[3] - 508)])
+def test_rope_outputs_over_what_is_read(lib, change):
+    """An output of 2048 bytes over one value of a gamma (512 bytes), the positions (32), turns (256) or axis (128)."""
+    assert _rope(lib, **change) == -3
+
+
+@pytest.mark.parametrize("change", [dict(g0=P[1] + 2048), dict(g0=P[1] - 512), dict(pos=P[1] - 32),
+                                    dict(turns=P[1] - 256), dict(axis=P[1] - 128), dict(g1=P[1])])
+def test_rope_outputs_beside_what_is_read(lib, change):
+    """Up to its edges an output is taken (a gamma of a part that the call lacks is not read): only the memory itself,
+    which is none of a device, is refused."""
+    assert _rope(lib, **change) in (-6, -7)
+
+
 def test_host_memory_is_refused(lib):
     """Pointers that are no device memory are -6 (or a failed query of them), never a launch."""
     assert _low_rank(lib) in (-6, -7)

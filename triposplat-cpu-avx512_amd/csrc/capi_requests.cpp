@@ -41,6 +41,9 @@ bool sane(const Rows& r) {
   return r.rows == 1 || (r.stride >= r.cols && r.stride <= (INT64_C(1) << 60) / r.rows);
 }
 
+// Values in a row, `floats` of 4 bytes.
+Rows whole(const void* p, int64_t floats) { return {static_cast<const float*>(p), floats, 1, floats}; }
+
 bool same(const Rows& a, const Rows& b) { return a.p == b.p && (a.rows == 1 || a.stride == b.stride); }
 
 // Whether no element belongs to both: apart as a whole, or column ranges of the same wider rows.
@@ -176,25 +179,25 @@ int tsplat_rope_axes_async(const float* x, int64_t part_stride, int64_t batch_st
   const int64_t in_last = (int64_t)last;
   float* outs[3] = {out0, parts > 1 ? out1 : nullptr, parts > 2 ? out2 : nullptr};
   const Rows in{x, in_last, 1, in_last};
-  const int64_t values = tokens * H * D;
+  const int64_t values = tokens * H * D, places = position_batches * (int64_t)L * axes;
+  // all that is read, in floats
+  const Rows reads[] = {in, whole(gamma0, (int64_t)H * D), whole(parts > 1 ? gamma1 : nullptr, (int64_t)H * D),
+                        whole(positions, places), whole(turns, D), whole(axis, D / 2)};
   if (!aligned4(x) || !aligned4(positions) || !aligned4(axis) || (reinterpret_cast<uintptr_t>(turns) & 7u) ||
       !aligned4(gamma0) || !aligned4(gamma1))
     return kErrAlign;
   for (int i = 0; i < parts; ++i) {
     const Rows o{outs[i], values, 1, values};
     if (!aligned4(outs[i])) return kErrAlign;
-    if (!disjoint(o, in)) return kErrRange;
+    for (const Rows& r : reads)
+      if (r.p && !disjoint(o, r)) return kErrRange;
     for (int j = 0; j < i; ++j)
       if (!disjoint(o, Rows{outs[j], values, 1, values})) return kErrRange;
   }
   DeviceRanges ptrs;
-  TSPLAT_CHECK(ptrs.check(x, in.bytes()));
   for (int i = 0; i < parts; ++i) TSPLAT_CHECK(ptrs.check(outs[i], values * 4));
-  if (gamma0) TSPLAT_CHECK(ptrs.check(gamma0, (int64_t)H * D * 4));
-  if (gamma1 && parts > 1) TSPLAT_CHECK(ptrs.check(gamma1, (int64_t)H * D * 4));
-  TSPLAT_CHECK(ptrs.check(positions, (int64_t)position_batches * L * axes * 4));
-  TSPLAT_CHECK(ptrs.check(turns, (int64_t)(D / 2) * 8));
-  TSPLAT_CHECK(ptrs.check(axis, (int64_t)(D / 2) * 4));
+  for (const Rows& r : reads)
+    if (r.p) TSPLAT_CHECK(ptrs.check(r.p, r.bytes()));
   RopeAxesParams p{x, part_stride, batch_stride, token_stride, head_stride, parts, {gamma0, gamma1},
                    {outs[0], outs[1], outs[2]}, positions, position_type, position_batches, axes, turns, axis,
                    interleaved ? 1 : 0, eps, B, L, H, D, out_bhld ? 1 : 0};

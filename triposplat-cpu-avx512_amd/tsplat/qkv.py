@@ -228,7 +228,8 @@ def rope_axes(x, positions, rope, *, gamma=None, eps=1.0e-12, out=None, out_bhld
 
     x: fp32 on the GPU, any strides that do not overlap, unit in D (a view into a projection's rows).  positions:
     [L, axes] or [B, L, axes], int32 or fp32 (fractional places); an angle is taken in 64 bits, so far positions
-    keep their precision.  rope: RopeAxes.  out may not lie in the memory that x spans.  No gradients."""
+    keep their precision.  rope: RopeAxes.  out may not lie in the memory that x spans, nor over anything else that is
+    read.  No gradients."""
     import torch
 
     if not (isinstance(x, torch.Tensor) and x.is_cuda and x.dtype == torch.float32 and x.dim() == 4):
