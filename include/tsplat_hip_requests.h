@@ -24,7 +24,7 @@ int tsplat_requests_abi_version(void);
  * out[m] = y[m] where rows[m] is not in [0, slots) or rank[a] <= 0 (nothing is written there when out is y).
  *
  * y, x, out: fp32, M rows of N, K, N values, y_stride / x_stride / out_stride floats apart.  out may be y itself
- * (same pointer and stride); it must not overlap y otherwise, nor x (-3).
+ * (same pointer and stride); it must not overlap y otherwise, nor anything else that is read (-3).
  * dtype of the adapters: 0 fp32, 1 bf16, 2 fp16.  Their values are laid out in tiles that one wave reads as one
  * piece, zero past K, N and each adapter's rank:
  *   down: [slots][ceil(R/16)][ceil(K/32)][4][16][8], value (r, k) at [r/16][k/32][k%32/8][r%16][k%8];
@@ -34,7 +34,7 @@ int tsplat_requests_abi_version(void);
  * to 2^20, slots up to 2^20 (-2).  A row of x that holds an infinity or NaN gives NaN.  The factors of the products (x,
  * the adapter, the inner sums) count in steps of 2^-133 where fp32's own are finer, below 2^-110.
  * scratch: at least tsplat_low_rank_scratch_bytes(...) of device memory that no other work uses until the call's
- * kernels are done (-5 when too small), 16-byte aligned. */
+ * kernels are done (-5 when too small, -3 over another argument), 16-byte aligned. */
 int64_t tsplat_low_rank_scratch_bytes(int M, int K, int N, int slots, int max_rank, int dtype);
 int tsplat_low_rank_add_async(const float* y, int64_t y_stride, const float* x, int64_t x_stride,
                               const int32_t* rows, const void* down, const void* up, const float* scale,

@@ -73,6 +73,25 @@ def test_low_rank_scratch(lib):
     assert lib.tsplat_low_rank_scratch_bytes(0, 64, 64, 2, 16, 1) == 0
 
 
+@pytest.mark.parametrize("change", [
+    dict(rows=P[7]), dict(rows=P[7] - 4 * 299), dict(rows=P[7] + 4 * (300 * 64 - 1)), dict(scale=P[7]),
+    dict(scale=P[7] - 4), dict(rank=P[7] + 64), dict(down=P[7]), dict(down=P[7] - 4080), dict(up=P[7] - 8176),
+    dict(rows=P[8]), dict(scale=P[8]), dict(rank=P[8] + 4), dict(down=P[8]), dict(up=P[8]),
+    dict(x=P[8]), dict(y=P[8]), dict(out=P[8]), dict(y=P[8], out=P[8]), dict(scratch=P[1] + 4 * 300 * 64 - 16)])
+def test_low_rank_memory_that_is_written_over_what_is_read(lib, change):
+    """out (300 rows) or scratch over one value of the rows, an adapter (2 slots: down 4096 bytes, up 8192), scale, rank;
+    scratch over x, y and out."""
+    assert _low_rank(lib, M=300, **change) == -3
+
+
+@pytest.mark.parametrize("change", [dict(rows=P[7] - 4 * 300), dict(rows=P[7] + 4 * 300 * 64), dict(scale=P[7] - 8),
+                                    dict(down=P[7] - 4096), dict(up=P[7] - 8192), dict(scratch=P[1] + 4 * 300 * 64),
+                                    dict(M=16, scratch=P[7]), dict(out=P[0])])
+def test_low_rank_memory_beside_what_is_read(lib, change):
+    """Up to the edges (and scratch that the call does not use): refused only as memory that is none of a device."""
+    assert _low_rank(lib, **{"M": 300, **change}) in (-6, -7)
+
+
 def _norm(lib, x=P[0], xs=32, h=P[1], hs=32, out=P[2], os=32, normed=P[3], ns=32, rows=4, cols=32, c=1.0, gate=None,
           gs=0, post=0, pw=None, pb=None, pe=1e-6, pre=1, w=None, b=None, e=1e-6, scale=None, shift=None, ms=0, per=2):
     return lib.tsplat_residual_norm_async(x, xs, h, hs, out, os, normed, ns, rows, cols, c, gate, gs, post, pw, pb,

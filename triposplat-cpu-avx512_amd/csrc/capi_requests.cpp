@@ -90,16 +90,19 @@ int tsplat_low_rank_add_async(const float* y, int64_t y_stride, const float* x, 
   const int64_t k_pad = ((int64_t)K + 31) / 32 * 32, n_pad = ((int64_t)N + 15) / 16 * 16;
   const int64_t down_values = ((int64_t)max_rank + 15) / 16 * 16 * k_pad;
   const int64_t up_values = ((int64_t)max_rank + 31) / 32 * 32 * n_pad;
+  const Rows room = whole(need > 0 ? scratch : nullptr, need / 4);
+  // what is only read besides y and x; y may be the output, but never scratch
+  const Rows reads[] = {whole(rows, M), whole(down, slots * down_values * size / 4),
+                        whole(up, slots * up_values * size / 4), whole(scale, slots), whole(rank, slots)};
+  for (const Rows& r : reads)
+    if (!disjoint(ro, r) || (room.p && !disjoint(room, r))) return kErrRange;
+  if (room.p && (!disjoint(room, ry) || !disjoint(room, rx) || !disjoint(room, ro))) return kErrRange;
   DeviceRanges ptrs;
   TSPLAT_CHECK(ptrs.check(x, rx.bytes()));
   TSPLAT_CHECK(ptrs.check(y, ry.bytes()));
   TSPLAT_CHECK(ptrs.check(out, ro.bytes()));
-  TSPLAT_CHECK(ptrs.check(rows, (int64_t)M * 4));
-  TSPLAT_CHECK(ptrs.check(down, slots * down_values * size));
-  TSPLAT_CHECK(ptrs.check(up, slots * up_values * size));
-  TSPLAT_CHECK(ptrs.check(scale, (int64_t)slots * 4));
-  TSPLAT_CHECK(ptrs.check(rank, (int64_t)slots * 4));
-  if (need > 0) TSPLAT_CHECK(ptrs.check(scratch, need));
+  for (const Rows& r : reads) TSPLAT_CHECK(ptrs.check(r.p, r.bytes()));
+  if (room.p) TSPLAT_CHECK(ptrs.check(scratch, need));
   LowRankParams p{y, x, rows, down, up, scale, rank, out, y_stride, x_stride, out_stride,
                   M, K, N, slots, max_rank, dtype, static_cast<float*>(scratch)};
   if (M == 1) p.y_stride = p.x_stride = p.out_stride = 0;

@@ -164,10 +164,9 @@ def low_rank_add(y, x, bank, rows, *, out=None, library=None):
     y [..., out] is the shared projection of x [..., in], both fp32 on the GPU with unit column stride and one row
     stride (column ranges of wider rows pass); rows [M] int32, contiguous.  A row whose number is no loaded slot of
     the bank (negative, out of range, unloaded) keeps y.  out: None for a new tensor, y itself (rows without an
-    adapter are not touched), or another that overlaps neither y nor x.  A row of x that
-    holds an infinity or NaN gives NaN; other rows are not affected.  fp32 factors below 2^-110 count in steps of
-    2^-133.  Runs on torch's current stream; capturable into
-    a HIP graph.  No gradients."""
+    adapter are not touched), or another that overlaps nothing that is read.  A row of x that holds an infinity or NaN
+    gives NaN; other rows are not affected.  fp32 factors below 2^-110 count in steps of 2^-133.  Runs on torch's
+    current stream; capturable into a HIP graph.  No gradients."""
     import torch
 
     if not isinstance(bank, AdapterBank):
