@@ -73,6 +73,20 @@ def test_many_requests_in_every_layout(cuda, hiplib, M, K, N, R, slots, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M,K,N,R,slots", [(40, 64, 3000, 33, 64), (130, 96, 3010, 20, 64), (130, 96, 3010, 20, 4),
+                                           (70, 64, 9000, 40, 2), (300, 64, 600, 40, 64), (90, 64, 2100, 34, 16)])
+def test_column_tiles_by_adapters(cuda, hiplib, M, K, N, R, slots, dtype):
+    """Few rows of few and of many adapters, on both sides of where a wave takes more columns."""
+    import torch
+
+    print(f"column tiles M={M} N={N} R={R} slots={slots} {dtype}", flush=True)
+    ranks = [1 + (R - 1) * (i % 4) // 3 for i in range(slots)]
+    x, y, bank, adapters, g = _case(torch, cuda, M, K, N, R, slots, dtype, seed=N + slots, ranks=ranks)
+    rows = torch.randint(-1, slots + 1, (M,), generator=g, device=cuda, dtype=torch.int32)
+    _check(torch, x, y, bank, adapters, rows, "columns")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("M,K,N,R,slots", [(64, 256, 192, 16, 64), (64, 256, 192, 32, 5), (300, 128, 160, 24, 7),
                                            (1100, 96, 64, 40, 3), (5000, 96, 80, 16, 9), (9100, 64, 48, 20, 30),
                                            (4600, 130, 70, 128, 6)])

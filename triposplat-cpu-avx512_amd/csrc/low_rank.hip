@@ -553,9 +553,12 @@ constexpr int kUnits = 256;  // compute units
 //     + 17 us with one workgroup a tile, 6.8 + 8.1 with 16 and 8.  Parts of K past that cost the second kernel more
 //     (1000 x 4096 x 4096, rank 128: two parts 44 us, four 57).
 //   - Eight column tiles read t and each adapter's border least, from where the waves come in many rounds (8202 x 6144:
-//     109 us, four 117; 12294 x 2900: 91, 98; but 14644 x 1743: 54, 49); two where there are fewer waves than three
-//     to two compute units (300 x 600: 8.2 us, four 8.7; but 64 x 6144 with 64 adapters 15.0, 14.5, and 300 x 6000 15.3,
-//     14.2), unless many parts of K make each wave add up t again (336 rows, 3099 -> 1046, six parts: 18.2, four 13.3).
+//     109 us, four 117; 12294 x 2900: 91, 98; but 14644 x 1743: 54, 49).  Two where few waves leave the chip idle (of 4
+//     adapters, rank 16: 300 x 600 7.9 us, four 8.4; 130 x 3000 7.9, 8.5; 130 x 5000 8.1, 8.7; rank 32 in fp16: 3000 x 400
+//     12.3, 11.7; 300 x 6000 12.0, 11.2).  A wave takes a turn for each adapter of its rows and loads their numbers and
+//     inner values anew, so those count as waves too, as many as slots spread over the rows let expect (of 64 adapters,
+//     rank 32 in fp16: 64 x 6144 14.5 us, four 13.8; 64 x 3000 12.7, 11.9; 130 x 3000 11.9, 11.7; but 300 x 600 9.8, 9.9).
+//     Many parts of K make each wave add up t again (336 rows, 3099 -> 1046, six parts: 18.2, four 13.3).
 struct Plan {
   int row_tiles, rank_tiles, splits, down_passes, column_tiles, up_passes;
 };
@@ -575,7 +578,8 @@ Plan plan_of(int M, int K, int N, int slots, int R, int dtype) {
   else if (slots > 1 && (workgroups - 1) % kUnits < kUnits * 7 / 8)
     pl.down_passes = 2;
   const int64_t waves = (int64_t)row_tiles * ceil_div(N, 64);
-  if (waves < 384 && pl.splits <= 2)
+  const int adapters = std::clamp((int)(INT64_C(16) * slots / M), 1, most);  // of a row tile
+  if (waves * adapters < 3 * kUnits && pl.splits <= 2)
     pl.column_tiles = 2;
   else if (waves >= 32768)
     pl.column_tiles = 8;
