@@ -73,6 +73,25 @@ def test_many_requests_in_every_layout(cuda, hiplib, M, K, N, R, slots, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M,K,N,R,slots", [(16400, 64, 40, 12, 2), (16400, 70, 33, 25, 2), (16370, 64, 40, 60, 2),
+                                           (16390, 40, 50, 100, 2), (24600, 33, 20, 40, 3), (33000, 40, 24, 70, 5),
+                                           (16300, 64, 40, 60, 2), (24500, 40, 24, 40, 3), (32700, 40, 24, 70, 5)])
+@pytest.mark.parametrize("order", ["requests", "every row another"])
+def test_row_tiles_with_and_without_a_border_pass(cuda, hiplib, M, K, N, R, slots, order, dtype):
+    """Two row tiles a workgroup and several adapters: so many rows that the workgroup of a border goes through all of
+    them by itself, and the last sizes below that."""
+    import torch
+
+    print(f"borders M={M} K={K} R={R} slots={slots} {order} {dtype}", flush=True)
+    ranks = [max(1, R - 11 * i) for i in range(slots)]
+    x, y, bank, adapters, g = _case(torch, cuda, M, K, N, R, slots, dtype, seed=M, ranks=ranks)
+    rows = torch.randint(-1, slots + 1, (M,), generator=g, device=cuda, dtype=torch.int32)
+    if order == "requests":
+        rows = rows[(torch.rand(M, generator=g, device=cuda) < 0.04).cumsum(0)]
+    _check(torch, x, y, bank, adapters, rows, "borders")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("M,K,N,R,slots", [(40, 64, 3000, 33, 64), (130, 96, 3010, 20, 64), (130, 96, 3010, 20, 4),
                                            (70, 64, 9000, 40, 2), (300, 64, 600, 40, 64), (90, 64, 2100, 34, 16)])
 def test_column_tiles_by_adapters(cuda, hiplib, M, K, N, R, slots, dtype):

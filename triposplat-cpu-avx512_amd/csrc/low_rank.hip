@@ -544,9 +544,12 @@ constexpr int kUnits = 256;  // compute units
 //     requests: 36 us, 22 with one; 2100 x 4096, rank 128 in fp32, 4 adapters: 56, 36 with one.  So a bank of one slot
 //     takes them sooner, and with large ranks sooner still (that call with one adapter: 45 us, one row tile 60; rank 64,
 //     4000 x 4096: 40, one 39).
-//   - With two row tiles the border between requests in a pass of its own: 7000 x 4096, rank 64, 2 to 6 adapters: 70-90 us
-//     -> 55-73; 12294 x 1024: 48-57 -> 44-53.  Not where the last round of workgroups is full and one more starts
-//     another (16384 x 4096, 2 adapters: 148 -> 157).
+//   - With two row tiles the border between requests in a pass of its own.  It pays while a border's workgroup, which
+//     takes twice its time, would end last, and adds a turn of workgroups that mostly end at once: where borders are many
+//     (slots) or the rounds few.  K 1024, fp32, rank 64, without and with: 7100 rows of 2 requests 23.0, 21.5 us; 12294:
+//     35.7, 33.2; 16384: 37.0, 39.7; 33000: 71.2, 74.8; of 12 requests in 4 slots 7100: 26.9, 24.7; 16500: 39.7, 38.1;
+//     33000: 59.0, 61.2.  A round of workgroups that it would just overfill costs less than it gains for most requests
+//     (8192 rows: 4 % slower of 2 requests, 4 to 14 % faster of 12 to 256).
 //   - Eight rank tiles, which read x once, only there and not for fp32's three planes, whose 96 registers are too many
 //     (16384 x 1024, rank 128: bf16 38 -> 26 us, fp16 52 -> 42; one row tile: fp16 45 -> 53).
 //   - Few rows leave the chip idle without the next two: 64 rows of an adapter each, K 1024 -> N 6144, rank 32, take 68
@@ -575,7 +578,7 @@ Plan plan_of(int M, int K, int N, int slots, int R, int dtype) {
   pl.splits = std::max(1, std::min({kUnits / workgroups, ceil_div(K, 32) / (2 * kDownWaves), 8}));
   if (pl.row_tiles == 1)
     pl.down_passes = std::max(1, std::min(1024 / (workgroups * pl.splits), most));
-  else if (slots > 1 && (workgroups - 1) % kUnits < kUnits * 7 / 8)
+  else if (slots > 1 && workgroups < kUnits * std::min(slots, 4))
     pl.down_passes = 2;
   const int64_t waves = (int64_t)row_tiles * ceil_div(N, 64);
   const int adapters = std::clamp((int)(INT64_C(16) * slots / M), 1, most);  // of a row tile
