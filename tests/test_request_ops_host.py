@@ -261,3 +261,34 @@ def test_rope_plan():
             RopeAxes(*bad, device="cpu")
     with pytest.raises(ValueError):
         RopeAxes(8, [4], 0.0, device="cpu")
+
+
+def test_a_library_is_found_by_what_its_name_means_now(lib, monkeypatch, tmp_path):
+    """The library of no name is found again at once; a name that is given is looked up in every call."""
+    import shutil
+
+    from tsplat import load_library
+    from tsplat._lib import DEFAULT_LIBRARY
+
+    monkeypatch.delenv("TSPLAT_HIP_LIBRARY", raising=False)
+    monkeypatch.chdir(tmp_path)
+    default = load_library()
+    assert load_library() is default and load_library(DEFAULT_LIBRARY) is default
+    with pytest.raises(FileNotFoundError):
+        load_library("")
+    other = tmp_path / "other.so"
+    shutil.copy(DEFAULT_LIBRARY, other)
+    link = tmp_path / "link.so"
+    for target in (DEFAULT_LIBRARY, other):
+        link.unlink(missing_ok=True)
+        link.symlink_to(target)
+        for _ in range(3):
+            assert load_library(str(link)) is load_library(target)
+            monkeypatch.setenv("TSPLAT_HIP_LIBRARY", str(link))
+            assert load_library() is load_library(target)
+            monkeypatch.delenv("TSPLAT_HIP_LIBRARY")
+    assert load_library(str(link)) is not default
+    link.unlink()
+    with pytest.raises(FileNotFoundError):
+        load_library(str(link))
+    assert load_library() is default

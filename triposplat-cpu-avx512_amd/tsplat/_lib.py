@@ -122,7 +122,7 @@ ABI_VERSION = 5
 # tsplat_requests_abi_version(), likewise, of REQUEST_SIGNATURES.
 REQUESTS_ABI_VERSION = 1
 
-_CACHE: dict[str, ctypes.CDLL] = {}
+_CACHE: dict[str | Path, ctypes.CDLL] = {}  # by resolved name; DEFAULT_LIBRARY also as it stands
 
 
 def library_path(path: str | os.PathLike | None = None) -> Path:
@@ -134,9 +134,10 @@ def library_path(path: str | os.PathLike | None = None) -> Path:
 
 def load_library(path: str | os.PathLike | None = None) -> ctypes.CDLL:
     """Open libtsplat_hip.so once per path and set every argtypes/restype."""
-    # the name as it is given, so that a loaded library is found again without touching the file system
-    given = os.environ.get("TSPLAT_HIP_LIBRARY", "") if path is None else path
-    lib = _CACHE.get(given) if isinstance(given, str) else None
+    # without a name there is nothing to resolve: small calls are bound by the host, and the look at the file system
+    # would take longer than the rest of them
+    unnamed = path is None and not os.environ.get("TSPLAT_HIP_LIBRARY")
+    lib = _CACHE.get(DEFAULT_LIBRARY) if unnamed else None
     if lib is not None:
         return lib
     import torch  # noqa: F401  (binds the library to torch's HIP runtime)
@@ -145,8 +146,8 @@ def load_library(path: str | os.PathLike | None = None) -> ctypes.CDLL:
     key = resolved.as_posix()
     lib = _CACHE.get(key)
     if lib is not None:
-        if isinstance(given, str) and (given == "" or os.path.isabs(given)):
-            _CACHE[given] = lib  # (a relative name means another file in another folder)
+        if unnamed:
+            _CACHE[DEFAULT_LIBRARY] = lib
         return lib
     if not resolved.is_file():
         raise FileNotFoundError(
