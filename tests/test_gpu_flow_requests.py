@@ -286,3 +286,29 @@ def test_refusals(cuda, hiplib):
             adapters.load(0, weights)
     with pytest.raises(ValueError):
         adapters.load(2, {})
+
+
+def test_tangents_are_refused(cuda, hiplib):
+    import torch
+    from tsplat.adapters import AdapterBank, low_rank_add
+    from tsplat.block_ops import residual_norm
+    from tsplat.qkv import RopeAxes, qkv_rope_axes, rope_axes
+
+    x, w = torch.randn(4, 192, device=cuda), torch.ones(192, device=cuda)
+    bank, rows = AdapterBank(1, 192, 192, 8, device=cuda), torch.zeros(4, dtype=torch.int32, device=cuda)
+    rope, pos = RopeAxes(64, [32], device=cuda), torch.arange(4, dtype=torch.int32, device=cuda)[:, None]
+    gamma = torch.ones(1, 64, device=cuda)
+    with torch.autograd.forward_ad.dual_level():
+        def dual(t):
+            return torch.autograd.forward_ad.make_dual(t.clone(), torch.ones_like(t))
+
+        for call in (lambda: low_rank_add(dual(x), x, bank, rows), lambda: low_rank_add(x, dual(x), bank, rows),
+                     lambda: residual_norm(dual(x), x), lambda: residual_norm(x, dual(x)),
+                     lambda: residual_norm(x, x, weight=dual(w)), lambda: residual_norm(x, x, gate=dual(w[None])),
+                     lambda: rope_axes(dual(x).view(1, 4, 3, 64), pos, rope),
+                     lambda: qkv_rope_axes(x, pos, rope, dual(gamma), gamma, 1, 4, 1),
+                     lambda: qkv_rope_axes(dual(x), pos, rope, gamma, gamma, 1, 4, 1)):
+            with pytest.raises(ValueError, match="forward"):
+                call()
+        low_rank_add(x, x, bank, rows)
+        residual_norm(x, x)

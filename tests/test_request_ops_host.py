@@ -292,3 +292,24 @@ def test_a_library_is_found_by_what_its_name_means_now(lib, monkeypatch, tmp_pat
     with pytest.raises(FileNotFoundError):
         load_library(str(link))
     assert load_library() is default
+
+
+def test_tangents_are_refused_like_gradients():
+    """A tensor with a forward-mode tangent has none afterwards: refused, with grad mode off too; others pass."""
+    import torch
+    from tsplat._lib import no_gradients
+
+    plain = torch.zeros(3)
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(plain.clone(), torch.ones(3))
+        with pytest.raises(ValueError, match="backward or forward"):
+            no_gradients(torch, plain, None, dual)
+        with torch.no_grad(), pytest.raises(ValueError, match="backward or forward"):
+            no_gradients(torch, dual)
+        no_gradients(torch, plain, None)
+    no_gradients(torch, plain)
+    leaf = torch.zeros(3, requires_grad=True)
+    with pytest.raises(ValueError, match="backward"):
+        no_gradients(torch, leaf)
+    with torch.no_grad():
+        no_gradients(torch, leaf)

@@ -223,10 +223,15 @@ def enqueue(lib, fn_name, index, *args) -> None:
 
 
 def no_gradients(torch, *tensors) -> None:
-    """These operators have no backward: a tensor that expects one is refused, not cut off in silence."""
+    """These operators have no backward and no forward mode: a tensor that expects a gradient or carries a tangent is
+    refused, not cut off in silence."""
+    forward = torch.autograd.forward_ad
+    duals = getattr(forward, "_current_level", 0) >= 0  # (outside of a dual level no tensor has a tangent)
     for t in tensors:
-        if t is not None and t.requires_grad and torch.is_grad_enabled():
-            raise ValueError("this operator has no backward: call it under torch.no_grad(), or detach its inputs")
+        if t is not None and (t.requires_grad and torch.is_grad_enabled()
+                              or duals and forward.unpack_dual(t).tangent is not None):
+            raise ValueError("this operator has no backward or forward mode of gradients: call it under "
+                             "torch.no_grad() and outside of dual levels, or detach its inputs")
 
 
 def rows_of(torch, name, t, cols) -> tuple[int, int]:
