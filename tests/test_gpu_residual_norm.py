@@ -292,3 +292,25 @@ def test_narrow_rows(cuda, hiplib, C, L):
     x, h, mod, vectors = _inputs(torch, cuda, 3, L, C, C + L)
     for post, pre in (("rms", "layer"), ("layer", "rms"), (None, "layer")):
         _check(torch, x, h, mod, vectors, post, pre, True, True, True, what=f"{post} {pre}")
+
+
+def test_a_row_of_the_most_columns(cuda, hiplib):
+    """2^31 - 1 columns in place: a column index one step past the end does not fit 31 bits.  Values of +-1 whose sums
+    are exact, so that the root's sum, the root, the division and the product are all that rounds: 3.5 u."""
+    import torch
+    from tsplat.block_ops import residual_norm as call
+
+    C, half = 2 ** 31 - 1, 2 ** 30 - 1
+    x, h = (torch.empty(C, device=cuda) for _ in range(2))
+    for t in (x, h):
+        t.fill_(0.5)
+        t[:-1].view(half, 2)[:, 1] = -0.5
+    print("2^31 - 1 columns", flush=True)
+    out, normed = call(x[None], h[None], out=x[None], normed=h[None])
+    torch.cuda.synchronize(cuda)
+    want = 1 / (1 + 1e-6) ** 0.5
+    for t, one, off in ((x, 1.0, 0.0), (h, want, 4 * U * want)):
+        pairs = t[:-1].view(half, 2)
+        for column, sign in ((pairs[:, 0], 1), (pairs[:, 1], -1), (t[-1:], 1)):
+            low, high = (float(v) * sign for v in torch.aminmax(column))
+            assert abs(low - one) <= off and abs(high - one) <= off, (sign, low, high)

@@ -173,17 +173,17 @@ __device__ float block_sum(float v, float* lds) {
 }
 
 template <typename F>
-__device__ Stats wide_stats(int kind, float eps, int cols, float* lds, F value) {
+__device__ Stats wide_stats(int kind, float eps, uint32_t cols, float* lds, F value) {
   if (kind == kNormNone) return {0.0f, 0.0f, 1.0f};
   const float n = (float)cols;
   float mean = 0.0f, left = 0.0f;
   if (kind == kNormLayer) {
     float s = 0.0f;
-    for (int c = threadIdx.x; c < cols; c += kWideThreads) s += value(c);
+    for (uint32_t c = threadIdx.x; c < cols; c += kWideThreads) s += value(c);
     mean = block_sum(s, lds) / n;
   }
   float s = 0.0f, q = 0.0f;
-  for (int c = threadIdx.x; c < cols; c += kWideThreads) {
+  for (uint32_t c = threadIdx.x; c < cols; c += kWideThreads) {
     const float d = value(c) - mean;
     s += d;
     q = fmaf(d, d, q);
@@ -196,7 +196,7 @@ __device__ Stats wide_stats(int kind, float eps, int cols, float* lds, F value) 
   return {mean, left, 1.0f / sqrtf(q + eps)};
 }
 
-__device__ __forceinline__ float wide_value(const NormSpec& s, const Stats& st, float v, int c) {
+__device__ __forceinline__ float wide_value(const NormSpec& s, const Stats& st, float v, uint32_t c) {
   if (s.kind == kNormNone) return v;
   v = (v - st.mean - st.left) * st.inv;
   if (s.weight) v *= s.weight[c];
@@ -208,20 +208,21 @@ __global__ __launch_bounds__(kWideThreads) void residual_norm_wide_kernel(Residu
   __shared__ float lds[kWideThreads / 64];
   const int64_t row = block_index();
   if (row >= p.rows) return;
+  const uint32_t cols = (uint32_t)p.cols;  // (a column past the last one may pass 2^31)
   const int64_t b = p.gate || p.scale ? (uint32_t)row / (uint32_t)p.rows_per_batch : 0;
   const float* x = p.x + row * p.x_stride;
   const float* h = p.h + row * p.h_stride;
   float* out = p.out + row * p.out_stride;
   float* normed = p.normed + row * p.normed_stride;
   const float* gate = p.gate ? p.gate + b * p.gate_stride : nullptr;
-  const Stats post = wide_stats(p.post.kind, p.post.eps, p.cols, lds, [&](int c) { return h[c]; });
-  for (int c = threadIdx.x; c < p.cols; c += kWideThreads) {
+  const Stats post = wide_stats(p.post.kind, p.post.eps, cols, lds, [&](uint32_t c) { return h[c]; });
+  for (uint32_t c = threadIdx.x; c < cols; c += kWideThreads) {
     const float v = wide_value(p.post, post, h[c], c);
     out[c] = fmaf(p.residual_scale, x[c], gate ? gate[c] * v : v);
   }
   // (a thread reads back what it wrote itself)
-  const Stats pre = wide_stats(p.pre.kind, p.pre.eps, p.cols, lds, [&](int c) { return out[c]; });
-  for (int c = threadIdx.x; c < p.cols; c += kWideThreads) {
+  const Stats pre = wide_stats(p.pre.kind, p.pre.eps, cols, lds, [&](uint32_t c) { return out[c]; });
+  for (uint32_t c = threadIdx.x; c < cols; c += kWideThreads) {
     float v = wide_value(p.pre, pre, out[c], c);
     if (p.scale) v = fmaf(v, 1.0f + p.scale[b * p.mod_stride + c], p.shift[b * p.mod_stride + c]);
     normed[c] = v;
