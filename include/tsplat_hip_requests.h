@@ -34,7 +34,8 @@ int tsplat_requests_abi_version(void);
  * to 2^20, slots up to 2^20 (-2).  A row of x that holds an infinity or NaN gives NaN.  The factors of the products (x,
  * the adapter, the inner sums) count in steps of 2^-133 where fp32's own are finer, below 2^-110.
  * scratch: at least tsplat_low_rank_scratch_bytes(...) of device memory that no other work uses until the call's
- * kernels are done (-5 when too small, -3 over another argument), 16-byte aligned. */
+ * kernels are done (-5 when too small, -3 over another argument), 16-byte aligned.
+ * The size is 0 for a call that needs none, and for sizes or a dtype that the call refuses. */
 int64_t tsplat_low_rank_scratch_bytes(int M, int K, int N, int slots, int max_rank, int dtype);
 int tsplat_low_rank_add_async(const float* y, int64_t y_stride, const float* x, int64_t x_stride,
                               const int32_t* rows, const void* down, const void* up, const float* scale,

@@ -92,6 +92,16 @@ def test_low_rank_memory_beside_what_is_read(lib, change):
     assert _low_rank(lib, **{"M": 300, **change}) in (-6, -7)
 
 
+@pytest.mark.parametrize("at,value", [(0, 2 ** 31 - 1), (0, (1 << 27) + 1), (0, -1), (1, 2 ** 31 - 1),
+                                      (1, (1 << 20) + 1), (1, 0), (2, 2 ** 31 - 1), (2, (1 << 20) + 1), (2, -5),
+                                      (3, (1 << 20) + 1), (3, 0), (4, 513), (4, 0), (5, 3), (5, -1)])
+def test_no_scratch_for_sizes_that_are_refused(lib, at, value):
+    sizes = [300, 64, 64, 2, 16, 1]
+    assert lib.tsplat_low_rank_scratch_bytes(*sizes) > 0
+    sizes[at] = value
+    assert lib.tsplat_low_rank_scratch_bytes(*sizes) == 0
+
+
 def _norm(lib, x=P[0], xs=32, h=P[1], hs=32, out=P[2], os=32, normed=P[3], ns=32, rows=4, cols=32, c=1.0, gate=None,
           gs=0, post=0, pw=None, pb=None, pe=1e-6, pre=1, w=None, b=None, e=1e-6, scale=None, shift=None, ms=0, per=2):
     return lib.tsplat_residual_norm_async(x, xs, h, hs, out, os, normed, ns, rows, cols, c, gate, gs, post, pw, pb,

@@ -17,6 +17,7 @@ namespace {
 
 constexpr int kRequestsAbiVersion = 1;
 constexpr int kMaxRank = 512;
+constexpr int kMaxRows = 1 << 27, kMaxFeatures = 1 << 20;  // (the launches' grids hold these)
 constexpr int kMaxSlots = 1 << 20;
 constexpr int kMaxHeadDim = 512;
 constexpr int kMaxHeads = 1 << 16;
@@ -57,6 +58,12 @@ bool disjoint(const Rows& a, const Rows& b) {
   return at >= a.cols * 4 && at + b.cols * 4 <= bytes;
 }
 
+bool low_rank_sizes(int M, int K, int N, int slots, int rank, int dtype) {
+  auto within = [](int n, int most) { return n > 0 && n <= most; };
+  return within(M, kMaxRows) && within(K, kMaxFeatures) && within(N, kMaxFeatures) && within(slots, kMaxSlots) &&
+         within(rank, kMaxRank) && (dtype == kAdapterF32 || dtype == kAdapterBf16 || dtype == kAdapterF16);
+}
+
 }  // namespace
 
 extern "C" {
@@ -64,7 +71,7 @@ extern "C" {
 int tsplat_requests_abi_version(void) { return kRequestsAbiVersion; }
 
 int64_t tsplat_low_rank_scratch_bytes(int M, int K, int N, int slots, int max_rank, int dtype) {
-  if (M <= 0 || K <= 0 || N <= 0 || slots <= 0 || slots > kMaxSlots || max_rank <= 0 || max_rank > kMaxRank) return 0;
+  if (!low_rank_sizes(M, K, N, slots, max_rank, dtype)) return 0;
   return low_rank_scratch_bytes(M, K, N, slots, max_rank, dtype);
 }
 
@@ -74,10 +81,7 @@ int tsplat_low_rank_add_async(const float* y, int64_t y_stride, const float* x, 
                               int slots, int max_rank, int dtype, void* scratch, int64_t scratch_bytes,
                               void* stream) {
   if (!y || !x || !rows || !down || !up || !scale || !rank || !out) return kErrNull;
-  if (M <= 0 || K <= 0 || N <= 0 || slots <= 0 || slots > kMaxSlots || max_rank <= 0 || max_rank > kMaxRank) return kErrDims;
-  if (dtype != kAdapterF32 && dtype != kAdapterBf16 && dtype != kAdapterF16) return kErrDims;
-  // (the launches' grids hold these)
-  if (M > (1 << 27) || K > (1 << 20) || N > (1 << 20)) return kErrDims;
+  if (!low_rank_sizes(M, K, N, slots, max_rank, dtype)) return kErrDims;
   const Rows ry{y, y_stride, M, N}, rx{x, x_stride, M, K}, ro{out, out_stride, M, N};
   if (!sane(ry) || !sane(rx) || !sane(ro)) return kErrRange;
   if ((!same(ro, ry) && !disjoint(ro, ry)) || !disjoint(ro, rx)) return kErrRange;
