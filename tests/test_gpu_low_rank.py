@@ -168,6 +168,45 @@ def test_every_bit_of_a_product(cuda, hiplib, M, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M,K,N,R", [(16, 200, 100, 20), (40, 300, 70, 64), (16, 4096, 64, 40), (700, 1600, 300, 129),
+                                     (6200, 70, 90, 12), (6300, 200, 72, 30), (6200, 130, 72, 64), (6300, 200, 72, 100),
+                                     (6200, 96, 50, 140), (7000, 1100, 70, 90), (9000, 40, 4200, 40)])
+def test_every_product_of_terms(cuda, hiplib, M, K, N, R, dtype):
+    """One value of x a row, and one of the adapter's second half a column, with all their bits: each output is a product
+    of three values, of which every product of their terms counts.  u = 2^-24.
+
+    What the split leaves out of a product is below 2^-22 of it with fp16 weights (4 u) and 2^-21 + 2^-30 with fp32 ones
+    (8.1 u); a sum is off by a step, 2 u, of what it holds at most, the whole once and 2^-6 of it before; two such
+    products, and u for the scale.  A term that was lost would cost 250 to 1000 u."""
+    import torch
+    from tsplat.adapters import AdapterBank, low_rank_add
+
+    print(f"terms M={M} K={K} N={N} R={R} {dtype}", flush=True)
+    dt, g = getattr(torch, dtype), torch.Generator(device=cuda).manual_seed(M + R)
+    # 1 + 2^-7 less a last bit, of 24 and of 11 bits: the largest second terms
+    most, most_weight = 1 + 2.0 ** -7 - 2.0 ** -23, {"float32": 1 + 2.0 ** -7 - 2.0 ** -23, "float16": 1 + 7 / 1024}
+    value = torch.randn(M, generator=g, device=cuda)
+    value[::4] = most
+    at = torch.randint(0, K, (M,), generator=g, device=cuda)
+    x = torch.zeros(M, K, device=cuda)
+    x[torch.arange(M), at] = value
+    down = torch.randn(2, R, K, generator=g, device=cuda).to(dt)
+    second = torch.randn(2, N, generator=g, device=cuda).to(dt)
+    down[:, ::3], second[:, ::2] = most_weight.get(dtype, 1.0), most_weight.get(dtype, 1.0)
+    rank_of = torch.arange(N, device=cuda) % R
+    up = torch.zeros(2, N, R, dtype=dt, device=cuda)
+    up[:, torch.arange(N), rank_of] = second
+    scale = torch.tensor([0.7, 1.3], device=cuda)
+    rows = torch.randint(0, 2, (M,), generator=g, device=cuda, dtype=torch.int32)
+    got = low_rank_add(torch.zeros(M, N, device=cuda), x, AdapterBank.stack(down, up, scale), rows)
+    a = rows.long()
+    inner = down.double()[a, :, at][:, rank_of]  # [M, N]
+    want = (scale.double()[a] * value.double())[:, None] * inner * second.double()[a]
+    off = 2 * {"float32": 8.1, "bfloat16": 0.0, "float16": 4.0}[dtype] + 2 * 2.1 + 1
+    assert_within(torch, got, want, 1.01 * off * 2.0 ** -24 * want.abs(), "terms")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_large_and_small_values(cuda, hiplib, dtype):
     """x up to near the end of fp32 and far below 1: nothing on the way overflows or goes to zero that the fp32
     product would keep."""

@@ -4,7 +4,7 @@
 // Two kernels: the inner values t = scale[a] x down[a]^T [M, R] go to scratch (R / K of x's bytes), the second joins
 // t up[a]^T to y.  Both run on the bf16 matrix cores at fp32 precision: an fp32 value is the sum of three bf16 values
 // (8 + 8 + 8 bits, split by truncation, so exactly and without overflow), a bf16 weight one, an fp16 weight two, an
-// fp32 weight three; the products below 2^-23 of the whole are left out.
+// fp32 weight three; the smallest products of terms are left out (kProducts says what that costs).
 //
 // What bounds it: 12294 x 1024 -> 4096, rank 16, HBM: 453 MB in 90-92 us (5.0 TB/s; x 15, y 74).  16384 x 4096 -> 1024,
 // rank 64 in fp32 (402 MB, 79 us at a copy's rate): 119 us for one adapter, 147 where two requests meet; every 32 rows
@@ -103,8 +103,10 @@ struct Weights<kAdapterF32> {  // three planes of the tile, split when the bank 
   }
 };
 
-// The products of an fp32 value's terms with a weight's that count: i + j <= 2 (the others are below 2^-23 of the
-// product), least first.
+// The products of an fp32 value's terms with a weight's that count: i + j <= 2, least first.  By truncation term 1 is
+// below 2^-7 of its value and term 2 below 2^-15, so what is left out is below 2^-22 of the product for fp16 weights (2
+// with 1), below 2^-21 for fp32 ones (1 with 2, 2 with 1, 2 with 2), nothing for bf16.  All terms have their value's sign:
+// it always takes from the product (0.7 x 2^-24 on average for fp32 weights, a sum's own roundings are more).
 template <int TERMS>
 constexpr int kProducts = TERMS == 1 ? 3 : TERMS == 2 ? 5 : 6;
 template <int TERMS>
