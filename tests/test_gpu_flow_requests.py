@@ -221,6 +221,50 @@ def test_a_captured_block_of_requests(cuda, hiplib):
         low_rank_add(qkv, z.view(B * L, C), bank, rows)
 
 
+@pytest.mark.parametrize("places", [False, True])
+def test_the_model_over_requests_waits_for_nothing(cuda, hiplib, places):
+    """velocity() copies nothing from the host, so a call neither waits for the stream nor stays out of a graph: captured,
+    with the slots as they were then, and replayed with eager calls of other slots between."""
+    import torch
+    from tsplat.flow_requests import FlowAdapters
+    from tsplat.qkv import RopeAxes
+
+    model = _model(cuda)
+    z, c, t, pos, g = _inputs(torch, cuda, model.cfg, 3, 7)
+    adapters = FlowAdapters(model, 3, 8)
+    for slot in (0, 2):
+        adapters.load(slot, _adapter(torch, cuda, model, g, 8, ["qkv", "xkv", "fc2"]))
+    kw = dict(adapters=adapters, slots=[2, -1, 0])
+    if places:
+        kw |= dict(positions=pos, rope=RopeAxes(64, SECTIONS, device=cuda))
+    want = model.velocity(z, c, t, **kw)
+    other = model.velocity(z, c, t, **(kw | dict(slots=[0, 2, -5])))
+    assert _rel(want, other.double()) > 1e-3
+    alone = model.velocity(z[:1], c[:1], t[:1], **(kw | dict(slots=[2]) | (dict(positions=pos[0]) if places else {})))
+    assert _rel(alone, want[:1].double()) <= LIMIT
+    torch.cuda.set_sync_debug_mode("error")
+    try:
+        again = model.velocity(z, c, t, **kw)
+    finally:
+        torch.cuda.set_sync_debug_mode("default")
+    assert torch.equal(again, want)
+    side = torch.cuda.Stream(device=cuda)
+    side.wait_stream(torch.cuda.current_stream(cuda))
+    with torch.cuda.stream(side):
+        model.velocity(z, c, t, **kw)  # (the stream's workspaces)
+    torch.cuda.synchronize(cuda)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        got = model.velocity(z, c, t, **kw)
+    for _ in range(4):
+        got.fill_(float("nan"))
+        torch.cuda.synchronize(cuda)
+        graph.replay()
+        torch.cuda.synchronize(cuda)
+        assert torch.equal(got, want)
+        assert torch.equal(model.velocity(z, c, t, **(kw | dict(slots=[0, 2, -5]))), other)
+
+
 def test_two_threads_on_two_streams(cuda, hiplib):
     """The operators keep nothing between calls: two host threads, each on a stream of its own, get what one gets."""
     import threading

@@ -46,7 +46,7 @@ from . import block_ops as bo
 from .native_sampler_backend import NativeSamplerBackend
 from .native_sdpa_ctypes import native_sdpa_f32_ex
 from .nf24 import bf16_planes, nf24_linear, precision_id, quantize_nf24_i16_per_output_channel
-from .qkv import gemm_nf24_qkv_direct
+from .qkv import RopeAxes, gemm_nf24_qkv_direct
 
 
 @dataclass(frozen=True)
@@ -211,6 +211,7 @@ class FlowModel:
         self.final_shift_table = _randn(torch, (2, C), 49999, device, 0.02)
         self.blocks = [FlowBlock(torch, cfg, i, device, 1010 + 10 * i) for i in range(nb)]
         self._freqs = {}
+        self._token_rope = None
         self.sampler = NativeSamplerBackend()
         self.precision = "fp32"
         self.attention_precision = "fp32"
@@ -222,6 +223,13 @@ class FlowModel:
         if L not in self._freqs:
             self._freqs[L] = rope_frequencies(self.torch, L, self.cfg.heads, self.cfg.rope_theta, self.device)
         return self._freqs[L]
+
+    def token_rope(self):
+        """The plan (qkv.RopeAxes) of freqs()'s positions: a token's index, on one axis."""
+        if self._token_rope is None:
+            self._token_rope = RopeAxes(self.cfg.head_dim, [self.cfg.head_dim // 2], self.cfg.rope_theta,
+                                        device=self.device)
+        return self._token_rope
 
     # -------------------------------------------------------------- pieces
     def timestep(self, t):

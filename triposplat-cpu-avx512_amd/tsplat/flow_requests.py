@@ -15,7 +15,7 @@ from __future__ import annotations
 from . import block_ops as bo
 from .adapters import AdapterBank, low_rank_add
 from .native_sdpa_ctypes import native_sdpa_f32_ex
-from .qkv import RopeAxes, qkv_rope_axes
+from .qkv import qkv_rope_axes
 
 
 class FlowAdapters:
@@ -66,7 +66,9 @@ def velocity(model, z, cond, t, *, adapters=None, slots=None, positions=None, ro
     """z [B, L, C], cond [B, Lc, C], t [B] (already x1000) -> v [B, L, C], as FlowModel.velocity.
     adapters: FlowAdapters, slots: one slot for each batch entry (-1 for none).  positions [L, axes] or
     [B, L, axes] with rope, a RopeAxes of the model's head size: the latent tokens' places; without them the
-    token's index on one axis, as in FlowModel.velocity."""
+    token's index on one axis, as in FlowModel.velocity.  Nothing is copied from the host: after one call on the
+    stream it can be captured into a HIP graph, which keeps the slots' numbers and reads what they hold when it is
+    replayed."""
     torch, cfg = model.torch, model.cfg
     B, L, C = (int(s) for s in z.shape)
     Lc, H = int(cond.shape[1]), cfg.heads
@@ -81,10 +83,13 @@ def velocity(model, z, cond, t, *, adapters=None, slots=None, positions=None, ro
         slots = [int(s) for s in slots]
         if len(slots) != B or any(s >= adapters.slots for s in slots):
             raise ValueError(f"slots must be {B} numbers below {adapters.slots}, negative for none")
-        of_entry = torch.tensor(slots, dtype=torch.int32, device=model.device)
-        rows, cond_rows = of_entry.repeat_interleave(L), of_entry.repeat_interleave(Lc)
+        # (filled entry by entry: a copy from the host would wait for the stream, and a graph cannot hold it)
+        of_entry = torch.empty(B, 1, dtype=torch.int32, device=model.device)
+        for b, s in enumerate(slots):
+            of_entry[b].fill_(max(s, -1))
+        rows, cond_rows = (of_entry.expand(B, n).contiguous().view(-1) for n in (L, Lc))
     if rope is None:
-        rope = RopeAxes(cfg.head_dim, [cfg.head_dim // 2], cfg.rope_theta, device=model.device)
+        rope = model.token_rope()
         positions = torch.arange(L, dtype=torch.int32, device=model.device)[:, None]
     t_emb, t_mod = model.timestep(t)
     x = model.input_layer(z.reshape(B * L, C)).view(B, L, C)
