@@ -323,3 +323,36 @@ def test_tangents_are_refused_like_gradients():
         no_gradients(torch, leaf)
     with torch.no_grad():
         no_gradients(torch, leaf)
+
+
+def test_a_load_that_fails_leaves_no_half_of_an_adapter(monkeypatch):
+    """An adapter's Linears are loaded one by one: where one fails, for memory or its type, the slot is empty."""
+    from types import SimpleNamespace
+
+    import torch
+    from tsplat import flow_requests
+
+    lin = {n: SimpleNamespace(in_features=8, out_features=6) for n in ("out", "fc1")}
+    model = SimpleNamespace(device="cpu", blocks=[SimpleNamespace(lin=lin)] * 2)
+    adapters = flow_requests.FlowAdapters(model, 2, 4)
+    good = (torch.ones(3, 8), torch.ones(6, 3))
+    weights = {(0, "out"): good, (1, "out"): good, (1, "fc1"): good}
+    adapters.load(0, weights)
+    adapters.load(1, weights)
+    bank = adapters.banks[1]["fc1"]
+
+    def fails(*_):
+        raise torch.OutOfMemoryError("no memory")
+
+    monkeypatch.setattr(bank, "load", fails)
+    with pytest.raises(torch.OutOfMemoryError):
+        adapters.load(1, weights)
+    for banks in adapters.banks:
+        for b in banks.values():
+            assert b.rank.tolist() == [3, 0]
+    monkeypatch.undo()
+    with pytest.raises(Exception):
+        adapters.load(1, {(0, "out"): good, (1, "out"): (good[0], torch.ones(6, 3).to_sparse())})
+    for banks in adapters.banks:
+        for b in banks.values():
+            assert b.rank.tolist() == [3, 0]

@@ -41,13 +41,17 @@ class FlowAdapters:
                 raise ValueError(f"the adapter of {name!r} in block {block} must be down [rank, {in_f}], "
                                  f"up [{out_f}, rank] of rank 1..{self.max_rank}")
         self.unload(slot)
-        for (block, name), (down, up) in weights.items():
-            bank = self.banks[block].get(name)
-            if bank is None:
-                bank = AdapterBank(self.slots, *self._sizes[block][name], self.max_rank, dtype=self.dtype,
-                                   device=self.device)
-            bank.load(slot, down, up, scale)
-            self.banks[block][name] = bank
+        try:
+            for (block, name), (down, up) in weights.items():
+                bank = self.banks[block].get(name)
+                if bank is None:
+                    bank = AdapterBank(self.slots, *self._sizes[block][name], self.max_rank, dtype=self.dtype,
+                                       device=self.device)
+                bank.load(slot, down, up, scale)
+                self.banks[block][name] = bank
+        except BaseException:
+            self.unload(slot)  # (an adapter of some of its Linears is none)
+            raise
 
     def unload(self, slot):
         if not 0 <= int(slot) < self.slots:
