@@ -122,7 +122,7 @@ ABI_VERSION = 5
 # tsplat_requests_abi_version(), likewise, of REQUEST_SIGNATURES.
 REQUESTS_ABI_VERSION = 1
 
-_CACHE: dict[str | Path, ctypes.CDLL] = {}  # by resolved name; DEFAULT_LIBRARY also as it stands
+_CACHE: dict[str | None, ctypes.CDLL] = {}  # by resolved name; None: DEFAULT_LIBRARY, which needs no resolving
 
 
 def library_path(path: str | os.PathLike | None = None) -> Path:
@@ -137,7 +137,7 @@ def load_library(path: str | os.PathLike | None = None) -> ctypes.CDLL:
     # without a name there is nothing to resolve: small calls are bound by the host, and the look at the file system
     # would take longer than the rest of them
     unnamed = path is None and not os.environ.get("TSPLAT_HIP_LIBRARY")
-    lib = _CACHE.get(DEFAULT_LIBRARY) if unnamed else None
+    lib = _CACHE.get(None) if unnamed else None
     if lib is not None:
         return lib
     import torch  # noqa: F401  (binds the library to torch's HIP runtime)
@@ -147,7 +147,7 @@ def load_library(path: str | os.PathLike | None = None) -> ctypes.CDLL:
     lib = _CACHE.get(key)
     if lib is not None:
         if unnamed:
-            _CACHE[DEFAULT_LIBRARY] = lib
+            _CACHE[None] = lib
         return lib
     if not resolved.is_file():
         raise FileNotFoundError(
