@@ -30,9 +30,11 @@ int tsplat_requests_abi_version(void);
  *   down: [slots][ceil(R/16)][ceil(K/32)][4][16][8], value (r, k) at [r/16][k/32][k%32/8][r%16][k%8];
  *   up:   [slots][ceil(N/16)][ceil(R/32)][4][16][8], value (n, r) at [n/16][r/32][r%32/8][n%16][r%8];
  * fp32: [slots][..][..][3][4][16][8] bf16, three planes whose sum is the value: its upper 16 bits, those of what is
- * left, and those of what is left then.  R = max_rank, 1..512; rank[a] <= R (a larger one counts as R).  16-byte aligned (-4).  M up to 2^27, K and N up
- * to 2^20, slots up to 2^20 (-2).  A row of x that holds an infinity or NaN gives NaN.  The factors of the products (x,
- * the adapter, the inner sums) count in steps of 2^-133 where fp32's own are finer, below 2^-110.
+ * left, and those of what is left then.  R = max_rank, 1..512; rank[a] <= R (a larger one counts as R).  16-byte
+ * aligned (-4).  M up to 2^27, K and N up to 2^20, slots up to 2^20 (-2).  A row of x that holds an infinity or NaN
+ * gives NaN.  A product of two factors is off by less than 2^-21 of it with fp32 adapters, 2^-22 with fp16, besides
+ * its sum's roundings.  The factors (x, the adapter, the inner sums) count in steps of 2^-133 where fp32's own are
+ * finer, below 2^-110.
  * scratch: at least tsplat_low_rank_scratch_bytes(...) of device memory that no other work uses until the call's
  * kernels are done (-5 when too small, -3 over another argument), 16-byte aligned.
  * The size is 0 for a call that needs none, and for sizes or a dtype that the call refuses. */
@@ -49,7 +51,8 @@ int tsplat_low_rank_add_async(const float* y, int64_t y_stride, const float* x, 
  * over `rows` (below 2^31) rows of `cols` fp32 values; b = row / rows_per_batch.
  * norm kinds: 0 none (post only), 1 LayerNorm, 2 RMS norm (x / sqrt(mean(x^2) + eps)); each with its weight and
  * bias [cols], either null.  gate null: 1; scale and shift: both or neither; their rows mod_stride floats apart
- * (gate: gate_stride), 0 for one row that serves every b.  x, h, out, normed rows are x_stride ... floats apart.  out may be x, normed may be h (same
+ * (gate: gate_stride), 0 for one row that serves every b.  x, h, out, normed rows are x_stride ... floats apart.
+ * Statistics are sums in fp32: a row whose squares pass its range has no norm.  out may be x, normed may be h (same
  * pointer and stride); other overlaps are refused (-3). */
 int tsplat_residual_norm_async(const float* x, int64_t x_stride, const float* h, int64_t h_stride, float* out,
                                int64_t out_stride, float* normed, int64_t normed_stride, int64_t rows, int cols,

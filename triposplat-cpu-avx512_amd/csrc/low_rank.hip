@@ -6,10 +6,11 @@
 // (8 + 8 + 8 bits, split by truncation, so exactly and without overflow), a bf16 weight one, an fp16 weight two, an
 // fp32 weight three; the smallest products of terms are left out (kProducts says what that costs).
 //
-// What bounds it: 12294 x 1024 -> 4096, rank 16, HBM: 453 MB in 90-92 us (5.0 TB/s; x 15, y 74).  16384 x 4096 -> 1024,
-// rank 64 in fp32 (402 MB, 79 us at a copy's rate): 119 us for one adapter, 147 where two requests meet; every 32 rows
-// read the adapter's 1.5 MB from L2, 1.05 GB at 11 TB/s, and the border tile's second adapter ends last.  Adapter values
-// staged in LDS for 64 or 128 rows were slower or no faster: a barrier a step of K, and t in parts.
+// What bounds it: 12294 x 1024 -> 4096, rank 16, HBM: 453 MB in 89-92 us (5.0 TB/s; x 18, y 74).  16384 x 4096 -> 1024,
+// rank 64 in fp32 (402 MB, 79 us at a copy's rate): 136-142 us for one adapter, 152 where two requests meet.  The first
+// kernel's waves wait for loads half of their time, two of them a SIMD for their 194 registers, while every 32 rows read
+// the adapter's 1.5 MB through L2 (0.97 GB at 9 TB/s, two thirds of it hits), and the border tile's second adapter ends
+// last.  Adapter values staged in LDS for 64 or 128 rows were slower or no faster: a barrier a step of K, and t in parts.
 //
 // Rows name their adapters in any order.  A workgroup handles a tile of rows and goes through the distinct adapters
 // that its rows name; the matrix products run over the whole row tile, and only the rows of that adapter are written,
@@ -104,9 +105,9 @@ struct Weights<kAdapterF32> {  // three planes of the tile, split when the bank 
 };
 
 // The products of an fp32 value's terms with a weight's that count: i + j <= 2, least first.  By truncation term 1 is
-// below 2^-7 of its value and term 2 below 2^-15, so what is left out is below 2^-22 of the product for fp16 weights (2
-// with 1), below 2^-21 for fp32 ones (1 with 2, 2 with 1, 2 with 2), nothing for bf16.  All terms have their value's sign:
-// it always takes from the product (0.7 x 2^-24 on average for fp32 weights, a sum's own roundings are more).
+// below 2^-7 of its value and term 2 below 2^-15, so what is left out is below 2^-22 of the product for fp16 weights
+// (2 with 1), below 2^-21 for fp32 ones (1 with 2, 2 with 1, 2 with 2), nothing for bf16.  All terms have their value's
+// sign: it always takes from the product (0.7 x 2^-24 on average for fp32 weights; a sum's own roundings are more).
 template <int TERMS>
 constexpr int kProducts = TERMS == 1 ? 3 : TERMS == 2 ? 5 : 6;
 template <int TERMS>
@@ -547,11 +548,11 @@ constexpr int kUnits = 256;  // compute units
 //     takes them sooner, and with large ranks sooner still (that call with one adapter: 45 us, one row tile 60; rank 64,
 //     4000 x 4096: 40, one 39).
 //   - With two row tiles the border between requests in a pass of its own.  It pays while a border's workgroup, which
-//     takes twice its time, would end last, and adds a turn of workgroups that mostly end at once: where borders are many
-//     (slots) or the rounds few.  K 1024, fp32, rank 64, without and with: 7100 rows of 2 requests 23.0, 21.5 us; 12294:
-//     35.7, 33.2; 16384: 37.0, 39.7; 33000: 71.2, 74.8; of 12 requests in 4 slots 7100: 26.9, 24.7; 16500: 39.7, 38.1;
-//     33000: 59.0, 61.2.  A round of workgroups that it would just overfill costs less than it gains for most requests
-//     (8192 rows: 4 % slower of 2 requests, 4 to 14 % faster of 12 to 256).
+//     takes twice its time, would end last, and adds a turn of workgroups that mostly end at once: where borders are
+//     many (slots) or the rounds few.  K 1024, fp32, rank 64, without and with: 7100 rows of 2 requests 23.0, 21.5 us;
+//     12294: 35.7, 33.2; 16384: 37.0, 39.7; 33000: 71.2, 74.8; of 12 requests in 4 slots 7100: 26.9, 24.7; 16500: 39.7,
+//     38.1; 33000: 59.0, 61.2.  Where it just overfills a round it still gains for most requests (8192 rows: 4 % slower
+//     of 2 requests, 4 to 14 % faster of 12 to 256).
 //   - Eight rank tiles, which read x once, only there and not for fp32's three planes, whose 96 registers are too many
 //     (16384 x 1024, rank 128: bf16 38 -> 26 us, fp16 52 -> 42; one row tile: fp16 45 -> 53).
 //   - Few rows leave the chip idle without the next two: 64 rows of an adapter each, K 1024 -> N 6144, rank 32, take 68
@@ -559,11 +560,11 @@ constexpr int kUnits = 256;  // compute units
 //     (1000 x 4096 x 4096, rank 128: two parts 44 us, four 57).
 //   - Eight column tiles read t and each adapter's border least, from where the waves come in many rounds (8202 x 6144:
 //     109 us, four 117; 12294 x 2900: 91, 98; but 14644 x 1743: 54, 49).  Two where few waves leave the chip idle (of 4
-//     adapters, rank 16: 300 x 600 7.9 us, four 8.4; 130 x 3000 7.9, 8.5; 130 x 5000 8.1, 8.7; rank 32 in fp16: 3000 x 400
-//     12.3, 11.7; 300 x 6000 12.0, 11.2).  A wave takes a turn for each adapter of its rows and loads their numbers and
-//     inner values anew, so those count as waves too, as many as slots spread over the rows let expect (of 64 adapters,
-//     rank 32 in fp16: 64 x 6144 14.5 us, four 13.8; 64 x 3000 12.7, 11.9; 130 x 3000 11.9, 11.7; but 300 x 600 9.8, 9.9).
-//     Many parts of K make each wave add up t again (336 rows, 3099 -> 1046, six parts: 18.2, four 13.3).
+//     adapters, rank 16: 300 x 600 7.9 us, four 8.4; 130 x 3000 7.9, 8.5; 130 x 5000 8.1, 8.7; rank 32 in fp16: 3000 x
+//     400 12.3, 11.7; 300 x 6000 12.0, 11.2).  A wave takes a turn for each adapter of its rows and loads their numbers
+//     and inner values anew, so those count as waves too, as many as slots spread over the rows let expect (of 64
+//     adapters, rank 32 in fp16: 64 x 6144 14.5 us, four 13.8; 64 x 3000 12.7, 11.9; 130 x 3000 11.9, 11.7; but 300 x
+//     600 9.8, 9.9).  Many parts of K make each wave add up t again (336 rows, 3099 -> 1046, six parts: 18.2, four 13.3).
 struct Plan {
   int row_tiles, rank_tiles, splits, down_passes, column_tiles, up_passes;
 };

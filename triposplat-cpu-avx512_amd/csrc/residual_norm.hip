@@ -164,7 +164,8 @@ __global__ __launch_bounds__(256) void residual_norm_kernel(ResidualNormParams p
   store_row(x, p.normed + row * p.normed_stride, c0, last);
 }
 
-// Rows too wide for registers: one workgroup a row, which is read again for each sum (1302 x 12288: 91 us, 2.8 TB/s).
+// Rows too wide for registers: one workgroup a row, which is read again for each sum (1302 x 12288: 93 us, 2.8 TB/s at
+// one pass' bytes; 174 with both norms).
 constexpr int kWideThreads = 1024;
 
 __device__ float block_sum(float v, float* lds) {
