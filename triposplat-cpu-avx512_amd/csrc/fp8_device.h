@@ -1,0 +1,77 @@
+// Device side of the 8-bit rows, shared by the kernels that make them and those that multiply them.
+#pragma once
+
+#include <hip/hip_bf16.h>
+#include <hip/hip_fp16.h>
+
+#include <type_traits>
+
+#include "fp8.h"
+#include "tsplat_common.h"
+
+namespace tsplat {
+
+typedef int intx4 __attribute__((ext_vector_type(4)));
+typedef int intx8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16_t;
+typedef _Float16 half_t;
+
+template <class T>
+struct Vec4;
+template <>
+struct Vec4<float> {
+  typedef float type __attribute__((ext_vector_type(4)));
+};
+template <>
+struct Vec4<bf16_t> {
+  typedef bf16_t type __attribute__((ext_vector_type(4)));
+};
+template <>
+struct Vec4<half_t> {
+  typedef half_t type __attribute__((ext_vector_type(4)));
+};
+
+// Values 4 at a time from k on, zero past K; VEC: the row's quadruples are aligned to their size.
+template <class T, bool VEC>
+__device__ __forceinline__ floatx4 load4(const T* row, int k, int K) {
+  floatx4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (VEC && k + 4 <= K) {
+    const typename Vec4<T>::type u = *reinterpret_cast<const typename Vec4<T>::type*>(row + k);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = (float)u[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (k + i < K) v[i] = (float)row[k + i];
+  }
+  return v;
+}
+
+// The bits of |v| where it is finite, else 0: their largest is that of the block's finite magnitudes.
+__device__ __forceinline__ uint32_t finite_bits(float v) {
+  const uint32_t u = __float_as_uint(v) & 0x7fffffffu;
+  return u < 0x7f800000u ? u : 0u;
+}
+
+// The exponent (+ 127) of the block's scale from its largest magnitude's bits: the smallest e with
+// largest / 2^e <= 448 = 1.75 * 2^8, at least -127; 0 for a block of zeros.
+__device__ __forceinline__ int scale_exponent(uint32_t top) {
+  const int e = (int)(top >> 23) - 8 + ((top & 0x7fffffu) > 0x600000u ? 1 : 0);
+  return top == 0 ? 127 : max(e, 0);
+}
+
+// 2^-(e - 127), a normal number: e is 247 at most.
+__device__ __forceinline__ float inverse_scale(int e) { return __uint_as_float((uint32_t)(254 - e) << 23); }
+
+// Four codes of v * inverse.  The product is exact (a subnormal one is far below half of the smallest code), so there
+// is one rounding, the conversion's, to nearest even; 448 is never passed.  An infinity becomes a NaN like a NaN.
+__device__ __forceinline__ int encode4(const floatx4& v, float inverse) {
+  float u[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    u[i] = (__float_as_uint(v[i]) & 0x7f800000u) == 0x7f800000u ? __uint_as_float(0x7fc00000u) : v[i] * inverse;
+  int w = __builtin_amdgcn_cvt_pk_fp8_f32(u[0], u[1], 0, false);
+  return __builtin_amdgcn_cvt_pk_fp8_f32(u[2], u[3], w, true);
+}
+
+}  // namespace tsplat

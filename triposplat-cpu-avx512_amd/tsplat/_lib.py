@@ -102,6 +102,15 @@ REQUEST_SIGNATURES = {
                                + [_i, ctypes.c_float] + [_i] * 5 + [_vp], _i),
 }
 
+# 8-bit rows and products; declared in include/tsplat_hip_fp8.h, with a version of their own.
+FP8_SIGNATURES = {
+    "tsplat_fp8_abi_version": ([], _i),
+    "tsplat_fp8_quantize_async": ([_vp, _i, _i64, _i, _i] + [_vp] * 3, _i),
+    "tsplat_fp8_linear_scratch_bytes": ([_i] * 4, _i64),
+    "tsplat_fp8_linear_async": ([_vp, _i, _i64] + [_vp] * 5 + [_i, _vp, _i64, _i64, _vp, _i64, _vp, _i, _i64]
+                                + [_i] * 3 + [_vp, _i64, _vp], _i),
+}
+
 STATUS_TEXT = {
     -1: "null pointer",
     -2: "bad sizes / stages / head dim",
@@ -121,6 +130,8 @@ STATUS_TEXT = {
 ABI_VERSION = 5
 # tsplat_requests_abi_version(), likewise, of REQUEST_SIGNATURES.
 REQUESTS_ABI_VERSION = 1
+# tsplat_fp8_abi_version(), of FP8_SIGNATURES.
+FP8_ABI_VERSION = 1
 
 _CACHE: dict[str | None, ctypes.CDLL] = {}  # by resolved name; None: DEFAULT_LIBRARY, which needs no resolving
 
@@ -165,18 +176,21 @@ def load_library(path: str | os.PathLike | None = None) -> ctypes.CDLL:
             f"{resolved} reports ABI version {found}, these bindings expect {ABI_VERSION}; "
             "rebuild it with `make -C triposplat-cpu-avx512_amd`"
         )
-    for name, (argtypes, restype) in REQUEST_SIGNATURES.items():
-        fn = getattr(lib, name, None)
-        if fn is None:
-            raise RuntimeError(f"{resolved} has no {name}; rebuild it with `make -C triposplat-cpu-avx512_amd`")
-        fn.argtypes = argtypes
-        fn.restype = restype
-    found = lib.tsplat_requests_abi_version()
-    if found != REQUESTS_ABI_VERSION:
-        raise RuntimeError(
-            f"{resolved} reports version {found} of its request operators, these bindings expect "
-            f"{REQUESTS_ABI_VERSION}; rebuild it with `make -C triposplat-cpu-avx512_amd`"
-        )
+    for signatures, version, expected, what in (
+            (REQUEST_SIGNATURES, "tsplat_requests_abi_version", REQUESTS_ABI_VERSION, "request operators"),
+            (FP8_SIGNATURES, "tsplat_fp8_abi_version", FP8_ABI_VERSION, "8-bit products")):
+        for name, (argtypes, restype) in signatures.items():
+            fn = getattr(lib, name, None)
+            if fn is None:
+                raise RuntimeError(f"{resolved} has no {name}; rebuild it with `make -C triposplat-cpu-avx512_amd`")
+            fn.argtypes = argtypes
+            fn.restype = restype
+        found = getattr(lib, version)()
+        if found != expected:
+            raise RuntimeError(
+                f"{resolved} reports version {found} of its {what}, these bindings expect {expected}; "
+                "rebuild it with `make -C triposplat-cpu-avx512_amd`"
+            )
     _CACHE[key] = lib
     return lib
 
@@ -234,10 +248,23 @@ def no_gradients(torch, *tensors) -> None:
                              "torch.no_grad() and outside of dual levels, or detach its inputs")
 
 
+def matrix_rows(torch, name, t, dtype) -> tuple[int, int, int]:
+    """(rows, columns, row stride) of a GPU tensor [..., columns] of this type whose rows lie at one stride."""
+    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype is dtype and t.dim() > 0 and t.shape[-1] > 0):
+        raise ValueError(f"{name} must be a [..., columns] GPU tensor of {dtype}")
+    cols = t.shape[-1]
+    rows, stride = _rows_at_one_stride(name, t, cols)
+    return rows, cols, stride
+
+
 def rows_of(torch, name, t, cols) -> tuple[int, int]:
     """(rows, row stride) of a GPU fp32 tensor [..., cols] whose rows lie at one stride; ValueError otherwise."""
     if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype is torch.float32):
         raise ValueError(f"{name} must be an fp32 GPU tensor")
+    return _rows_at_one_stride(name, t, cols)
+
+
+def _rows_at_one_stride(name, t, cols) -> tuple[int, int]:
     shape = t.shape
     if len(shape) == 0 or shape[-1] != cols:
         raise ValueError(f"{name} must have {cols} columns, its shape is {list(shape)}")
