@@ -1,0 +1,57 @@
+// The plan of a ragged cross attention: its layout, what its header says, and the tiles that the kernels take.
+#pragma once
+
+#include <stdint.h>
+
+namespace tsplat {
+
+// The plan's ints: the header, then `items` work items of kCrossItem ints, then `joins` of kCrossJoin.
+enum CrossHeader : int {
+  kPlanMagic = 0, kPlanInts, kPlanItems, kPlanJoins, kPlanParts, kPlanRows, kPlanStates, kPlanHeads, kPlanKvHeads,
+  kPlanDim, kPlanType, kPlanTerms, kPlanFew, kPlanHeaderInts = 16
+};
+constexpr int32_t kPlanMagicValue = 0x54435031;
+
+// One workgroup's work for one key head: `rows` rows from row0 of a request's query rows, where a row is a query token
+// and one of the group's heads (row = token * group + head), against `keys` states from key0 on.
+// part: where the partial result goes, or -1: the result itself.
+struct CrossItem {
+  int32_t token0;  // the request's first query token
+  int32_t row0, rows;
+  int32_t key0, keys;
+  int32_t part;
+  int32_t unused[2];
+};
+// The same rows' partial results, `parts` of them from first_part on, become the result.
+struct CrossJoin {
+  int32_t token0, row0, rows, first_part, parts;
+  int32_t unused[3];
+};
+constexpr int kCrossItem = sizeof(CrossItem) / 4, kCrossJoin = sizeof(CrossJoin) / 4;
+
+// Head sizes are padded to one of these.
+constexpr int cross_padded_dim(int dim) { return dim <= 64 ? 64 : dim <= 96 ? 96 : 128; }
+
+// A workgroup: wq waves of 32 rows times wk waves that share the keys of a tile, kb blocks of 32 keys each, bufs buffers.
+// few: at most 32 rows a request, where reading the keys is all.
+struct CrossTile {
+  int wq, wk, kb, bufs;
+};
+constexpr CrossTile cross_tile(int padded, int terms, bool few) {
+  if (few) return terms == 3 && padded > 64 ? CrossTile{1, 2, 1, 1} : CrossTile{1, 4, 1, 1};
+  if (terms == 3) return CrossTile{8, 1, padded > 64 ? 1 : 2, 2};
+  if (terms == 2) return CrossTile{8, 1, padded > 64 ? 1 : 2, 2};
+  return CrossTile{4, 1, 2, 2};
+}
+
+// Writes the plan (null: only counts); its size in ints, or a negative status.
+int64_t make_cross_plan(const int32_t* q_lengths, const int32_t* k_lengths, int requests, int heads, int kv_heads,
+                        int head_dim, int dtype, int precision, int compute_units, int32_t* plan, int64_t plan_ints);
+
+// Floats of one part and key head: the rows' sums of padded columns, then their maxima, then their denominators.
+inline int64_t cross_part_floats(const int32_t* header) {
+  const int padded = cross_padded_dim(header[kPlanDim]);
+  return (int64_t)cross_tile(padded, header[kPlanTerms], header[kPlanFew] != 0).wq * 32 * (padded + 2);
+}
+
+}  // namespace tsplat

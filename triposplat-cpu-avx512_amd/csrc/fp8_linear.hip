@@ -431,11 +431,7 @@ int launch_out(const Fp8LinearParams& p, hipStream_t stream) {
     if (st != kOk) return st;
     xc = codes, xe = exps;
   }
-#ifdef CFG
-  return launch_tiles<CFG, TO>(p, xc, xe, f, veco, stream);
-#else
   return launch_tiles<128, 256, 2, 2, 64, 3, TO>(p, xc, xe, f, veco, stream);
-#endif
 }
 
 }  // namespace

@@ -111,6 +111,15 @@ FP8_SIGNATURES = {
                                 + [_i] * 3 + [_vp, _i64, _vp], _i),
 }
 
+# Cross attention over requests of their own lengths; declared in include/tsplat_hip_cross.h, with a version of its own.
+CROSS_SIGNATURES = {
+    "tsplat_cross_abi_version": ([], _i),
+    "tsplat_cross_plan": ([_vp] * 2 + [_i] * 6 + [_vp, _i64], _i64),
+    "tsplat_cross_scratch_bytes": ([_vp], _i64),
+    "tsplat_cross_attention_async": ([_vp, _i64, _i64] * 3 + [_vp, ctypes.c_float, _vp, _i64, _i64] + [_vp] * 3
+                                     + [_i64, _vp], _i),
+}
+
 STATUS_TEXT = {
     -1: "null pointer",
     -2: "bad sizes / stages / head dim",
@@ -132,6 +141,8 @@ ABI_VERSION = 5
 REQUESTS_ABI_VERSION = 1
 # tsplat_fp8_abi_version(), of FP8_SIGNATURES.
 FP8_ABI_VERSION = 1
+# tsplat_cross_abi_version(), of CROSS_SIGNATURES.
+CROSS_ABI_VERSION = 1
 
 _CACHE: dict[str | None, ctypes.CDLL] = {}  # by resolved name; None: DEFAULT_LIBRARY, which needs no resolving
 
@@ -178,7 +189,8 @@ def load_library(path: str | os.PathLike | None = None) -> ctypes.CDLL:
         )
     for signatures, version, expected, what in (
             (REQUEST_SIGNATURES, "tsplat_requests_abi_version", REQUESTS_ABI_VERSION, "request operators"),
-            (FP8_SIGNATURES, "tsplat_fp8_abi_version", FP8_ABI_VERSION, "8-bit products")):
+            (FP8_SIGNATURES, "tsplat_fp8_abi_version", FP8_ABI_VERSION, "8-bit products"),
+            (CROSS_SIGNATURES, "tsplat_cross_abi_version", CROSS_ABI_VERSION, "cross attention")):
         for name, (argtypes, restype) in signatures.items():
             fn = getattr(lib, name, None)
             if fn is None:
