@@ -19,7 +19,8 @@ int tsplat_fp8_abi_version(void);
 
 /* Rows of K values in 8 bits.  codes: [rows][Kp], Kp = K rounded up to 128, e4m3 (1 sign, 4 exponent, 3 fraction bits,
  * largest 448, no infinity), zero past K; exponents: [rows][Ke], Ke = Kp / 128 rounded up to 4, block b of a row
- * stands for codes * 2^(exponents[b] - 127); 127 past the last block.  Both 16-byte aligned (-4).
+ * stands for codes * 2^(exponents[b] - 127); 127 past the last block.  codes 16-byte aligned, exponents 4-byte (-4): a
+ * run of rows is such rows again.
  *
  * The scale is the smallest power of two, 2^-127 at least, that brings the block's largest finite magnitude to 448 or
  * below (1 for a block without one), a code the nearest value of x / scale, ties to even; an infinity or NaN gives a

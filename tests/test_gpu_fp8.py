@@ -211,3 +211,28 @@ def test_graph_and_streams(cuda, hiplib):
         torch.cuda.synchronize()
         for (_, y), e in zip(graphs, eager):
             assert torch.equal(y, e), turn
+
+
+def test_refusals(cuda, hiplib):
+    import torch
+    from tsplat.fp8 import fp8_linear, quantize_blocks
+
+    x, w, bias, residual, _ = _linear_case(torch, cuda, 70, 130, 40, "float32", 1)
+    weight, gate = quantize_blocks(w), torch.ones(2, 40, device=cuda)
+    for bad in (x.double(), x.cpu(), x.t(), None, x[:, :0], x.clone().requires_grad_()):
+        with pytest.raises(ValueError):
+            quantize_blocks(bad)
+        with pytest.raises(ValueError):
+            fp8_linear(bad, weight)
+    for args, kwargs in (((x, w), {}), ((x[:, :129], weight), {}), ((x, weight, bias[:39]), {}),
+                         ((x, weight, bias.half()), {}), ((x, weight), dict(activation="relu")),
+                         ((x, weight), dict(gate=gate[:, :39])), ((x, weight), dict(gate=torch.ones(3, 40, device=cuda))),
+                         ((x, weight), dict(gate=gate.double())), ((x, weight), dict(residual=residual[:69])),
+                         ((x, weight), dict(residual=residual, out_dtype=torch.half)),
+                         ((x, weight), dict(out=residual[:, :39])), ((x, weight), dict(out_dtype=torch.float64)),
+                         ((x, weight), dict(gate=gate[:1].expand(2, -1))), ((x, weight, bias.clone().requires_grad_()), {})):
+        with pytest.raises(ValueError):
+            fp8_linear(*args, **kwargs)
+    with pytest.raises(RuntimeError, match="-3"):
+        fp8_linear(x, weight, out=x[:, :40])
+    assert quantize_blocks(x[:0]).codes.shape == (0, 130) and fp8_linear(x[:0], weight).shape == (0, 40)

@@ -40,7 +40,7 @@ int tsplat_fp8_quantize_async(const void* x, int dtype, int64_t x_stride, int ro
   const Span in = span_rows(x, x_stride, rows, K, size_of(dtype));
   const Span c = span_whole(codes, rows * fp8_code_stride(K)), e = span_whole(exponents, rows * fp8_exponent_stride(K));
   if (!apart(c, in) || !apart(e, in) || !apart(c, e)) return kErrRange;
-  if (!aligned_to(x, size_of(dtype)) || !aligned16(codes) || !aligned16(exponents)) return kErrAlign;
+  if (!aligned_to(x, size_of(dtype)) || !aligned16(codes) || !aligned_to(exponents, 4)) return kErrAlign;
   DeviceRanges ptrs;
   TSPLAT_CHECK(ptrs.check(x, in.bytes()));
   TSPLAT_CHECK(ptrs.check(codes, c.bytes()));
@@ -88,8 +88,8 @@ int tsplat_fp8_linear_async(const void* x, int x_dtype, int64_t x_stride, const 
   if (residual && !same_rows(so, sr) && !apart(so, sr)) return kErrRange;
   if (room.p && (!apart(room, so) || (residual && !apart(room, sr)))) return kErrRange;
   if ((x && !aligned_to(x, xs)) || !aligned_to(out, os) || !aligned_to(residual, os) || !aligned_to(bias, 4) ||
-      !aligned_to(gate, 4) || !aligned16(w_codes) || !aligned16(w_exponents) || !aligned16(scratch) ||
-      (!x && (!aligned16(x_codes) || !aligned16(x_exponents))))
+      !aligned_to(gate, 4) || !aligned16(w_codes) || !aligned_to(w_exponents, 4) || !aligned16(scratch) ||
+      (!x && (!aligned16(x_codes) || !aligned_to(x_exponents, 4))))
     return kErrAlign;
   DeviceRanges ptrs;
   TSPLAT_CHECK(ptrs.check(out, so.bytes()));

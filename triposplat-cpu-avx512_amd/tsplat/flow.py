@@ -43,10 +43,13 @@ import math
 from dataclasses import dataclass
 
 from . import block_ops as bo
+from .cross_attention import CrossPlan
+from .fp8 import Fp8Rows, fp8_linear, quantize_blocks
 from .native_sampler_backend import NativeSamplerBackend
 from .native_sdpa_ctypes import native_sdpa_f32_ex
-from .nf24 import bf16_planes, nf24_linear, precision_id, quantize_nf24_i16_per_output_channel
-from .qkv import RopeAxes, gemm_nf24_qkv_direct
+from .nf24 import (bf16_planes, decode_nf24_i16_weight, nf24_linear, precision_id,
+                   quantize_nf24_i16_per_output_channel)
+from .qkv import RopeAxes, gemm_nf24_qkv_direct, qkv_rope_rmsnorm_pack
 
 
 @dataclass(frozen=True)
@@ -88,12 +91,21 @@ class PackedLinear:
         self.out_features = int(code01_t.shape[1])
         self.precision = "fp32"  # GEMM product precision (tsplat.nf24.PRECISIONS)
         self.planes = None       # bf16 weight planes of self.precision (tsplat.nf24.bf16_planes)
+        self.rows8 = None        # the weight in 8 bits of precision "fp8" (tsplat.fp8.quantize_blocks)
 
     def set_precision(self, precision, planes=True):
         """Product precision of this Linear; with planes, a bf16 mode reads
         the weights from bf16 planes built here once (same results, 2 or 4
-        bytes per weight) instead of decoding the codes in every call."""
+        bytes per weight) instead of decoding the codes in every call.
+        "fp8": the weight in 8 bits, built here once, and the activations
+        brought to 8 bits in every call."""
+        if precision == "fp8":
+            if self.rows8 is None:
+                self.rows8 = quantize_blocks(decode_nf24_i16_weight(self.code01_t, self.q2_t, self.scale))
+            self.precision, self.planes = precision, None
+            return
         precision_id(precision)
+        self.rows8 = None
         self.precision = precision
         if precision == "fp32" or not planes:
             self.planes = None
@@ -108,18 +120,42 @@ class PackedLinear:
         codes, scales, _ = quantize_nf24_i16_per_output_channel(w)
         return cls(codes[0], codes[1], scales[0], b)
 
+    @property
+    def kv_layout(self):
+        """The layout of qkv_direct's k/v that this Linear's precision stores itself, for the SDPA after it."""
+        return "packed" if self.precision == "fp8" else "bhld"
+
     def __call__(self, x2, out=None, output_start=0, output_count=None):
+        """x2: [M, K] fp32, or its Fp8Rows in precision "fp8"."""
+        if self.precision == "fp8":
+            count = self.out_features - output_start if output_count is None else output_count
+            if output_start == 0 and count == self.out_features:
+                return fp8_linear(x2, self.rows8, self.bias, out=out)
+            return fp8_linear(x2, self.rows8.narrow(output_start, count), self.bias[output_start:output_start + count],
+                              out=out)
         return nf24_linear(x2, self.code01_t, self.q2_t, self.scale, self.bias, out=out,
                            output_start=output_start, output_count=output_count, precision=self.precision,
                            planes=self.planes)
 
     def epilogue(self, x2, kind, out=None, gate=None):
         """This Linear with a fused elementwise epilogue (block_ops.EPILOGUE_*)."""
+        if self.precision == "fp8":
+            if kind == bo.EPILOGUE_GELU:
+                return fp8_linear(x2, self.rows8, self.bias, activation="gelu", out=out)
+            if kind not in (bo.EPILOGUE_GATED, bo.EPILOGUE_ADD) or out is None or (
+                    (gate is None) != (kind == bo.EPILOGUE_ADD)):
+                raise ValueError("the residual epilogues update `out` in place, EPILOGUE_GATED with a gate")
+            return fp8_linear(x2, self.rows8, self.bias, gate=gate, residual=out, out=out)
         return bo.nf24_linear_epilogue(x2, self.code01_t, self.q2_t, self.scale, self.bias, kind,
                                        out=out, gate=gate, precision=self.precision, planes=self.planes)
 
     def qkv_direct(self, x2, freqs, q_gamma, k_gamma, B, L, H, kv_layout="packed"):
-        """Fused QKV projection + RoPE/RMSNorm (tsplat.qkv.gemm_nf24_qkv_direct)."""
+        """Fused QKV projection + RoPE/RMSNorm (tsplat.qkv.gemm_nf24_qkv_direct); in precision "fp8" the
+        projection and the postprocess after it, which stores k/v packed only."""
+        if self.precision == "fp8":
+            if kv_layout != "packed":
+                raise ValueError("precision 'fp8' stores k/v packed (PackedLinear.kv_layout)")
+            return qkv_rope_rmsnorm_pack(self(x2), freqs, q_gamma, k_gamma, B, L, H)
         return gemm_nf24_qkv_direct(x2, self.code01_t, self.q2_t, self.scale, self.bias, freqs,
                                     q_gamma, k_gamma, B, L, H, precision=self.precision,
                                     kv_layout=kv_layout, planes=self.planes)
@@ -130,11 +166,15 @@ class PackedLinear:
 
 def set_model_precision(model, precision, include=("blocks",), planes=True):
     """Product precision of a flow model ("fp32" strict, or the opt-in
-    "bf16" / "bf16x3"): "blocks" in include sets the block Linears, "io" the
-    timestep / input / output Linears, "attention" the SDPA products (Q K^T
-    and P V); what include does not name stays fp32.  planes: the bf16-mode
-    Linears build their bf16 weight planes now (PackedLinear.set_precision)."""
-    precision_id(precision)
+    "bf16" / "bf16x3" / "fp8"): "blocks" in include sets the block Linears,
+    "io" the timestep / input / output Linears, "attention" the SDPA products
+    (Q K^T and P V; not in "fp8"); what include does not name stays fp32.
+    planes: the bf16-mode Linears build their bf16 weight planes now
+    (PackedLinear.set_precision)."""
+    if precision != "fp8":
+        precision_id(precision)
+    elif "attention" in include:
+        raise ValueError("precision 'fp8' is of Linears, not of the attention's products")
     for blk in model.blocks:
         for lin in blk.lin.values():
             lin.set_precision(precision if "blocks" in include else "fp32", planes)
@@ -240,10 +280,9 @@ class FlowModel:
         return t_emb, t_mod
 
     def block_forward(self, blk: FlowBlock, x, cond, t_mod):
-        """x [B, L, C] (updated in place and returned), cond [B, Lc, C], t_mod [B, 6C]."""
+        """x [B, L, C] (updated in place and returned), cond [B, Lc, C] or condition_rows of it, t_mod [B, 6C]."""
         cfg = self.cfg
         B, L, C = (int(s) for s in x.shape)
-        Lc = int(cond.shape[1])
         H = cfg.heads
         mod = t_mod.clone()  # [B, 6C] = t_mod + shift_table, chunks (shift, scale, gate) x 2
         for b in range(B):
@@ -257,14 +296,16 @@ class FlowModel:
         # [B, H, L, 64], exact SDPA, NF24 out with the gated residual in its epilogue
         h = bo.layer_norm(x, cfg.ln_eps, scale=scale_msa, shift=shift_msa)
         q, k, v = lin["qkv"].qkv_direct(h.view(B * L, C), self.freqs(L), blk.q_gamma, blk.k_gamma,
-                                        B, L, H, kv_layout="bhld")
-        a = native_sdpa_f32_ex(q, k, v, out_layout="blhd", precision=self.attention_precision)
+                                        B, L, H, kv_layout=lin["qkv"].kv_layout)
+        a = native_sdpa_f32_ex(q, k, v, kv_packed=lin["qkv"].kv_layout == "packed", key_count=L, out_layout="blhd",
+                               precision=self.attention_precision)
         lin["out"].epilogue(a.view(B * L, C), bo.EPILOGUE_GATED, out=x2, gate=gate_msa)
 
         # cross attention to the condition tokens (no RoPE)
         h = bo.layer_norm(x, cfg.ln_eps, blk.xnorm_w, blk.xnorm_b)
         xq = bo.head_rmsnorm(lin["xq"](h.view(B * L, C)), blk.xq_gamma, B, L, H)
-        kv = lin["xkv"](cond.reshape(B * Lc, C))  # [B*Lc, 2C] = [k | v]
+        kv = lin["xkv"](cond if isinstance(cond, Fp8Rows) else cond.reshape(-1, C))  # [B*Lc, 2C] = [k | v]
+        Lc = kv.shape[0] // B
         xk = bo.head_rmsnorm(kv, blk.xk_gamma, B, Lc, H, token_stride=2 * C)
         xv = bo.head_rmsnorm(kv[:, C:], None, B, Lc, H, token_stride=2 * C, normalize=False)
         a = native_sdpa_f32_ex(xq, xk, xv, out_layout="blhd", precision=self.attention_precision)
@@ -276,25 +317,44 @@ class FlowModel:
         lin["fc2"].epilogue(h, bo.EPILOGUE_GATED, out=x2, gate=gate_mlp)
         return x
 
-    def velocity(self, z, cond, t, observe=None, *, adapters=None, slots=None, positions=None, rope=None):
+    def condition_plan(self, tokens, lengths):
+        """The plan of a batch whose entries bring conditions of their own
+        lengths, any of them 0, for velocity(cond_plan=...): tokens latent
+        tokens in each entry.  Made once, for all steps and blocks; it keeps
+        the attention precision that the model has now."""
+        return CrossPlan([tokens] * len(lengths), lengths, self.cfg.heads, self.cfg.head_dim,
+                         precision=self.attention_precision, device=self.device)
+
+    def condition_rows(self, cond2):
+        """cond2 [rows, C] as the blocks' condition Linears read it: in 8 bits, once for all blocks, where all of
+        them multiply in precision "fp8"."""
+        if cond2.shape[0] and self.blocks and all(blk.lin["xkv"].precision == "fp8" for blk in self.blocks):
+            return quantize_blocks(cond2)
+        return cond2
+
+    def velocity(self, z, cond, t, observe=None, *, adapters=None, slots=None, positions=None, rope=None,
+                 cond_plan=None):
         """z [B, L, C], cond [B, Lc, C], t [B] (already x1000) -> v [B, L, C].
         adapters (flow_requests.FlowAdapters) with slots, one of them per
-        batch entry, or positions with rope (qkv.RopeAxes): the batch's
-        requests with their own adapters and latent positions
-        (flow_requests.velocity).
+        batch entry, positions with rope (qkv.RopeAxes), or cond_plan
+        (condition_plan; cond is then [rows, C], the entries' conditions one
+        after the other): the batch's requests with their own adapters,
+        latent positions and conditions (flow_requests.velocity).
         observe(i, x), when given, sees the hidden state x entering block i,
         and observe(len(blocks), x) the state the final layer receives (for
         checks that recompute single blocks elsewhere; x is updated in place
         afterwards, so keep a copy)."""
-        if adapters is not None or slots is not None or positions is not None or rope is not None:
+        if any(a is not None for a in (adapters, slots, positions, rope, cond_plan)):
             from . import flow_requests
 
             return flow_requests.velocity(self, z, cond, t, adapters=adapters, slots=slots, positions=positions,
-                                          rope=rope, observe=observe)
+                                          rope=rope, cond_plan=cond_plan, observe=observe)
         torch = self.torch
         B, L, C = (int(s) for s in z.shape)
         t_emb, t_mod = self.timestep(t)
         x = self.input_layer(z.reshape(B * L, C)).view(B, L, C)
+        rows = self.condition_rows(cond.reshape(-1, C))
+        cond = rows if isinstance(rows, Fp8Rows) else cond
         for i, blk in enumerate(self.blocks):
             if observe is not None:
                 observe(i, x)

@@ -150,9 +150,9 @@ class JointFlowModel:
         lin = blk.lin
         h = bo.layer_norm(x, cfg.ln_eps, scale=cm, shift=sm)
         q, k, v = lin["qkv"].qkv_direct(h.view(Ltot, C), self.freqs(L, Ltot - L), blk.q_gamma,
-                                        blk.k_gamma, 1, Ltot, H, kv_layout="bhld")
-        a = native_sdpa_f32_ex(q, k, v, key_bias=key_bias, out_layout="blhd",
-                               precision=self.attention_precision)
+                                        blk.k_gamma, 1, Ltot, H, kv_layout=lin["qkv"].kv_layout)
+        a = native_sdpa_f32_ex(q, k, v, kv_packed=lin["qkv"].kv_layout == "packed", key_count=Ltot,
+                               key_bias=key_bias, out_layout="blhd", precision=self.attention_precision)
         x2 = x.view(Ltot, C)
         lin["out"].epilogue(a.view(Ltot, C), bo.EPILOGUE_GATED, out=x2, gate=gm)
         h = bo.layer_norm(x, cfg.ln_eps, scale=c2, shift=s2)

@@ -1,9 +1,11 @@
-"""The flow model over a batch of requests with adapters and latent positions of their own.
+"""The flow model over a batch of requests with adapters, latent positions and conditions of their own.
 
-The graph is FlowModel.velocity's (flow.py), with two additions: each batch
+The graph is FlowModel.velocity's (flow.py), with three additions: each batch
 entry may name a slot of low-rank adapters beside the blocks' packed Linears
-(FlowAdapters), and the latent tokens' rotary positions may have several axes
-(time, height, width) and differ from request to request (qkv.RopeAxes).
+(FlowAdapters), the latent tokens' rotary positions may have several axes
+(time, height, width) and differ from request to request (qkv.RopeAxes), and
+the entries' conditions may have lengths of their own, none among them
+(cross_attention.CrossPlan).
 An adapter's part has to be added before what follows the projection, so the
 GEMM's fused epilogues do not apply: a Linear stores its projection,
 low_rank_add adds to it in place, and the step after it is a pass of its own
@@ -14,6 +16,7 @@ from __future__ import annotations
 
 from . import block_ops as bo
 from .adapters import AdapterBank, low_rank_add
+from .cross_attention import CrossPlan, cross_attention
 from .native_sdpa_ctypes import native_sdpa_f32_ex
 from .qkv import qkv_rope_axes
 
@@ -61,21 +64,38 @@ class FlowAdapters:
                 bank.unload(slot)
 
 
-def _adapted(lin, x2, bank, rows):
-    out = lin(x2)
+def _adapted(lin, x2, bank, rows, made=None):
+    """made: x2 as the packed Linear reads it, where that is another form."""
+    out = lin(x2 if made is None else made)
     return out if bank is None or rows is None else low_rank_add(out, x2, bank, rows, out=out)
 
 
-def velocity(model, z, cond, t, *, adapters=None, slots=None, positions=None, rope=None, observe=None):
+def _check_plan(model, plan, cond, B, L):
+    """That this plan is of this batch: its lengths are not read again."""
+    if not isinstance(plan, CrossPlan):
+        raise ValueError("cond_plan must be a CrossPlan (FlowModel.condition_plan)")
+    if plan.q_lengths != [L] * B or (plan.heads, plan.kv_heads, plan.head_dim) != (
+            model.cfg.heads, model.cfg.heads, model.cfg.head_dim) or plan.dtype is not model.torch.float32:
+        raise ValueError(f"cond_plan must be of {B} entries of {L} latent tokens and the model's heads, in fp32")
+    if cond.dim() != 2 or cond.shape[0] != plan.states:
+        raise ValueError(f"with this cond_plan cond is [{plan.states}, {model.cfg.hidden}]")
+
+
+def velocity(model, z, cond, t, *, adapters=None, slots=None, positions=None, rope=None, cond_plan=None, observe=None):
     """z [B, L, C], cond [B, Lc, C], t [B] (already x1000) -> v [B, L, C], as FlowModel.velocity.
     adapters: FlowAdapters, slots: one slot for each batch entry (-1 for none).  positions [L, axes] or
     [B, L, axes] with rope, a RopeAxes of the model's head size: the latent tokens' places; without them the
-    token's index on one axis, as in FlowModel.velocity.  Nothing is copied from the host: after one call on the
+    token's index on one axis, as in FlowModel.velocity.  cond_plan: FlowModel.condition_plan of the entries' lengths;
+    cond is then [rows, C], their conditions one after the other, and an entry without one gets nothing from the cross
+    attention but its output Linear's bias.  Nothing is copied from the host: after one call on the
     stream it can be captured into a HIP graph, which keeps the slots' numbers and reads what they hold when it is
     replayed."""
     torch, cfg = model.torch, model.cfg
     B, L, C = (int(s) for s in z.shape)
-    Lc, H = int(cond.shape[1]), cfg.heads
+    H = cfg.heads
+    if cond_plan is not None:
+        _check_plan(model, cond_plan, cond, B, L)
+    lengths = [int(cond.shape[1])] * B if cond_plan is None else cond_plan.k_lengths
     if (positions is None) != (rope is None):
         raise ValueError("positions and rope go together")
     if (adapters is None) != (slots is None):
@@ -91,19 +111,24 @@ def velocity(model, z, cond, t, *, adapters=None, slots=None, positions=None, ro
         of_entry = torch.empty(B, 1, dtype=torch.int32, device=model.device)
         for b, s in enumerate(slots):
             of_entry[b].fill_(max(s, -1))
-        rows, cond_rows = (of_entry.expand(B, n).contiguous().view(-1) for n in (L, Lc))
+        rows = of_entry.expand(B, L).contiguous().view(-1)
+        cond_rows, start = torch.empty(sum(lengths), dtype=torch.int32, device=model.device), 0
+        for n, s in zip(lengths, slots):
+            cond_rows[start:start + n].fill_(max(s, -1))
+            start += n
     if rope is None:
         rope = model.token_rope()
         positions = torch.arange(L, dtype=torch.int32, device=model.device)[:, None]
     t_emb, t_mod = model.timestep(t)
     x = model.input_layer(z.reshape(B * L, C)).view(B, L, C)
-    cond2 = cond.reshape(B * Lc, C)
+    cond2 = cond.reshape(sum(lengths), C)
+    cond_made = model.condition_rows(cond2)
     branch = gate = None  # the last branch's output, not yet added to x, and its gate
     for i, blk in enumerate(model.blocks):
         banks = adapters.banks[i] if adapters is not None else {}
 
-        def linear(name, x2, at=rows):
-            return _adapted(blk.lin[name], x2, banks.get(name), at)
+        def linear(name, x2, at=rows, made=None):
+            return _adapted(blk.lin[name], x2, banks.get(name), at, made)
 
         mod = t_mod.clone()  # [B, 6C] = t_mod + shift_table, chunks (shift, scale, gate) x 2
         for b in range(B):
@@ -128,17 +153,31 @@ def velocity(model, z, cond, t, *, adapters=None, slots=None, positions=None, ro
         # cross attention to the condition tokens (no RoPE)
         _, h = bo.residual_norm(x, branch, gate=gate_msa, weight=blk.xnorm_w, bias=blk.xnorm_b, eps=cfg.ln_eps,
                                 out=x, normed=branch)
-        xq = bo.head_rmsnorm(linear("xq", h.view(B * L, C)), blk.xq_gamma, B, L, H)
-        kv = linear("xkv", cond2, cond_rows)  # [B*Lc, 2C] = [k | v]
-        xk = bo.head_rmsnorm(kv, blk.xk_gamma, B, Lc, H, token_stride=2 * C)
-        xv = bo.head_rmsnorm(kv[:, C:], None, B, Lc, H, token_stride=2 * C, normalize=False)
-        a = native_sdpa_f32_ex(xq, xk, xv, out_layout="blhd", precision=model.attention_precision)
+        xq = linear("xq", h.view(B * L, C))
+        if cond_plan is None:
+            Lc = lengths[0]
+            xq = bo.head_rmsnorm(xq, blk.xq_gamma, B, L, H)
+            kv = linear("xkv", cond2, cond_rows, cond_made)  # [B*Lc, 2C] = [k | v]
+            xk = bo.head_rmsnorm(kv, blk.xk_gamma, B, Lc, H, token_stride=2 * C)
+            xv = bo.head_rmsnorm(kv[:, C:], None, B, Lc, H, token_stride=2 * C, normalize=False)
+            a = native_sdpa_f32_ex(xq, xk, xv, out_layout="blhd", precision=model.attention_precision)
+        elif cond_plan.states:
+            xq = bo.head_rmsnorm(xq, blk.xq_gamma, 1, B * L, H, out_bhld=False)[0]
+            kv = linear("xkv", cond2, cond_rows, cond_made)
+            xk = bo.head_rmsnorm(kv, blk.xk_gamma, 1, kv.shape[0], H, token_stride=2 * C, out_bhld=False)[0]
+            a = cross_attention(xq, xk, kv[:, C:].unflatten(1, (H, -1)), cond_plan)
+        else:
+            a = torch.zeros_like(xq)
         branch = linear("xout", a.view(B * L, C)).view(B, L, C)
 
         # MLP
         _, h = bo.residual_norm(x, branch, eps=cfg.ln_eps, scale=scale_mlp, shift=shift_mlp, out=x, normed=branch)
-        f = linear("fc1", h.view(B * L, C))
-        branch, gate = linear("fc2", bo.gelu_tanh(f, out=f)).view(B, L, C), gate_mlp
+        if blk.lin["fc1"].precision == "fp8" and banks.get("fc1") is None:  # (nothing joins before the GELU)
+            f = blk.lin["fc1"].epilogue(h.view(B * L, C), bo.EPILOGUE_GELU)
+        else:
+            f = linear("fc1", h.view(B * L, C))
+            f = bo.gelu_tanh(f, out=f)
+        branch, gate = linear("fc2", f).view(B, L, C), gate_mlp
 
     fs = t_emb[:, None, :].expand(B, 2, C).contiguous()  # [B, (shift, scale), C]
     for b in range(B):

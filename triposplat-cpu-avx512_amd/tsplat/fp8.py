@@ -49,6 +49,12 @@ class Fp8Rows:
         """[rows, ceil(K / 128)] uint8, a view: a block's scale is 2^(exponent - 127)."""
         return self._exponents[:, :-(-self.features // BLOCK)]
 
+    def narrow(self, start, count):
+        """Rows start .. start + count - 1, a view (of a weight: a run of its outputs)."""
+        if start < 0 or count < 0 or start + count > self.rows:
+            raise ValueError(f"rows {start}..{start + count} of {self.rows}")
+        return Fp8Rows((self._codes[start:start + count], self._exponents[start:start + count]), count, self.features)
+
     def dequantize(self):
         """The values that the codes stand for, fp32 [rows, K] (exact)."""
         import torch
