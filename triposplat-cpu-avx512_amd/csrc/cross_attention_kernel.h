@@ -93,23 +93,28 @@ __device__ __forceinline__ void split8(const float (&x)[8], shortx8 (&out)[TERMS
   }
 }
 
-// Eight values of a row from dim on, as they are in memory; zero past the vector's end.
+// Eight values of a row of D from dim on, as they are in memory (VEC: CrossParams::vec); past the row's end some others,
+// which past_end makes zero: nothing waits for a load before its values are used.
 template <class T>
 struct Raw {
   T x[8];
 };
-template <class T>
-__device__ __forceinline__ Raw<T> load_raw(const T* row, int dim, int D, bool vec) {
+template <class T, bool VEC>
+__device__ __forceinline__ Raw<T> load_eight(const T* row, int dim, int D) {
   Raw<T> r;
-  if (vec) {
-    if (dim < D)
-      __builtin_memcpy(&r, __builtin_assume_aligned(row + dim, 16), sizeof(r));
-    else
-      __builtin_memset(&r, 0, sizeof(r));
+  if constexpr (VEC) {
+    __builtin_memcpy(&r, __builtin_assume_aligned(row + min(dim, D - 8), 16), sizeof(r));
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) r.x[i] = dim + i < D ? row[dim + i] : (T)0.0f;
+    for (int i = 0; i < 8; ++i) r.x[i] = row[min(dim + i, D - 1)];
   }
+  return r;
+}
+template <class T, bool VEC>
+__device__ __forceinline__ Raw<T> past_end(Raw<T> r, int dim, int D, bool none) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (none || dim + (VEC ? 0 : i) >= D) r.x[i] = (T)0.0f;
   return r;
 }
 
@@ -138,97 +143,181 @@ __device__ __forceinline__ floatx16 products(const shortx8 (&a)[TERMS], const sh
   return c;
 }
 
-template <class T, int TERMS, int DP, bool FEW, bool BIAS>
-__global__ __launch_bounds__(cross_tile(DP, TERMS, FEW).wq* cross_tile(DP, TERMS, FEW).wk * 64) void cross_kernel(
-    CrossParams p) {
-  typedef typename Element<T>::type E;
-  constexpr CrossTile kTile = cross_tile(DP, TERMS, FEW);
-  constexpr int WQ = kTile.wq, WK = kTile.wk, KB = kTile.kb, BUFS = kTile.bufs;
-  constexpr int kThreads = WQ * WK * 64, kKeys = WK * KB * 32, kBlocks = DP / 32, kSlices = DP / 16;
-  constexpr int kAllUnits = kKeys * DP / 8, kUnits = (kAllUnits + kThreads - 1) / kThreads;  // of 8 values
-  constexpr int kRowK = DP + 8, kRowV = DP + 16;  // values from row to row
-  constexpr int kPlaneK = kKeys * kRowK, kPlaneV = kKeys * kRowV;
-  constexpr int kBuffer = TERMS * (kPlaneK + kPlaneV);
-  constexpr int kMerge = (WK - 1) * WQ * (DP / 2 + 2) * 64 * 2;  // shorts of the waves' sums that meet at the end
-  constexpr int kLds = BUFS * kBuffer > kMerge ? BUFS * kBuffer : kMerge;
-  __shared__ __attribute__((aligned(16))) short lds[kLds];
-  __shared__ float biases[BUFS][kKeys];
+// The second product's operand: eight states (four, and the four that lie 8 rows on) of a lane's column.
+__device__ __forceinline__ shortx8 transposed(const short* from, int pitch) {
+  const shortx4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) shortx4*)(from));
+  const shortx4 hi =
+      __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) shortx4*)(from + 8 * pitch));
+  return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+}
 
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wq = wave / WK, wk = wave % WK;
-  const int l32 = lane & 31, half = lane >> 5;
-  // neighbours on an XCD share a key head
+// A workgroup's number among the grid's, such that neighbours are on one XCD.
+__device__ __forceinline__ int xcd_order() {
   const int count = gridDim.x, per = count / 8, more = count % 8, xcd = blockIdx.x % 8;
-  const int id = xcd * per + min(xcd, more) + blockIdx.x / 8;
-  const CrossItem item = p.items[id % p.item_count];
-  const int kv = id / p.item_count;
-  const bool vec = p.vec;
-  const int D = p.dim;
+  return xcd * per + min(xcd, more) + blockIdx.x / 8;
+}
 
-  // this lane's row
-  const int row = wq * 32 + l32;
-  const bool live = row < item.rows;
-  const int at = item.row0 + (live ? row : 0);
-  const int64_t token = item.token0 + at / p.group;
-  const int head = kv * p.group + at % p.group;
+// The query row of a lane: where q's vector and the result's lie.
+struct Row {
+  int64_t token;
+  int head;
+};
+__device__ __forceinline__ Row row_of(const CrossParams& p, const CrossItem& item, int kv, int row) {
+  const int at = item.row0 + row;
+  return {item.token0 + at / p.group, kv * p.group + at % p.group};
+}
 
-  // Q: columns 16 c + 8 half + i of the row in slice c
-  shortx8 q[kSlices][TERMS];
-  const T* qrow = static_cast<const T*>(p.q) + token * p.q_token + head * p.q_head;
+// Columns 16 c + 8 half + i of a lane's query row in slice c; odd: an infinity or NaN among them.
+template <class T, class E, int TERMS, bool VEC, int SLICES>
+__device__ __forceinline__ void load_queries(const CrossParams& p, const Row& at, int half, shortx8 (&q)[SLICES][TERMS],
+                                             bool& odd) {
+  const T* row = static_cast<const T*>(p.q) + at.token * p.q_token + at.head * p.q_head;
+  odd = false;
 #pragma unroll
-  for (int c = 0; c < kSlices; ++c) {
-    Raw<T> r = load_raw<T>(qrow, 16 * c + 8 * half, D, vec);
+  for (int c = 0; c < SLICES; ++c) {
+    Raw<T> r = past_end<T, VEC>(load_eight<T, VEC>(row, 16 * c + 8 * half, p.dim), 16 * c + 8 * half, p.dim, false);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) odd |= !(fabsf((float)r.x[i]) < INFINITY);
     if constexpr (sizeof(T) == 4) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) r.x[i] *= p.scale * kLog2e;
     }
     terms_of<T, E, TERMS>(r, q[c]);
   }
+}
+
+// A bias in log2 units; a finite one stays finite (the type's lowest masks against others, not by itself).
+__device__ __forceinline__ float bias_log2(float b) {
+  const float b2 = fmaxf(b * kLog2e, -3.4028234663852886e38f);
+  return b == -INFINITY || b != b ? b : b2;
+}
+
+// A product brought to T: rounded to fp32 first, whichever instructions the compiler would fuse it into.
+template <class T>
+__device__ __forceinline__ T rounded(float y) {
+  asm("" : "+v"(y));
+  return (T)y;
+}
+
+// What a block's sums become: a part, or the result.  The lane's row, 16 columns of each 32 in registers.
+template <class T, int DP, bool VEC, int BLOCKS>
+__device__ __forceinline__ void finish(const CrossParams& p, const CrossItem& item, int kv, int row, int tile_rows,
+                                       const Row& at, int half, const floatx16 (&o)[BLOCKS], float m, float l) {
+  if (item.part >= 0) {
+    float* part = p.partial + ((int64_t)item.part * p.kv_heads + kv) * (tile_rows * (DP + 2));
+#pragma unroll
+    for (int b = 0; b < BLOCKS; ++b)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        *reinterpret_cast<floatx4*>(part + row * DP + b * 32 + g * 8 + half * 4) =
+            floatx4{o[b][4 * g], o[b][4 * g + 1], o[b][4 * g + 2], o[b][4 * g + 3]};
+    if (half == 0) {
+      part[tile_rows * DP + row] = m;
+      part[tile_rows * (DP + 1) + row] = l;
+    }
+    return;
+  }
+  const float scale = l == 0.0f ? 0.0f : 1.0f / l;  // (nothing seen: zeros)
+  T* out = static_cast<T*>(p.out) + at.token * p.out_token + at.head * p.out_head;
+#pragma unroll
+  for (int b = 0; b < BLOCKS; ++b)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int dim = b * 32 + g * 8 + half * 4;
+      T y[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] = rounded<T>(o[b][4 * g + e] * scale);
+      if (VEC) {
+        if (dim < p.dim) __builtin_memcpy(__builtin_assume_aligned(out + dim, 4 * sizeof(T)), y, sizeof(y));
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (dim + e < p.dim) out[dim + e] = y[e];
+      }
+    }
+}
+
+// The weights of a block's 16 scores in log2 units and their sum; m the reference.
+template <bool SCALED>
+__device__ __forceinline__ float weights(floatx16& s, float to_log2, float m) {
+  float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+    s[r] = __builtin_amdgcn_exp2f(SCALED ? s[r] - m : fmaf(s[r], to_log2, -m));
+    sum[r & 3] += s[r];
+  }
+  return (sum[0] + sum[1]) + (sum[2] + sum[3]);
+}
+
+// Many rows: a tile of states serves all of a workgroup's waves.
+template <class T, int TERMS, int DP, bool BIAS, bool VEC>
+__global__ __launch_bounds__(cross_tile(DP, TERMS, false).wq * 64, 2) void cross_kernel(CrossParams p) {
+  typedef typename Element<T>::type E;
+  constexpr CrossTile kTile = cross_tile(DP, TERMS, false);
+  constexpr int KB = kTile.kb, kThreads = kTile.wq * 64, kKeys = KB * 32, kBlocks = DP / 32, kSlices = DP / 16;
+  constexpr int kAllUnits = kKeys * DP / 8, kUnits = (kAllUnits + kThreads - 1) / kThreads;  // of 8 values
+  constexpr int kRowK = DP + 8, kRowV = DP + 16;  // values from row to row
+  constexpr int kPlaneK = kKeys * kRowK, kPlaneV = kKeys * kRowV;
+  constexpr int kBuffer = TERMS * (kPlaneK + kPlaneV);
+  __shared__ __attribute__((aligned(16))) short lds[2 * kBuffer];
+  __shared__ __attribute__((aligned(16))) float biases[2][kKeys];
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int l32 = lane & 31, half = lane >> 5;
+  // An XCD takes all tiles of the same key heads, which share their states in its L2, the longest first.
+  const bool whole = p.kv_heads % 8 == 0;
+  const int id = whole ? blockIdx.x / 8 : xcd_order(), heads = whole ? p.kv_heads / 8 : 1;
+  const CrossItem item = p.items[whole ? id / heads : id % p.item_count];
+  const int kv = whole ? blockIdx.x % 8 * heads + id % heads : id / p.item_count;
+  const int D = p.dim;
+
+  // this lane's row
+  const int row = wave * 32 + l32;
+  const bool live = row < item.rows;
+  const Row place = row_of(p, item, kv, live ? row : 0);
+  shortx8 q[kSlices][TERMS];
+  bool odd;
+  load_queries<T, E, TERMS, VEC>(p, place, half, q, odd);
+  odd = __any(odd);
   const float to_log2 = sizeof(T) == 4 ? 1.0f : p.scale * kLog2e;
 
   const T* kbase = static_cast<const T*>(p.k) + (int64_t)item.key0 * p.k_token + kv * p.k_head;
   const T* vbase = static_cast<const T*>(p.v) + (int64_t)item.key0 * p.v_token + kv * p.v_head;
-  const float* bias = p.bias + (BIAS ? item.key0 : 0);
+  const float* bias = p.bias ? p.bias + item.key0 : nullptr;
+  auto bias_of = [&](int64_t key) { return VEC || bias ? bias[key] : 0.0f; };  // (unaligned calls: with or without one)
 
   Raw<T> kr[kUnits], vr[kUnits];
-  uint32_t masked = 0;  // a bit for each unit
-  float b2 = 0.0f;
+  float br[kUnits], b2 = 0.0f;  // the biases of the units' states, of state key0 + tid
   auto load = [&](int key0) {
-    masked = 0;
 #pragma unroll
     for (int u = 0; u < kUnits; ++u) {
-      const int unit = tid + u * kThreads, key = key0 + unit / (DP / 8), dim = unit % (DP / 8) * 8;
-      const bool real = key < item.keys && unit < kAllUnits;
-      const int64_t from = real ? key : 0;
-      kr[u] = load_raw<T>(kbase + from * p.k_token, dim, D, vec);
-      vr[u] = load_raw<T>(vbase + from * p.v_token, dim, D, vec);
-      if (!real || (BIAS && bias[from] == -INFINITY)) masked |= 1u << u;
+      const int unit = tid + u * kThreads, dim = unit % (DP / 8) * 8;
+      const int64_t from = min(key0 + unit / (DP / 8), item.keys - 1);
+      kr[u] = load_eight<T, VEC>(kbase + from * p.k_token, dim, D);
+      vr[u] = load_eight<T, VEC>(vbase + from * p.v_token, dim, D);
+      if (BIAS) br[u] = bias_of(from);
     }
-    if (BIAS && tid < kKeys) {
-      // log2 units; a finite bias stays finite (the type's lowest masks against others, not by itself)
-      const float b = key0 + tid < item.keys ? bias[key0 + tid] : -INFINITY;
-      b2 = b == -INFINITY ? b : fmaxf(b * kLog2e, -3.4028234663852886e38f);
-      if (b != b) b2 = b;
-    }
+    if (BIAS && tid < kKeys) b2 = bias_of(min(key0 + tid, item.keys - 1));
   };
-  auto store = [&](int buf) {
+  auto store = [&](int key0, int buf) {
     short* kp = lds + buf * kBuffer;
     short* vp = kp + TERMS * kPlaneK;
 #pragma unroll
     for (int u = 0; u < kUnits; ++u) {
       const int unit = tid + u * kThreads, key = unit / (DP / 8), dim = unit % (DP / 8) * 8;
       if (kAllUnits % kThreads && unit >= kAllUnits) break;
+      const bool none = key0 + key >= item.keys || (BIAS && br[u] == -INFINITY);
       shortx8 kt[TERMS], vt[TERMS];
-      terms_of<T, E, TERMS>(kr[u], kt);
-      terms_of<T, E, TERMS>(vr[u], vt);
+      terms_of<T, E, TERMS>(past_end<T, VEC>(kr[u], dim, D, none), kt);
+      terms_of<T, E, TERMS>(past_end<T, VEC>(vr[u], dim, D, none), vt);
 #pragma unroll
       for (int t = 0; t < TERMS; ++t) {
-        if (masked >> u & 1) kt[t] = vt[t] = shortx8{0, 0, 0, 0, 0, 0, 0, 0};
         *reinterpret_cast<shortx8*>(kp + t * kPlaneK + key * kRowK + dim) = kt[t];
         *reinterpret_cast<shortx8*>(vp + t * kPlaneV + key * kRowV + dim) = vt[t];
       }
     }
-    if (BIAS && tid < kKeys) biases[buf][tid] = b2;
+    if (BIAS && tid < kKeys) biases[buf][tid] = key0 + tid < item.keys ? bias_log2(b2) : -INFINITY;
   };
 
   floatx16 o[kBlocks];
@@ -239,18 +328,16 @@ __global__ __launch_bounds__(cross_tile(DP, TERMS, FEW).wq* cross_tile(DP, TERMS
   float m_run = -INFINITY, l_run = 0.0f;  // l_run: this lane's half of the row's sum
 
   const int tiles = (item.keys + kKeys - 1) / kKeys;
-  const bool wave_live = wq * 32 < item.rows;
+  const bool wave_live = wave * 32 < item.rows;
   if (tiles > 0) load(0);
   for (int t = 0; t < tiles; ++t) {
-    const int buf = BUFS == 2 ? t & 1 : 0;
-    if (BUFS == 1 && t > 0) __syncthreads();  // the tile before has been read
-    store(buf);
+    const int buf = t & 1;
+    store(t * kKeys, buf);
     __syncthreads();
     if (t + 1 < tiles) load((t + 1) * kKeys);
-    const int first = wk * KB * 32;  // this wave's states of the tile
-    if (!wave_live || t * kKeys + first >= item.keys) continue;
-    const short* kp = lds + buf * kBuffer + (first + l32) * kRowK + 8 * half;
-    const short* vp = lds + buf * kBuffer + TERMS * kPlaneK + (first + 4 * half + (lane & 15) / 4) * kRowV +
+    if (!wave_live) continue;
+    const short* kp = lds + buf * kBuffer + l32 * kRowK + 8 * half;
+    const short* vp = lds + buf * kBuffer + TERMS * kPlaneK + (4 * half + (lane & 15) / 4) * kRowV +
                       (lane >> 4 & 1) * 16 + (lane & 3) * 4;
 
     floatx16 s[KB];
@@ -267,14 +354,16 @@ __global__ __launch_bounds__(cross_tile(DP, TERMS, FEW).wq* cross_tile(DP, TERMS
         s[b] = products<E, TERMS>(kt, q[c], s[b]);
       }
       if constexpr (BIAS) {
-        const float* br = &biases[buf][first + b * 32 + 4 * half];
+        const float* br = &biases[buf][b * 32 + 4 * half];
+        if (odd) {  // (a masked state's zeros times an infinity)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const float add = br[r / 4 * 8 + r % 4];
-          s[b][r] = add == -INFINITY ? add : fmaf(s[b][r], to_log2, add);
+          for (int r = 0; r < 16; ++r)
+            if (br[r / 4 * 8 + r % 4] == -INFINITY) s[b][r] = 0.0f;
         }
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[b][r] = fmaf(s[b][r], to_log2, br[r / 4 * 8 + r % 4]);
       } else {
-        const int left = item.keys - (t * kKeys + first + b * 32) - 4 * half;  // states of this block from this lane's first
+        const int left = item.keys - (t * kKeys + b * 32) - 4 * half;  // states of this block from this lane's first
         if (left < 32) {
 #pragma unroll
           for (int r = 0; r < 16; ++r)
@@ -303,13 +392,7 @@ __global__ __launch_bounds__(cross_tile(DP, TERMS, FEW).wq* cross_tile(DP, TERMS
     const float m = m_run == -INFINITY ? 0.0f : m_run;
 #pragma unroll
     for (int b = 0; b < KB; ++b) {
-      float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        s[b][r] = __builtin_amdgcn_exp2f(BIAS ? s[b][r] - m : fmaf(s[b][r], to_log2, -m));
-        sum[r & 3] += s[b][r];
-      }
-      l_run += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      l_run += weights<BIAS>(s[b], to_log2, m);
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         float x[8];
@@ -321,104 +404,219 @@ __global__ __launch_bounds__(cross_tile(DP, TERMS, FEW).wq* cross_tile(DP, TERMS
         for (int d = 0; d < kBlocks; ++d) {
           shortx8 vt[TERMS];
 #pragma unroll
-          for (int i = 0; i < TERMS; ++i) {
-            const short* from = vp + i * kPlaneV + (b * 32 + 16 * c) * kRowV + 32 * d;
-            const shortx4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                (__attribute__((address_space(3))) shortx4*)(from));
-            const shortx4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                (__attribute__((address_space(3))) shortx4*)(from + 8 * kRowV));
-            vt[i] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-          }
+          for (int i = 0; i < TERMS; ++i)
+            vt[i] = transposed(vp + i * kPlaneV + (b * 32 + 16 * c) * kRowV + 32 * d, kRowV);
           o[d] = products<E, TERMS>(vt, pt, o[d]);
         }
       }
     }
   }
 
-  float l = l_run + other_half(l_run);
-  if constexpr (WK > 1) {
-    float* merge = reinterpret_cast<float*>(lds);
-    constexpr int kWave = (DP / 2 + 2) * 64;
-    __syncthreads();
-    if (wk > 0) {
-      float* mine = merge + ((wk - 1) * WQ + wq) * kWave;
+  const float l = l_run + other_half(l_run);
+  if (live) finish<T, DP, VEC>(p, item, kv, row, kTile.wq * 32, place, half, o, m_run, l);
+}
+
+// At most 32 rows a request, where reading the states is all: each wave takes every fourth block of 32 states by itself,
+// without a barrier, K and V through the wave's own LDS; the next block's loads are under way while this
+// one is multiplied.  The waves'
+// sums meet at the end.
+template <class T, int TERMS, int DP, bool BIAS, bool VEC>
+__global__ __launch_bounds__(kFewWaves * 64, TERMS > 1 && DP > 64 ? 1 : 2) void cross_few_kernel(CrossParams p) {
+  typedef typename Element<T>::type E;
+  constexpr int kBlocks = DP / 32, kSlices = DP / 16, kUnits = DP / 16;  // a lane's eights of 32 states' values
+  constexpr int kRowK = DP + 8, kRowV = DP + 16;
+  constexpr int kMerge = (kFewWaves - 1) * (DP / 2 + 2) * 64 * 2;  // shorts of the sums that meet
+  constexpr int kPlane = 32 * kRowV, kRows = kFewWaves * TERMS * kPlane;  // (K's rows fit as well)
+  constexpr int kLds = kRows > kMerge ? kRows : kMerge;
+  __shared__ __attribute__((aligned(16))) short lds[kLds];
+  __shared__ __attribute__((aligned(16))) float biases[kFewWaves][32];
+
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int l32 = lane & 31, half = lane >> 5;
+  // (an item's key heads are neighbours: their states lie side by side in memory)
+  const int id = xcd_order();
+  const CrossItem item = p.items[id / p.kv_heads];
+  const int kv = id % p.kv_heads;
+  const int D = p.dim;
+  const bool live = l32 < item.rows;
+  const Row place = row_of(p, item, kv, live ? l32 : 0);
+  shortx8 q[kSlices][TERMS];
+  bool odd;
+  load_queries<T, E, TERMS, VEC>(p, place, half, q, odd);
+  const float to_log2 = sizeof(T) == 4 ? 1.0f : p.scale * kLog2e;
+
+  const T* kbase = static_cast<const T*>(p.k) + (int64_t)item.key0 * p.k_token + kv * p.k_head;
+  const T* vbase = static_cast<const T*>(p.v) + (int64_t)item.key0 * p.v_token + kv * p.v_head;
+  const float* bias = p.bias ? p.bias + item.key0 : nullptr;
+  short* wlds = lds + wave * TERMS * kPlane;
+  Raw<T> kr[kUnits], vr[kUnits];
+  float b2 = 0.0f;
+  const int last = item.keys - 1;  // (past the last state: its values, which count for nothing)
+  auto load_rows = [&](Raw<T>(&r)[kUnits], const T* base, int64_t step, int key0) {
 #pragma unroll
-      for (int b = 0; b < kBlocks; ++b)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) mine[(b * 16 + r) * 64 + lane] = o[b][r];
-      mine[DP / 2 * 64 + lane] = m_run;
-      mine[(DP / 2 + 1) * 64 + lane] = l;
+    for (int u = 0; u < kUnits; ++u) {
+      const int unit = lane + u * 64;
+      r[u] = load_eight<T, VEC>(base + min(key0 + unit / (DP / 8), last) * step, unit % (DP / 8) * 8, D);
     }
-    __syncthreads();
-    if (wk > 0) return;
+  };
+  auto load_k = [&](int key0) {
+    load_rows(kr, kbase, p.k_token, key0);
+    if (BIAS) b2 = VEC || bias ? bias[min(key0 + l32, last)] : 0.0f;
+  };
+  auto load_v = [&](int key0) { load_rows(vr, vbase, p.v_token, key0); };
+  // Their terms to the wave's LDS, a plane of rows of `pitch` for each; zeros where nothing counts.  (A wave's LDS
+  // operations are done in order.)
+  auto put_rows = [&](const Raw<T>(&r)[kUnits], int pitch, int left) {
 #pragma unroll
-    for (int w = 0; w < WK - 1; ++w) {
-      const float* theirs = merge + (w * WQ + wq) * kWave;
-      const float m2 = theirs[DP / 2 * 64 + lane], l2 = theirs[(DP / 2 + 1) * 64 + lane];
-      const float m_new = fmaxf(m_run, m2);
-      const float keep = m_run == m_new ? 1.0f : __builtin_amdgcn_exp2f(m_run - m_new);
-      const float take = m2 == m_new ? 1.0f : __builtin_amdgcn_exp2f(m2 - m_new);
-      m_run = m_new;
-      l = l * keep + l2 * take;
+    for (int u = 0; u < kUnits; ++u) {
+      const int unit = lane + u * 64, state = unit / (DP / 8), dim = unit % (DP / 8) * 8;
+      const bool none = state >= left || (BIAS && biases[wave][state] == -INFINITY);
+      shortx8 out[TERMS];
+      terms_of<T, E, TERMS>(past_end<T, VEC>(r[u], dim, D, none), out);
 #pragma unroll
-      for (int b = 0; b < kBlocks; ++b)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) o[b][r] = o[b][r] * keep + theirs[(b * 16 + r) * 64 + lane] * take;
+      for (int t = 0; t < TERMS; ++t)
+        *reinterpret_cast<shortx8*>(wlds + t * kPlane + state * pitch + dim) = out[t];
     }
-  }
-  if (!live) return;
-  if (item.part >= 0) {
-    constexpr int kRows = WQ * 32;
-    float* part = p.partial + ((int64_t)item.part * p.kv_heads + kv) * (kRows * (DP + 2));
-#pragma unroll
-    for (int b = 0; b < kBlocks; ++b)
-#pragma unroll
-      for (int g = 0; g < 4; ++g)
-        *reinterpret_cast<floatx4*>(part + row * DP + b * 32 + g * 8 + half * 4) =
-            floatx4{o[b][4 * g], o[b][4 * g + 1], o[b][4 * g + 2], o[b][4 * g + 3]};
-    if (half == 0) {
-      part[kRows * DP + row] = m_run;
-      part[kRows * (DP + 1) + row] = l;
-    }
-    return;
-  }
-  const float scale = l == 0.0f ? 0.0f : 1.0f / l;  // (nothing seen: zeros)
-  T* out = static_cast<T*>(p.out) + token * p.out_token + head * p.out_head;
+    __builtin_amdgcn_wave_barrier();
+  };
+  const short* kp = wlds + l32 * kRowK + 8 * half;
+  const short* vp = wlds + (4 * half + (lane & 15) / 4) * kRowV + (lane >> 4 & 1) * 16 + (lane & 3) * 4;
+  const float* br = &biases[wave][4 * half];
+
+  floatx16 o[kBlocks];
 #pragma unroll
   for (int b = 0; b < kBlocks; ++b)
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const int dim = b * 32 + g * 8 + half * 4;
-      T y[4];
+    for (int r = 0; r < 16; ++r) o[b][r] = 0.0f;
+  float m_run = -INFINITY, l_run = 0.0f;
+  constexpr int kStep = kFewWaves * 32;
+  int key0 = wave * 32;
+  if (key0 <= last) {
+    load_k(key0);
+    load_v(key0);
+  }
+  for (; key0 <= last; key0 += kStep) {
+    const int left = item.keys - key0;  // states from this block's first on
+    if (BIAS) {
+      biases[wave][l32] = l32 < left ? bias_log2(b2) : -INFINITY;  // (both halves write the same)
+      __builtin_amdgcn_wave_barrier();
+    }
+    const bool more = key0 + kStep <= last;
+    floatx16 s;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) y[e] = (T)(o[b][4 * g + e] * scale);
-      if (vec) {
-        if (dim < D) __builtin_memcpy(__builtin_assume_aligned(out + dim, 4 * sizeof(T)), y, sizeof(y));
+    for (int r = 0; r < 16; ++r) s[r] = 0.0f;
+    put_rows(kr, kRowK, left);
+    if (more) load_k(key0 + kStep);
+#pragma unroll
+    for (int c = 0; c < kSlices; ++c) {
+      shortx8 kt[TERMS];
+#pragma unroll
+      for (int t = 0; t < TERMS; ++t) kt[t] = *reinterpret_cast<const shortx8*>(kp + t * kPlane + 16 * c);
+      s = products<E, TERMS>(kt, q[c], s);
+    }
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int key = r / 4 * 8 + r % 4;
+      if constexpr (BIAS) {
+        const float add = br[key];
+        s[r] = add == -INFINITY ? add : fmaf(s[r], to_log2, add);
       } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (dim + e < D) out[dim + e] = y[e];
+        s[r] = key + 4 * half < left ? s[r] : -INFINITY;
       }
     }
+    float top = s[0];
+#pragma unroll
+    for (int r = 1; r < 16; ++r) top = fmaxf(top, s[r]);
+    top = fmaxf(top, other_half(top));
+    const float ref = BIAS ? top - kLift<E> : fmaf(top, to_log2, -kLift<E>);
+    if (__any(ref > m_run + kSlack)) {
+      const float m_new = fmaxf(m_run, ref);
+      const float keep = m_run == m_new ? 1.0f : __builtin_amdgcn_exp2f(m_run - m_new);
+      l_run *= keep;
+#pragma unroll
+      for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[b][r] *= keep;
+      m_run = m_new;
+    }
+    l_run += weights<BIAS>(s, to_log2, m_run == -INFINITY ? 0.0f : m_run);
+    shortx8 pt[2][TERMS];
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      float x[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = s[8 * c + i];
+      split8<E, TERMS>(x, pt[c]);
+    }
+    put_rows(vr, kRowV, left);
+    if (more) load_v(key0 + kStep);
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+      for (int d = 0; d < kBlocks; ++d) {
+        shortx8 vt[TERMS];
+#pragma unroll
+        for (int t = 0; t < TERMS; ++t) vt[t] = transposed(vp + t * kPlane + 16 * c * kRowV + 32 * d, kRowV);
+        o[d] = products<E, TERMS>(vt, pt[c], o[d]);
+      }
+    __builtin_amdgcn_wave_barrier();
+  }
+
+  float l = l_run + other_half(l_run);
+  float* merge = reinterpret_cast<float*>(lds);
+  constexpr int kWave = (DP / 2 + 2) * 64;
+  __syncthreads();
+  if (wave > 0) {
+    float* mine = merge + (wave - 1) * kWave;
+#pragma unroll
+    for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) mine[(b * 16 + r) * 64 + lane] = o[b][r];
+    mine[DP / 2 * 64 + lane] = m_run;
+    mine[(DP / 2 + 1) * 64 + lane] = l;
+  }
+  __syncthreads();
+  if (wave > 0) return;
+#pragma unroll
+  for (int w = 0; w < kFewWaves - 1; ++w) {
+    const float* theirs = merge + w * kWave;
+    const float m2 = theirs[DP / 2 * 64 + lane], l2 = theirs[(DP / 2 + 1) * 64 + lane];
+    const float m_new = fmaxf(m_run, m2);
+    const float keep = m_run == m_new ? 1.0f : __builtin_amdgcn_exp2f(m_run - m_new);
+    const float take = m2 == m_new ? 1.0f : __builtin_amdgcn_exp2f(m2 - m_new);
+    m_run = m_new;
+    l = l * keep + l2 * take;
+#pragma unroll
+    for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[b][r] = o[b][r] * keep + theirs[(b * 16 + r) * 64 + lane] * take;
+  }
+  if (live) finish<T, DP, VEC>(p, item, kv, l32, 32, place, half, o, m_run, l);
 }
 
-template <class T, int TERMS, int DP, bool FEW>
-int launch_tile(const CrossParams& p, hipStream_t stream) {
-  constexpr CrossTile kTile = cross_tile(DP, TERMS, FEW);
+template <class T, int TERMS, int DP, bool BIAS, bool VEC>
+int launch_kernel(const CrossParams& p, hipStream_t stream) {
   const int grid = p.item_count * p.kv_heads;
-  if (p.bias)
-    cross_kernel<T, TERMS, DP, FEW, true><<<grid, kTile.wq * kTile.wk * 64, 0, stream>>>(p);
+  if (p.few)
+    cross_few_kernel<T, TERMS, DP, BIAS, VEC><<<grid, kFewWaves * 64, 0, stream>>>(p);
   else
-    cross_kernel<T, TERMS, DP, FEW, false><<<grid, kTile.wq * kTile.wk * 64, 0, stream>>>(p);
+    cross_kernel<T, TERMS, DP, BIAS, VEC><<<grid, cross_tile(DP, TERMS, false).wq * 64, 0, stream>>>(p);
   return hipGetLastError() == hipSuccess ? kOk : kErrLaunch;
+}
+
+template <class T, int TERMS, int DP>
+int launch_dim(const CrossParams& p, hipStream_t stream) {
+  if (!p.vec) return launch_kernel<T, TERMS, DP, true, false>(p, stream);
+  return p.bias ? launch_kernel<T, TERMS, DP, true, true>(p, stream) : launch_kernel<T, TERMS, DP, false, true>(p, stream);
 }
 
 template <class T, int TERMS>
 int launch_terms(const CrossParams& p, hipStream_t stream) {
   switch (cross_padded_dim(p.dim)) {
-    case 64: return p.few ? launch_tile<T, TERMS, 64, true>(p, stream) : launch_tile<T, TERMS, 64, false>(p, stream);
-    case 96: return p.few ? launch_tile<T, TERMS, 96, true>(p, stream) : launch_tile<T, TERMS, 96, false>(p, stream);
-    default: return p.few ? launch_tile<T, TERMS, 128, true>(p, stream) : launch_tile<T, TERMS, 128, false>(p, stream);
+    case 64: return launch_dim<T, TERMS, 64>(p, stream);
+    case 96: return launch_dim<T, TERMS, 96>(p, stream);
+    default: return launch_dim<T, TERMS, 128>(p, stream);
   }
 }
 

@@ -31,14 +31,16 @@ int64_t make_cross_plan(const int32_t* q_lengths, const int32_t* k_lengths, int 
   const int terms = dtype != 0 ? 1 : precision == 0 ? 3 : precision;
   const bool few = longest <= 32;
   const CrossTile tile = cross_tile(padded, terms, few);
-  const int tile_rows = tile.wq * 32, tile_keys = tile.wk * tile.kb * 32;
-  // Tiles of keys over all workgroups: an even share of them for each of `slots` workgroups that run at once is the
-  // length of a part, at least four tiles (fewer and the parts' sums cost more than they save).
+  const int tile_rows = tile.wq * 32, tile_keys = tile.kb * 32;
+  // Tiles of keys over all workgroups: an even share of them for each workgroup that runs at once is the length of a part.
+  // Few rows: a part's sums are small, so four times as many parts, two tiles at least.  Many: four tiles at least (fewer
+  // and the parts' sums cost more than they save).
   const int64_t slots = (int64_t)compute_units * 2;
   int64_t work = 0;
   for (int i = 0; i < requests; ++i)
     work += ((int64_t)q_lengths[i] * group + tile_rows - 1) / tile_rows * ((k_lengths[i] + tile_keys - 1) / tile_keys);
-  const int64_t share = std::max<int64_t>(4, (work * kv_heads + slots - 1) / slots);
+  const int64_t at_once = few ? 4 * slots : slots;
+  const int64_t share = std::max<int64_t>(few ? 2 : 4, (work * kv_heads + at_once - 1) / at_once);
 
   int64_t items = 0, joins = 0, parts = 0;
   const int64_t room_items = plan ? (plan_ints - kPlanHeaderInts) / kCrossItem : 0;
@@ -72,7 +74,13 @@ int64_t make_cross_plan(const int32_t* q_lengths, const int32_t* k_lengths, int 
   std::copy(header, header + kPlanHeaderInts, plan);
   CrossJoin* join = reinterpret_cast<CrossJoin*>(plan + kPlanHeaderInts + items * kCrossItem);
   parts = 0;
+  CrossItem* const first = item;
   each([&](const CrossItem& it) { *item++ = it; }, [&](const CrossJoin& j) { *join++ = j; });
+  // the longest first: what starts last is short
+  std::sort(first, item, [](const CrossItem& a, const CrossItem& b) {
+    if (a.keys != b.keys) return a.keys > b.keys;
+    return a.key0 != b.key0 ? a.key0 < b.key0 : a.token0 != b.token0 ? a.token0 < b.token0 : a.row0 < b.row0;
+  });
   return need;
 }
 

@@ -32,16 +32,16 @@ constexpr int kCrossItem = sizeof(CrossItem) / 4, kCrossJoin = sizeof(CrossJoin)
 // Head sizes are padded to one of these.
 constexpr int cross_padded_dim(int dim) { return dim <= 64 ? 64 : dim <= 96 ? 96 : 128; }
 
-// A workgroup: wq waves of 32 rows times wk waves that share the keys of a tile, kb blocks of 32 keys each, bufs buffers.
-// few: at most 32 rows a request, where reading the keys is all.
+// A workgroup's tile: wq waves of 32 rows each against kb blocks of 32 states; few: 32 rows, a block of 32 states to each
+// of kFewWaves waves.
+constexpr int kFewWaves = 4;
 struct CrossTile {
-  int wq, wk, kb, bufs;
+  int wq, kb;
 };
 constexpr CrossTile cross_tile(int padded, int terms, bool few) {
-  if (few) return terms == 3 && padded > 64 ? CrossTile{1, 2, 1, 1} : CrossTile{1, 4, 1, 1};
-  if (terms == 3) return CrossTile{8, 1, padded > 64 ? 1 : 2, 2};
-  if (terms == 2) return CrossTile{8, 1, padded > 64 ? 1 : 2, 2};
-  return CrossTile{4, 1, 2, 2};
+  if (few) return {1, kFewWaves};
+  if (terms > 1) return {8, padded > 64 ? 1 : 2};
+  return {4, 2};
 }
 
 // Writes the plan (null: only counts); its size in ints, or a negative status.
