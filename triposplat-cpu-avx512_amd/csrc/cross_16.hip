@@ -12,7 +12,7 @@ namespace {
 
 // out = sum_p 2^(m_p - M) o_p / sum_p 2^(m_p - M) l_p, M the largest m_p.  Four columns of a row a thread; the grid's
 // third dimension goes over an item's rows.
-constexpr int kJoinThreads = 256;
+constexpr int kJoinThreads = 256, kJoinAhead = 8;
 template <class T>
 __global__ __launch_bounds__(kJoinThreads) void cross_join_kernel(CrossParams p, int padded, int tile_rows) {
   const CrossJoin join = p.joins[blockIdx.x];
@@ -24,15 +24,25 @@ __global__ __launch_bounds__(kJoinThreads) void cross_join_kernel(CrossParams p,
   const float* m = base + tile_rows * padded + row;
   float top = -INFINITY, l = 0.0f;
   floatx4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (int n = 0; n < join.parts; ++n) {
-    const float mn = m[n * next], ln = m[n * next + tile_rows];
-    const floatx4 o = *reinterpret_cast<const floatx4*>(base + n * next + row * padded + dim);
-    const float new_top = fmaxf(top, mn);
-    const float keep = top == new_top ? 1.0f : __builtin_amdgcn_exp2f(top - new_top);
-    const float take = mn == new_top ? 1.0f : __builtin_amdgcn_exp2f(mn - new_top);
-    l = l * keep + ln * take;
-    sum = sum * keep + o * take;
-    top = new_top;
+  for (int n0 = 0; n0 < join.parts; n0 += kJoinAhead) {  // (so many parts' loads are under way at once)
+    float mn[kJoinAhead], ln[kJoinAhead];
+    floatx4 o[kJoinAhead];
+#pragma unroll
+    for (int j = 0; j < kJoinAhead; ++j) {
+      const int64_t at = min(n0 + j, join.parts - 1) * next;
+      mn[j] = m[at], ln[j] = m[at + tile_rows];
+      o[j] = *reinterpret_cast<const floatx4*>(base + at + row * padded + dim);
+    }
+#pragma unroll
+    for (int j = 0; j < kJoinAhead; ++j) {
+      if (n0 + j >= join.parts) break;
+      const float new_top = fmaxf(top, mn[j]);
+      const float keep = top == new_top ? 1.0f : __builtin_amdgcn_exp2f(top - new_top);
+      const float take = mn[j] == new_top ? 1.0f : __builtin_amdgcn_exp2f(mn[j] - new_top);
+      l = l * keep + ln[j] * take;
+      sum = sum * keep + o[j] * take;
+      top = new_top;
+    }
   }
   const float scale = l == 0.0f ? 0.0f : 1.0f / l;
   const int at = join.row0 + row;

@@ -167,12 +167,11 @@ __device__ __forceinline__ Row row_of(const CrossParams& p, const CrossItem& ite
   return {item.token0 + at / p.group, kv * p.group + at % p.group};
 }
 
-// Columns 16 c + 8 half + i of a lane's query row in slice c; odd: an infinity or NaN among them.
+// Columns 16 c + 8 half + i of a lane's query row in slice c; whether an infinity or NaN is among them.
 template <class T, class E, int TERMS, bool VEC, int SLICES>
-__device__ __forceinline__ void load_queries(const CrossParams& p, const Row& at, int half, shortx8 (&q)[SLICES][TERMS],
-                                             bool& odd) {
+__device__ __forceinline__ bool load_queries(const CrossParams& p, const Row& at, int half, shortx8 (&q)[SLICES][TERMS]) {
   const T* row = static_cast<const T*>(p.q) + at.token * p.q_token + at.head * p.q_head;
-  odd = false;
+  bool odd = false;
 #pragma unroll
   for (int c = 0; c < SLICES; ++c) {
     Raw<T> r = past_end<T, VEC>(load_eight<T, VEC>(row, 16 * c + 8 * half, p.dim), 16 * c + 8 * half, p.dim, false);
@@ -184,6 +183,7 @@ __device__ __forceinline__ void load_queries(const CrossParams& p, const Row& at
     }
     terms_of<T, E, TERMS>(r, q[c]);
   }
+  return odd;
 }
 
 // A bias in log2 units; a finite one stays finite (the type's lowest masks against others, not by itself).
@@ -277,9 +277,7 @@ __global__ __launch_bounds__(cross_tile(DP, TERMS, false).wq * 64, 2) void cross
   const bool live = row < item.rows;
   const Row place = row_of(p, item, kv, live ? row : 0);
   shortx8 q[kSlices][TERMS];
-  bool odd;
-  load_queries<T, E, TERMS, VEC>(p, place, half, q, odd);
-  odd = __any(odd);
+  const bool odd = __any(load_queries<T, E, TERMS, VEC>(p, place, half, q));
   const float to_log2 = sizeof(T) == 4 ? 1.0f : p.scale * kLog2e;
 
   const T* kbase = static_cast<const T*>(p.k) + (int64_t)item.key0 * p.k_token + kv * p.k_head;
@@ -440,9 +438,6 @@ __global__ __launch_bounds__(kFewWaves * 64, TERMS > 1 && DP > 64 ? 1 : 2) void 
   const int D = p.dim;
   const bool live = l32 < item.rows;
   const Row place = row_of(p, item, kv, live ? l32 : 0);
-  shortx8 q[kSlices][TERMS];
-  bool odd;
-  load_queries<T, E, TERMS, VEC>(p, place, half, q, odd);
   const float to_log2 = sizeof(T) == 4 ? 1.0f : p.scale * kLog2e;
 
   const T* kbase = static_cast<const T*>(p.k) + (int64_t)item.key0 * p.k_token + kv * p.k_head;
@@ -495,6 +490,8 @@ __global__ __launch_bounds__(kFewWaves * 64, TERMS > 1 && DP > 64 ? 1 : 2) void 
     load_k(key0);
     load_v(key0);
   }
+  shortx8 q[kSlices][TERMS];
+  load_queries<T, E, TERMS, VEC>(p, place, half, q);
   for (; key0 <= last; key0 += kStep) {
     const int left = item.keys - key0;  // states from this block's first on
     if (BIAS) {

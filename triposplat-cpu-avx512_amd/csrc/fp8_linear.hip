@@ -40,14 +40,28 @@ __device__ __forceinline__ floatx4 columns4(const T* row, int n, int N) {
   return VEC ? load4<T, true>(row, min(n, N - 4), N) : load4<T, false>(row, n, N);
 }
 
-// What follows the sums of COUNT pieces of row m, piece i of them columns n(i) .. n(i) + 3.
-template <class TO, bool VEC, int COUNT, class N>
-__device__ __forceinline__ void finish(const Finish& f, floatx4 (&y)[COUNT], int m, N n) {
-  const int64_t row = min(m, f.M - 1);
-  if (f.bias) {
+// The gate's row of row m.
+__device__ __forceinline__ const float* gate_row(const Finish& f, int m) {
+  return f.gate + (f.gate_stride ? (uint32_t)m / (uint32_t)f.rows_per_batch * f.gate_stride : 0);
+}
+
+// What follows the sums of columns n .. n + 3 in COUNT rows m(i); none is written past row M or column N.  bias: of these
+// columns.  All of a piece's rows are asked for before the first is used.
+template <class TO, bool VEC, int COUNT, class Rows>
+__device__ __forceinline__ void finish(const Finish& f, floatx4 (&y)[COUNT], const floatx4& bias, int n, Rows m) {
+  floatx4 gate[COUNT], residual[COUNT];
+  if (f.gate) {
 #pragma unroll
-    for (int i = 0; i < COUNT; ++i) y[i] += columns4<float, VEC>(f.bias, n(i), f.N);
+    for (int i = 0; i < COUNT; ++i) gate[i] = columns4<float, VEC>(gate_row(f, min(m(i), f.M - 1)), n, f.N);
   }
+  if (f.residual) {
+#pragma unroll
+    for (int i = 0; i < COUNT; ++i)
+      residual[i] = columns4<TO, VEC>(
+          static_cast<const TO*>(f.residual) + (int64_t)min(m(i), f.M - 1) * f.residual_stride, n, f.N);
+  }
+#pragma unroll
+  for (int i = 0; i < COUNT; ++i) y[i] += bias;
   if (f.activation) {
 #pragma unroll
     for (int i = 0; i < COUNT; ++i)
@@ -55,30 +69,33 @@ __device__ __forceinline__ void finish(const Finish& f, floatx4 (&y)[COUNT], int
       for (int e = 0; e < 4; ++e) y[i][e] = gelu(y[i][e]);
   }
   if (f.gate) {
-    const float* gate = f.gate + (f.gate_stride ? row / f.rows_per_batch * f.gate_stride : 0);
 #pragma unroll
-    for (int i = 0; i < COUNT; ++i) y[i] *= columns4<float, VEC>(gate, n(i), f.N);
+    for (int i = 0; i < COUNT; ++i) y[i] *= gate[i];
   }
   if (f.residual) {
-    const TO* residual = static_cast<const TO*>(f.residual) + row * f.residual_stride;
 #pragma unroll
-    for (int i = 0; i < COUNT; ++i) y[i] += columns4<TO, VEC>(residual, n(i), f.N);
+    for (int i = 0; i < COUNT; ++i) y[i] += residual[i];
   }
-  if (m >= f.M) return;
-  TO* out = static_cast<TO*>(f.out) + row * f.out_stride;
 #pragma unroll
   for (int i = 0; i < COUNT; ++i) {
+    if (m(i) >= f.M) continue;
+    TO* out = static_cast<TO*>(f.out) + (int64_t)m(i) * f.out_stride;
     if constexpr (VEC) {
       typename Vec4<TO>::type o;
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[e] = (TO)y[i][e];
-      if (n(i) < f.N) *reinterpret_cast<typename Vec4<TO>::type*>(out + n(i)) = o;
+      if (n < f.N) *reinterpret_cast<typename Vec4<TO>::type*>(out + n) = o;
     } else {
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        if (n(i) + e < f.N) out[n(i) + e] = (TO)y[i][e];
+        if (n + e < f.N) out[n + e] = (TO)y[i][e];
     }
   }
+}
+
+template <bool VEC>
+__device__ __forceinline__ floatx4 bias_of(const Finish& f, int n) {
+  return f.bias ? columns4<float, VEC>(f.bias, n, f.N) : floatx4{0.0f, 0.0f, 0.0f, 0.0f};
 }
 
 __device__ __forceinline__ intx8 join(const intx4& a, const intx4& b) {
@@ -133,30 +150,37 @@ __device__ __forceinline__ bf16x8 widen8(int lo, int hi, float scale) {
   return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
-// ---- many rows: tiles of BM x BN through LDS, STAGES buffers of BK codes of each row.
-// A row's BK bytes are pieces of 16, and a wave reads one piece of each of 32 rows at once, eight lanes (rows) in a cycle
-// of all banks: piece c of row r lies at place c ^ (r % 8) (BK 128), or c ^ (r / 2 % 4) (BK 64).  The copies to LDS write
-// in lane order, so the lane picks its piece.
-template <int BM, int BN, int WM, int WN, int BK, int STAGES, class TO, bool VEC>
-__global__ __launch_bounds__(WM* WN * 64, 2) void fp8_tile_kernel(const uint8_t* __restrict__ xc,
+// ---- many rows: tiles of BM x BN through LDS, STAGES buffers of 64 codes of each row.
+// A row's 64 bytes are pieces of 16, and a wave reads one piece of each of 32 rows at once, eight lanes (rows) in a cycle
+// of all banks: piece c of row r lies at place c ^ (r / 2 % 4).  The copies to LDS write in lane order, so the lane picks
+// its piece.
+// A stage is multiplied in two steps, of 32 codes each (EXACT) or of half of the weights' rows.  The operands of each step
+// are read into registers while the one before is multiplied (where 128 sums leave room for that), so a stage's buffer is free, and the copies of the stage
+// that comes STAGES later may begin, before its last step is multiplied.
+constexpr int kStage = 64;
+
+template <int BM, int BN, int WM, int WN, int STAGES, class TO, bool VEC>
+__global__ __launch_bounds__(WM* WN * 64, BM * BN > 128 * 128 ? 2 : 3) void fp8_tile_kernel(const uint8_t* __restrict__ xc,
                                                                   const uint8_t* __restrict__ xe,
                                                                   const uint8_t* __restrict__ wc,
                                                                   const uint8_t* __restrict__ we, Finish f,
                                                                   int code_stride, int exp_stride, int tiles_n) {
   constexpr bool kExact = sizeof(TO) == 4;
-  constexpr int kWaves = WM * WN, kPieces = BK / 16, kRowsACopy = 64 / kPieces;
+  constexpr int kWaves = WM * WN, kPieces = kStage / 16, kRowsACopy = 64 / kPieces;
   constexpr int kCopies = (BM + BN) / kRowsACopy / kWaves;
   constexpr int MI = BM / WM / 32, NI = BN / WN / 32;
-  constexpr int kStepsAScale = kFp8Block / BK, kExpCopies = (BM + BN) / 64;
+  constexpr int NS = kExact ? NI : NI / 2;  // of the weights' 32 rows, in a step
+  constexpr int kExpCopies = (BM + BN) / 64;
   static_assert((BM + BN) % 64 == 0 && BM % 64 == 0, "whole copies of exponents");
   static_assert(kCopies * kRowsACopy * kWaves == BM + BN && BM % kRowsACopy == 0, "whole copies");
-  __shared__ __attribute__((aligned(16))) uint8_t lds[STAGES][(BM + BN) * BK];
+  __shared__ __attribute__((aligned(16))) uint8_t lds[STAGES][(BM + BN) * kStage];
   __shared__ __attribute__((aligned(16))) uint8_t exps[2][(BM + BN) * 4];
+  constexpr bool kAhead = kExact;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int tile = tile_of(blockIdx.x, gridDim.x);
   const int m0 = tile / tiles_n * BM, n0 = tile % tiles_n * BN;
-  const int steps = code_stride / BK;
-  auto place = [](int r, int c) { return c ^ (BK == 128 ? r & 7 : (r >> 1) & 3); };
+  const int blocks = code_stride / kFp8Block, stages = blocks * (kFp8Block / kStage);
+  auto place = [](int r, int c) { return c ^ ((r >> 1) & 3); };
 
   const uint8_t* from[kCopies];
 #pragma unroll
@@ -176,15 +200,16 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void fp8_tile_kernel(const uint8_t*
       copy4_to_lds((r < BM ? xe : we) + row * exp_stride + four * 4, &exps[four & 1][r0 * 4]);
     }
   };
-  auto fetch = [&](int step) {
-    if (step % (4 * kStepsAScale) == 0) fetch_exps(step / (4 * kStepsAScale));
+  auto fetch = [&](int stage, int buffer) {
+    if (stage % 8 == 0) fetch_exps(stage / 8);
 #pragma unroll
     for (int j = 0; j < kCopies; ++j)
-      copy16_to_lds(from[j] + step * BK, &lds[step % STAGES][(j * kWaves + wave) * kRowsACopy * BK]);
+      copy16_to_lds(from[j] + stage * kStage, &lds[buffer][(j * kWaves + wave) * kRowsACopy * kStage]);
   };
 
   const int wm = wave / WN * (BM / WM), wn = wave % WN * (BN / WN);
   const int l32 = lane & 31, half = lane >> 5;
+  const bool busy = m0 + wm < f.M && n0 + wn < f.N;  // (a ragged last tile: its waves without rows only copy)
   floatx16 acc[NI][MI];
 #pragma unroll
   for (int i = 0; i < NI; ++i)
@@ -193,83 +218,130 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void fp8_tile_kernel(const uint8_t*
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
 
-#pragma unroll
-  for (int s = 0; s < STAGES - 1; ++s)
-    if (s < steps) fetch(s);
-  for (int step = 0; step < steps; ++step) {
-    // the oldest stage's copies are done when at most those of the STAGES - 2 after it are not (exponents are asked for
-    // before the codes of their step)
-    if (step + STAGES - 2 < steps)
-      wait_and_meet<kCopies*(STAGES - 2)>();
-    else
-      wait_and_meet<0>();
-    if (step + STAGES - 1 < steps) fetch(step + STAGES - 1);
-    const uint8_t* a = &lds[step % STAGES][(BM + wn + l32) * BK];
-    const uint8_t* b = &lds[step % STAGES][(wm + l32) * BK];
-    auto piece = [&](const uint8_t* row, int i, int c) {
-      return *reinterpret_cast<const intx4*>(row + i * 32 * BK + place(l32, c) * 16);
+  // A step's operands: pieces of the weights' rows and of x's, and the exponents of their block.
+  struct Step {
+    typedef std::conditional_t<kExact, intx4, intx8> Codes;
+    Codes w[NS], x[MI];
+  };
+  struct Scales {
+    uint32_t w[NI], x[MI];
+  };
+  auto read_step = [&](Step& to, int buffer, int step) {
+    const uint8_t* a = &lds[buffer][(BM + wn + l32) * kStage];
+    const uint8_t* b = &lds[buffer][(wm + l32) * kStage];
+    auto codes = [&](const uint8_t* row) {
+      const intx4 lo = *reinterpret_cast<const intx4*>(row + place(l32, (kExact ? 2 * step : 0) + half) * 16);
+      if constexpr (kExact)
+        return lo;
+      else
+        return join(lo, *reinterpret_cast<const intx4*>(row + place(l32, 2 + half) * 16));
     };
-    const int block = step / kStepsAScale;
+#pragma unroll
+    for (int i = 0; i < NS; ++i) to.w[i] = codes(a + ((kExact ? 0 : step * NS) + i) * 32 * kStage);
+#pragma unroll
+    for (int i = 0; i < MI; ++i) to.x[i] = codes(b + i * 32 * kStage);
+  };
+  auto read_scales = [&](Scales& to, int block) {
     const uint8_t* e = &exps[block >> 2 & 1][block & 3];
-    uint32_t wq[NI], xq[MI];
 #pragma unroll
-    for (int i = 0; i < NI; ++i) wq[i] = e[(BM + wn + i * 32 + l32) * 4];
+    for (int i = 0; i < NI; ++i) to.w[i] = e[(BM + wn + i * 32 + l32) * 4];
 #pragma unroll
-    for (int i = 0; i < MI; ++i) xq[i] = e[(wm + i * 32 + l32) * 4];
+    for (int i = 0; i < MI; ++i) to.x[i] = e[(wm + i * 32 + l32) * 4];
+  };
+  auto multiply = [&](const Step& s, const Scales& q, int step) {
     if constexpr (kExact) {
-      float wf[NI], xf[MI];
 #pragma unroll
-      for (int i = 0; i < NI; ++i) wf[i] = scale_of(wq[i]);
+      for (int h = 0; h < 2; ++h) {
+        bf16x8 wb[NI], xb[MI];
 #pragma unroll
-      for (int i = 0; i < MI; ++i) xf[i] = scale_of(xq[i]);
+        for (int i = 0; i < MI; ++i) xb[i] = widen8(s.x[i][2 * h], s.x[i][2 * h + 1], scale_of(q.x[i]));
 #pragma unroll
-      for (int s = 0; s < BK / 32; ++s) {
-        intx4 wv[NI], xv[MI];
-#pragma unroll
-        for (int i = 0; i < NI; ++i) wv[i] = piece(a, i, 2 * s + half);
-#pragma unroll
-        for (int i = 0; i < MI; ++i) xv[i] = piece(b, i, 2 * s + half);
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          bf16x8 wb[NI], xb[MI];
-#pragma unroll
-          for (int i = 0; i < NI; ++i) wb[i] = widen8(wv[i][2 * h], wv[i][2 * h + 1], wf[i]);
-#pragma unroll
-          for (int i = 0; i < MI; ++i) xb[i] = widen8(xv[i][2 * h], xv[i][2 * h + 1], xf[i]);
-#pragma unroll
-          for (int i = 0; i < NI; ++i)
-#pragma unroll
-            for (int j = 0; j < MI; ++j)
-              acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wb[i], xb[j], acc[i][j], 0, 0, 0);
-        }
-      }
-    } else {
-#pragma unroll
-      for (int s = 0; s < BK / 64; ++s) {
-        intx8 wv[NI], xv[MI];
-#pragma unroll
-        for (int i = 0; i < NI; ++i) wv[i] = join(piece(a, i, 4 * s + half), piece(a, i, 4 * s + 2 + half));
-#pragma unroll
-        for (int i = 0; i < MI; ++i) xv[i] = join(piece(b, i, 4 * s + half), piece(b, i, 4 * s + 2 + half));
+        for (int i = 0; i < NI; ++i) wb[i] = widen8(s.w[i][2 * h], s.w[i][2 * h + 1], scale_of(q.w[i]));
 #pragma unroll
         for (int i = 0; i < NI; ++i)
 #pragma unroll
           for (int j = 0; j < MI; ++j)
-            acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wv[i], xv[j], acc[i][j], 0, 0, 0, (int)wq[i], 0,
-                                                                       (int)xq[j]);
+            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wb[i], xb[j], acc[i][j], 0, 0, 0);
       }
+    } else {
+#pragma unroll
+      for (int i = 0; i < NS; ++i)
+#pragma unroll
+        for (int j = 0; j < MI; ++j) {
+          floatx16& c = acc[step * NS + i][j];
+          c = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(s.w[i], s.x[j], c, 0, 0, 0, (int)q.w[step * NS + i], 0,
+                                                             (int)q.x[j]);
+        }
     }
-  }
+  };
 
 #pragma unroll
+  for (int i = 0; i < STAGES; ++i)
+    if (i < stages) fetch(i, i);
+  if (stages >= STAGES)
+    wait_and_meet<(STAGES - 1) * kCopies>();
+  else
+    wait_and_meet<0>();
+  Step now, next;
+  Scales scales, scales_next;
+  if (kAhead && busy) read_step(now, 0, 0);
+  read_scales(scales, 0);
+  int buffer = 0;
+  for (int block = 0; block < blocks; ++block) {
+#pragma unroll
+    for (int half_block = 0; half_block < 2; ++half_block) {
+      const int stage = 2 * block + half_block;
+      if (busy) {
+        if (!kAhead) read_step(now, buffer, 0);
+        read_step(next, buffer, 1);
+        multiply(now, scales, 0);
+        if (!kAhead) multiply(next, scales, 1);
+      }
+      const int after = buffer == STAGES - 1 ? 0 : buffer + 1;
+      if (stage + 1 < stages) {
+        // The next stage's copies are done when at most those of the STAGES - 2 after it are under way (exponents are asked
+        // for before the codes of their stage); this stage is in every wave's registers then.
+        if (stage + STAGES - 1 < stages)
+          wait_and_meet<(STAGES - 2) * kCopies>();
+        else
+          wait_and_meet<0>();
+        if (kAhead && busy) read_step(now, after, 0);
+        if (half_block == 1) read_scales(scales_next, block + 1);
+        if (stage + STAGES < stages) fetch(stage + STAGES, buffer);
+      }
+      if (kAhead && busy) multiply(next, scales, 1);
+      buffer = after;
+    }
+    scales = scales_next;
+  }
+
+  // A lane holds four columns of one row, 32 rows to a store: through LDS (a wave's 32 rows at a time, its own) a store
+  // and the loads beside it take whole rows of the wave's tile instead.
+  constexpr int kPitch = NI * 32 + 4, kLanesARow = NI * 8, kRowsAtOnce = 64 / kLanesARow,
+                kBatch = NI * MI > 4 ? 8 : 4;  // (rows to a lane at once, as registers allow)
+  static_assert(kWaves * 32 * kPitch * 4 <= (int)sizeof(lds), "the waves' rows fit");
+  float* rows = reinterpret_cast<float*>(&lds[0][0]) + wave * 32 * kPitch;
+  const int n = n0 + wn + lane % kLanesARow * 4, r0 = lane / kLanesARow;
+  const floatx4 bias = bias_of<VEC>(f, n);
+  __syncthreads();
+  if (!busy) return;
+#pragma unroll
   for (int j = 0; j < MI; ++j) {
-    floatx4 y[NI * 4];
 #pragma unroll
-    for (int i = 0; i < NI * 4; ++i)
+    for (int i = 0; i < NI; ++i)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) y[i][e] = acc[i / 4][j][i % 4 * 4 + e];
-    finish<TO, VEC>(f, y, m0 + wm + j * 32 + l32,
-                    [&](int i) { return n0 + wn + i / 4 * 32 + i % 4 * 8 + half * 4; });
+      for (int g = 0; g < 4; ++g)
+        *reinterpret_cast<floatx4*>(rows + l32 * kPitch + i * 32 + g * 8 + half * 4) =
+            floatx4{acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
+    __builtin_amdgcn_wave_barrier();
+    for (int r = r0; r < 32; r += kBatch * kRowsAtOnce) {
+      floatx4 y[kBatch];
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i)
+        y[i] = *reinterpret_cast<const floatx4*>(rows + (r + i * kRowsAtOnce) * kPitch + lane % kLanesARow * 4);
+      finish<TO, VEC>(f, y, bias, n, [&](int i) { return m0 + wm + j * 32 + r + i * kRowsAtOnce; });
+    }
+    __builtin_amdgcn_wave_barrier();
   }
 }
 
@@ -358,7 +430,7 @@ __global__ __launch_bounds__(kFewWaves * 64) void fp8_few_kernel(const T* __rest
     floatx4 y[1] = {part[0][tile][at]};
 #pragma unroll
     for (int w = 1; w < kFewWaves; ++w) y[0] += part[w][tile][at];
-    finish<TO, VECO>(f, y, m, [&](int) { return n; });
+    finish<TO, VECO>(f, y, bias_of<VECO>(f, n), n, [&](int) { return m; });
   }
 }
 
@@ -396,7 +468,7 @@ int launch_few(const Fp8LinearParams& p, const Finish& f, bool veco, hipStream_t
   return launch_few_rows<T, false, 4, TO>(p, f, veco, stream);
 }
 
-template <int BM, int BN, int WM, int WN, int BK, int STAGES, class TO>
+template <int BM, int BN, int WM, int WN, int STAGES, class TO>
 int launch_tiles(const Fp8LinearParams& p, const uint8_t* xc, const uint8_t* xe, const Finish& f, bool veco,
                  hipStream_t stream) {
   const int tiles_n = (p.N + BN - 1) / BN;
@@ -407,8 +479,8 @@ int launch_tiles(const Fp8LinearParams& p, const uint8_t* xc, const uint8_t* xe,
                                                     (int)fp8_exponent_stride(p.K), tiles_n);
     return hipGetLastError() == hipSuccess ? kOk : kErrLaunch;
   };
-  return veco ? go(fp8_tile_kernel<BM, BN, WM, WN, BK, STAGES, TO, true>)
-              : go(fp8_tile_kernel<BM, BN, WM, WN, BK, STAGES, TO, false>);
+  return veco ? go(fp8_tile_kernel<BM, BN, WM, WN, STAGES, TO, true>)
+              : go(fp8_tile_kernel<BM, BN, WM, WN, STAGES, TO, false>);
 }
 
 template <class TO>
@@ -431,7 +503,9 @@ int launch_out(const Fp8LinearParams& p, hipStream_t stream) {
     if (st != kOk) return st;
     xc = codes, xe = exps;
   }
-  return launch_tiles<128, 256, 2, 2, 64, 3, TO>(p, xc, xe, f, veco, stream);
+  const int64_t wide = (int64_t)((p.M + 127) / 128) * ((p.N + 255) / 256);
+  if (wide < 2 * compute_units()) return launch_tiles<128, 128, 2, 2, 3, TO>(p, xc, xe, f, veco, stream);
+  return launch_tiles<128, 256, 2, 2, 3, TO>(p, xc, xe, f, veco, stream);
 }
 
 }  // namespace
