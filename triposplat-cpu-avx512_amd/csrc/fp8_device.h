@@ -47,10 +47,29 @@ __device__ __forceinline__ floatx4 load4(const T* row, int k, int K) {
   return v;
 }
 
-// The bits of |v| where it is finite, else 0: their largest is that of the block's finite magnitudes.
-__device__ __forceinline__ uint32_t finite_bits(float v) {
-  const uint32_t u = __float_as_uint(v) & 0x7fffffffu;
-  return u < 0x7f800000u ? u : 0u;
+// The bits of the largest finite magnitude of a lane's COUNT quadruples and of its neighbours' by `over`, which agrees on
+// the largest of a float's bits.  Values that are not finite are rare: only a wave that meets an infinity looks at each
+// value (a NaN is passed over by the maximum).
+template <int COUNT, class Over>
+__device__ __forceinline__ uint32_t largest_bits(const floatx4 (&v)[COUNT], Over over) {
+  float top = 0.0f;
+#pragma unroll
+  for (int i = 0; i < COUNT; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) top = fmaxf(top, fabsf(v[i][e]));
+  uint32_t bits = over(__float_as_uint(top));
+  if (__any(bits >= 0x7f800000u)) {
+    bits = 0;
+#pragma unroll
+    for (int i = 0; i < COUNT; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t u = __float_as_uint(v[i][e]) & 0x7fffffffu;
+        bits = max(bits, u < 0x7f800000u ? u : 0u);
+      }
+    bits = over(bits);
+  }
+  return bits;
 }
 
 // The exponent (+ 127) of the block's scale from its largest magnitude's bits: the smallest e with
@@ -64,12 +83,16 @@ __device__ __forceinline__ int scale_exponent(uint32_t top) {
 __device__ __forceinline__ float inverse_scale(int e) { return __uint_as_float((uint32_t)(254 - e) << 23); }
 
 // Four codes of v * inverse.  The product is exact (a subnormal one is far below half of the smallest code), so there
-// is one rounding, the conversion's, to nearest even; 448 is never passed.  An infinity becomes a NaN like a NaN.
+// is one rounding, the conversion's, to nearest even; 448 is never passed by a finite value.  An infinity becomes a NaN
+// like a NaN (the conversion makes 448 of it).
 __device__ __forceinline__ int encode4(const floatx4& v, float inverse) {
   float u[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    u[i] = (__float_as_uint(v[i]) & 0x7f800000u) == 0x7f800000u ? __uint_as_float(0x7fc00000u) : v[i] * inverse;
+  for (int i = 0; i < 4; ++i) u[i] = v[i] * inverse;
+  if (__any(!(fmaxf(fmaxf(fabsf(u[0]), fabsf(u[1])), fmaxf(fabsf(u[2]), fabsf(u[3]))) <= 448.0f))) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) u[i] = fabsf(u[i]) <= 448.0f ? u[i] : __uint_as_float(0x7fc00000u);
+  }
   int w = __builtin_amdgcn_cvt_pk_fp8_f32(u[0], u[1], 0, false);
   return __builtin_amdgcn_cvt_pk_fp8_f32(u[2], u[3], w, true);
 }

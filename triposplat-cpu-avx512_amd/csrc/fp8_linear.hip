@@ -175,7 +175,7 @@ __global__ __launch_bounds__(WM* WN * 64, BM * BN > 128 * 128 ? 2 : 3) void fp8_
   static_assert(kCopies * kRowsACopy * kWaves == BM + BN && BM % kRowsACopy == 0, "whole copies");
   __shared__ __attribute__((aligned(16))) uint8_t lds[STAGES][(BM + BN) * kStage];
   __shared__ __attribute__((aligned(16))) uint8_t exps[2][(BM + BN) * 4];
-  constexpr bool kAhead = kExact;
+  constexpr bool kAhead = true;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int tile = tile_of(blockIdx.x, gridDim.x);
   const int m0 = tile / tiles_n * BM, n0 = tile % tiles_n * BN;
@@ -391,15 +391,12 @@ __global__ __launch_bounds__(kFewWaves * 64) void fp8_few_kernel(const T* __rest
       int xq;
       if (x) {
         floatx4 v[8];
-        uint32_t top = 0;
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = load4<T, VEC>(x + m * x_stride, block * kFp8Block + quarter * 32 + i * 4, K);
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) top = max(top, finite_bits(v[i][e]));
-        top = max(top, (uint32_t)__shfl_xor((int)top, 16));
-        top = max(top, (uint32_t)__shfl_xor((int)top, 32));
+        const uint32_t top = largest_bits(v, [](uint32_t bits) {
+          bits = max(bits, (uint32_t)__shfl_xor((int)bits, 16));
+          return max(bits, (uint32_t)__shfl_xor((int)bits, 32));
+        });
         xq = scale_exponent(top);
 #pragma unroll
         for (int i = 0; i < 8; ++i) xv[i] = encode4(v[i], inverse_scale(xq));
@@ -444,7 +441,7 @@ int size_of(int dtype) { return dtype == kValueF32 ? 4 : 2; }
 
 template <class T, bool VEC, int MB, class TO>
 int launch_few_rows(const Fp8LinearParams& p, const Finish& f, bool veco, hipStream_t stream) {
-  constexpr int NB = 1;
+  constexpr int NB = MB >= 2 ? 2 : 1;
   const int grid = (p.N + 16 * NB - 1) / (16 * NB);
   auto go = [&](auto kernel) {
     kernel<<<grid, kFewWaves * 64, 0, stream>>>(static_cast<const T*>(p.x), p.x_stride, p.x_codes, p.x_exponents,

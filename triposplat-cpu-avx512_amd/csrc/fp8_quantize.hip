@@ -41,9 +41,12 @@ __global__ __launch_bounds__(kThreads) void fp8_quantize_kernel(Fp8QuantizeParam
 #pragma unroll
     for (int j = 0; j < kAhead; ++j) {
       if (i0 + j * kGroups >= items) break;
-      uint32_t top = max(max(finite_bits(v[j][0]), finite_bits(v[j][1])), max(finite_bits(v[j][2]), finite_bits(v[j][3])));
+      const floatx4 one[1] = {v[j]};
+      const uint32_t top = largest_bits(one, [](uint32_t bits) {
 #pragma unroll
-      for (int d = 16; d > 0; d >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, d, 32));
+        for (int d = 16; d > 0; d >>= 1) bits = max(bits, (uint32_t)__shfl_xor((int)bits, d, 32));
+        return bits;
+      });
       const int e = scale_exponent(top);
       if (block[j] < blocks)
         *reinterpret_cast<int*>(codes + (int64_t)row[j] * code_stride + block[j] * kFp8Block + lane * 4) =
