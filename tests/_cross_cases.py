@@ -7,8 +7,9 @@ U = 2.0 ** -24
 STEP = {"float32": 2.0 ** -24, "bfloat16": 2.0 ** -8, "float16": 2.0 ** -11}  # half a step of the type
 LEAST = {"float32": 2.0 ** -150, "bfloat16": 2.0 ** -134, "float16": 2.0 ** -25}  # half of its smallest value
 # What a product of fp32 factors loses relative to |a| |b|: bf16 terms hold 2^-8, 2^-16, 2^-24 of a factor, and the
-# products of the terms i and j with i + j of the number of terms or more are left out.
-LOST = {"fp32": 5 * 2.0 ** -24, "bf16x3": 3.1 * 2.0 ** -16, "bf16": 2.01 * 2.0 ** -8}
+# products of the terms i and j with i + j of the number of terms or more are left out.  Pairs of fp16 values hold a factor
+# to 2^-23 (half a step of 2^-12 of what is left, which is 2^-11 at most) and leave out a product of 2^-11 by 2^-11: 2^-21.
+LOST = {"fp32": 8.1 * 2.0 ** -24, "bf16x3": 3.1 * 2.0 ** -16, "bf16": 2.01 * 2.0 ** -8}
 
 
 def cross(torch, q, k, v, q_lengths, k_lengths, bias=None, scale=None, precision="fp32"):
@@ -20,7 +21,8 @@ def cross(torch, q, k, v, q_lengths, k_lengths, bias=None, scale=None, precision
     |x - m| + 8, the exponential 1 ulp.  A relative error d of each weight moves the result by 2 d sum w |v|; the sums over
     n states (and one more for each of the parts that they are cut into, fewer than n / 32 + 8) by 2 U each addition, in the
     numerator and the denominator; a 16-bit weight is rounded by half a step, in the numerator only, and in fp16 by 2^-25
-    of what is lifted by 2^7, 2^-32 of the largest weight."""
+    of what is lifted by 2^7, 2^-32 of the largest weight.  fp32 values in pairs of fp16: 2^-22 more of a score (twice: k's
+    small values and q's), 2^-25 of v scaled to 2^9 at least for its first tile's largest, 2^-25 of weights lifted by 2^11."""
     name = str(q.dtype).split(".")[-1]
     rows, heads, D = q.shape
     group = heads // k.shape[1]
@@ -39,6 +41,8 @@ def cross(torch, q, k, v, q_lengths, k_lengths, bias=None, scale=None, precision
             size = scale * torch.bmm(qq.abs(), kk.abs().transpose(1, 2).contiguous())
             lost = LOST[precision] if name == "float32" else 0.0
             off = ((2 * D * (1 + 2.0 ** -5) + 6) * U + lost) * size
+            if name == "float32" and precision == "fp32":
+                off = off + 2 * 2.0 ** -22
             if bias is not None:
                 b = bias[keep].double()
                 s = s + b
@@ -63,6 +67,8 @@ def cross(torch, q, k, v, q_lengths, k_lengths, bias=None, scale=None, precision
                     moved = moved + 2.0 ** -32 * vv.abs().sum(1, keepdim=True) / total
             else:
                 moved = moved + lost * wv
+                if precision == "fp32":
+                    moved = moved + 2.0 ** -34 * vv.abs().amax() + 2.0 ** -36 * vv.abs().sum(1, keepdim=True) / total
             out[q0:q0 + nq] = o.transpose(0, 1)
             bound[q0:q0 + nq] = moved.transpose(0, 1)
         q0, k0 = q0 + nq, k0 + nk

@@ -181,6 +181,7 @@ def test_strides_and_alignment(cuda, hiplib, dtype):
     plan = _plan(torch, cuda, queries, keys, heads, kv_heads, D, dtype)
     want = cross_attention(q, k, v, plan, key_bias=bias)
     assert not want[43:].any() and want.shape == q.shape
+    exact, bound = cross(torch, q, k, v, queries, keys, bias)
     flat = torch.randn(48 * heads * 80 + 9, generator=g, device=cuda).to(dt)
     for offset, token, head in ((0, heads * 80, 80), (1, heads * 80, 80), (3, heads * 65, 65), (8, 72, 48 * 72), (2, 70, 48 * 70)):
         q2 = flat.as_strided((48, heads, D), (token, head, 1), offset)
@@ -190,9 +191,68 @@ def test_strides_and_alignment(cuda, hiplib, dtype):
         buffer = torch.full((48 * heads * 80 + 9,), 7.0, device=cuda, dtype=dt)
         out = buffer.as_strided((48, heads, D), (token, head, 1), offset)
         assert cross_attention(q2, k2, v, plan, key_bias=bias, out=out) is out
-        assert torch.equal(out[:43], want[:43])
+        if dtype == "float32":  # (aligned calls go by pairs of fp16 values, others by bf16 terms)
+            assert_within(torch, out[:43].double(), exact[:43], bound[:43], "strides")
+        else:
+            assert torch.equal(out[:43], want[:43])
         out[:43] = 7.0
         assert bool((buffer == 7).all())
+
+
+def _outliers(torch, kind, q, k, v):
+    """Values that pairs of fp16 under one scale do not hold; the weights of the outlying states are zero or all."""
+    if kind == "k early":
+        k[3] = -1e6 * q[0, 0].sign()
+    elif kind == "k late":
+        k[400] = -1e6 * q[0, 0].sign()
+    elif kind == "q":
+        q[7] *= 1e5
+    elif kind == "v early":
+        v[2] = 1e12
+    elif kind == "v late":
+        v[401] = 1e12
+    elif kind == "v small":
+        v[:, :, 8:16] *= 1e-9
+    elif kind == "v steps":
+        v[:] *= torch.logspace(-12, 12, len(v), device=v.device)[:, None, None]
+    elif kind == "zeros first":
+        k[:200], v[:200] = 0.0, 0.0
+    elif kind == "all small":
+        q *= 1e-15
+        k *= 1e-15
+        v *= 1e-15
+    elif kind == "all large":
+        q *= 1e12
+        k *= 1e-12
+        v *= 1e30
+    elif kind == "zero":
+        q[:], k[:], v[:] = 0.0, 0.0, 0.0
+
+
+@pytest.mark.parametrize("kind", ["k early", "k late", "q", "v early", "v late", "v small", "v steps", "zeros first",
+                                  "all small", "all large", "zero"])
+@pytest.mark.parametrize("D", [64, 128])
+def test_values_of_unlike_sizes(cuda, hiplib, kind, D):
+    """fp32 accuracy whatever the values' sizes: what one state or feature holds costs no other one anything, and a result
+    does not depend on the other requests of the batch."""
+    import torch
+    from tsplat.cross_attention import cross_attention
+
+    queries, keys = [300, 40, 300], [500, 90, 500]
+    q, k, v, bias, g = _inputs(torch, cuda, queries, keys, 2, 2, D, "float32", 12)
+    k, v = k.contiguous(), v.contiguous()
+    plain = cross_attention(q, k, v, _plan(torch, cuda, queries, keys, 2, 2, D, "float32"))
+    _outliers(torch, kind, q[:300], k[:500], v[:500])
+    plan = _plan(torch, cuda, queries, keys, 2, 2, D, "float32")
+    for b in (None, bias):
+        want, bound = cross(torch, q, k, v, queries, keys, b)
+        got = cross_attention(q, k, v, plan, key_bias=b)
+        if kind == "q":  # scores of 1e5: the bound's first order says nothing for those rows
+            rows = torch.arange(640, device=cuda) != 7
+            got, want, bound = got[rows], want[rows], bound[rows]
+        assert_within(torch, got.double(), want, bound, kind)
+        if b is None:
+            assert torch.equal(got[-340:], plain[-340:])
 
 
 def test_offsets_past_32_bits(cuda, hiplib):

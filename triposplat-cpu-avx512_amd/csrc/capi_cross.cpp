@@ -47,8 +47,10 @@ bool is_header(const int32_t* h) {
          h[kPlanTerms] <= 3 && (h[kPlanType] == 0 || h[kPlanTerms] == 1);
 }
 
+// The parts' sums, then the pairs' flags.
+int64_t part_bytes(const int32_t* h) { return (int64_t)h[kPlanParts] * h[kPlanKvHeads] * cross_part_floats(h) * 4; }
 int64_t scratch_bytes(const int32_t* h) {
-  return (int64_t)h[kPlanParts] * h[kPlanKvHeads] * cross_part_floats(h) * 4;
+  return part_bytes(h) + (cross_has_pairs(h) ? ((int64_t)h[kPlanItems] * h[kPlanKvHeads] * 4 + 15) / 16 * 16 : 0);
 }
 
 bool multiple(int64_t stride, int64_t count, int of) { return count == 1 || stride % of == 0; }
@@ -129,6 +131,11 @@ int tsplat_cross_attention_async(const void* q, int64_t q_token, int64_t q_head,
                            multiple(k_head, kv_heads, eights) && multiple(v_token, states, eights) &&
                            multiple(v_head, kv_heads, eights)));
   const hipStream_t s = static_cast<hipStream_t>(stream);
+  if (cross_has_pairs(h) && p.vec) {
+    p.flags = reinterpret_cast<int32_t*>(static_cast<char*>(scratch) + part_bytes(h));
+    const int st = launch_cross_pairs(p, s);
+    if (st != kOk) return launched(st);
+  }
   const int st = p.type != 0 ? launch_cross_16(p, s) : p.terms == 3 ? launch_cross_f32(p, s) : launch_cross_f32_fast(p, s);
   if (st != kOk || p.join_count == 0) return launched(st);
   return launched(launch_cross_join(p, s));

@@ -19,10 +19,12 @@ struct CrossParams {
   const CrossJoin* joins;
   int item_count, join_count, parts;
   float* partial;
+  int32_t* flags;  // of pairs: a workgroup's (item, key head) that they do not serve; null: no pairs
   int vec;  // q, k, v in eights and out in fours are aligned, and dim is a multiple of 8
 };
 int launch_cross_f32(const CrossParams& p, hipStream_t stream);
 int launch_cross_f32_fast(const CrossParams& p, hipStream_t stream);
+int launch_cross_pairs(const CrossParams& p, hipStream_t stream);
 int launch_cross_16(const CrossParams& p, hipStream_t stream);
 // The partial results' join.
 int launch_cross_join(const CrossParams& p, hipStream_t stream);

@@ -157,6 +157,20 @@ __device__ __forceinline__ int xcd_order() {
   return xcd * per + min(xcd, more) + blockIdx.x / 8;
 }
 
+// Many rows: which item and key head a workgroup takes.  An XCD takes all tiles of the same key heads, which share their
+// states in its L2, the longest first.
+struct Work {
+  int item, kv;
+};
+__device__ __forceinline__ Work work_of(const CrossParams& p) {
+  if (p.kv_heads % 8 != 0) {
+    const int id = xcd_order();
+    return {id % p.item_count, id / p.item_count};
+  }
+  const int id = blockIdx.x / 8, heads = p.kv_heads / 8;
+  return {id / heads, (int)(blockIdx.x % 8) * heads + id % heads};
+}
+
 // The query row of a lane: where q's vector and the result's lie.
 struct Row {
   int64_t token;
@@ -265,12 +279,10 @@ __global__ __launch_bounds__(cross_tile(DP, TERMS, false).wq * 64, 2) void cross
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l32 = lane & 31, half = lane >> 5;
-  // An XCD takes all tiles of the same key heads, which share their states in its L2, the longest first.
-  const bool whole = p.kv_heads % 8 == 0;
-  const int id = whole ? blockIdx.x / 8 : xcd_order(), heads = whole ? p.kv_heads / 8 : 1;
-  const CrossItem item = p.items[whole ? id / heads : id % p.item_count];
-  const int kv = whole ? blockIdx.x % 8 * heads + id % heads : id / p.item_count;
-  const int D = p.dim;
+  const Work work = work_of(p);
+  if (p.flags && p.flags[(int64_t)work.item * p.kv_heads + work.kv] == 0) return;  // (done by the pairs)
+  const CrossItem item = p.items[work.item];
+  const int kv = work.kv, D = p.dim;
 
   // this lane's row
   const int row = wave * 32 + l32;

@@ -54,4 +54,9 @@ inline int64_t cross_part_floats(const int32_t* header) {
   return (int64_t)cross_tile(padded, header[kPlanTerms], header[kPlanFew] != 0).wq * 32 * (padded + 2);
 }
 
+// Whether a call may go by pairs of fp16 values (cross_pairs.hip): fp32 at fp32 accuracy, many rows.
+inline bool cross_has_pairs(const int32_t* header) {
+  return header[kPlanType] == 0 && header[kPlanTerms] == 3 && header[kPlanFew] == 0;
+}
+
 }  // namespace tsplat
