@@ -1,6 +1,6 @@
 // Cross attention of fp32 values as pairs of fp16 values, for many rows: three products of 16-bit terms where bf16 terms
 // take six.
-//   q' sq = qh + ql,  k sk = kh + kl,  v sv = vh + vl,  2^7 p = ph + pl
+//   q' sq = qh + ql,  k sk = kh + kl,  v sv = vh + vl,  p = ph + pl
 //   S = qh kh + ql kh + qh kl,  O = ph vh + pl vh + ph vl
 // A pair holds its value to 2^-23 of it and to 2^-25; products of fp16 values are exact in fp32 and the dropped ones are
 // below 2^-22 of the product.  sq, a power of two of the row's own, brings q's largest magnitude to [2^14, 2^15); sk and sv
@@ -13,8 +13,9 @@
 // than 2^-21 of themselves); an infinity or NaN in q.  It then leaves its result to the kernel of bf16 terms, which is
 // launched behind this one and does what is flagged: any input has fp32's accuracy, an unusual one at that kernel's time.
 //
-// p = 2^(x - m) for a reference m that is 4 below the row's largest x, or up to 8 (few tiles rescale), and 2^7 times that is
-// below 2^15; the lift comes after the exponential, whose argument keeps its last place.
+// p = 2^(x - m) for a reference m that is 11 below the row's largest x, or up to 15 (few tiles rescale): below 2^15, and a
+// weight 2^-36 of the largest is still held.  (The exponential's argument is rounded by 2^-21 at most there, 3e-7 of a
+// weight, which its sum has as well; a factor after the exponential instead takes 16 more instructions a block.)
 //
 // Everything else as in cross_attention_kernel.h: a workgroup of eight waves of 32 rows, S^T = K Q^T, O^T = V^T P^T.
 
@@ -24,17 +25,22 @@ namespace tsplat {
 namespace cross {
 
 typedef _Float16 halfx2 __attribute__((ext_vector_type(2)));
+typedef float floatx2 __attribute__((ext_vector_type(2)));
 
-constexpr float kPairSlack = 4.0f, kPairBase = 4.0f, kPairLift = 128.0f;
+constexpr float kPairSlack = 4.0f, kPairBase = 11.0f;
 constexpr float kPairTop = 0x1p15f, kPairLeast = 0x1p-4f, kPairScores = 8.0f;
 
 // Eight values as pairs.
 __device__ __forceinline__ void pair8(const float (&x)[8], shortx8 (&out)[2]) {
   intx4 hi, lo;
+  float minus = -1.0f;
+  asm("" : "+s"(minus));  // (a product that the compiler does not turn back into two conversions and a difference)
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const halfx2 h = {(half_t)x[2 * i], (half_t)x[2 * i + 1]};
-    const halfx2 l = {(half_t)(x[2 * i] - (float)h[0]), (half_t)(x[2 * i + 1] - (float)h[1])};
+    const halfx2 h = __builtin_convertvector(floatx2{x[2 * i], x[2 * i + 1]}, halfx2);
+    // (fused products take the halves where they are; exact)
+    const halfx2 l = __builtin_convertvector(
+        floatx2{fmaf((float)h[0], minus, x[2 * i]), fmaf((float)h[1], minus, x[2 * i + 1])}, halfx2);
     hi[i] = __builtin_bit_cast(int, h);
     lo[i] = __builtin_bit_cast(int, l);
   }
@@ -63,8 +69,9 @@ __device__ __forceinline__ floatx16 pair_products(const shortx8 (&a)[2], const s
 template <int DP, bool BIAS>
 __global__ __launch_bounds__(cross_tile(DP, 3, false).wq * 64, 2) void cross_pair_kernel(CrossParams p) {
   constexpr CrossTile kTile = cross_tile(DP, 3, false);
-  constexpr int KB = kTile.kb, kWaves = kTile.wq, kThreads = kWaves * 64, kKeys = KB * 32, kBlocks = DP / 32,
-                kSlices = DP / 16;
+  // (two runs of KB blocks between barriers where LDS holds them: waves that are apart multiply while others take exponents)
+  constexpr int KB = kTile.kb, kRuns = DP == 64 ? 2 : 1, kWaves = kTile.wq, kThreads = kWaves * 64,
+                kKeys = kRuns * KB * 32, kBlocks = DP / 32, kSlices = DP / 16;
   constexpr int kAllUnits = kKeys * DP / 8, kUnits = (kAllUnits + kThreads - 1) / kThreads;  // of 8 values
   constexpr int kRowK = DP + 8, kRowV = DP + 16;  // values from row to row
   constexpr int kPlaneK = kKeys * kRowK, kPlaneV = kKeys * kRowV, kBuffer = 2 * (kPlaneK + kPlaneV);
@@ -207,9 +214,12 @@ __global__ __launch_bounds__(cross_tile(DP, 3, false).wq * 64, 2) void cross_pai
     __syncthreads();
     if (t + 1 < tiles) load((t + 1) * kKeys);
     if (!wave_live) continue;
-    const short* kp = lds + buf * kBuffer + l32 * kRowK + 8 * half;
-    const short* vp = lds + buf * kBuffer + 2 * kPlaneK + (4 * half + (lane & 15) / 4) * kRowV + (lane >> 4 & 1) * 16 +
-                      (lane & 3) * 4;
+#pragma unroll 1
+    for (int first = 0; first < kKeys; first += KB * 32) {
+    if (t * kKeys + first >= item.keys) break;
+    const short* kp = lds + buf * kBuffer + (first + l32) * kRowK + 8 * half;
+    const short* vp = lds + buf * kBuffer + 2 * kPlaneK + (first + 4 * half + (lane & 15) / 4) * kRowV +
+                      (lane >> 4 & 1) * 16 + (lane & 3) * 4;
     floatx16 s[KB];
 #pragma unroll
     for (int b = 0; b < KB; ++b) {
@@ -224,11 +234,11 @@ __global__ __launch_bounds__(cross_tile(DP, 3, false).wq * 64, 2) void cross_pai
         s[b] = pair_products(kt, q[c], s[b]);
       }
       if constexpr (BIAS) {
-        const float* add = &biases[buf][b * 32 + 4 * half];
+        const float* add = &biases[buf][first + b * 32 + 4 * half];
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[b][r] = fmaf(s[b][r], to_log2, add[r / 4 * 8 + r % 4]);
       } else {
-        const int left = item.keys - (t * kKeys + b * 32) - 4 * half;  // states of this block from this lane's first
+        const int left = item.keys - (t * kKeys + first + b * 32) - 4 * half;  // states of this block from this lane's first
         if (left < 32) {
 #pragma unroll
           for (int r = 0; r < 16; ++r)
@@ -261,7 +271,7 @@ __global__ __launch_bounds__(cross_tile(DP, 3, false).wq * 64, 2) void cross_pai
       for (int c = 0; c < 2; ++c) {
         float x[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = s[b][8 * c + i] * kPairLift;
+        for (int i = 0; i < 8; ++i) x[i] = s[b][8 * c + i];
         shortx8 pt[2];
         pair8(x, pt);
 #pragma unroll
@@ -274,13 +284,14 @@ __global__ __launch_bounds__(cross_tile(DP, 3, false).wq * 64, 2) void cross_pai
         }
       }
     }
+    }
   }
 
   bad |= !(most < kPairTop) || least < kPairLeast;
   bad = __syncthreads_or(bad);
   if (tid == 0) *flag = bad;
   if (bad || !live) return;
-  const float l = l_run + other_half(l_run), down = power(-ev) / kPairLift;
+  const float l = l_run + other_half(l_run), down = power(-ev);
 #pragma unroll
   for (int b = 0; b < kBlocks; ++b)
 #pragma unroll
