@@ -25,7 +25,10 @@ def _codes_equal(torch, q, x):
     assert torch.equal(q.exponents.to(torch.int64), e)
     assert torch.equal(torch.nan_to_num(got, nan=999.0), torch.nan_to_num(code[:, :K], nan=999.0))
     # what lies past K and past the last block
-    assert not q._codes[:, K:].any() and bool((q._exponents[:, e.shape[1]:] == 127).all())
+    B = q.blocks
+    codes = q._buffer[:x.shape[0] * 128 * B].view(-1, 128 * B)
+    exponents = q._buffer[x.shape[0] * 128 * B:].view(x.shape[0], -1)
+    assert not codes[:, K:].any() and bool((exponents[:, B:] == 127).all())
 
 
 @pytest.mark.parametrize("dtype", TYPES)

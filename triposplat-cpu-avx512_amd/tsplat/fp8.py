@@ -32,28 +32,36 @@ class Fp8Rows:
     """Rows of K values in 8 bits: values [rows, K] = codes * 2^(exponents - 127), an exponent for each 128 of a row.
     Made by quantize_blocks."""
 
-    def __init__(self, buffers, rows, features):
-        self._codes, self._exponents = buffers  # [rows, K rounded up to 128], [rows, blocks rounded up to 4], uint8
+    def __init__(self, buffer, at, rows, features):
+        # uint8: the codes' rows, K rounded up to 128 bytes each, and the exponents', blocks rounded up to 4, at `at`
+        self._buffer, self._at = buffer, at
         self.rows, self.features = rows, features
-        self.device, self.index = self._codes.device, self._codes.get_device()
+        self.blocks = -(-features // BLOCK)
+        self.device, self.index = buffer.device, buffer.get_device()
+        base = buffer.data_ptr()
+        self.codes_ptr, self.exponents_ptr = base + at[0], base + at[1]
+
+    def _rows_of(self, which, width, step):
+        return self._buffer.as_strided((self.rows, width), (step, 1), self._at[which])
 
     @property
     def codes(self):
         """[rows, K] float8_e4m3fn, a view."""
         import torch
 
-        return self._codes.view(torch.float8_e4m3fn)[:, :self.features]
+        return self._rows_of(0, self.features, self.blocks * BLOCK).view(torch.float8_e4m3fn)
 
     @property
     def exponents(self):
         """[rows, ceil(K / 128)] uint8, a view: a block's scale is 2^(exponent - 127)."""
-        return self._exponents[:, :-(-self.features // BLOCK)]
+        return self._rows_of(1, self.blocks, _fours(self.blocks))
 
     def narrow(self, start, count):
         """Rows start .. start + count - 1, a view (of a weight: a run of its outputs)."""
         if start < 0 or count < 0 or start + count > self.rows:
             raise ValueError(f"rows {start}..{start + count} of {self.rows}")
-        return Fp8Rows((self._codes[start:start + count], self._exponents[start:start + count]), count, self.features)
+        at = self._at[0] + start * self.blocks * BLOCK, self._at[1] + start * _fours(self.blocks)
+        return Fp8Rows(self._buffer, at, count, self.features)
 
     def dequantize(self):
         """The values that the codes stand for, fp32 [rows, K] (exact)."""
@@ -61,8 +69,13 @@ class Fp8Rows:
 
         # (2^(e - 127) by its bits in 64 bits: 2^-127 is subnormal in fp32)
         scale = ((self.exponents.to(torch.int64) + 896) << 52).view(torch.float64)
-        padded = self._codes.view(torch.float8_e4m3fn).float().view(self.rows, -1, BLOCK)
-        return (padded.double() * scale[:, :, None]).float().view(self.rows, -1)[:, :self.features].contiguous()
+        padded = self._rows_of(0, self.blocks * BLOCK, self.blocks * BLOCK).view(torch.float8_e4m3fn).float()
+        padded = padded.unflatten(1, (self.blocks, BLOCK)).double() * scale[:, :, None]
+        return padded.float().flatten(1)[:, :self.features].contiguous()
+
+
+def _fours(n):
+    return (n + 3) // 4 * 4
 
 
 def quantize_blocks(x, *, library=None):
@@ -82,12 +95,13 @@ def quantize_blocks(x, *, library=None):
     no_gradients(torch, x)
     _limits(M, K, 1)
     blocks = -(-K // BLOCK)
-    codes = torch.empty((M, blocks * BLOCK), dtype=torch.uint8, device=x.device)
-    exponents = torch.empty((M, -(-blocks // 4) * 4), dtype=torch.uint8, device=x.device)
+    codes = M * blocks * BLOCK
+    # (one piece of memory for both: an allocation takes the host longer than the smallest rows take the GPU)
+    rows = Fp8Rows(torch.empty(codes + M * _fours(blocks), dtype=torch.uint8, device=x.device), (0, codes), M, K)
     if M:
-        enqueue(load_library(library), "tsplat_fp8_quantize_async", x.get_device(), x.data_ptr(), types[kind], stride,
-                M, K, codes.data_ptr(), exponents.data_ptr())
-    return Fp8Rows((codes, exponents), M, K)
+        enqueue(load_library(library), "tsplat_fp8_quantize_async", rows.index, x.data_ptr(), types[kind], stride, M, K,
+                rows.codes_ptr, rows.exponents_ptr)
+    return rows
 
 
 def _limits(M, K, N):
@@ -170,8 +184,8 @@ def fp8_linear(x, weight, bias=None, *, activation=None, gate=None, residual=Non
     need = lib.tsplat_fp8_linear_scratch_bytes(M, K, N, not ready)
     scratch = torch.empty(need, dtype=torch.uint8, device=weight.device) if need else None
     enqueue(lib, "tsplat_fp8_linear_async", at, None if ready else x.data_ptr(), types[kind], x_stride,
-            x._codes.data_ptr() if ready else None, x._exponents.data_ptr() if ready else None,
-            weight._codes.data_ptr(), weight._exponents.data_ptr(), bias.data_ptr() if bias is not None else None,
+            x.codes_ptr if ready else None, x.exponents_ptr if ready else None,
+            weight.codes_ptr, weight.exponents_ptr, bias.data_ptr() if bias is not None else None,
             int(activation is not None), gate_ptr, gate_stride, per, res_ptr, res_stride, out.data_ptr(),
             types[result], out_stride, M, K, N, scratch.data_ptr() if need else None, need)
     return out
