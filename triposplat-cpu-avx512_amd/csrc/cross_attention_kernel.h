@@ -151,6 +151,12 @@ __device__ __forceinline__ shortx8 transposed(const short* from, int pitch) {
   return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
+// Keeps what follows behind what came before, where the compiler's order would need more registers than there are.
+template <bool NOW>
+__device__ __forceinline__ void in_order() {
+  if constexpr (NOW) __builtin_amdgcn_sched_barrier(0);
+}
+
 // A workgroup's number among the grid's, such that neighbours are on one XCD.
 __device__ __forceinline__ int xcd_order() {
   const int count = gridDim.x, per = count / 8, more = count % 8, xcd = blockIdx.x % 8;
@@ -181,23 +187,31 @@ __device__ __forceinline__ Row row_of(const CrossParams& p, const CrossItem& ite
   return {item.token0 + at / p.group, kv * p.group + at % p.group};
 }
 
-// Columns 16 c + 8 half + i of a lane's query row in slice c; whether an infinity or NaN is among them.
+// The thread's number again: what is made of it after a loop is not held in registers meanwhile.
+__device__ __forceinline__ int thread_again() {
+  int tid = threadIdx.x;
+  asm volatile("" : "+v"(tid));
+  return tid;
+}
+
+// Columns 16 c + 8 half + i of a lane's query row in slice c; whether an infinity or NaN may be
+// among them.
 template <class T, class E, int TERMS, bool VEC, int SLICES>
 __device__ __forceinline__ bool load_queries(const CrossParams& p, const Row& at, int half, shortx8 (&q)[SLICES][TERMS]) {
   const T* row = static_cast<const T*>(p.q) + at.token * p.q_token + at.head * p.q_head;
-  bool odd = false;
+  float sum = 0.0f;
 #pragma unroll
   for (int c = 0; c < SLICES; ++c) {
     Raw<T> r = past_end<T, VEC>(load_eight<T, VEC>(row, 16 * c + 8 * half, p.dim), 16 * c + 8 * half, p.dim, false);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) odd |= !(fabsf((float)r.x[i]) < INFINITY);
+    for (int i = 0; i < 8; ++i) sum += fabsf((float)r.x[i]);
     if constexpr (sizeof(T) == 4) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) r.x[i] *= p.scale * kLog2e;
     }
     terms_of<T, E, TERMS>(r, q[c]);
   }
-  return odd;
+  return !(sum < INFINITY);
 }
 
 // A bias in log2 units; a finite one stays finite (the type's lowest masks against others, not by itself).
@@ -265,12 +279,14 @@ __device__ __forceinline__ float weights(floatx16& s, float to_log2, float m) {
 
 // Many rows: a tile of states serves all of a workgroup's waves.
 template <class T, int TERMS, int DP, bool BIAS, bool VEC>
-__global__ __launch_bounds__(cross_tile(DP, TERMS, false).wq * 64, 2) void cross_kernel(CrossParams p) {
+__global__ __launch_bounds__(cross_tile(DP, TERMS, false).wq * 64, !VEC && DP > 64 && TERMS == 1 ? 1 : 2) void cross_kernel(
+    CrossParams p) {
   typedef typename Element<T>::type E;
   constexpr CrossTile kTile = cross_tile(DP, TERMS, false);
   constexpr int KB = kTile.kb, kThreads = kTile.wq * 64, kKeys = KB * 32, kBlocks = DP / 32, kSlices = DP / 16;
   constexpr int kAllUnits = kKeys * DP / 8, kUnits = (kAllUnits + kThreads - 1) / kThreads;  // of 8 values
   constexpr int kRowK = DP + 8, kRowV = DP + 16;  // values from row to row
+  constexpr bool kTight = DP > 96 && sizeof(T) == 4 && (TERMS == 1 || !VEC);
   constexpr int kPlaneK = kKeys * kRowK, kPlaneV = kKeys * kRowV;
   constexpr int kBuffer = TERMS * (kPlaneK + kPlaneV);
   __shared__ __attribute__((aligned(16))) short lds[2 * kBuffer];
@@ -286,8 +302,7 @@ __global__ __launch_bounds__(cross_tile(DP, TERMS, false).wq * 64, 2) void cross
 
   // this lane's row
   const int row = wave * 32 + l32;
-  const bool live = row < item.rows;
-  const Row place = row_of(p, item, kv, live ? row : 0);
+  const Row place = row_of(p, item, kv, row < item.rows ? row : 0);
   shortx8 q[kSlices][TERMS];
   const bool odd = __any(load_queries<T, E, TERMS, VEC>(p, place, half, q));
   const float to_log2 = sizeof(T) == 4 ? 1.0f : p.scale * kLog2e;
@@ -305,8 +320,10 @@ __global__ __launch_bounds__(cross_tile(DP, TERMS, false).wq * 64, 2) void cross
       const int unit = tid + u * kThreads, dim = unit % (DP / 8) * 8;
       const int64_t from = min(key0 + unit / (DP / 8), item.keys - 1);
       kr[u] = load_eight<T, VEC>(kbase + from * p.k_token, dim, D);
+      in_order<kTight>();
       vr[u] = load_eight<T, VEC>(vbase + from * p.v_token, dim, D);
       if (BIAS) br[u] = bias_of(from);
+      in_order<kTight>();
     }
     if (BIAS && tid < kKeys) b2 = bias_of(min(key0 + tid, item.keys - 1));
   };
@@ -320,12 +337,12 @@ __global__ __launch_bounds__(cross_tile(DP, TERMS, false).wq * 64, 2) void cross
       const bool none = key0 + key >= item.keys || (BIAS && br[u] == -INFINITY);
       shortx8 kt[TERMS], vt[TERMS];
       terms_of<T, E, TERMS>(past_end<T, VEC>(kr[u], dim, D, none), kt);
+#pragma unroll
+      for (int t = 0; t < TERMS; ++t) *reinterpret_cast<shortx8*>(kp + t * kPlaneK + key * kRowK + dim) = kt[t];
+      in_order<kTight>();
       terms_of<T, E, TERMS>(past_end<T, VEC>(vr[u], dim, D, none), vt);
 #pragma unroll
-      for (int t = 0; t < TERMS; ++t) {
-        *reinterpret_cast<shortx8*>(kp + t * kPlaneK + key * kRowK + dim) = kt[t];
-        *reinterpret_cast<shortx8*>(vp + t * kPlaneV + key * kRowV + dim) = vt[t];
-      }
+      for (int t = 0; t < TERMS; ++t) *reinterpret_cast<shortx8*>(vp + t * kPlaneV + key * kRowV + dim) = vt[t];
     }
     if (BIAS && tid < kKeys) biases[buf][tid] = key0 + tid < item.keys ? bias_log2(b2) : -INFINITY;
   };
@@ -339,12 +356,14 @@ __global__ __launch_bounds__(cross_tile(DP, TERMS, false).wq * 64, 2) void cross
 
   const int tiles = (item.keys + kKeys - 1) / kKeys;
   const bool wave_live = wave * 32 < item.rows;
-  if (tiles > 0) load(0);
+  constexpr bool kLate = DP > 96 && TERMS == 3 && !VEC;  // (no registers to hold a tile while another is multiplied)
+  if (!kLate && tiles > 0) load(0);
   for (int t = 0; t < tiles; ++t) {
     const int buf = t & 1;
+    if (kLate) load(t * kKeys);
     store(t * kKeys, buf);
     __syncthreads();
-    if (t + 1 < tiles) load((t + 1) * kKeys);
+    if (!kLate && t + 1 < tiles) load((t + 1) * kKeys);
     if (!wave_live) continue;
     const short* kp = lds + buf * kBuffer + l32 * kRowK + 8 * half;
     const short* vp = lds + buf * kBuffer + TERMS * kPlaneK + (4 * half + (lane & 15) / 4) * kRowV +
@@ -362,6 +381,7 @@ __global__ __launch_bounds__(cross_tile(DP, TERMS, false).wq * 64, 2) void cross
         for (int i = 0; i < TERMS; ++i)
           kt[i] = *reinterpret_cast<const shortx8*>(kp + i * kPlaneK + b * 32 * kRowK + 16 * c);
         s[b] = products<E, TERMS>(kt, q[c], s[b]);
+        in_order<kTight>();
       }
       if constexpr (BIAS) {
         const float* br = &biases[buf][b * 32 + 4 * half];
@@ -417,13 +437,16 @@ __global__ __launch_bounds__(cross_tile(DP, TERMS, false).wq * 64, 2) void cross
           for (int i = 0; i < TERMS; ++i)
             vt[i] = transposed(vp + i * kPlaneV + (b * 32 + 16 * c) * kRowV + 32 * d, kRowV);
           o[d] = products<E, TERMS>(vt, pt, o[d]);
+          in_order<kTight>();
         }
       }
     }
   }
 
   const float l = l_run + other_half(l_run);
-  if (live) finish<T, DP, VEC>(p, item, kv, row, kTile.wq * 32, place, half, o, m_run, l);
+  const int again = thread_again(), out_row = (again >> 6) * 32 + (again & 31);
+  if (out_row < item.rows)
+    finish<T, DP, VEC>(p, item, kv, out_row, kTile.wq * 32, row_of(p, item, kv, out_row), again >> 5 & 1, o, m_run, l);
 }
 
 // At most 32 rows a request, where reading the states is all: each wave takes every fourth block of 32 states by itself,
@@ -431,10 +454,11 @@ __global__ __launch_bounds__(cross_tile(DP, TERMS, false).wq * 64, 2) void cross
 // one is multiplied.  The waves'
 // sums meet at the end.
 template <class T, int TERMS, int DP, bool BIAS, bool VEC>
-__global__ __launch_bounds__(kFewWaves * 64, TERMS > 1 && DP > 64 ? 1 : 2) void cross_few_kernel(CrossParams p) {
+__global__ __launch_bounds__(kFewWaves * 64, DP > 64 && (sizeof(T) == 4 || !VEC) ? 1 : 2) void cross_few_kernel(CrossParams p) {
   typedef typename Element<T>::type E;
   constexpr int kBlocks = DP / 32, kSlices = DP / 16, kUnits = DP / 16;  // a lane's eights of 32 states' values
   constexpr int kRowK = DP + 8, kRowV = DP + 16;
+  constexpr bool kTight = DP > 96;
   constexpr int kMerge = (kFewWaves - 1) * (DP / 2 + 2) * 64 * 2;  // shorts of the sums that meet
   constexpr int kPlane = 32 * kRowV, kRows = kFewWaves * TERMS * kPlane;  // (K's rows fit as well)
   constexpr int kLds = kRows > kMerge ? kRows : kMerge;
@@ -522,6 +546,7 @@ __global__ __launch_bounds__(kFewWaves * 64, TERMS > 1 && DP > 64 ? 1 : 2) void 
 #pragma unroll
       for (int t = 0; t < TERMS; ++t) kt[t] = *reinterpret_cast<const shortx8*>(kp + t * kPlane + 16 * c);
       s = products<E, TERMS>(kt, q[c], s);
+      in_order<kTight>();
     }
     __builtin_amdgcn_wave_barrier();
 #pragma unroll
@@ -568,6 +593,7 @@ __global__ __launch_bounds__(kFewWaves * 64, TERMS > 1 && DP > 64 ? 1 : 2) void 
 #pragma unroll
         for (int t = 0; t < TERMS; ++t) vt[t] = transposed(vp + t * kPlane + 16 * c * kRowV + 32 * d, kRowV);
         o[d] = products<E, TERMS>(vt, pt[c], o[d]);
+        in_order<kTight>();
       }
     __builtin_amdgcn_wave_barrier();
   }

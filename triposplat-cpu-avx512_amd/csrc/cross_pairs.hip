@@ -74,6 +74,7 @@ __global__ __launch_bounds__(cross_tile(DP, 3, false).wq * 64, 2) void cross_pai
                 kKeys = kRuns * KB * 32, kBlocks = DP / 32, kSlices = DP / 16;
   constexpr int kAllUnits = kKeys * DP / 8, kUnits = (kAllUnits + kThreads - 1) / kThreads;  // of 8 values
   constexpr int kRowK = DP + 8, kRowV = DP + 16;  // values from row to row
+  constexpr bool kTight = DP > 96;
   constexpr int kPlaneK = kKeys * kRowK, kPlaneV = kKeys * kRowV, kBuffer = 2 * (kPlaneK + kPlaneV);
   __shared__ __attribute__((aligned(16))) short lds[2 * kBuffer];
   __shared__ __attribute__((aligned(16))) float biases[2][kKeys];
@@ -114,11 +115,9 @@ __global__ __launch_bounds__(cross_tile(DP, 3, false).wq * 64, 2) void cross_pai
 
   // this lane's row
   const int row = wave * 32 + l32;
-  const bool live = row < item.rows;
-  const Row place = row_of(p, item, kv, live ? row : 0);
+  const Row place = row_of(p, item, kv, row < item.rows ? row : 0);
   shortx8 q[kSlices][2];
-  float from_scaled, q_sum = 0.0f;  // 1 / sq, |q'|_1
-  bool bad = false;
+  float from_scaled, q_sum = 0.0f;  // 1 / sq, |q'|_1: no number where q holds an infinity or NaN
   {
     Raw<float> qr[kSlices];
     const float* from = static_cast<const float*>(p.q) + place.token * p.q_token + place.head * p.q_head;
@@ -129,7 +128,6 @@ __global__ __launch_bounds__(cross_tile(DP, 3, false).wq * 64, 2) void cross_pai
       qr[c] = past_end<float, true>(load_eight<float, true>(from, dim, D), dim, D, false);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        bad |= !(fabsf(qr[c].x[i]) < INFINITY);
         qr[c].x[i] *= p.scale * kLog2e;
         q_sum += fabsf(qr[c].x[i]);
       }
@@ -169,7 +167,7 @@ __global__ __launch_bounds__(cross_tile(DP, 3, false).wq * 64, 2) void cross_pai
   const int ek = exponent_to(k_top, 9), ev = exponent_to(v_top, 9);
   const float k_scale = power(ek), v_scale = power(ev);
   const float to_log2 = from_scaled * power(-ek);
-  bad |= !(q_sum * power(-ek) < kPairScores);
+  bool bad = !(q_sum * power(-ek) < kPairScores);
 
   float most = 0.0f, least = INFINITY;  // of the scaled values; of fours of v's that are not all zero
   auto store = [&](int key0, int buf) {
@@ -232,6 +230,7 @@ __global__ __launch_bounds__(cross_tile(DP, 3, false).wq * 64, 2) void cross_pai
         for (int i = 0; i < 2; ++i)
           kt[i] = *reinterpret_cast<const shortx8*>(kp + i * kPlaneK + b * 32 * kRowK + 16 * c);
         s[b] = pair_products(kt, q[c], s[b]);
+        in_order<kTight>();
       }
       if constexpr (BIAS) {
         const float* add = &biases[buf][first + b * 32 + 4 * half];
@@ -281,6 +280,7 @@ __global__ __launch_bounds__(cross_tile(DP, 3, false).wq * 64, 2) void cross_pai
           for (int i = 0; i < 2; ++i)
             vt[i] = transposed(vp + i * kPlaneV + (b * 32 + 16 * c) * kRowV + 32 * d, kRowV);
           o[d] = pair_products(vt, pt, o[d]);
+          in_order<kTight>();
         }
       }
     }
@@ -290,13 +290,14 @@ __global__ __launch_bounds__(cross_tile(DP, 3, false).wq * 64, 2) void cross_pai
   bad |= !(most < kPairTop) || least < kPairLeast;
   bad = __syncthreads_or(bad);
   if (tid == 0) *flag = bad;
-  if (bad || !live) return;
+  const int again = thread_again(), out_row = (again >> 6) * 32 + (again & 31);
+  if (bad || out_row >= item.rows) return;
   const float l = l_run + other_half(l_run), down = power(-ev);
 #pragma unroll
   for (int b = 0; b < kBlocks; ++b)
 #pragma unroll
     for (int r = 0; r < 16; ++r) o[b][r] *= down;
-  finish<float, DP, true>(p, item, kv, row, kWaves * 32, place, half, o, m_run, l);
+  finish<float, DP, true>(p, item, kv, out_row, kWaves * 32, row_of(p, item, kv, out_row), again >> 5 & 1, o, m_run, l);
 }
 
 template <int DP>
