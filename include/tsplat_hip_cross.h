@@ -18,9 +18,10 @@ int tsplat_cross_abi_version(void);
 /* The plan of a batch, made on the host and kept while the lengths stay: which workgroup takes which rows and keys.
  * q_lengths, k_lengths [requests] (host): rows and states of each request, in order, either may be 0.  heads a multiple
  * of kv_heads (query head h reads key head h / (heads / kv_heads)), head_dim 1..128; dtype of q, k, v and out: 0 fp32,
- * 1 bf16, 2 fp16; precision of fp32 products: 0 three bf16 terms of each factor (fp32 accuracy), 2 two terms, 1 one term
- * (0 for 16-bit types).
- * Returns the plan's size in ints, or a negative status (-1, -2: sizes).  With plan (host memory of plan_ints ints) it
+ * 1 bf16, 2 fp16; precision of fp32 products: 0 pairs of fp16 values or three bf16 terms of each factor (fp32
+ * accuracy), 2 two bf16 terms, 1 one (0 for 16-bit types).
+ * Returns the plan's size in ints, or a negative status (-1, -2: sizes; at most 65535 heads, 2^30 - 1 rows times heads of a
+ * group, as many states, and 2^32 - 1 threads of a launch).  With plan (host memory of plan_ints ints) it
  * is written there (-3 when too small).  The first TSPLAT_CROSS_HEADER ints describe it. */
 #define TSPLAT_CROSS_HEADER 16
 int64_t tsplat_cross_plan(const int32_t* q_lengths, const int32_t* k_lengths, int requests, int heads, int kv_heads,
@@ -34,7 +35,8 @@ int64_t tsplat_cross_scratch_bytes(const int32_t* header);
  * q, out: [rows][heads][head_dim], k, v: [states][kv_heads][head_dim] of the plan's type, unit stride within a vector,
  * token and head strides in values (vectors must not overlap, -3); rows and states at least the sums of the plan's lengths; rows past
  * them are not touched.  bias: fp32 [states] or null; a state whose bias is -infinity is not read into any result,
- * whatever it holds.  scale: positive and finite (-2).
+ * whatever it holds; one of +infinity or NaN makes its request's results NaN, and one below -2.3e38 counts as the type's
+ * lowest.  An infinity in q, or in k or v of a state that counts, may come out as a NaN.  scale: positive and finite (-2).
  * header: the plan's first ints (host); plan: all of it on the device, as tsplat_cross_plan wrote it.
  * out must not overlap anything that is read (-3).  scratch: tsplat_cross_scratch_bytes of device memory that no other
  * work uses until the call's kernels are done (-5 when too small, -3 over another argument), 16-byte aligned.  The call

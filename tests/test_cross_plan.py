@@ -101,11 +101,17 @@ def test_plans_cover_everything_once(lib, dtype, precision):
 
 @pytest.mark.parametrize("change", [dict(queries=[-1]), dict(keys=[-1]), dict(heads=0), dict(kv=0), dict(kv=3),
                                     dict(dim=0), dict(dim=129), dict(dtype=3), dict(dtype=-1), dict(precision=3),
-                                    dict(precision=-1), dict(dtype=1, precision=1), dict(heads=(1 << 16) + 2, kv=1),
+                                    dict(precision=-1), dict(dtype=1, precision=1), dict(heads=1 << 16, kv=1),
                                     dict(queries=[2 ** 31 - 1]), dict(keys=[2 ** 31 - 1])])
 def test_plan_refusals(lib, change):
     args = {"queries": [3], "keys": [5], **change}
     assert make(lib, **args) == -2
+
+
+def test_plan_of_more_workgroups_than_a_launch_has(lib):
+    n = 1 << 18
+    assert len(make(lib, [1] * n, [1] * n, heads=16, kv=16)) == INTS + 8 * n
+    assert make(lib, [1] * n, [1] * n, heads=128, kv=128) == -2
 
 
 def test_plan_of_too_little_room_or_no_lengths(lib):

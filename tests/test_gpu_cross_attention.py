@@ -345,3 +345,28 @@ def test_refusals(cuda, hiplib):
                          (([1 << 30, 1 << 30], [1, 1], 4, 64), {}), (([1, 1], [1 << 30, 1 << 30], 4, 64), {})):
         with pytest.raises(ValueError):
             CrossPlan(*args, **{"device": cuda, **kwargs})
+
+
+def test_handles_used_on_another_stream(cuda, hiplib):
+    """A plan and 8-bit rows that are gone before another stream has read them: the allocator keeps their memory."""
+    import torch
+    from tsplat.cross_attention import cross_attention
+    from tsplat.fp8 import fp8_linear, quantize_blocks
+
+    q, k, v, _, g = _inputs(torch, cuda, [300], [2000], 4, 4, 64, "float32", 3)
+    w = torch.randn(256, 256, generator=g, device=cuda)
+    x = torch.randn(200, 256, generator=g, device=cuda)
+    want = cross_attention(q, k, v, _plan(torch, cuda, [300], [2000], 4, 4, 64, "float32"))
+    want8 = fp8_linear(x, quantize_blocks(w))
+    side = torch.cuda.Stream()
+    for _ in range(5):
+        plan, weight = _plan(torch, cuda, [300], [2000], 4, 4, 64, "float32"), quantize_blocks(w)
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            for _ in range(20):
+                got, got8 = cross_attention(q, k, v, plan), fp8_linear(x, weight)
+        del plan, weight
+        trash = [torch.full((n,), 0x7F, dtype=torch.uint8, device=cuda) for n in (512, 1024, 4096, 70000, 66560) for _ in range(4)]
+        torch.cuda.synchronize()
+        assert torch.equal(got, want) and torch.equal(got8, want8)
+        del trash

@@ -14,7 +14,7 @@ static_assert(kPlanHeaderInts == TSPLAT_CROSS_HEADER, "the header's size is part
 
 int64_t make_cross_plan(const int32_t* q_lengths, const int32_t* k_lengths, int requests, int heads, int kv_heads,
                         int head_dim, int dtype, int precision, int compute_units, int32_t* plan, int64_t plan_ints) {
-  if (requests < 0 || requests > (1 << 20) || heads < 1 || heads > (1 << 16) || kv_heads < 1 || heads % kv_heads != 0 ||
+  if (requests < 0 || requests > (1 << 20) || heads < 1 || heads >= (1 << 16) || kv_heads < 1 || heads % kv_heads != 0 ||
       head_dim < 1 || head_dim > 128 || dtype < 0 || dtype > 2 || precision < 0 || precision > 2 ||
       (dtype != 0 && precision != 0))
     return kErrDims;
@@ -65,7 +65,8 @@ int64_t make_cross_plan(const int32_t* q_lengths, const int32_t* k_lengths, int 
   };
   each([&](const CrossItem&) { ++items; }, [&](const CrossJoin&) { ++joins; });
   const int64_t need = kPlanHeaderInts + items * kCrossItem + joins * kCrossJoin;
-  if (items * kv_heads > INT32_MAX || need > INT32_MAX) return kErrDims;
+  const int64_t threads = (few ? kFewWaves : tile.wq) * 64;
+  if (items * kv_heads * threads > UINT32_MAX || need > INT32_MAX) return kErrDims;  // (a launch's threads in 32 bits)
   if (!plan) return need;
   if (plan_ints < need || room_items < items) return kErrRange;
   const int32_t header[kPlanHeaderInts] = {kPlanMagicValue, (int32_t)need, (int32_t)items, (int32_t)joins,

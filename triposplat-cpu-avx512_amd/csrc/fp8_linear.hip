@@ -470,7 +470,7 @@ int launch_tiles(const Fp8LinearParams& p, const uint8_t* xc, const uint8_t* xe,
                  hipStream_t stream) {
   const int tiles_n = (p.N + BN - 1) / BN;
   const int64_t tiles = (int64_t)((p.M + BM - 1) / BM) * tiles_n;
-  if (tiles > INT32_MAX) return kErrDims;
+  if (tiles * WM * WN * 64 > UINT32_MAX) return kErrDims;  // (a launch's threads in 32 bits)
   auto go = [&](auto kernel) {
     kernel<<<(int)tiles, WM * WN * 64, 0, stream>>>(xc, xe, p.w_codes, p.w_exponents, f, (int)fp8_code_stride(p.K),
                                                     (int)fp8_exponent_stride(p.K), tiles_n);

@@ -59,7 +59,8 @@ __global__ __launch_bounds__(kThreads) void fp8_quantize_kernel(Fp8QuantizeParam
 template <class T>
 int launch(const Fp8QuantizeParams& p, hipStream_t stream) {
   const int code_stride = (int)fp8_code_stride(p.K), exp_stride = (int)fp8_exponent_stride(p.K);
-  const int rows_per = std::max(1, kGroups * kAhead / exp_stride);
+  // (a launch's threads are counted in 32 bits: more rows to a workgroup for very many)
+  const int rows_per = std::max({1, kGroups * kAhead / exp_stride, (p.rows >> 23) + 1});
   const dim3 grid((p.rows + rows_per - 1) / rows_per);
   const bool vec = reinterpret_cast<uintptr_t>(p.x) % (4 * sizeof(T)) == 0 && (p.rows == 1 || p.x_stride % 4 == 0);
   if (vec)

@@ -248,6 +248,18 @@ def enqueue(lib, fn_name, index, *args) -> None:
         check_status(status, fn_name)
 
 
+def made_on(index: int) -> int:
+    """The stream that memory made now belongs to, for used_here."""
+    return _raw_stream(index)
+
+
+def used_here(torch, tensor, index, stream) -> None:
+    """For memory that a handle keeps, made on `stream`: a use on another one is told to torch's allocator, which else
+    could give the memory away while that stream still reads it."""
+    if _raw_stream(index) != stream:
+        tensor.record_stream(torch.cuda.current_stream(index))
+
+
 def no_gradients(torch, *tensors) -> None:
     """These operators have no backward and no forward mode: a tensor that expects a gradient or carries a tangent is
     refused, not cut off in silence."""

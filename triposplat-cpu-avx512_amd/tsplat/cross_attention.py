@@ -9,7 +9,7 @@ from __future__ import annotations
 import ctypes
 import math
 
-from ._lib import check_status, enqueue, load_library, no_gradients
+from ._lib import check_status, enqueue, load_library, made_on, no_gradients, used_here
 from .fp8 import type_ids
 from .nf24 import precision_id
 
@@ -32,7 +32,7 @@ class CrossPlan:
     dtype: the type of q, k, v and the result, torch.float32 (default), bfloat16 or float16.  precision: of fp32
     products, "fp32" or the opt-in "bf16x3" / "bf16" (tsplat.nf24.PRECISIONS).  Making one copies it to the GPU and
     waits for that, so it is not made while a graph is captured; calls only read it, and any number of them on any
-    streams may share it."""
+    streams may share it.  A captured graph reads it too: keep the plan as long as the graph."""
 
     def __init__(self, q_lengths, k_lengths, heads, head_dim, *, kv_heads=None, dtype=None, precision="fp32",
                  device=None, library=None):
@@ -47,7 +47,7 @@ class CrossPlan:
         self.dtype = torch.float32 if dtype is None else dtype
         if self.dtype not in type_ids(torch):
             raise ValueError("dtype is torch.float32, bfloat16 or float16")
-        if not 1 <= self.kv_heads <= self.heads <= 1 << 16 or self.heads % self.kv_heads:
+        if not 1 <= self.kv_heads <= self.heads < 1 << 16 or self.heads % self.kv_heads:
             raise ValueError(f"{self.heads} heads are not a multiple of {self.kv_heads} key heads, or too many")
         if not 1 <= self.head_dim <= 128:
             raise ValueError(f"head_dim is 1..128, not {self.head_dim}")
@@ -68,7 +68,7 @@ class CrossPlan:
                 raise ValueError("too many requests, rows or states for one plan")
             plan = torch.empty(ints, dtype=torch.int32)
             check_status(min(0, self.library.tsplat_cross_plan(*sizes, plan.data_ptr(), ints)), "tsplat_cross_plan")
-            self._plan = plan.to(torch.device("cuda", index))
+            self._plan, self._stream = plan.to(torch.device("cuda", index)), made_on(index)
         self.device, self.index = self._plan.device, index
         self._header = (ctypes.c_int32 * HEADER_INTS)(*plan[:HEADER_INTS].tolist())
         self.rows, self.states = self._header[_ROWS], self._header[_STATES]
@@ -98,7 +98,8 @@ def cross_attention(q, k, v, plan, *, key_bias=None, scale=None, out=None):
     q [rows, heads, head_dim], k, v [states, kv_heads, head_dim]: of the plan's type, unit stride within a vector, the
     other strides free (k and v may be views of one fused projection); at least as many rows and states as the plan's
     lengths add up to.  key_bias [states] fp32: a state whose bias is -infinity is not read into any result, whatever it
-    holds.  scale: head_dim ** -0.5 by default.  out: None for a new tensor like q, its rows behind the last request
+    holds (one of +infinity or NaN makes its request's results NaN, and one below -2.3e38 counts as the type's lowest).  An
+    infinity in q, or in k or v of a state that counts, may come out as a NaN.  scale: head_dim ** -0.5 by default.  out: None for a new tensor like q, its rows behind the last request
     zero, or a tensor that overlaps nothing that is read, whose rows behind the last request stay as they are.
     Sums, maxima and exponents are fp32; fp32 products as the plan's precision says.  Runs on torch's current stream;
     capturable into a HIP graph.  No gradients."""
@@ -127,6 +128,7 @@ def cross_attention(q, k, v, plan, *, key_bias=None, scale=None, out=None):
     out_ptr, out_token, out_head = _vectors(torch, "out", out, plan, plan.heads, plan.rows)
     if plan.rows == 0:
         return out
+    used_here(torch, plan._plan, plan.index, plan._stream)
     need = plan._scratch_bytes
     scratch = torch.empty(need, dtype=torch.uint8, device=plan.device) if need else None
     enqueue(plan.library, "tsplat_cross_attention_async", plan.index, q_ptr, q_token, q_head, k_ptr, k_token, k_head,

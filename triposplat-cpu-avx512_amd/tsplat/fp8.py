@@ -11,7 +11,7 @@ signs is off by about 4 % of its result's norm, which the caller opts into
 """
 from __future__ import annotations
 
-from ._lib import enqueue, load_library, matrix_rows, no_gradients
+from ._lib import enqueue, load_library, made_on, matrix_rows, no_gradients, used_here
 
 BLOCK = 128
 # the library's limits
@@ -32,9 +32,9 @@ class Fp8Rows:
     """Rows of K values in 8 bits: values [rows, K] = codes * 2^(exponents - 127), an exponent for each 128 of a row.
     Made by quantize_blocks."""
 
-    def __init__(self, buffer, at, rows, features):
+    def __init__(self, buffer, at, rows, features, stream):
         # uint8: the codes' rows, K rounded up to 128 bytes each, and the exponents', blocks rounded up to 4, at `at`
-        self._buffer, self._at = buffer, at
+        self._buffer, self._at, self._stream = buffer, at, stream
         self.rows, self.features = rows, features
         self.blocks = -(-features // BLOCK)
         self.device, self.index = buffer.device, buffer.get_device()
@@ -61,7 +61,7 @@ class Fp8Rows:
         if start < 0 or count < 0 or start + count > self.rows:
             raise ValueError(f"rows {start}..{start + count} of {self.rows}")
         at = self._at[0] + start * self.blocks * BLOCK, self._at[1] + start * _fours(self.blocks)
-        return Fp8Rows(self._buffer, at, count, self.features)
+        return Fp8Rows(self._buffer, at, count, self.features, self._stream)
 
     def dequantize(self):
         """The values that the codes stand for, fp32 [rows, K] (exact)."""
@@ -97,7 +97,8 @@ def quantize_blocks(x, *, library=None):
     blocks = -(-K // BLOCK)
     codes = M * blocks * BLOCK
     # (one piece of memory for both: an allocation takes the host longer than the smallest rows take the GPU)
-    rows = Fp8Rows(torch.empty(codes + M * _fours(blocks), dtype=torch.uint8, device=x.device), (0, codes), M, K)
+    rows = Fp8Rows(torch.empty(codes + M * _fours(blocks), dtype=torch.uint8, device=x.device), (0, codes), M, K,
+                   made_on(x.get_device()))
     if M:
         enqueue(load_library(library), "tsplat_fp8_quantize_async", rows.index, x.data_ptr(), types[kind], stride, M, K,
                 rows.codes_ptr, rows.exponents_ptr)
@@ -180,6 +181,8 @@ def fp8_linear(x, weight, bias=None, *, activation=None, gate=None, residual=Non
         raise ValueError("x, weight and out must be on one GPU")
     if M == 0:
         return out
+    for rows in (x, weight) if ready else (weight,):
+        used_here(torch, rows._buffer, at, rows._stream)
     lib = load_library(library)
     need = lib.tsplat_fp8_linear_scratch_bytes(M, K, N, not ready)
     scratch = torch.empty(need, dtype=torch.uint8, device=weight.device) if need else None
