@@ -3,8 +3,15 @@
 // Both operands are e4m3 codes with a power-of-two scale for each 128 of a row: products of codes are exact, the scales
 // are taken by the instructions that widen or multiply the codes, and the sums stay in fp32 registers.  The operands'
 // lane layout along K does not matter as long as both agree (a sum has no order of its own).
-// The weights are the first operand: a lane then holds four neighbouring columns of one row of the result, which it
-// loads and stores as one piece.
+// The weights are the first operand: a lane then holds four neighbouring columns of one row of the result.
+//
+// What bounds it, and measured (with the rows' conversion, which is HBM's time: 17 and 58 us of these):
+// 16384x1024x4096 in fp32 with GELU 177 us, 16384x4096x1024 onto a gated residual 187: products through bf16 at 1.18
+// PFLOP/s, what the matrix cores hold at their clock under that load (a library's 8192^3 in bf16: 1.12), and the result's
+// bytes, which the products hide in part (the former 149 us, 40 of them its 268 MB).  Without the conversions to bf16 6
+// us less, without the copies into LDS 9.  8-bit products (results of 16 bits): 16384x4096x4096 295 us, 1.86 PFLOP/s
+// (a library's: 2.64); 4101x1024x2048 27 us, of which 6 convert the rows and 10 are a launch and its chain of loads.
+// One row of 1024x1024 4.4 us (the call 11: the host), 64 rows of 1024x6144 13.
 
 #include <algorithm>
 
@@ -157,6 +164,8 @@ __device__ __forceinline__ bf16x8 widen8(int lo, int hi, float scale) {
 // A stage is multiplied in two steps, of 32 codes each (EXACT) or of half of the weights' rows.  The operands of each step
 // are read into registers while the one before is multiplied (where 128 sums leave room for that), so a stage's buffer is free, and the copies of the stage
 // that comes STAGES later may begin, before its last step is multiplied.
+// 128x256 tiles, two workgroups a CU; 128x128 where there are fewer than two of the wide ones for each CU (4101x1024x2048:
+// 23 against 25 us; 16384x1024x4096 in 16 bits the wide ones, half the reads of x).
 constexpr int kStage = 64;
 
 template <int BM, int BN, int WM, int WN, int STAGES, class TO, bool VEC>
@@ -347,7 +356,9 @@ __global__ __launch_bounds__(WM* WN * 64, BM * BN > 128 * 128 ? 2 : 3) void fp8_
 
 // ---- few rows (up to 64): bound by reading the weights once.  A workgroup takes 16 NB columns and all rows, its eight
 // waves every eighth block of K each, straight from memory to registers; their sums meet in LDS.  x is brought to 8
-// bits on the way (a lane holds 32 values of a row, four lanes its block of 128): one launch, no scratch.
+// bits on the way (a lane holds 32 values of a row, four lanes its block of 128): one launch, no scratch.  Two column
+// tiles from 17 rows on, which halves the workgroups that convert x (64 rows of 1024x6144 23 -> 13 us); one for a few
+// rows, whose time is a chain of loads (4.4 us).  Products through bf16: their rate does not matter here.
 constexpr int kFewWaves = 8;
 
 template <class T, bool VEC, int MB, int NB, class TO, bool VECO>
