@@ -264,6 +264,11 @@ def test_refusals(cuda, hiplib):
                     ((z, c, t), "plan")):
         with pytest.raises(ValueError):
             model.velocity(*args, cond_plan=p)
+    for precision in ("fp32", "fp8"):  # one condition for two entries
+        model.set_precision(precision)
+        with pytest.raises(ValueError):
+            model.velocity(z, c[None, :20], t)
+    model.set_precision("fp32")
     for include in (("blocks", "attention"), ("attention",)):
         with pytest.raises(ValueError):
             model.set_precision("fp8", include=include)

@@ -304,8 +304,8 @@ class FlowModel:
         # cross attention to the condition tokens (no RoPE)
         h = bo.layer_norm(x, cfg.ln_eps, blk.xnorm_w, blk.xnorm_b)
         xq = bo.head_rmsnorm(lin["xq"](h.view(B * L, C)), blk.xq_gamma, B, L, H)
-        kv = lin["xkv"](cond if isinstance(cond, Fp8Rows) else cond.reshape(-1, C))  # [B*Lc, 2C] = [k | v]
-        Lc = kv.shape[0] // B
+        Lc = cond.rows // B if isinstance(cond, Fp8Rows) else int(cond.shape[1])
+        kv = lin["xkv"](cond if isinstance(cond, Fp8Rows) else cond.reshape(B * Lc, C))  # [B*Lc, 2C] = [k | v]
         xk = bo.head_rmsnorm(kv, blk.xk_gamma, B, Lc, H, token_stride=2 * C)
         xv = bo.head_rmsnorm(kv[:, C:], None, B, Lc, H, token_stride=2 * C, normalize=False)
         a = native_sdpa_f32_ex(xq, xk, xv, out_layout="blhd", precision=self.attention_precision)
@@ -325,12 +325,12 @@ class FlowModel:
         return CrossPlan([tokens] * len(lengths), lengths, self.cfg.heads, self.cfg.head_dim,
                          precision=self.attention_precision, device=self.device)
 
-    def condition_rows(self, cond2):
-        """cond2 [rows, C] as the blocks' condition Linears read it: in 8 bits, once for all blocks, where all of
-        them multiply in precision "fp8"."""
-        if cond2.shape[0] and self.blocks and all(blk.lin["xkv"].precision == "fp8" for blk in self.blocks):
-            return quantize_blocks(cond2)
-        return cond2
+    def condition_rows(self, cond):
+        """cond [..., C] as the blocks' condition Linears read it: its rows in 8 bits, once for all blocks, where all
+        of them multiply in precision "fp8", else itself."""
+        if cond.numel() and self.blocks and all(blk.lin["xkv"].precision == "fp8" for blk in self.blocks):
+            return quantize_blocks(cond.reshape(-1, cond.shape[-1]))
+        return cond
 
     def velocity(self, z, cond, t, observe=None, *, adapters=None, slots=None, positions=None, rope=None,
                  cond_plan=None):
@@ -353,8 +353,9 @@ class FlowModel:
         B, L, C = (int(s) for s in z.shape)
         t_emb, t_mod = self.timestep(t)
         x = self.input_layer(z.reshape(B * L, C)).view(B, L, C)
-        rows = self.condition_rows(cond.reshape(-1, C))
-        cond = rows if isinstance(rows, Fp8Rows) else cond
+        if cond.shape[0] != B:
+            raise ValueError(f"cond must be [{B}, rows, {C}], its shape is {list(cond.shape)}")
+        cond = self.condition_rows(cond)
         for i, blk in enumerate(self.blocks):
             if observe is not None:
                 observe(i, x)
