@@ -32,15 +32,22 @@ int64_t make_cross_plan(const int32_t* q_lengths, const int32_t* k_lengths, int 
   const bool few = longest <= 32;
   const CrossTile tile = cross_tile(padded, terms, few);
   const int tile_rows = tile.wq * 32, tile_keys = tile.kb * 32;
-  // Tiles of keys over all workgroups: an even share of them for each workgroup that runs at once is the length of a part.
-  // Few rows: a part's sums are small, so four times as many parts, two tiles at least.  Many: four tiles at least (fewer
-  // and the parts' sums cost more than they save).
+  // Tiles of keys over all workgroups: an even share of them for each workgroup that runs at once is the length of a part
+  // (four times as many parts for few rows, whose sums are small).  Where that is short, the length that makes one part's
+  // tiles, in a chain, and the join of a request's parts together shortest: their number halved, its root.  (Two single
+  // tokens over 2049 and 4101 states in fp32: parts of 1, 2, 3, 4 tiles take 34, 27, 26, 23 us; one over 500: 9.9, 11.5,
+  // 11.5, 14; 64 over 4096: 2, 3, 4, 6 take 38, 37, 26, 26; three of 200 over 700 in 16 bits: 2, 3, 4 take 14.1, 12.4, 12.5.)
   const int64_t slots = (int64_t)compute_units * 2;
-  int64_t work = 0;
-  for (int i = 0; i < requests; ++i)
-    work += ((int64_t)q_lengths[i] * group + tile_rows - 1) / tile_rows * ((k_lengths[i] + tile_keys - 1) / tile_keys);
+  int64_t work = 0, most = 0;
+  for (int i = 0; i < requests; ++i) {
+    const int64_t tiles = (k_lengths[i] + (int64_t)tile_keys - 1) / tile_keys;
+    work += ((int64_t)q_lengths[i] * group + tile_rows - 1) / tile_rows * tiles;
+    if (q_lengths[i] > 0) most = std::max(most, tiles);
+  }
   const int64_t at_once = few ? 4 * slots : slots;
-  const int64_t share = std::max<int64_t>(few ? 2 : 4, (work * kv_heads + at_once - 1) / at_once);
+  int64_t share = few ? 1 : terms > 1 ? 2 : 3;
+  while ((share + 1) * (share + 1) * 2 <= most) ++share;
+  share = std::max<int64_t>(share, (work * kv_heads + at_once - 1) / at_once);
 
   int64_t items = 0, joins = 0, parts = 0;
   const int64_t room_items = plan ? (plan_ints - kPlanHeaderInts) / kCrossItem : 0;
