@@ -18,7 +18,8 @@
 // in bf16 92 us, 0.44 PFLOP/s: 784 workgroups of 22 and 32 tiles on 768 places (more parts than the plan makes cost more
 // than they even out: 123).  fp32 values in three bf16 terms (unaligned, or flagged by cross_pairs.hip) 1340 us for the
 // former, 1.23 PFLOP/s of bf16 products.  Few rows: HBM, 64 single tokens over 1.09 GB of bf16 states 221 us, 4.9 TB/s
-// (a copy: 5.0); two single tokens over 50 MB of fp32 ones 21, of which about 5 join the parts and 6 are a launch and first loads.
+// (a copy: 5.0); two single tokens over 50 MB of fp32 ones 21, of which about 5 join the parts and 6 are a
+// launch and first loads.
 //
 // States go from memory through registers to LDS, a tile ahead of the products; states that the bias masks, or past the
 // request's last, are put there as zeros, so what memory holds in their place does not matter.  Rows of LDS are padded so

@@ -219,76 +219,76 @@ __global__ __launch_bounds__(cross_tile(DP, 3, false).wq * 64, 2) void cross_pai
     if (!wave_live) continue;
 #pragma unroll 1
     for (int first = 0; first < kKeys; first += KB * 32) {
-    if (t * kKeys + first >= item.keys) break;
-    const short* kp = lds + buf * kBuffer + (first + l32) * kRowK + 8 * half;
-    const short* vp = lds + buf * kBuffer + 2 * kPlaneK + (first + 4 * half + (lane & 15) / 4) * kRowV +
-                      (lane >> 4 & 1) * 16 + (lane & 3) * 4;
-    floatx16 s[KB];
+      if (t * kKeys + first >= item.keys) break;
+      const short* kp = lds + buf * kBuffer + (first + l32) * kRowK + 8 * half;
+      const short* vp = lds + buf * kBuffer + 2 * kPlaneK + (first + 4 * half + (lane & 15) / 4) * kRowV +
+                        (lane >> 4 & 1) * 16 + (lane & 3) * 4;
+      floatx16 s[KB];
 #pragma unroll
-    for (int b = 0; b < KB; ++b) {
+      for (int b = 0; b < KB; ++b) {
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[b][r] = 0.0f;
+        for (int r = 0; r < 16; ++r) s[b][r] = 0.0f;
 #pragma unroll
-      for (int c = 0; c < kSlices; ++c) {
-        shortx8 kt[2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-          kt[i] = *reinterpret_cast<const shortx8*>(kp + i * kPlaneK + b * 32 * kRowK + 16 * c);
-        s[b] = pair_products(kt, q[c], s[b]);
-        in_order<kTight>();
-      }
-      if constexpr (BIAS) {
-        const float* add = &biases[buf][first + b * 32 + 4 * half];
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s[b][r] = fmaf(s[b][r], to_log2, add[r / 4 * 8 + r % 4]);
-      } else {
-        const int left = item.keys - (t * kKeys + first + b * 32) - 4 * half;  // states of this block from this lane's first
-        if (left < 32) {
-#pragma unroll
-          for (int r = 0; r < 16; ++r)
-            if (r / 4 * 8 + r % 4 >= left) s[b][r] = -INFINITY;
-        }
-      }
-    }
-    float top = s[0][0];
-#pragma unroll
-    for (int b = 0; b < KB; ++b)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) top = fmaxf(top, s[b][r]);
-    top = fmaxf(top, other_half(top));
-    const float ref = BIAS ? top - kPairBase : fmaf(top, to_log2, -kPairBase);
-    if (__any(ref > m_run + kPairSlack)) {
-      const float m_new = fmaxf(m_run, ref);
-      const float keep = m_run == m_new ? 1.0f : __builtin_amdgcn_exp2f(m_run - m_new);
-      l_run *= keep;
-#pragma unroll
-      for (int b = 0; b < kBlocks; ++b)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) o[b][r] *= keep;
-      m_run = m_new;
-    }
-    const float m = m_run == -INFINITY ? 0.0f : m_run;
-#pragma unroll
-    for (int b = 0; b < KB; ++b) {
-      l_run += weights<BIAS>(s[b], to_log2, m);
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        float x[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = s[b][8 * c + i];
-        shortx8 pt[2];
-        pair8(x, pt);
-#pragma unroll
-        for (int d = 0; d < kBlocks; ++d) {
-          shortx8 vt[2];
+        for (int c = 0; c < kSlices; ++c) {
+          shortx8 kt[2];
 #pragma unroll
           for (int i = 0; i < 2; ++i)
-            vt[i] = transposed(vp + i * kPlaneV + (b * 32 + 16 * c) * kRowV + 32 * d, kRowV);
-          o[d] = pair_products(vt, pt, o[d]);
+            kt[i] = *reinterpret_cast<const shortx8*>(kp + i * kPlaneK + b * 32 * kRowK + 16 * c);
+          s[b] = pair_products(kt, q[c], s[b]);
           in_order<kTight>();
         }
+        if constexpr (BIAS) {
+          const float* add = &biases[buf][first + b * 32 + 4 * half];
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[b][r] = fmaf(s[b][r], to_log2, add[r / 4 * 8 + r % 4]);
+        } else {
+          const int left = item.keys - (t * kKeys + first + b * 32) - 4 * half;  // states of this block from this lane's first
+          if (left < 32) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+              if (r / 4 * 8 + r % 4 >= left) s[b][r] = -INFINITY;
+          }
+        }
       }
-    }
+      float top = s[0][0];
+#pragma unroll
+      for (int b = 0; b < KB; ++b)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) top = fmaxf(top, s[b][r]);
+      top = fmaxf(top, other_half(top));
+      const float ref = BIAS ? top - kPairBase : fmaf(top, to_log2, -kPairBase);
+      if (__any(ref > m_run + kPairSlack)) {
+        const float m_new = fmaxf(m_run, ref);
+        const float keep = m_run == m_new ? 1.0f : __builtin_amdgcn_exp2f(m_run - m_new);
+        l_run *= keep;
+#pragma unroll
+        for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) o[b][r] *= keep;
+        m_run = m_new;
+      }
+      const float m = m_run == -INFINITY ? 0.0f : m_run;
+#pragma unroll
+      for (int b = 0; b < KB; ++b) {
+        l_run += weights<BIAS>(s[b], to_log2, m);
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          float x[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[i] = s[b][8 * c + i];
+          shortx8 pt[2];
+          pair8(x, pt);
+#pragma unroll
+          for (int d = 0; d < kBlocks; ++d) {
+            shortx8 vt[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+              vt[i] = transposed(vp + i * kPlaneV + (b * 32 + 16 * c) * kRowV + 32 * d, kRowV);
+            o[d] = pair_products(vt, pt, o[d]);
+            in_order<kTight>();
+          }
+        }
+      }
     }
   }
 
