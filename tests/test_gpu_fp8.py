@@ -239,3 +239,18 @@ def test_refusals(cuda, hiplib):
     with pytest.raises(RuntimeError, match="-3"):
         fp8_linear(x, weight, out=x[:, :40])
     assert quantize_blocks(x[:0]).codes.shape == (0, 130) and fp8_linear(x[:0], weight).shape == (0, 40)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M,K,N", [(4200, 136, 4100), (16500, 300, 1030), (1100, 520, 15000), (8192, 1024, 2048)])
+def test_linear_of_many_tiles(cuda, hiplib, M, K, N, dtype):
+    """More than two of the wide tiles to a CU: ragged bands of rows and runs of columns, each written once."""
+    import torch
+    from tsplat.fp8 import fp8_linear, quantize_blocks
+
+    print(f"many tiles M={M} K={K} N={N} {dtype}", flush=True)
+    x, w, bias, residual, g = _linear_case(torch, cuda, M, K, N, dtype, 21)
+    weight, gate = quantize_blocks(w), torch.randn(2, N, generator=g, device=cuda)
+    for what, args in (("gelu", dict(bias=bias, activation="gelu")), ("gated", dict(bias=bias, gate=gate, residual=residual))):
+        want, bound = linear(torch, x, w, args.get("bias"), args.get("activation"), args.get("gate"), args.get("residual"), dtype)
+        assert_within(torch, fp8_linear(x, weight, **args).double(), want, bound, what)
