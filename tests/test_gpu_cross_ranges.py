@@ -1,0 +1,70 @@
+"""cross_attention at the ends of its values' range, and where neighbouring features are of unlike sizes."""
+from __future__ import annotations
+
+import math
+
+import pytest
+
+from _cross_ranges import FEATURE, KINDS, feature_off, ranges, small_features
+from _request_cases import assert_within
+
+pytestmark = pytest.mark.gpu
+
+INF = math.inf
+
+
+def _inputs(torch, cuda, rows, n, heads, D, dtype, seed, aligned=True):
+    """q, k, v; unaligned: the same values in rows of an odd pitch, which take another kernel."""
+    g = torch.Generator(device=cuda).manual_seed(seed)
+    made = [torch.randn(m, heads, D, generator=g, device=cuda).to(getattr(torch, dtype)) for m in (rows, n, n)]
+    return made if aligned else [_unaligned(t) for t in made]
+
+
+def _unaligned(t):
+    wide = t.new_zeros(t.shape[0], t.shape[1], t.shape[2] + 1)
+    wide[..., 1:] = t
+    return wide[..., 1:]
+
+
+def _plan(torch, cuda, rows, n, heads, D, dtype, precision="fp32"):
+    from tsplat.cross_attention import CrossPlan
+
+    return CrossPlan([rows], [n], heads, D, dtype=getattr(torch, dtype), precision=precision, device=cuda)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("D", [64, 96, 128])
+def test_features_of_unlike_sizes(cuda, hiplib, kind, D):
+    """A feature far below its neighbours keeps fp32's accuracy, whether or not its neighbours are small as well."""
+    import torch
+    from tsplat.cross_attention import cross_attention
+
+    for rows, n, aligned in ((300, 500, True), (300, 500, False), (3, 500, True), (70, 4000, True)):
+        q, k, v = _inputs(torch, cuda, rows, n, 2, D, "float32", 4)
+        v = small_features(kind, v)
+        if not aligned:
+            q, k, v = (_unaligned(t) for t in (q, k, v))
+        bias = torch.where(torch.arange(n, device=cuda) % 5 == 0, -INF, 0.0)
+        plan = _plan(torch, cuda, rows, n, 2, D, "float32")
+        for b in (None, bias):
+            want, bound = ranges(torch, q, k, v, [rows], [n], b)
+            got = cross_attention(q, k, v, plan, key_bias=b)
+            assert_within(torch, got.double(), want, bound, kind)
+            assert feature_off(torch, got, want) <= FEATURE
+
+
+def test_values_of_unlike_sizes_by_feature(cuda, hiplib):
+    """States of sizes from 1e-12 to 1e12, and a feature that is zero among the first states."""
+    import torch
+    from tsplat.cross_attention import cross_attention
+
+    q, k, v = _inputs(torch, cuda, 300, 500, 2, 64, "float32", 5)
+    plan = _plan(torch, cuda, 300, 500, 2, 64, "float32")
+    steps = v * torch.logspace(-12, 12, 500, device=cuda)[:, None, None]
+    late = v.clone()
+    late[:200, :, 11], late[200:, :, 11] = 0.0, late[200:, :, 11] * 1e-9
+    for values in (steps, late):
+        want, bound = ranges(torch, q, k, values, [300], [500])
+        got = cross_attention(q, k, values, plan)
+        assert_within(torch, got.double(), want, bound, "by feature")
+        assert feature_off(torch, got, want) <= FEATURE

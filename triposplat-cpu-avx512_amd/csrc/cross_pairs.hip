@@ -9,15 +9,17 @@
 //
 // What the pairs do not serve, and the workgroup finds while it reads the states: a magnitude of 2^15 and more of the
 // scaled values (an infinity too); scores that may lose 2^-22 log2 units to the 2^-25 of k's values (|q'|_1 / sk of 8 and
-// more); four neighbouring values of v, not all zero, below 2^-4 (they would keep less
-// than 2^-21 of themselves); an infinity or NaN in q.  It then leaves its result to the kernel of bf16 terms, which is
-// launched behind this one and does what is flagged: any input has fp32's accuracy, an unusual one at that kernel's time.
+// more); four neighbouring values of v, not all zero, below 2^-4, or a feature of v, not all zero, that stays below 2^-4 in
+// all of the states; an infinity or NaN in q.  It then leaves its result to the kernel of bf16 terms, which is launched
+// behind this one and does what is flagged, at that kernel's time.  So a value of v is held to 2^-23 of it or to 2^-21 of
+// the larger of its feature's largest, over the workgroup's states, and its neighbours'.  (Each value by itself cannot be
+// asked for 2^-4: one in 2000 of a normal distribution is below.)
 //
 // p = 2^(x - m) for a reference m that is 11 below the row's largest x, or up to 15 (few tiles rescale): below 2^15, and a
 // weight 2^-36 of the largest is still held.  (The exponential's argument is rounded by 2^-21 at most there, 3e-7 of a
 // weight, which its sum has as well; a factor after the exponential instead takes 16 more instructions a block.)
 //
-// 2 x 16384 x 2048, 16 heads of 64: 858 us (bf16 terms 1340; the flags' launch 5), 0.32 PFLOP/s of the operator's
+// 2 x 16384 x 2048, 16 heads of 64: 880 us (the check by features 20 of them; bf16 terms 1340; the flags' launch 5), 0.32 PFLOP/s of the operator's
 // operations, 0.96 of fp16 products.  What bounds it: products (46 % of the SIMDs' cycles) and vector instructions (50 %)
 // that hardly overlap, as a SIMD's two waves do the same at the same time: waves of unlike priority, and a block's products
 // between the exponents of the one before, did not change that (870 and spills).
@@ -31,6 +33,7 @@ namespace cross {
 
 typedef _Float16 halfx2 __attribute__((ext_vector_type(2)));
 typedef float floatx2 __attribute__((ext_vector_type(2)));
+typedef unsigned short ushortx2 __attribute__((ext_vector_type(2)));
 
 constexpr float kPairSlack = 4.0f, kPairBase = 11.0f;
 constexpr float kPairTop = 0x1p15f, kPairLeast = 0x1p-4f, kPairScores = 8.0f;
@@ -84,6 +87,7 @@ __global__ __launch_bounds__(cross_tile(DP, 3, false).wq * 64, 2) void cross_pai
   __shared__ __attribute__((aligned(16))) short lds[2 * kBuffer];
   __shared__ __attribute__((aligned(16))) float biases[2][kKeys];
   __shared__ float largest[2][kWaves];
+  __shared__ uint32_t features[DP];  // the upper bits of v's largest magnitudes
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l32 = lane & 31, half = lane >> 5;
@@ -166,6 +170,7 @@ __global__ __launch_bounds__(cross_tile(DP, 3, false).wq * 64, 2) void cross_pai
     }
   }
   if (lane == 0) largest[0][wave] = k_top, largest[1][wave] = v_top;
+  if (tid < DP) features[tid] = 0;
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < kWaves; ++w) k_top = fmaxf(k_top, largest[0][w]), v_top = fmaxf(v_top, largest[1][w]);
@@ -175,6 +180,9 @@ __global__ __launch_bounds__(cross_tile(DP, 3, false).wq * 64, 2) void cross_pai
   bool bad = !(q_sum * power(-ek) < kPairScores);
 
   float most = 0.0f, least = INFINITY;  // of the scaled values; of fours of v's that are not all zero
+  // The upper 16 bits of the largest magnitudes of the eight features that this thread brings, the same in all of its units.
+  static_assert(kUnits == 1 || kThreads % (DP / 8) == 0, "a thread's features");
+  ushortx2 feature[4] = {};
   auto store = [&](int key0, int buf) {
     short* kp = lds + buf * kBuffer;
     short* vp = kp + 2 * kPlaneK;
@@ -183,6 +191,12 @@ __global__ __launch_bounds__(cross_tile(DP, 3, false).wq * 64, 2) void cross_pai
       const int unit = tid + u * kThreads, key = unit / (DP / 8), dim = unit % (DP / 8) * 8;
       if (kAllUnits % kThreads && unit >= kAllUnits) break;
       clean(u, key0);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t two = __builtin_amdgcn_perm(__float_as_uint(vr[u].x[2 * i + 1]), __float_as_uint(vr[u].x[2 * i]),
+                                                   0x07060302u) & 0x7fff7fffu;
+        feature[i] = __builtin_elementwise_max(feature[i], __builtin_bit_cast(ushortx2, two));
+      }
 #pragma unroll
       for (int i = 0; i < 8; ++i) kr[u].x[i] *= k_scale, vr[u].x[i] *= v_scale;
       most = fmaxf(most, fmaxf(largest4(kr[u].x), largest4(kr[u].x + 4)));
@@ -292,6 +306,10 @@ __global__ __launch_bounds__(cross_tile(DP, 3, false).wq * 64, 2) void cross_pai
     }
   }
 
+#pragma unroll
+  for (int i = 0; i < 8; ++i) atomicMax(&features[tid % (DP / 8) * 8 + i], (uint32_t)feature[i / 2][i % 2]);
+  __syncthreads();
+  if (tid < DP && features[tid] != 0) bad |= __uint_as_float(features[tid] << 16) * v_scale < kPairLeast;
   bad |= !(most < kPairTop) || least < kPairLeast;
   bad = __syncthreads_or(bad);
   if (tid == 0) *flag = bad;
