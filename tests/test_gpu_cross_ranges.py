@@ -32,6 +32,23 @@ def _plan(torch, cuda, rows, n, heads, D, dtype, precision="fp32"):
     return CrossPlan([rows], [n], heads, D, dtype=getattr(torch, dtype), precision=precision, device=cuda)
 
 
+@pytest.mark.parametrize("D", [64, 96, 128])
+@pytest.mark.parametrize("q_size,k_size", [(1e-19, 1e-19), (1e-20, 1e-20), (1e-38, 1e-5), (1e-30, 1e-37), (1e-38, 1.0)])
+def test_scores_next_to_zero(cuda, hiplib, q_size, k_size, D):
+    """Scores that fp32 cannot tell from zero: the mean of the values, with a last block of states that is not full."""
+    import torch
+    from tsplat.cross_attention import cross_attention
+
+    q, k, v = _inputs(torch, cuda, 300, 500, 2, D, "float32", 1)
+    q, k = q * q_size, k * k_size
+    q[7] = 0.0
+    bias = torch.zeros(500, device=cuda)
+    for b in (None, bias):
+        want, bound = ranges(torch, q, k, v, [300], [500], b)
+        got = cross_attention(q, k, v, _plan(torch, cuda, 300, 500, 2, D, "float32"), key_bias=b)
+        assert_within(torch, got.double(), want, bound, "bias" if b is not None else "plain")
+
+
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("D", [64, 96, 128])
 def test_features_of_unlike_sizes(cuda, hiplib, kind, D):

@@ -176,7 +176,9 @@ __global__ __launch_bounds__(cross_tile(DP, 3, false).wq * 64, 2) void cross_pai
   for (int w = 0; w < kWaves; ++w) k_top = fmaxf(k_top, largest[0][w]), v_top = fmaxf(v_top, largest[1][w]);
   const int ek = exponent_to(k_top, 9), ev = exponent_to(v_top, 9);
   const float k_scale = power(ek), v_scale = power(ev);
-  const float to_log2 = from_scaled * power(-ek);
+  // (never zero, which would make no number of a state past the end at -infinity; scaled scores are below 2^37, and such
+  // tiny ones are zero either way)
+  const float to_log2 = fmaxf(from_scaled * power(-ek), 0x1p-126f);
   bool bad = !(q_sum * power(-ek) < kPairScores);
 
   float most = 0.0f, least = INFINITY;  // of the scaled values; of fours of v's that are not all zero
