@@ -49,6 +49,23 @@ def test_scores_next_to_zero(cuda, hiplib, q_size, k_size, D):
         assert_within(torch, got.double(), want, bound, "bias" if b is not None else "plain")
 
 
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("n,size", [(2000, 1e32), (2000, 1e34), (2000, 1.5e35), (20000, 1e34)])
+def test_sums_of_large_values(cuda, hiplib, n, size, D):
+    """Equal scores over values whose sum fp32 holds: no weight above 1 may carry it past the type's range.  20000 states
+    are cut into parts."""
+    import torch
+    from tsplat.cross_attention import cross_attention
+
+    q, k, v = _inputs(torch, cuda, 300, n, 1, D, "float32", 2)
+    q = torch.zeros_like(q)
+    v = (1 + 0.1 * v) * size
+    for b in (None, torch.zeros(n, device=cuda)):
+        want, bound = ranges(torch, q, k, v, [300], [n], b)
+        got = cross_attention(q, k, v, _plan(torch, cuda, 300, n, 1, D, "float32"), key_bias=b)
+        assert_within(torch, got.double(), want, bound, "large")
+
+
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("D", [64, 96, 128])
 def test_features_of_unlike_sizes(cuda, hiplib, kind, D):

@@ -317,12 +317,15 @@ __global__ __launch_bounds__(cross_tile(DP, 3, false).wq * 64, 2) void cross_pai
   if (tid == 0) *flag = bad;
   const int again = thread_again(), out_row = (again >> 6) * 32 + (again & 31);
   if (bad || out_row >= item.rows) return;
-  const float l = l_run + other_half(l_run), down = power(-ev);
+  // Weights of 1 at most before v's scale is undone: sums that fp32 holds stay within it.
+  constexpr float kMost = kPairBase + kPairSlack, kDown = 1.0f / (1 << (int)kMost);
+  const float l = (l_run + other_half(l_run)) * kDown, down = power(-ev);
 #pragma unroll
   for (int b = 0; b < kBlocks; ++b)
 #pragma unroll
-    for (int r = 0; r < 16; ++r) o[b][r] *= down;
-  finish<float, DP, true>(p, item, kv, out_row, kWaves * 32, row_of(p, item, kv, out_row), again >> 5 & 1, o, m_run, l);
+    for (int r = 0; r < 16; ++r) o[b][r] = o[b][r] * kDown * down;
+  finish<float, DP, true>(p, item, kv, out_row, kWaves * 32, row_of(p, item, kv, out_row), again >> 5 & 1, o,
+                          m_run + kMost, l);
 }
 
 template <int DP>
