@@ -5,6 +5,7 @@ import math
 
 import pytest
 
+from _cross_cases import cross
 from _cross_ranges import FEATURE, KINDS, feature_off, ranges, small_features
 from _request_cases import assert_within
 
@@ -64,6 +65,30 @@ def test_sums_of_large_values(cuda, hiplib, n, size, D):
         want, bound = ranges(torch, q, k, v, [300], [n], b)
         got = cross_attention(q, k, v, _plan(torch, cuda, 300, n, 1, D, "float32"), key_bias=b)
         assert_within(torch, got.double(), want, bound, "large")
+
+
+@pytest.mark.parametrize("dtype,precision", [("float32", "fp32"), ("float32", "bf16x3"), ("float32", "bf16"),
+                                             ("bfloat16", "fp32")])
+@pytest.mark.parametrize("aligned", [True, False])
+@pytest.mark.parametrize("rows", [2, 100])
+def test_sums_of_large_values_with_rising_scores(cuda, hiplib, rows, aligned, dtype, precision):
+    """The same, with half of the states' scores 5.4 above the first ones', which a reference that lags behind the largest
+    score makes weights of 2^7.8."""
+    import torch
+    from tsplat.cross_attention import cross_attention
+
+    n = 2000
+    q, k, v = _inputs(torch, cuda, rows, n, 1, 64, dtype, 3)
+    q[:], k[:] = 0, 0
+    q[..., 0] = 8.0
+    k[:, :, 0] = torch.where(torch.arange(n, device=cuda) % 256 < 128, 0.0, 5.375)[:, None].to(k.dtype)
+    v = ((1 + 0.1 * v.float()) * 1e35).to(v.dtype)
+    if not aligned:
+        q, k, v = (_unaligned(t) for t in (q, k, v))
+    want, bound = cross(torch, q, k, v, [rows], [n], precision=precision)
+    got = cross_attention(q, k, v, _plan(torch, cuda, rows, n, 1, 64, dtype, precision))
+    assert bool(torch.isfinite(want).all())
+    assert_within(torch, got.double(), want, bound, precision)
 
 
 @pytest.mark.parametrize("kind", KINDS)

@@ -46,10 +46,11 @@ typedef int intx4 __attribute__((ext_vector_type(4)));
 constexpr float kLog2e = 1.4426950408889634f;
 // Weights are 2^(x - m) for a reference m that follows a row's largest x (log2 units) only when that has passed it by more
 // than kSlack: most tiles rescale nothing.  fp16 weights lie 2^7 higher, below 2^15 at most, so that a weight 2^-31 of the
-// largest is still held (many small ones add up); bf16 has fp32's range.
+// largest is still held (many small ones add up; sums of fp16 values are far from fp32's range).  bf16 has fp32's range, and
+// so may its values: weights of 1 at most, 2^-8 where m has just moved, keep every sum that fp32 holds within it.
 constexpr float kSlack = 8.0f;
 template <class E>
-constexpr float kLift = std::is_same_v<E, half_t> ? 7.0f : 0.0f;
+constexpr float kLift = std::is_same_v<E, half_t> ? 7.0f : -kSlack;
 
 template <class T>
 struct Element {
