@@ -127,3 +127,34 @@ def test_values_of_unlike_sizes_by_feature(cuda, hiplib):
         got = cross_attention(q, k, values, plan)
         assert_within(torch, got.double(), want, bound, "by feature")
         assert feature_off(torch, got, want) <= FEATURE
+
+
+@pytest.mark.parametrize("precision", ["fp32", "bf16x3"])
+@pytest.mark.parametrize("aligned", [True, False])
+@pytest.mark.parametrize("rows", [2, 100])
+def test_largest_finite_values(cuda, hiplib, rows, aligned, precision):
+    """Values between bf16's largest and fp32's: finite ones, in q, k and v."""
+    import torch
+    from tsplat.cross_attention import cross_attention
+
+    top = torch.finfo(torch.float32).max
+    for n in (1, 70):
+        q, k, v = _inputs(torch, cuda, rows, n, 2, 64, "float32", 6)
+        v[:, :, 2], v[:, :, 5] = top / n, -3.4e38 / n
+        v[0, :, 7] = top
+        v[1:, :, 7] = 0.0
+        k[:, :, 0], q[:, :, 0] = top, 0.0
+        k[:, :, 1], q[:, :, 1] = 0.0, -top
+        if not aligned:
+            q, k, v = (_unaligned(t) for t in (q, k, v))
+        # (scale * log2 e * top is 3.3997e38, above bf16's largest)
+        scale = 0.6925
+        want, bound = cross(torch, q, k, v, [rows], [n], scale=scale, precision=precision)
+        got = cross_attention(q, k, v, _plan(torch, cuda, rows, n, 2, 64, "float32", precision), scale=scale).double()
+        # A result that may be off by `bound` may round past fp32's largest where it lies closer to it than that: the value
+        # top itself, whose weight and denominator are each rounded.  3.4e38 does not (2.8e35 away; 3.1 * 2^-16 of it: 1.6e34).
+        past = torch.isinf(got) & (want.abs() + bound > top)
+        assert bool((got[past].sign() == want[past].sign()).all()) and not past[..., 5].any()
+        got = torch.where(past, want, got)
+        assert bool(torch.isfinite(got).all())
+        assert_within(torch, got, want, bound, precision)

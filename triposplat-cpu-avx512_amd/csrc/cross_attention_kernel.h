@@ -70,15 +70,20 @@ __device__ __forceinline__ floatx16 multiply(const shortx8& a, const shortx8& b,
 }
 
 // Pairs of values to 16 bits, nearest even; `left` what is left of them (exact).
+constexpr float kBf16Top = 3.3895313892515355e38f;  // the largest
+template <bool CAP>
 __device__ __forceinline__ int bf16_pair(float a, float b, float& left_a, float& left_b) {
-  const int w = __builtin_bit_cast(int, bf16x2{(bf16_t)a, (bf16_t)b});
+  const bf16x2 first = CAP ? bf16x2{(bf16_t)__builtin_amdgcn_fmed3f(a, -kBf16Top, kBf16Top),
+                                    (bf16_t)__builtin_amdgcn_fmed3f(b, -kBf16Top, kBf16Top)}
+                           : bf16x2{(bf16_t)a, (bf16_t)b};
+  const int w = __builtin_bit_cast(int, first);
   left_a = a - __int_as_float(w << 16);
   left_b = b - __int_as_float(w & 0xffff0000);
   return w;
 }
 
-// Eight values as TERMS vectors of 16-bit terms.
-template <class E, int TERMS>
+// Eight values as TERMS vectors of 16-bit terms; CAP: the first terms within bf16's range.
+template <class E, int TERMS, bool CAP = false>
 __device__ __forceinline__ void split8(const float (&x)[8], shortx8 (&out)[TERMS]) {
   if constexpr (std::is_same_v<E, half_t>) {
     halfx8 h;
@@ -95,7 +100,8 @@ __device__ __forceinline__ void split8(const float (&x)[8], shortx8 (&out)[TERMS
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         float a, b;
-        w[i] = bf16_pair(left[2 * i], left[2 * i + 1], a, b);
+        w[i] = t == 0 ? bf16_pair<CAP>(left[2 * i], left[2 * i + 1], a, b)
+                      : bf16_pair<false>(left[2 * i], left[2 * i + 1], a, b);
         left[2 * i] = a, left[2 * i + 1] = b;
       }
       out[t] = __builtin_bit_cast(shortx8, w);
@@ -128,13 +134,14 @@ __device__ __forceinline__ Raw<T> past_end(Raw<T> r, int dim, int D, bool none) 
   return r;
 }
 
-// The terms of eight values; of T's own 16 bits as they are.
+// The terms of eight values; of T's own 16 bits as they are.  A first term is bf16's largest at most, so that a finite value
+// past it keeps finite terms (an infinity or NaN remains in the second).  A term alone rounds as bf16 does.
 template <class T, class E, int TERMS>
 __device__ __forceinline__ void terms_of(const Raw<T>& r, shortx8 (&out)[TERMS]) {
   if constexpr (sizeof(T) == 2) {
     out[0] = __builtin_bit_cast(shortx8, r);
   } else {
-    split8<E, TERMS>(r.x, out);
+    split8<E, TERMS, (TERMS > 1)>(r.x, out);
   }
 }
 
