@@ -37,8 +37,9 @@ int64_t tsplat_cross_scratch_bytes(const int32_t* header);
  * q, out: [rows][heads][head_dim], k, v: [states][kv_heads][head_dim] of the plan's type, unit stride within a vector,
  * token and head strides in values (vectors must not overlap, -3); rows and states at least the sums of the plan's lengths; rows past
  * them are not touched.  bias: fp32 [states] or null; a state whose bias is -infinity is not read into any result,
- * whatever it holds; one of +infinity or NaN makes its request's results NaN, and one below -2.3e38 counts as the type's
- * lowest.  An infinity in q, or in k or v of a state that counts, may come out as a NaN.  scale: positive and finite (-2).
+ * whatever it holds; one of +infinity or NaN makes its request's results NaN, and one past 2.3e38 of either sign counts as
+ * the type's largest or lowest.  An infinity in q, or in k or v of a state that counts, may come out as a NaN.  scale:
+ * positive and finite (-2).
  * header: the plan's first ints (host); plan: all of it on the device, as tsplat_cross_plan wrote it.
  * out must not overlap anything that is read (-3).  scratch: tsplat_cross_scratch_bytes of device memory that no other
  * work uses until the call's kernels are done (-5 when too small, -3 over another argument), 16-byte aligned.  The call

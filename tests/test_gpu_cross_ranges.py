@@ -158,3 +158,24 @@ def test_largest_finite_values(cuda, hiplib, rows, aligned, precision):
         got = torch.where(past, want, got)
         assert bool(torch.isfinite(got).all())
         assert_within(torch, got, want, bound, precision)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16", "float16"])
+@pytest.mark.parametrize("rows", [1, 100])
+@pytest.mark.parametrize("aligned", [True, False])
+def test_largest_bias(cuda, hiplib, aligned, rows, dtype):
+    """A finite bias is never taken for an infinity: fp32's largest leaves its own state alone."""
+    import torch
+    from tsplat.cross_attention import cross_attention
+
+    q, k, v = _inputs(torch, cuda, rows, 300, 2, 64, dtype, 7, aligned)
+    plan = _plan(torch, cuda, rows, 300, 2, 64, dtype)
+    for at, value in ((0, 2.4e38), (150, 3e38), (299, torch.finfo(torch.float32).max)):
+        bias = torch.zeros(300, device=cuda)
+        bias[at] = value
+        got = cross_attention(q, k, v, plan, key_bias=bias).double()
+        want = v[at].double().expand_as(got)
+        # one weight, which division by itself makes 1 to 2 ulp, a pair's 2^-23 of the value, the result's rounding
+        assert_within(torch, got, want, (torch.finfo(v.dtype).eps / 2 + 2.0 ** -21) * want.abs(), str(value))
+        bias[at] = INF
+        assert bool(torch.isnan(cross_attention(q, k, v, plan, key_bias=bias)).all())

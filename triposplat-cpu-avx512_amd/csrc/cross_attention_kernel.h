@@ -231,10 +231,11 @@ __device__ __forceinline__ bool load_queries(const CrossParams& p, const Row& at
   return !(sum < INFINITY);
 }
 
-// A bias in log2 units; a finite one stays finite (the type's lowest masks against others, not by itself).
+// A bias in log2 units; a finite one stays finite (the type's lowest masks against others, not by itself; its largest leaves
+// its own state alone).
 __device__ __forceinline__ float bias_log2(float b) {
-  const float b2 = fmaxf(b * kLog2e, -3.4028234663852886e38f);
-  return b == -INFINITY || b != b ? b : b2;
+  constexpr float kTop = 3.4028234663852886e38f;
+  return fabsf(b) < INFINITY ? __builtin_amdgcn_fmed3f(b * kLog2e, -kTop, kTop) : b;
 }
 
 // A product brought to T: rounded to fp32 first, whichever instructions the compiler would fuse it into.
