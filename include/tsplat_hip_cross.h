@@ -39,7 +39,7 @@ int64_t tsplat_cross_scratch_bytes(const int32_t* header);
  * them are not touched.  bias: fp32 [states] or null; a state whose bias is -infinity is not read into any result,
  * whatever it holds; one of +infinity or NaN makes its request's results NaN, and one past 2.3e38 of either sign counts as
  * the type's largest or lowest.  An infinity in q, or in k or v of a state that counts, may come out as a NaN.  scale:
- * positive and finite (-2).
+ * positive, and finite times log2 e (-2).
  * header: the plan's first ints (host); plan: all of it on the device, as tsplat_cross_plan wrote it.
  * out must not overlap anything that is read (-3).  scratch: tsplat_cross_scratch_bytes of device memory that no other
  * work uses until the call's kernels are done (-5 when too small, -3 over another argument), 16-byte aligned.  The call

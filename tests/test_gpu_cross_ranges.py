@@ -179,3 +179,30 @@ def test_largest_bias(cuda, hiplib, aligned, rows, dtype):
         assert_within(torch, got, want, (torch.finfo(v.dtype).eps / 2 + 2.0 ** -21) * want.abs(), str(value))
         bias[at] = INF
         assert bool(torch.isnan(cross_attention(q, k, v, plan, key_bias=bias)).all())
+
+
+def test_scale_whose_product_is_no_number(cuda, hiplib):
+    """scale * log2 e has to be finite as well."""
+    import torch
+    from tsplat.cross_attention import cross_attention
+
+    q, k, v = _inputs(torch, cuda, 40, 50, 2, 64, "float32", 8)
+    plan = _plan(torch, cuda, 40, 50, 2, 64, "float32")
+    q = torch.zeros_like(q)
+    assert bool(torch.isfinite(cross_attention(q, k, v, plan, scale=2.3e38)).all())
+    for scale in (2.4e38, 2.9e38):
+        with pytest.raises(ValueError):
+            cross_attention(q, k, v, plan, scale=scale)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16", "float16"])
+@pytest.mark.parametrize("rows", [1, 100])
+def test_smallest_scale(cuda, hiplib, rows, dtype):
+    """Scores of zero, and states past the last one that still count for nothing: the values' mean."""
+    import torch
+    from tsplat.cross_attention import cross_attention
+
+    q, k, v = _inputs(torch, cuda, rows, 50, 2, 64, dtype, 9)
+    plan = _plan(torch, cuda, rows, 50, 2, 64, dtype)
+    want, bound = cross(torch, q, k, v, [rows], [50], scale=1.4e-45)
+    assert_within(torch, cross_attention(q, k, v, plan, scale=1.4e-45).double(), want, bound, dtype)

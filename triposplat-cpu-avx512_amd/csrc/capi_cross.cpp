@@ -15,6 +15,7 @@ using namespace tsplat;
 namespace {
 
 constexpr int kCrossAbiVersion = 1;
+constexpr float kLog2e = 1.4426950408889634f;  // (the kernels' exponents are base 2)
 
 int launched(int st) {
   if (st == kErrLaunch) (void)note(hipErrorLaunchFailure);
@@ -76,7 +77,7 @@ int tsplat_cross_attention_async(const void* q, int64_t q_token, int64_t q_head,
                                  float scale, void* out, int64_t out_token, int64_t out_head, const int32_t* header,
                                  const int32_t* plan, void* scratch, int64_t scratch_size, void* stream) {
   if (!header) return kErrNull;
-  if (!is_header(header) || !(scale > 0.0f) || !std::isfinite(scale)) return kErrDims;
+  if (!is_header(header) || !(scale > 0.0f) || !std::isfinite(scale * kLog2e)) return kErrDims;
   const int32_t* h = header;
   const int64_t rows = h[kPlanRows], states = h[kPlanStates];
   const int heads = h[kPlanHeads], kv_heads = h[kPlanKvHeads], dim = h[kPlanDim], size = h[kPlanType] == 0 ? 4 : 2;

@@ -14,6 +14,7 @@ from .fp8 import type_ids
 from .nf24 import precision_id
 
 HEADER_INTS = 16
+MAX_SCALE = 2.3e38  # times log2 e within fp32
 # where the header holds the plan's items and the sums of its lengths
 _ITEMS, _ROWS, _STATES = 2, 5, 6
 
@@ -120,8 +121,8 @@ def cross_attention(q, k, v, plan, *, key_bias=None, scale=None, out=None):
             raise ValueError(f"key_bias must be a contiguous [{plan.states} or more] fp32 tensor on the plan's GPU")
         bias_ptr = key_bias.data_ptr()
     scale = plan._scale if scale is None else float(scale)
-    if not 0.0 < scale < 3e38:
-        raise ValueError(f"scale must be positive and finite, not {scale}")
+    if not 0.0 < scale <= MAX_SCALE:
+        raise ValueError(f"scale must be positive and at most {MAX_SCALE}, not {scale}")
     if out is None:
         out = torch.empty((q.shape[0], plan.heads, plan.head_dim), dtype=plan.dtype, device=plan.device)
         if q.shape[0] > plan.rows:
