@@ -145,10 +145,10 @@ __device__ __forceinline__ int tile_of(int id, int count) {
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
-// 2^(e - 127) for e >= 1.  e = 0 makes zero: values under such a scale are below 2^-118.
+// 2^(e - 127): the conversions below take the scale's exponent field alone, 0 among its values.
 __device__ __forceinline__ float scale_of(uint32_t e) { return __uint_as_float((e & 0xffu) << 23); }
 
-// Eight codes as bf16, times the scale.
+// Eight codes as bf16, times the scale: exact down to 2^-126, below that to bf16's smallest step of 2^-133.
 __device__ __forceinline__ bf16x8 widen8(int lo, int hi, float scale) {
   const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, false);
   const bf16x2 b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, true);
