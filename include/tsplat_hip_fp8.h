@@ -24,7 +24,7 @@ int tsplat_fp8_abi_version(void);
  *
  * The scale is the smallest power of two, 2^-127 at least, that brings the block's largest finite magnitude to 448 or
  * below (1 for a block without one), a code the nearest value of x / scale, ties to even; an infinity or NaN gives a
- * NaN.
+ * NaN.  (An fp32 value of 248 * 2^120 and more rounds to 2^128, which is an infinity to fp32.)
  * dtype of x: 0 fp32, 1 bf16, 2 fp16; rows x_stride values apart.  rows up to 2^27, K up to 2^20 (-2).  codes and
  * exponents must not overlap each other or x (-3). */
 int tsplat_fp8_quantize_async(const void* x, int dtype, int64_t x_stride, int rows, int K, uint8_t* codes,
@@ -34,7 +34,12 @@ int tsplat_fp8_quantize_async(const void* x, int dtype, int64_t x_stride, int ro
  * out[m][n] = y * gate[m / rows_per_batch][n] + residual[m][n].
  *
  * x8: the 8-bit rows of x (dtype, x_stride as above), made within the call, or with x null the rows at x_codes,
- * x_exponents; w8: N rows of K as above.  Products of codes are exact, their sums are held in fp32.
+ * x_exponents; w8: N rows of K as above.  Sums are held in fp32.  Products:
+ *   out_dtype 0, or at most 64 rows: exact (a value below 2^-126 is first rounded to a multiple of 2^-133);
+ *   out_dtype 1 and 2 beyond 64 rows: those of each 8 neighbouring values are brought to the largest one's exponent and
+ *   cut at 2^-13 of its power of two: 2^-10 of the magnitudes that are summed at most, 1.5e-5 of a sum of random signs or
+ *   so.  Where the terms cancel that is more of the sum, and the same row may differ by it between a call of 64 rows and
+ *   one of more.
  * bias [N], gate (rows gate_stride floats apart, 0 for one row that serves all) and residual may be null; residual and
  * out are of out_dtype, rows residual_stride and out_stride values apart; out may be residual itself (same pointer and
  * stride) and must not overlap anything else that is read (-3).
