@@ -162,8 +162,8 @@ __device__ __forceinline__ bf16x8 widen8(int lo, int hi, float scale) {
 // of all banks: piece c of row r lies at place c ^ (r / 2 % 4).  The copies to LDS write in lane order, so the lane picks
 // its piece.
 // A stage is multiplied in two steps, of 32 codes each (EXACT) or of half of the weights' rows.  The operands of each step
-// are read into registers while the one before is multiplied (where 128 sums leave room for that), so a stage's buffer is free, and the copies of the stage
-// that comes STAGES later may begin, before its last step is multiplied.
+// are read into registers while the one before is multiplied, so a stage's buffer is free, and the copies of the stage that
+// comes STAGES later may begin, before its last step is multiplied.
 // 128x256 tiles, two workgroups a CU; 128x128 where there are fewer than two of the wide ones for each CU (4101x1024x2048:
 // 23 against 25 us; 16384x1024x4096 in 16 bits the wide ones, half the reads of x).
 constexpr int kStage = 64;
@@ -184,7 +184,6 @@ __global__ __launch_bounds__(WM* WN * 64, BM * BN > 128 * 128 ? 2 : 3) void fp8_
   static_assert(kCopies * kRowsACopy * kWaves == BM + BN && BM % kRowsACopy == 0, "whole copies");
   __shared__ __attribute__((aligned(16))) uint8_t lds[STAGES][(BM + BN) * kStage];
   __shared__ __attribute__((aligned(16))) uint8_t exps[2][(BM + BN) * 4];
-  constexpr bool kAhead = true;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   // Wide tiles: bands of 16 row tiles, in them runs of 4 column tiles, whose operands stay in the XCD's L2 (16384x1024x4096
   // in fp32 163 -> 157 us, 16384x4096x4096 in bf16 306 -> 292); small ones, few enough, row after row.
@@ -303,7 +302,7 @@ __global__ __launch_bounds__(WM* WN * 64, BM * BN > 128 * 128 ? 2 : 3) void fp8_
     wait_and_meet<0>();
   Step now, next;
   Scales scales, scales_next;
-  if (kAhead && busy) read_step(now, 0, 0);
+  if (busy) read_step(now, 0, 0);
   read_scales(scales, 0);
   int buffer = 0;
   for (int block = 0; block < blocks; ++block) {
@@ -311,10 +310,8 @@ __global__ __launch_bounds__(WM* WN * 64, BM * BN > 128 * 128 ? 2 : 3) void fp8_
     for (int half_block = 0; half_block < 2; ++half_block) {
       const int stage = 2 * block + half_block;
       if (busy) {
-        if (!kAhead) read_step(now, buffer, 0);
         read_step(next, buffer, 1);
         multiply(now, scales, 0);
-        if (!kAhead) multiply(next, scales, 1);
       }
       const int after = buffer == STAGES - 1 ? 0 : buffer + 1;
       if (stage + 1 < stages) {
@@ -324,11 +321,11 @@ __global__ __launch_bounds__(WM* WN * 64, BM * BN > 128 * 128 ? 2 : 3) void fp8_
           wait_and_meet<(STAGES - 2) * kCopies>();
         else
           wait_and_meet<0>();
-        if (kAhead && busy) read_step(now, after, 0);
+        if (busy) read_step(now, after, 0);
         if (half_block == 1) read_scales(scales_next, block + 1);
         if (stage + STAGES < stages) fetch(stage + STAGES, buffer);
       }
-      if (kAhead && busy) multiply(next, scales, 1);
+      if (busy) multiply(next, scales, 1);
       buffer = after;
     }
     scales = scales_next;
