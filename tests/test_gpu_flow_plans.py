@@ -1,0 +1,63 @@
+"""What the flow model refuses of conditions and their plans, and what it does not do for each entry."""
+from __future__ import annotations
+
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+
+def _model(cuda, blocks=1, L=40):
+    from tsplat.flow import FlowConfig, FlowModel
+
+    return FlowModel(FlowConfig(hidden=128, heads=2, blocks=blocks, latent_tokens=L, cond_tokens=33), cuda)
+
+
+def _inputs(torch, cuda, lengths, seed=1, L=40):
+    g = torch.Generator(device=cuda).manual_seed(seed)
+    B = len(lengths)
+    z = torch.randn(B, L, 128, generator=g, device=cuda)
+    return z, torch.randn(sum(lengths), 128, generator=g, device=cuda), torch.rand(B, generator=g, device=cuda) * 1000
+
+
+def test_plan_of_another_attention_precision(cuda, hiplib):
+    """A plan made for one precision of the attention's products does not serve another in silence."""
+    import torch
+
+    model = _model(cuda)
+    z, c, t = _inputs(torch, cuda, [20, 5])
+    plans = {}
+    for precision in ("bf16", "bf16x3", "fp32"):
+        model.set_precision(precision, include=("attention",))
+        plans[precision] = model.condition_plan(40, [20, 5])
+    for now in plans:
+        model.set_precision(now, include=("attention",))
+        for made, plan in plans.items():
+            if made == now:
+                assert torch.isfinite(model.velocity(z, c, t, cond_plan=plan)).all()
+            else:
+                with pytest.raises(ValueError, match="precision"):
+                    model.velocity(z, c, t, cond_plan=plan)
+
+
+def test_eight_bits_of_the_other_linears(cuda, hiplib):
+    """Precision "fp8" of the timestep, input and output Linears, alone and with the blocks, in both models."""
+    import torch
+    from tsplat.flow import FlowConfig
+    from tsplat.flow_joint import JointFlowModel
+
+    model = _model(cuda, blocks=2)
+    z, c, t = _inputs(torch, cuda, [33, 33])
+    joint = JointFlowModel(FlowConfig(hidden=128, heads=2, blocks=2, latent_tokens=40, cond_tokens=33), cuda)
+    cam = torch.randn(1, 5, generator=torch.Generator(device=cuda).manual_seed(3), device=cuda)
+    for m, args in ((model, (z, c.view(2, 33, 128), t)), (joint, (z[0], c[:33], cam, t[:1]))):
+        before = m.velocity(*args)
+        for include in (("io",), ("blocks", "io")):
+            m.set_precision("fp8", include=include)
+            got = m.velocity(*args)
+            m.set_precision("fp32", include=include)
+            for a, b in zip(*((x if isinstance(x, tuple) else (x,)) for x in (got, before))):
+                # (a few per cent a Linear; other results than fp32's)
+                assert 1e-4 < float((a.double() - b.double()).norm() / b.double().norm()) < 0.3
+        after = m.velocity(*args)
+        for a, b in zip(*((x if isinstance(x, tuple) else (x,)) for x in (after, before))):
+            assert torch.equal(a, b)

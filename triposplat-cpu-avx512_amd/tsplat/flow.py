@@ -320,8 +320,9 @@ class FlowModel:
     def condition_plan(self, tokens, lengths):
         """The plan of a batch whose entries bring conditions of their own
         lengths, any of them 0, for velocity(cond_plan=...): tokens latent
-        tokens in each entry.  Made once, for all steps and blocks; it keeps
-        the attention precision that the model has now."""
+        tokens in each entry.  Made once, for all steps and blocks, in the
+        attention precision that the model has now: in another one velocity
+        refuses it."""
         return CrossPlan([tokens] * len(lengths), lengths, self.cfg.heads, self.cfg.head_dim,
                          precision=self.attention_precision, device=self.device)
 

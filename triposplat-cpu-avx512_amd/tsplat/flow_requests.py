@@ -77,6 +77,9 @@ def _check_plan(model, plan, cond, B, L):
     if plan.q_lengths != [L] * B or (plan.heads, plan.kv_heads, plan.head_dim) != (
             model.cfg.heads, model.cfg.heads, model.cfg.head_dim) or plan.dtype is not model.torch.float32:
         raise ValueError(f"cond_plan must be of {B} entries of {L} latent tokens and the model's heads, in fp32")
+    if plan.precision != model.attention_precision:
+        raise ValueError(f"cond_plan is of precision {plan.precision!r}, the model's attention now of "
+                         f"{model.attention_precision!r}: make another (FlowModel.condition_plan)")
     if cond.dim() != 2 or cond.shape[0] != plan.states:
         raise ValueError(f"with this cond_plan cond is [{plan.states}, {model.cfg.hidden}]")
 
