@@ -39,6 +39,31 @@ def test_plan_of_another_attention_precision(cuda, hiplib):
                     model.velocity(z, c, t, cond_plan=plan)
 
 
+def test_refused_before_anything_runs(cuda, hiplib, monkeypatch):
+    """A condition that does not fit the batch is refused by its shape, before the first kernel."""
+    import torch
+    from tsplat.flow_requests import FlowAdapters
+
+    model = _model(cuda)
+    z, c, t = _inputs(torch, cuda, [20, 20])
+    plan, adapters = model.condition_plan(40, [20, 20]), FlowAdapters(model, 2, 4)
+
+    def never(_):
+        raise AssertionError("a kernel ran")
+
+    monkeypatch.setattr(model, "timestep", never)
+    wide = torch.zeros(2, 20, 64, device=cuda)
+    for cond in (c[None, :20], c.view(1, 40, 128), c, c.view(4, 10, 128), wide, c[0]):
+        for kwargs in ({}, dict(adapters=adapters, slots=[0, -1])):
+            with pytest.raises(ValueError):
+                model.velocity(z, cond, t, **kwargs)
+    for cond in (c[:39], c.view(2, 20, 128), c[:, :64], c.view(80, 64)):
+        with pytest.raises(ValueError):
+            model.velocity(z, cond, t, cond_plan=plan)
+    with pytest.raises(AssertionError):
+        model.velocity(z, c, t, cond_plan=plan)
+
+
 def test_eight_bits_of_the_other_linears(cuda, hiplib):
     """Precision "fp8" of the timestep, input and output Linears, alone and with the blocks, in both models."""
     import torch

@@ -326,6 +326,11 @@ class FlowModel:
         return CrossPlan([tokens] * len(lengths), lengths, self.cfg.heads, self.cfg.head_dim,
                          precision=self.attention_precision, device=self.device)
 
+    def check_condition(self, cond, entries):
+        """Refuses a condition that is not [entries, rows, C]."""
+        if cond.dim() != 3 or cond.shape[0] != entries or cond.shape[2] != self.cfg.hidden:
+            raise ValueError(f"cond must be [{entries}, rows, {self.cfg.hidden}], its shape is {list(cond.shape)}")
+
     def condition_rows(self, cond):
         """cond [..., C] as the blocks' condition Linears read it: its rows in 8 bits, once for all blocks, where all
         of them multiply in precision "fp8", else itself."""
@@ -352,10 +357,9 @@ class FlowModel:
                                           rope=rope, cond_plan=cond_plan, observe=observe)
         torch = self.torch
         B, L, C = (int(s) for s in z.shape)
+        self.check_condition(cond, B)
         t_emb, t_mod = self.timestep(t)
         x = self.input_layer(z.reshape(B * L, C)).view(B, L, C)
-        if cond.shape[0] != B:
-            raise ValueError(f"cond must be [{B}, rows, {C}], its shape is {list(cond.shape)}")
         cond = self.condition_rows(cond)
         for i, blk in enumerate(self.blocks):
             if observe is not None:

@@ -80,7 +80,7 @@ def _check_plan(model, plan, cond, B, L):
     if plan.precision != model.attention_precision:
         raise ValueError(f"cond_plan is of precision {plan.precision!r}, the model's attention now of "
                          f"{model.attention_precision!r}: make another (FlowModel.condition_plan)")
-    if cond.dim() != 2 or cond.shape[0] != plan.states:
+    if tuple(cond.shape) != (plan.states, model.cfg.hidden):
         raise ValueError(f"with this cond_plan cond is [{plan.states}, {model.cfg.hidden}]")
 
 
@@ -96,7 +96,9 @@ def velocity(model, z, cond, t, *, adapters=None, slots=None, positions=None, ro
     torch, cfg = model.torch, model.cfg
     B, L, C = (int(s) for s in z.shape)
     H = cfg.heads
-    if cond_plan is not None:
+    if cond_plan is None:
+        model.check_condition(cond, B)
+    else:
         _check_plan(model, cond_plan, cond, B, L)
     lengths = [int(cond.shape[1])] * B if cond_plan is None else cond_plan.k_lengths
     if (positions is None) != (rope is None):
