@@ -64,6 +64,30 @@ def test_refused_before_anything_runs(cuda, hiplib, monkeypatch):
         model.velocity(z, c, t, cond_plan=plan)
 
 
+def test_one_fill_for_each_entry(cuda, hiplib):
+    """Conditions of one length: the entries' slots are written once and spread to both kinds of rows."""
+    import torch
+    from torch.utils._python_dispatch import TorchDispatchMode
+    from tsplat.flow_requests import FlowAdapters
+
+    class Fills(TorchDispatchMode):
+        count = 0
+
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            self.count += "fill_" in func.name()
+            return func(*args, **(kwargs or {}))
+
+    model = _model(cuda)
+    adapters = FlowAdapters(model, 2, 4)
+    counts = {}
+    for B in (2, 9):
+        z, c, t = _inputs(torch, cuda, [20] * B)
+        with Fills() as fills:
+            model.velocity(z, c.view(B, 20, 128), t, adapters=adapters, slots=[0] * B)
+        counts[B] = fills.count
+    assert counts[9] - counts[2] == 7, counts
+
+
 def test_eight_bits_of_the_other_linears(cuda, hiplib):
     """Precision "fp8" of the timestep, input and output Linears, alone and with the blocks, in both models."""
     import torch

@@ -117,10 +117,13 @@ def velocity(model, z, cond, t, *, adapters=None, slots=None, positions=None, ro
         for b, s in enumerate(slots):
             of_entry[b].fill_(max(s, -1))
         rows = of_entry.expand(B, L).contiguous().view(-1)
-        cond_rows, start = torch.empty(sum(lengths), dtype=torch.int32, device=model.device), 0
-        for n, s in zip(lengths, slots):
-            cond_rows[start:start + n].fill_(max(s, -1))
-            start += n
+        if cond_plan is None:
+            cond_rows = of_entry.expand(B, lengths[0]).contiguous().view(-1)
+        else:
+            cond_rows, start = torch.empty(sum(lengths), dtype=torch.int32, device=model.device), 0
+            for n, s in zip(lengths, slots):
+                cond_rows[start:start + n].fill_(max(s, -1))
+                start += n
     if rope is None:
         rope = model.token_rope()
         positions = torch.arange(L, dtype=torch.int32, device=model.device)[:, None]
