@@ -44,8 +44,11 @@ bool is_header(const int32_t* h) {
   return h[kPlanItems] >= 0 && h[kPlanJoins] >= 0 && h[kPlanParts] >= 0 && h[kPlanParts] <= h[kPlanItems] &&
          h[kPlanJoins] <= h[kPlanParts] && h[kPlanInts] == ints && h[kPlanRows] >= 0 && h[kPlanStates] >= 0 &&
          h[kPlanKvHeads] >= 1 && h[kPlanHeads] >= h[kPlanKvHeads] && h[kPlanHeads] % h[kPlanKvHeads] == 0 &&
-         h[kPlanDim] >= 1 && h[kPlanDim] <= 128 && h[kPlanType] >= 0 && h[kPlanType] <= 2 && h[kPlanTerms] >= 1 &&
-         h[kPlanTerms] <= 3 && (h[kPlanType] == 0 || h[kPlanTerms] == 1);
+         h[kPlanHeads] < 1 << 16 && h[kPlanDim] >= 1 && h[kPlanDim] <= 128 && h[kPlanType] >= 0 && h[kPlanType] <= 2 &&
+         h[kPlanTerms] >= 1 && h[kPlanTerms] <= 3 && (h[kPlanType] == 0 || h[kPlanTerms] == 1) &&
+         (h[kPlanFew] == 0 || h[kPlanFew] == 1) &&
+         cross_launch_fits(h[kPlanItems], h[kPlanKvHeads],
+                           cross_tile(cross_padded_dim(h[kPlanDim]), h[kPlanTerms], h[kPlanFew] != 0), h[kPlanFew] != 0);
 }
 
 // The parts' sums, then the pairs' flags.

@@ -73,8 +73,7 @@ int64_t make_cross_plan(const int32_t* q_lengths, const int32_t* k_lengths, int 
   };
   each([&](const CrossItem&) { ++items; }, [&](const CrossJoin&) { ++joins; });
   const int64_t need = kPlanHeaderInts + items * kCrossItem + joins * kCrossJoin;
-  const int64_t threads = (few ? kFewWaves : tile.wq) * 64;
-  if (items * kv_heads * threads > UINT32_MAX || need > INT32_MAX) return kErrDims;  // (a launch's threads in 32 bits)
+  if (!cross_launch_fits(items, kv_heads, tile, few) || need > INT32_MAX) return kErrDims;
   if (!plan) return need;
   if (plan_ints < need || room_items < items) return kErrRange;
   const int32_t header[kPlanHeaderInts] = {kPlanMagicValue, (int32_t)need, (int32_t)items, (int32_t)joins,

@@ -44,6 +44,11 @@ constexpr CrossTile cross_tile(int padded, int terms, bool few) {
   return {4, 2};
 }
 
+// Whether a launch holds a workgroup for each item and key head: its threads are counted in 32 bits.
+inline bool cross_launch_fits(int64_t items, int64_t kv_heads, const CrossTile& tile, bool few) {
+  return items * kv_heads * ((few ? kFewWaves : tile.wq) * 64) <= UINT32_MAX;
+}
+
 // Writes the plan (null: only counts); its size in ints, or a negative status.
 int64_t make_cross_plan(const int32_t* q_lengths, const int32_t* k_lengths, int requests, int heads, int kv_heads,
                         int head_dim, int dtype, int precision, int compute_units, int32_t* plan, int64_t plan_ints);
