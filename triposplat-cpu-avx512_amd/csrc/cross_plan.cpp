@@ -37,8 +37,9 @@ int64_t make_cross_plan(const int32_t* q_lengths, const int32_t* k_lengths, int 
   // tiles, in a chain, and the join of a request's parts together shortest: their number halved, its root.  (Two single
   // tokens over 2049 and 4101 states in fp32: parts of 1, 2, 3, 4 tiles take 34, 27, 26, 23 us; one over 500: 9.9, 11.5,
   // 11.5, 14; 64 over 4096: 2, 3, 4, 6 take 38, 37, 26, 26; three of 200 over 700 in 16 bits: 2, 3, 4 take 14.1, 12.4, 12.5.)
-  // A workgroup of eight waves has a CU to itself (fp32, 2000 rows over 2000 states, 16 heads: 69 us, for two at once 83),
-  // of four waves two run at once (16 bits, five ragged requests of 1 to 8193 rows: 92, for one 105).
+  // The even share counts one workgroup of eight waves a CU (fp32, 2000 rows over 2000 states, 16 heads: 69 us, for two at
+  // once 83), which is what fits, and two of four waves (16 bits, five ragged requests of 1 to 8193 rows: 92, for one 105),
+  // of which three fit for heads up to 64 and two for wider ones.
   const int64_t at_once = (int64_t)compute_units * (few ? 8 : terms > 1 ? 1 : 2);
   int64_t work = 0, most = 0;
   for (int i = 0; i < requests; ++i) {
