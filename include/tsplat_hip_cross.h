@@ -34,6 +34,10 @@ int64_t tsplat_cross_scratch_bytes(const int32_t* header);
 /* out[t][h] = sum_j softmax_j(scale q[t][h] . k[j][g] + bias[j]) v[j][g], g = h / (heads / kv_heads), over the states j of
  * the request that row t belongs to; zero where it has none, or every bias is -infinity.
  *
+ * Sums, maxima and exponents are fp32.  Products of 16-bit types are of the values as they are, summed before scale is
+ * multiplied in (those sums must be finite), and of the weights rounded to that type: half a step of each, about as much
+ * again as the result's own rounding.
+ *
  * q, out: [rows][heads][head_dim], k, v: [states][kv_heads][head_dim] of the plan's type, unit stride within a vector,
  * token and head strides in values (vectors must not overlap, -3); rows and states at least the sums of the plan's lengths; rows past
  * them are not touched.  bias: fp32 [states] or null; a state whose bias is -infinity is not read into any result,

@@ -14,12 +14,12 @@
 //
 // What bounds it, and measured: many rows, the exponents and what surrounds them in the vector units (a block of 32 x 32
 // takes 125 vector instructions, 16 of them exponents at a quarter of the rate, and 8 products of 64 values a head): 275
-// GFLOP of 2 x 16384 x 2048 in bf16 at 0.71 PFLOP/s, 387 us, 0.81 at 128 values a head.  Five ragged requests with a bias
+// GFLOP of 2 x 16384 x 2048 in bf16 at 0.71 PFLOP/s, 386 us, 0.80 at 128 values a head.  Five ragged requests with a bias
 // in bf16 92 us, 0.44 PFLOP/s: 784 workgroups of 22 and 32 tiles on 768 places (more parts than the plan makes cost more
-// than they even out: 123).  fp32 values in three bf16 terms (unaligned, or flagged by cross_pairs.hip) 1340 us for the
-// former, 1.23 PFLOP/s of bf16 products.  Few rows: HBM, 64 single tokens over 1.09 GB of bf16 states 221 us, 4.9 TB/s
-// (a copy: 5.0); two single tokens over 50 MB of fp32 ones 21, of which about 5 join the parts and 6 are a
-// launch and first loads.
+// than they even out: 123).  fp32 values in three bf16 terms 1350 us for the former, 1.22 PFLOP/s of bf16 products, which is
+// what a flagged call of cross_pairs.hip takes besides (unaligned 1630: loads of single values); in two terms 836, in one
+// 428.  Few rows: HBM, 64 single tokens over 1.09 GB of bf16 states 221 us, 4.9 TB/s (a copy: 5.0); two single tokens over
+// 50 MB of fp32 ones 22, of which about 5 join the parts and 6 are a launch and first loads.
 //
 // States go from memory through registers to LDS, a tile ahead of the products; states that the bias masks, or past the
 // request's last, are put there as zeros, so what memory holds in their place does not matter.  Rows of LDS are padded so

@@ -6,12 +6,13 @@
 // The weights are the first operand: a lane then holds four neighbouring columns of one row of the result.
 //
 // What bounds it, and measured (with the rows' conversion, which is HBM's time: 17 and 58 us of these):
-// 16384x1024x4096 in fp32 with GELU 175 us, 16384x4096x1024 onto a gated residual 186: products through bf16 at 1.18
+// 16384x1024x4096 in fp32 with GELU 181 us, 16384x4096x1024 onto a gated residual 188: products through bf16 at 1.18
 // PFLOP/s, what the matrix cores hold at their clock under that load (a library's 8192^3 in bf16: 1.12), and the result's
 // bytes, which the products hide in part (the former 149 us, 40 of them its 268 MB).  Without the conversions to bf16 6
-// us less, without the copies into LDS 9.  8-bit products (results of 16 bits): 16384x4096x4096 292 us, 1.88 PFLOP/s
-// (a library's: 2.64); 4101x1024x2048 27 us, of which 6 convert the rows and 10 are a launch and its chain of loads.
-// One row of 1024x1024 4.4 us (the call 11: the host), 64 rows of 1024x6144 13.
+// us less, without the copies into LDS 9.  8-bit products (results of 16 bits): 16384x4096x4096 323 us, 1.70 PFLOP/s
+// (a library's: 2.64), and 52 the conversion; 4101x1024x2048 28 us, of which 6 convert the rows and 10 are a launch and its
+// chain of loads.  One row of 1024x1024 4.4 us (the call 11: the host), 64 rows of 1024x6144 13.  77 to 1370 rows of
+// 1024x1024 18 us, of 4096x1024 42 to 48: 8 to 88 workgroups, each the whole of K long.
 
 #include <algorithm>
 
@@ -186,7 +187,7 @@ __global__ __launch_bounds__(WM* WN * 64, BM * BN > 128 * 128 ? 2 : 3) void fp8_
   __shared__ __attribute__((aligned(16))) uint8_t exps[2][(BM + BN) * 4];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   // Wide tiles: bands of 16 row tiles, in them runs of 4 column tiles, whose operands stay in the XCD's L2 (16384x1024x4096
-  // in fp32 163 -> 157 us, 16384x4096x4096 in bf16 306 -> 292); small ones, few enough, row after row.
+  // in fp32 163 -> 157 us, 16384x4096x4096 in bf16 5 % less); small ones, few enough, row after row.
   constexpr int kBand = BM * BN > 128 * 128 ? 16 : 1, kRun = 4;
   int tile = tile_of(blockIdx.x, gridDim.x), m0 = tile / tiles_n * BM, n0 = tile % tiles_n * BN;
   if constexpr (kBand > 1) {

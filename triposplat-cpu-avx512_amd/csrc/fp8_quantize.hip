@@ -1,7 +1,8 @@
 // Rows to 8 bits: a block of 128 values of a row becomes e4m3 codes and the exponent of one power-of-two scale,
 //   e = the smallest with max |x| <= 448 * 2^e,  code = e4m3(x / 2^e).
 // One pass: 32 lanes read a block (4 values each), agree on its largest magnitude in registers and write 4 codes each.
-// Bound by HBM: b + 1 bytes a value.  16384 x 4096 in fp32: 58 us, 5.8 TB/s read and written (a 1 GiB device copy: 5.0).
+// Bound by HBM: b + 1 bytes a value.  16384 x 4096 in fp32: 58 us, 5.8 TB/s read and written (a 1 GiB device copy: 5.0);
+// in bf16 and fp16 46 us, 4.4 TB/s (a lane's loads are 8 bytes there).
 // Blocks of a workgroup are asked for four at a time; 3 x 1001 in fp16 takes 3.7 us, a launch (the call 11, the host).
 
 #include <algorithm>

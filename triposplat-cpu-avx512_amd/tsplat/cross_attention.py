@@ -97,13 +97,15 @@ def cross_attention(q, k, v, plan, *, key_bias=None, scale=None, out=None):
     states j of the request that row t belongs to; zeros where it has none, or where every bias is -infinity.
 
     q [rows, heads, head_dim], k, v [states, kv_heads, head_dim]: of the plan's type, unit stride within a vector, the
-    other strides free (k and v may be views of one fused projection); at least as many rows and states as the plan's
-    lengths add up to.  key_bias [states] fp32: a state whose bias is -infinity is not read into any result, whatever it
+    other strides free (k and v may be views of one fused projection) as long as no vectors overlap: shared key heads are
+    kv_heads, not an expanded tensor; at least as many rows and states as the plan's lengths add up to.  key_bias [states] fp32: a state whose bias is -infinity is not read into any result, whatever it
     holds (one of +infinity or NaN makes its request's results NaN, and one past 2.3e38 of either sign counts as the type's
     largest or lowest).  An infinity in q, or in k or v of a state that counts, may come out as a NaN.  scale:
     head_dim ** -0.5 by default.  out: None for a new tensor like q, its rows behind the last request zero, or a tensor
     that overlaps nothing that is read, whose rows behind the last request stay as they are.
-    Sums, maxima and exponents are fp32; fp32 products as the plan's precision says.  Runs on torch's current stream;
+    Sums, maxima and exponents are fp32; fp32 products as the plan's precision says.  With bf16 and fp16 values the weights
+    are rounded to that type before they meet v (half a step of each: in bf16 2.2e-3 of the result's norm, with the
+    result's own rounding, which alone is 1.7e-3), and q . k is summed before scale is multiplied in.  Runs on torch's current stream;
     capturable into a HIP graph.  No gradients."""
     import torch
 
