@@ -206,3 +206,32 @@ def test_smallest_scale(cuda, hiplib, rows, dtype):
     plan = _plan(torch, cuda, rows, 50, 2, 64, dtype)
     want, bound = cross(torch, q, k, v, [rows], [50], scale=1.4e-45)
     assert_within(torch, cross_attention(q, k, v, plan, scale=1.4e-45).double(), want, bound, dtype)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_small_query_features(cuda, hiplib, D):
+    """Query features 2^-32 of the row's largest against keys 2^6 of the first states': two states count, and their
+    difference is the small features' score."""
+    import torch
+    from tsplat.cross_attention import cross_attention
+
+    # (so many states that a part holds 192 of them at least; scale * log2 e is 1 to 1e-7)
+    n, late, rows, scale = 3200, 150, 64, 0.6931472
+    q = torch.full((rows, 1, D), 100.49 * 2.0 ** -27, device=cuda)
+    q[..., 0] = 4000.0
+    k = torch.zeros(n, 1, D, device=cuda)
+    k[:, :, 1:] = 1.0 / 64
+    k[0, :, 1:] = 1.0
+    k[1] = 0.0
+    k[late, :, 1:] = 63.0
+    v = torch.zeros(n, 1, D, device=cuda)
+    v[1], v[late] = -1.0, 1.0
+    bias = torch.full((n,), -200.0, device=cuda)
+    bias[1] = bias[late] = 0.0
+    s = scale * (q.double()[:, 0] * k.double()[late, 0]).sum(1)
+    want = torch.tanh(s / 2)[:, None, None].expand(rows, 1, D)
+    got = cross_attention(q, k, v, _plan(torch, cuda, rows, n, 1, D, "float32"), key_bias=bias, scale=scale).double()
+    # In log2 units: 2^-22 each for q's and k's small values, half a step of 16 for each state's exponent, 2 D U of a score;
+    # the exponential 1 ulp, and as much again for sums and the division.  The result moves by half of a score (in units of e).
+    bound = 0.5 * (math.log(2) * (2 * 2.0 ** -22 + 2 * 2.0 ** -21) + 2 * D * 2.0 ** -24 * float(s.max()) + 8 * 2.0 ** -24)
+    assert float((got - want).abs().max()) <= bound, (float((got - want).abs().max()), bound)

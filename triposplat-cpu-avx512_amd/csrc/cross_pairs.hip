@@ -9,7 +9,7 @@
 //
 // What the pairs do not serve, and the workgroup finds while it reads the states: a magnitude of 2^15 and more of the
 // scaled values (an infinity too); scores that may lose 2^-22 log2 units to the 2^-25 of k's values (|q'|_1 / sk of 8 and
-// more); four neighbouring values of v, not all zero, below 2^-4, or a feature of v, not all zero, that stays below 2^-4 in
+// more) or of q's (D times k's largest, over sq, likewise); four neighbouring values of v, not all zero, below 2^-4, or a feature of v, not all zero, that stays below 2^-4 in
 // all of the states; an infinity or NaN in q.  It then leaves its result to the kernel of bf16 terms, which is launched
 // behind this one and does what is flagged, at that kernel's time.  So a value of v is held to 2^-23 of it or to 2^-21 of
 // the larger of its feature's largest, over the workgroup's states, and its neighbours'.  (Each value by itself cannot be
@@ -90,6 +90,7 @@ __global__ __launch_bounds__(cross_tile(DP, 3, false).wq * 64, 2) void cross_pai
   __shared__ __attribute__((aligned(16))) float biases[2][kKeys];
   __shared__ float largest[2][kWaves];
   __shared__ uint32_t features[DP];  // the upper bits of v's largest magnitudes
+  __shared__ uint32_t k_largest;     // the bits of the scaled k's
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l32 = lane & 31, half = lane >> 5;
@@ -173,6 +174,7 @@ __global__ __launch_bounds__(cross_tile(DP, 3, false).wq * 64, 2) void cross_pai
   }
   if (lane == 0) largest[0][wave] = k_top, largest[1][wave] = v_top;
   if (tid < DP) features[tid] = 0;
+  if (tid == 0) k_largest = 0;
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < kWaves; ++w) k_top = fmaxf(k_top, largest[0][w]), v_top = fmaxf(v_top, largest[1][w]);
@@ -183,7 +185,8 @@ __global__ __launch_bounds__(cross_tile(DP, 3, false).wq * 64, 2) void cross_pai
   const float to_log2 = fmaxf(from_scaled * power(-ek), 0x1p-126f);
   bool bad = !(q_sum * power(-ek) < kPairScores);
 
-  float most = 0.0f, least = INFINITY;  // of the scaled values; of fours of v's that are not all zero
+  // Of the scaled values; least: of fours of v's that are not all zero.
+  float k_most = 0.0f, v_most = 0.0f, least = INFINITY;
   // The upper 16 bits of the largest magnitudes of the eight features that this thread brings, the same in all of its units.
   static_assert(kUnits == 1 || kThreads % (DP / 8) == 0, "a thread's features");
   ushortx2 feature[4] = {};
@@ -203,11 +206,11 @@ __global__ __launch_bounds__(cross_tile(DP, 3, false).wq * 64, 2) void cross_pai
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i) kr[u].x[i] *= k_scale, vr[u].x[i] *= v_scale;
-      most = fmaxf(most, fmaxf(largest4(kr[u].x), largest4(kr[u].x + 4)));
+      k_most = fmaxf(k_most, fmaxf(largest4(kr[u].x), largest4(kr[u].x + 4)));
 #pragma unroll
       for (int i = 0; i < 8; i += 4) {
         const float four = largest4(vr[u].x + i);
-        most = fmaxf(most, four);
+        v_most = fmaxf(v_most, four);
         least = fminf(least, four == 0.0f ? INFINITY : four);
       }
       shortx8 kt[2], vt[2];
@@ -312,9 +315,11 @@ __global__ __launch_bounds__(cross_tile(DP, 3, false).wq * 64, 2) void cross_pai
 
 #pragma unroll
   for (int i = 0; i < 8; ++i) atomicMax(&features[tid % (DP / 8) * 8 + i], (uint32_t)feature[i / 2][i % 2]);
+  atomicMax(&k_largest, __float_as_uint(k_most));
   __syncthreads();
+  const float k_all = __uint_as_float(k_largest);
+  bad |= !(k_all < kPairTop) || !(v_most < kPairTop) || least < kPairLeast || !(to_log2 * k_all * (float)D < kPairScores);
   if (tid < DP && features[tid] != 0) bad |= __uint_as_float(features[tid] << 16) * v_scale < kPairLeast;
-  bad |= !(most < kPairTop) || least < kPairLeast;
   bad = __syncthreads_or(bad);
   if (tid == 0) *flag = bad;
   const int again = thread_again(), out_row = (again >> 6) * 32 + (again & 31);
