@@ -20,9 +20,9 @@ int tsplat_cross_abi_version(void);
  * of kv_heads (query head h reads key head h / (heads / kv_heads)), head_dim 1..128; dtype of q, k, v and out: 0 fp32,
  * 1 bf16, 2 fp16; precision of fp32 products: 0 pairs of fp16 values or three bf16 terms of each factor (fp32
  * accuracy: a score to 2^-21 log2 units besides fp32's own error, a weight to 2^-36 of its row's largest, a value of v to
- * 2^-23 of it or 2^-21 of the largest of its feature or of its four neighbours), 2 two bf16 terms, 1 one (0 for 16-bit
- * types).  Fewer than three terms round finite values to infinities, as bf16 does: one from 3.3962e38 on, two from
- * 3.4027e38 on.
+ * 2^-23 of it or 2^-21 of the largest of its feature or of its four neighbours, and none of q, k, v more finely than to
+ * 2^-134), 2 two bf16 terms, 1 one (0 for 16-bit types).  Fewer than three terms round finite values to infinities, as
+ * bf16 does: one from 3.3962e38 on, two from 3.4027e38 on.
  * Returns the plan's size in ints, or a negative status (-1, -2: sizes; at most 65535 heads, 2^30 - 1 rows times heads of a
  * group, as many states, and 2^32 - 1 threads of a launch).  With plan (host memory of plan_ints ints) it
  * is written there (-3 when too small).  The first TSPLAT_CROSS_HEADER ints describe it. */

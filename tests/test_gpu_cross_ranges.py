@@ -235,3 +235,22 @@ def test_small_query_features(cuda, hiplib, D):
     # the exponential 1 ulp, and as much again for sums and the division.  The result moves by half of a score (in units of e).
     bound = 0.5 * (math.log(2) * (2 * 2.0 ** -22 + 2 * 2.0 ** -21) + 2 * D * 2.0 ** -24 * float(s.max()) + 8 * 2.0 ** -24)
     assert float((got - want).abs().max()) <= bound, (float((got - want).abs().max()), bound)
+
+
+@pytest.mark.parametrize("aligned", [True, False])
+@pytest.mark.parametrize("rows", [2, 100])
+@pytest.mark.parametrize("size", [1e-33, 1e-36, 1e-40])
+def test_smallest_values(cuda, hiplib, size, rows, aligned):
+    """Values whose last bf16 term is subnormal, and subnormal ones: an absolute step of 2^-133 is what is left of them."""
+    import torch
+    from tsplat.cross_attention import cross_attention
+
+    q, k, v = _inputs(torch, cuda, rows, 50, 2, 64, "float32", 10)
+    v *= size
+    if not aligned:
+        q, k, v = (_unaligned(t) for t in (q, k, v))
+    want, bound = ranges(torch, q, k, v, [rows], [50])
+    got = cross_attention(q, k, v, _plan(torch, cuda, rows, 50, 2, 64, "float32"))
+    # half of bf16's smallest step, 2^-134, of each value, whose weights add up to 1; half of fp32's, 2^-150, of each of 50
+    # sums of them at weights of 2^-8: 50 * 2^-142 < 2^-136
+    assert_within(torch, got.double(), want, bound + 2.0 ** -134 + 2.0 ** -136, str(size))
