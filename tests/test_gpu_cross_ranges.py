@@ -254,3 +254,19 @@ def test_smallest_values(cuda, hiplib, size, rows, aligned):
     # half of bf16's smallest step, 2^-134, of each value, whose weights add up to 1; half of fp32's, 2^-150, of each of 50
     # sums of them at weights of 2^-8: 50 * 2^-142 < 2^-136
     assert_within(torch, got.double(), want, bound + 2.0 ** -134 + 2.0 ** -136, str(size))
+
+
+@pytest.mark.parametrize("at", [0, 150])
+def test_values_far_below_the_first_ones(cuda, hiplib, at):
+    """States that scaling by the first ones' largest would bring to zero are not zeros."""
+    import torch
+    from tsplat.cross_attention import cross_attention
+
+    q, k, v = _inputs(torch, cuda, 100, 200, 2, 64, "float32", 11)
+    v *= 1e-12
+    v[at] = 1e38 if at == 0 else 1e31
+    bias = torch.zeros(200, device=cuda)
+    bias[at] = -300.0  # its weight is below 1e-120
+    want, _ = ranges(torch, q, k, torch.where(bias[:, None, None] < 0, 0.0, v), [100], [200], bias)
+    got = cross_attention(q, k, v, _plan(torch, cuda, 100, 200, 2, 64, "float32"), key_bias=bias)
+    assert feature_off(torch, got, want) <= FEATURE

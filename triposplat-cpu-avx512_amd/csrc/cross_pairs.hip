@@ -9,11 +9,11 @@
 //
 // What the pairs do not serve, and the workgroup finds while it reads the states: a magnitude of 2^15 and more of the
 // scaled values (an infinity too); scores that may lose 2^-22 log2 units to the 2^-25 of k's values (|q'|_1 / sk of 8 and
-// more) or of q's (D times k's largest, over sq, likewise); four neighbouring values of v, not all zero, below 2^-4, or a feature of v, not all zero, that stays below 2^-4 in
-// all of the states; an infinity or NaN in q.  It then leaves its result to the kernel of bf16 terms, which is launched
-// behind this one and does what is flagged, at that kernel's time.  So a value of v is held to 2^-23 of it or to 2^-21 of
-// the larger of its feature's largest, over the workgroup's states, and its neighbours'.  (Each value by itself cannot be
-// asked for 2^-4: one in 2000 of a normal distribution is below.)
+// more) or of q's (D times k's largest, over sq, likewise); four neighbouring values of v, not all zero, below 2^-4, or a
+// feature of v, not all zero, that stays below 2^-4 in all of the states; an infinity or NaN in q.  It then leaves its result
+// to the kernel of bf16 terms, which is launched behind this one and does what is flagged, at that kernel's time.  So a value
+// of v is held to 2^-23 of it or to 2^-21 of the larger of its feature's largest, over the workgroup's states, and its
+// neighbours'.  (Each value by itself cannot be asked for 2^-4: one in 2000 of a normal distribution is below.)
 //
 // p = 2^(x - m) for a reference m that is 11 below the row's largest x, or up to 15 (few tiles rescale): below 2^15, and a
 // weight 2^-36 of the largest is still held.  (The exponential's argument is rounded by 2^-21 at most there, 3e-7 of a
@@ -185,7 +185,7 @@ __global__ __launch_bounds__(cross_tile(DP, 3, false).wq * 64, 2) void cross_pai
   const float to_log2 = fmaxf(from_scaled * power(-ek), 0x1p-126f);
   bool bad = !(q_sum * power(-ek) < kPairScores);
 
-  // Of the scaled values; least: of fours of v's that are not all zero.
+  // Largest of the scaled k's and of v's; least: of fours of v's that are not all zero (which scaled ones may become).
   float k_most = 0.0f, v_most = 0.0f, least = INFINITY;
   // The upper 16 bits of the largest magnitudes of the eight features that this thread brings, the same in all of its units.
   static_assert(kUnits == 1 || kThreads % (DP / 8) == 0, "a thread's features");
@@ -205,14 +205,14 @@ __global__ __launch_bounds__(cross_tile(DP, 3, false).wq * 64, 2) void cross_pai
         feature[i] = __builtin_elementwise_max(feature[i], __builtin_bit_cast(ushortx2, two));
       }
 #pragma unroll
-      for (int i = 0; i < 8; ++i) kr[u].x[i] *= k_scale, vr[u].x[i] *= v_scale;
-      k_most = fmaxf(k_most, fmaxf(largest4(kr[u].x), largest4(kr[u].x + 4)));
-#pragma unroll
       for (int i = 0; i < 8; i += 4) {
         const float four = largest4(vr[u].x + i);
         v_most = fmaxf(v_most, four);
         least = fminf(least, four == 0.0f ? INFINITY : four);
       }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) kr[u].x[i] *= k_scale, vr[u].x[i] *= v_scale;
+      k_most = fmaxf(k_most, fmaxf(largest4(kr[u].x), largest4(kr[u].x + 4)));
       shortx8 kt[2], vt[2];
       pair8(kr[u].x, kt);
       pair8(vr[u].x, vt);
@@ -318,7 +318,8 @@ __global__ __launch_bounds__(cross_tile(DP, 3, false).wq * 64, 2) void cross_pai
   atomicMax(&k_largest, __float_as_uint(k_most));
   __syncthreads();
   const float k_all = __uint_as_float(k_largest);
-  bad |= !(k_all < kPairTop) || !(v_most < kPairTop) || least < kPairLeast || !(to_log2 * k_all * (float)D < kPairScores);
+  bad |= !(k_all < kPairTop) || !(to_log2 * k_all * (float)D < kPairScores);
+  bad |= !(v_most * v_scale < kPairTop) || least * v_scale < kPairLeast;
   if (tid < DP && features[tid] != 0) bad |= __uint_as_float(features[tid] << 16) * v_scale < kPairLeast;
   bad = __syncthreads_or(bad);
   if (tid == 0) *flag = bad;
