@@ -14,11 +14,11 @@
 //
 // What bounds it, and measured: many rows, the exponents and what surrounds them in the vector units (a block of 32 x 32
 // takes 125 vector instructions, 16 of them exponents at a quarter of the rate, and 8 products of 64 values a head): 275
-// GFLOP of 2 x 16384 x 2048 in bf16 at 0.71 PFLOP/s, 386 us, 0.80 at 128 values a head.  Five ragged requests with a bias
+// GFLOP of 2 x 16384 x 2048 in bf16 at 0.73 PFLOP/s, 375 us, 0.82 at 128 values a head.  Five ragged requests with a bias
 // in bf16 92 us, 0.44 PFLOP/s: 784 workgroups of 22 and 32 tiles on 768 places (more parts than the plan makes cost more
-// than they even out: 123).  fp32 values in three bf16 terms 1350 us for the former, 1.22 PFLOP/s of bf16 products, which is
-// what a flagged call of cross_pairs.hip takes besides (unaligned 1630: loads of single values); in two terms 836, in one
-// 428.  Few rows: HBM, 64 single tokens over 1.09 GB of bf16 states 221 us, 4.9 TB/s (a copy: 5.0); two single tokens over
+// than they even out: 123).  fp32 values in three bf16 terms 1300 us for the former, 1.27 PFLOP/s of bf16 products, which is
+// what a flagged call of cross_pairs.hip takes besides (unaligned 1570: loads of single values); in two terms 815, in one
+// 425.  Few rows: HBM, 64 single tokens over 1.09 GB of bf16 states 221 us, 4.9 TB/s (a copy: 5.0); two single tokens over
 // 50 MB of fp32 ones 22, of which about 5 join the parts and 6 are a launch and first loads.
 //
 // States go from memory through registers to LDS, a tile ahead of the products; states that the bias masks, or past the
@@ -47,10 +47,13 @@ constexpr float kLog2e = 1.4426950408889634f;
 // Weights are 2^(x - m) for a reference m that follows a row's largest x (log2 units) only when that has passed it by more
 // than kSlack: most tiles rescale nothing.  fp16 weights lie 2^7 higher, below 2^15 at most, so that a weight 2^-31 of the
 // largest is still held (many small ones add up; sums of fp16 values are far from fp32's range).  bf16 has fp32's range, and
-// so may its values: weights of 1 at most, 2^-8 where m has just moved, keep every sum that fp32 holds within it.
-constexpr float kSlack = 8.0f;
-template <class E>
-constexpr float kLift = std::is_same_v<E, half_t> ? 7.0f : -kSlack;
+// so may its values: weights of 1 at most, 2^-kSlack where m has just moved, keep every sum that fp32 holds within it.  fp32
+// values: a slack of 2, as x - m is rounded at its own size (8 rows over 30 states are off by 1.7e-7, with a slack of 8 by
+// 2.4e-7; a normal row's largest score rises by less than that after its first tile).
+template <class T>
+constexpr float kSlack = sizeof(T) == 4 ? 2.0f : 8.0f;
+template <class T>
+constexpr float kLift = std::is_same_v<T, half_t> ? 7.0f : -kSlack<T>;
 
 template <class T>
 struct Element {
@@ -425,8 +428,8 @@ __global__ __launch_bounds__(cross_tile(DP, TERMS, false).wq * 64, !VEC && DP > 
 #pragma unroll
       for (int r = 0; r < 16; ++r) top = fmaxf(top, s[b][r]);
     top = fmaxf(top, other_half(top));
-    const float ref = BIAS ? top - kLift<E> : fmaf(top, to_log2, -kLift<E>);
-    if (__any(ref > m_run + kSlack)) {
+    const float ref = BIAS ? top - kLift<T> : fmaf(top, to_log2, -kLift<T>);
+    if (__any(ref > m_run + kSlack<T>)) {
       const float m_new = fmaxf(m_run, ref);
       // (-inf where nothing has been seen: its sums are zero)
       const float keep = m_run == m_new ? 1.0f : __builtin_amdgcn_exp2f(m_run - m_new);
@@ -581,8 +584,8 @@ __global__ __launch_bounds__(kFewWaves * 64, DP > 64 && (sizeof(T) == 4 || !VEC)
 #pragma unroll
     for (int r = 1; r < 16; ++r) top = fmaxf(top, s[r]);
     top = fmaxf(top, other_half(top));
-    const float ref = BIAS ? top - kLift<E> : fmaf(top, to_log2, -kLift<E>);
-    if (__any(ref > m_run + kSlack)) {
+    const float ref = BIAS ? top - kLift<T> : fmaf(top, to_log2, -kLift<T>);
+    if (__any(ref > m_run + kSlack<T>)) {
       const float m_new = fmaxf(m_run, ref);
       const float keep = m_run == m_new ? 1.0f : __builtin_amdgcn_exp2f(m_run - m_new);
       l_run *= keep;

@@ -19,9 +19,9 @@
 // weight 2^-36 of the largest is still held.  (The exponential's argument is rounded by 2^-21 at most there, 3e-7 of a
 // weight, which its sum has as well; a factor after the exponential instead takes 16 more instructions a block.)
 //
-// 2 x 16384 x 2048, 16 heads of 64: 877 us (the check by features 20 of them; bf16 terms 1350; the flags' launch 5), 0.31
-// PFLOP/s of the operator's operations, 0.94 of fp16 products.  A request whose first tile is masked throughout (128 states
-// for heads up to 64, 32 for wider ones) has no scale from it and goes to the bf16 terms: 2240 us.  What bounds the kernel:
+// 2 x 16384 x 2048, 16 heads of 64: 861 us (22 of them the checks by feature and key; bf16 terms 1300; the flags' launch 5),
+// 0.32 PFLOP/s of the operator's operations, 0.96 of fp16 products.  A request whose first tile is masked throughout (128 states
+// for heads up to 64, 32 for wider ones) has no scale from it and goes to the bf16 terms: 2150 us.  What bounds the kernel:
 // products (45 % of the SIMDs' cycles) and vector instructions (52 %) that hardly overlap, as a SIMD's two waves do the same
 // at the same time: waves of unlike priority, and a block's products between the exponents of the one before, did not change
 // that (12 us more, and spills).
