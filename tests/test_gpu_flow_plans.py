@@ -64,6 +64,18 @@ def test_refused_before_anything_runs(cuda, hiplib, monkeypatch):
         model.velocity(z, c, t, cond_plan=plan)
 
 
+def test_condition_split_into_heads(cuda, hiplib):
+    """[entries, rows, heads, 64] is the same memory as [entries, rows, C], and taken alike by both routes."""
+    import torch
+
+    model = _model(cuda)
+    z, c, t = _inputs(torch, cuda, [20, 20])
+    positions = torch.arange(40, dtype=torch.int32, device=cuda)[:, None]
+    for kwargs in ({}, dict(positions=positions, rope=model.token_rope())):
+        want = model.velocity(z, c.view(2, 20, 128), t, **kwargs)
+        assert torch.equal(model.velocity(z, c.view(2, 20, 2, 64), t, **kwargs), want)
+
+
 def test_one_fill_for_each_entry(cuda, hiplib):
     """Conditions of one length: the entries' slots are written once and spread to both kinds of rows."""
     import torch

@@ -327,8 +327,8 @@ class FlowModel:
                          precision=self.attention_precision, device=self.device)
 
     def check_condition(self, cond, entries):
-        """Refuses a condition that is not [entries, rows, C]."""
-        if cond.dim() != 3 or cond.shape[0] != entries or cond.shape[2] != self.cfg.hidden:
+        """Refuses a condition that is not [entries, rows, C], where C may be split into heads."""
+        if cond.dim() < 3 or cond.shape[0] != entries or math.prod(cond.shape[2:]) != self.cfg.hidden:
             raise ValueError(f"cond must be [{entries}, rows, {self.cfg.hidden}], its shape is {list(cond.shape)}")
 
     def condition_rows(self, cond):
