@@ -71,9 +71,11 @@ def test_condition_split_into_heads(cuda, hiplib):
     model = _model(cuda)
     z, c, t = _inputs(torch, cuda, [20, 20])
     positions = torch.arange(40, dtype=torch.int32, device=cuda)[:, None]
-    for kwargs in ({}, dict(positions=positions, rope=model.token_rope())):
-        want = model.velocity(z, c.view(2, 20, 128), t, **kwargs)
-        assert torch.equal(model.velocity(z, c.view(2, 20, 2, 64), t, **kwargs), want)
+    for precision in ("fp32", "fp8"):
+        model.set_precision(precision)
+        for kwargs in ({}, dict(positions=positions, rope=model.token_rope())):
+            want = model.velocity(z, c.view(2, 20, 128), t, **kwargs)
+            assert torch.equal(model.velocity(z, c.view(2, 20, 2, 64), t, **kwargs), want)
 
 
 def test_one_fill_for_each_entry(cuda, hiplib):

@@ -335,7 +335,7 @@ class FlowModel:
         """cond [..., C] as the blocks' condition Linears read it: its rows in 8 bits, once for all blocks, where all
         of them multiply in precision "fp8", else itself."""
         if cond.numel() and self.blocks and all(blk.lin["xkv"].precision == "fp8" for blk in self.blocks):
-            return quantize_blocks(cond.reshape(-1, cond.shape[-1]))
+            return quantize_blocks(cond.reshape(-1, self.cfg.hidden))
         return cond
 
     def velocity(self, z, cond, t, observe=None, *, adapters=None, slots=None, positions=None, rope=None,
